@@ -28,7 +28,8 @@ DEV_FLAG_NAMES = {1: "bad slot", 2: "bad block id", 4: "context longer than its 
 EXPORTS = ("cx_version", "cx_last_error", "cx_device_error", "cx_kv_append", "cx_kv_gather",
            "cx_block_copy", "cx_paged_workspace_bytes", "cx_paged_decode", "cx_paged_verify",
            "cx_attention_dense", "cx_paged_decode_static", "cx_paged_kernel_kind",
-           "cx_kv_append_rope", "cx_set_wait_limit_ns")
+           "cx_kv_append_rope", "cx_set_wait_limit_ns", "cx_kv_append_norm_rope",
+           "cx_paged_attend", "cx_paged_attend_workspace_bytes", "cx_paged_attend_kind")
 KERNEL_KINDS = {0: "generic", 1: "mma", 2: "tcgen05", 3: "fma"}
 
 
@@ -46,6 +47,29 @@ class CxAttnBatch(ctypes.Structure):
                 ("batch", ctypes.c_int64), ("max_q_len", ctypes.c_int64),
                 ("n_q_heads", ctypes.c_int64), ("scale", ctypes.c_float),
                 ("reserved", ctypes.c_int32), ("window", ctypes.c_int64)]
+
+
+class CxQkv(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+                ("k_token_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+                ("v_token_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64),
+                ("n_tokens", ctypes.c_int64), ("n_q_heads", ctypes.c_int64),
+                ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class CxNormRope(ctypes.Structure):
+    _fields_ = [("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p),
+                ("q_weight_dtype", ctypes.c_int32), ("k_weight_dtype", ctypes.c_int32),
+                ("eps", ctypes.c_float), ("interleaved", ctypes.c_int32),
+                ("cos_table", ctypes.c_void_p), ("sin_table", ctypes.c_void_p),
+                ("table_rows", ctypes.c_int64), ("rot_dim", ctypes.c_int64)]
+
+
+class CxAttnMods(ctypes.Structure):
+    _fields_ = [("softcap", ctypes.c_float), ("out_dtype", ctypes.c_int32),
+                ("alibi_slopes", ctypes.c_void_p), ("prefix_lens", ctypes.c_void_p),
+                ("q_stride", ctypes.c_int64)]
 
 
 class CxError(RuntimeError):
@@ -79,6 +103,15 @@ _SIGS = {
     "cx_set_wait_limit_ns": ([ctypes.c_uint64], None),
     "cx_kv_append_rope": ([ctypes.POINTER(CxPool), _I64, _VP, _VP, _I32, _VP, _VP, _I64, _VP, _VP,
                            _I64, _I32, _VP, _I64, _VP, _I32, _VP], ctypes.c_int),
+    "cx_kv_append_norm_rope": ([ctypes.POINTER(CxPool), _I64, ctypes.POINTER(CxQkv), _VP, _VP,
+                                ctypes.POINTER(CxNormRope), _VP, _I32, _VP], ctypes.c_int),
+    "cx_paged_attend": ([ctypes.POINTER(CxPool), _I64, ctypes.POINTER(CxAttnBatch),
+                         ctypes.POINTER(CxAttnMods), _VP, _I32, _VP, _VP, ctypes.c_size_t, _I32,
+                         _VP], ctypes.c_int),
+    "cx_paged_attend_workspace_bytes": ([ctypes.POINTER(CxPool), ctypes.POINTER(CxAttnBatch)],
+                                        ctypes.c_size_t),
+    "cx_paged_attend_kind": ([ctypes.POINTER(CxPool), ctypes.POINTER(CxAttnBatch), _I32],
+                             ctypes.c_int),
 }
 
 
@@ -124,6 +157,34 @@ def require_cuda(device=None) -> torch.device:
     if dev.type != "cuda":
         raise CxError(f"chenxing_b200 runs on CUDA devices only, got {dev}")
     return dev
+
+
+def same_device(a: torch.device, b: torch.device) -> bool:
+    """Whether two CUDA devices are one; no index means the current device."""
+    if a.type != b.type:
+        return False
+    cur = torch.cuda.current_device() if a.index is None or b.index is None else 0
+    return (cur if a.index is None else a.index) == (cur if b.index is None else b.index)
+
+
+class on_device:
+    """Makes ``device`` the current one while a kernel is launched on it (a
+    launch on a stream of another device than the current one fails); does
+    nothing when it already is."""
+    __slots__ = ("_dev", "_prev")
+
+    def __init__(self, device: torch.device) -> None:
+        self._dev = device.index
+
+    def __enter__(self) -> None:
+        prev = torch.cuda.current_device()
+        self._prev = None if self._dev is None or self._dev == prev else prev
+        if self._prev is not None:
+            torch.cuda.set_device(self._dev)
+
+    def __exit__(self, *exc) -> None:
+        if self._prev is not None:
+            torch.cuda.set_device(self._prev)
 
 
 def cx_dtype(dt: torch.dtype) -> int:

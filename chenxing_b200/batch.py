@@ -8,6 +8,9 @@ whole batch as device arrays, so one ``cx_kv_append`` and one
 ``cx_paged_decode`` / ``cx_paged_verify`` launch serve every sequence of a
 layer.  Tables and lengths are exactly the reference's ``Sequence.block_table``
 and ``n_tokens`` values; nothing here changes them.
+
+A batch may also change the scores (``softcap``, ``alibi_slopes``,
+``prefix_lens``) or ask for a 16-bit output; ``cx_paged_attend`` serves those.
 """
 from __future__ import annotations
 
@@ -18,7 +21,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._arrays import to_device, upload
+from ._arrays import rows_on_device, to_device, upload
 
 __all__ = ["PagedBatch", "slot_mapping", "decode_batch", "verify_batch"]
 
@@ -61,11 +64,26 @@ class PagedBatch:
     per sequence INCLUDING the query tokens being attended (they are appended
     first, as in transformer.py:87-88); q_lens: query tokens per sequence
     (None = decode, one each); window: sliding window or None.
+
+    Score modifiers, none by default (the scaled score of a query at position
+    ``pos`` and a key at ``j`` is ``s``):
+
+    * ``softcap``: ``s`` becomes ``softcap * tanh(s / softcap)``;
+    * ``alibi_slopes`` (n_q_heads values >= 0): ``s -= slope[h] * |pos - j|``,
+      after the cap;
+    * ``prefix_lens`` (one per sequence): keys ``j < prefix_lens[b]`` are seen by
+      every query row of the sequence, past the causal limit (a prompt whose
+      first tokens see one another) and the window (tokens that a long stream
+      keeps); what lies past the context is cut off.
+
+    A batch holds one workspace: its calls run in order on one stream, the one
+    it was made on.
     """
 
     def __init__(self, cache, block_tables, ctx_lens, *, n_q_heads: int, q_lens=None,
                  window: int | None = None, scale: float | None = None,
-                 table_stride: int | None = None) -> None:
+                 table_stride: int | None = None, softcap: float | None = None,
+                 alibi_slopes=None, prefix_lens=None) -> None:
         self.cache = cache
         self.device = cache.device
         self.n_q_heads = int(n_q_heads)
@@ -77,13 +95,28 @@ class PagedBatch:
         self.scale = (1.0 / math.sqrt(cache.head_dim)) if scale is None else float(scale)
         self.verify = q_lens is not None
         self.table_stride = table_stride
+        self.softcap = None if softcap is None else float(softcap)
+        if softcap is not None and not (0 < self.softcap < math.inf):
+            raise ValueError("softcap must be positive and finite (or None)")
+        self.alibi_slopes = None
+        if alibi_slopes is not None:
+            sl = alibi_slopes.detach().cpu().numpy() if isinstance(alibi_slopes, torch.Tensor) \
+                else alibi_slopes
+            sl = np.asarray(sl, dtype=np.float32).reshape(-1)
+            if sl.shape[0] != self.n_q_heads or not np.all(np.isfinite(sl)) or np.any(sl < 0):
+                raise ValueError(f"alibi_slopes must be {self.n_q_heads} finite values >= 0")
+            self.alibi_slopes = upload(sl, self.device)
+        self.prefix_lens = None
+        self.prefix_host = None
+        self._planned_by = None          # entry point that made the workspace's plan
         self._ws = None
         self._ws_bytes = 0
-        self.set(block_tables, ctx_lens, q_lens)
+        self.set(block_tables, ctx_lens, q_lens, prefix_lens)
 
     # ------------------------------------------------------------------ #
-    def set(self, block_tables, ctx_lens, q_lens=None) -> None:
-        """(Re)load tables and lengths; the next attention call re-plans."""
+    def set(self, block_tables, ctx_lens, q_lens=None, prefix_lens=None) -> None:
+        """(Re)load tables and lengths; the next attention call re-plans.  Without
+        ``prefix_lens`` a batch that has some keeps them (for as many sequences)."""
         bs = self.cache.block_size
         B = len(block_tables)
         ctx = np.asarray(ctx_lens, dtype=np.int64).reshape(-1)
@@ -96,6 +129,14 @@ class PagedBatch:
             raise ValueError("a block table is longer than table_stride")
         if np.any(ctx < 0) or np.any(ctx > lens * bs):
             raise ValueError("context length outside [0, len(block_table) * block_size]")
+        if prefix_lens is None:
+            pre = self.prefix_host
+            if pre is not None and pre.shape[0] != B:
+                raise ValueError("prefix_lens must be given again for another batch size")
+        else:
+            pre = np.asarray(prefix_lens, dtype=np.int64).reshape(-1)
+            if pre.shape[0] != B or np.any(pre < 0):
+                raise ValueError("prefix_lens must be one value >= 0 per sequence")
         ids = np.fromiter(itertools.chain.from_iterable(block_tables), dtype=np.int64,
                           count=int(lens.sum()))
         if ids.size and (ids.min() < 0 or ids.max() >= self.cache.n_blocks):
@@ -127,7 +168,11 @@ class PagedBatch:
                                    self.ctx_lens.data_ptr(),
                                    _lib.ptr(self.q_start), B, self.max_q, self.n_q_heads,
                                    self.scale, 0, self.window)
-        need = int(_lib.lib().cx_paged_workspace_bytes(self.cache.cx_pool(), self._c))
+        if pre is not None:
+            self.prefix_host = np.minimum(pre, np.iinfo(np.int32).max)
+            self.prefix_lens = upload(self.prefix_host.astype(np.int32), self.device)
+        need = max(int(_lib.lib().cx_paged_workspace_bytes(self.cache.cx_pool(), self._c)),
+                   int(_lib.lib().cx_paged_attend_workspace_bytes(self.cache.cx_pool(), self._c)))
         if need > self._ws_bytes:
             self._ws = torch.zeros(need, dtype=torch.uint8, device=self.device)
             self._ws_bytes = need
@@ -143,14 +188,24 @@ class PagedBatch:
         """Keys attended per layer (KV token-layers of one step and layer)."""
         if self.window:
             lo = np.maximum(0, self.ctx_host - self.q_lens_host - self.window + 1)
-            return int(np.sum(self.ctx_host - lo))
+            pre = 0 if self.prefix_host is None else np.minimum(self.prefix_host, lo)
+            return int(np.sum(self.ctx_host - lo + pre))
         return int(self.ctx_host.sum())
 
     def kernel_kind(self, q_dtype=torch.bfloat16) -> str:
         """Which libcxkv kernel attends this batch: "generic", "mma" or "tcgen05"."""
+        if self.scored:
+            return _lib.KERNEL_KINDS[_lib.lib().cx_paged_attend_kind(
+                self.cache.cx_pool(), self._c, _lib.cx_dtype(q_dtype))]
         k = _lib.lib().cx_paged_kernel_kind(self.cache.cx_pool(), self._c,
                                             _lib.cx_dtype(q_dtype), int(self.verify))
         return _lib.KERNEL_KINDS[k]
+
+    @property
+    def scored(self) -> bool:
+        """Whether the batch changes the scores or the visible keys."""
+        return self.softcap is not None or self.alibi_slopes is not None \
+            or self.prefix_lens is not None
 
     def c_struct(self) -> _lib.CxAttnBatch:
         return self._c
@@ -160,9 +215,13 @@ class PagedBatch:
         return self._ws
 
 
-def _attend(cache, layer: int, q, batch: PagedBatch, out, replan, fn_name: str):
+def _attend(cache, layer: int, q, batch: PagedBatch, out, replan, out_dtype, fn_name: str):
     if batch.cache is not cache:
         raise ValueError("PagedBatch belongs to a different cache")
+    if out_dtype is None:
+        out_dtype = torch.float32 if out is None else out.dtype
+    if batch.scored or out_dtype != torch.float32:
+        return _attend_scored(cache, layer, q, batch, out, replan, out_dtype)
     qt = to_device(q, cache.device)
     expect = (batch.total_q, batch.n_q_heads, cache.head_dim)
     if tuple(qt.shape) != expect:
@@ -171,26 +230,68 @@ def _attend(cache, layer: int, q, batch: PagedBatch, out, replan, fn_name: str):
         out = torch.empty(expect, dtype=torch.float32, device=cache.device)
     elif tuple(out.shape) != expect or out.dtype != torch.float32 or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous float32 tensor of shape {expect}")
-    do_plan = batch.needs_plan if replan is None else bool(replan)
+    do_plan = _plans(batch, replan, "plain")
     fn = getattr(_lib.lib(), fn_name)
     _lib.check(fn(cache.cx_pool(), int(layer), batch.c_struct(), qt.data_ptr(),
                   _lib.cx_dtype(qt.dtype), out.data_ptr(), batch.workspace.data_ptr(),
                   batch.workspace.numel(), int(do_plan), _lib.stream_ptr(cache.device)), fn_name)
     if do_plan:
         batch.needs_plan = False
+        batch._planned_by = "plain"
     return out
 
 
-def decode_batch(cache, layer: int, q, batch: PagedBatch, out=None, replan=None):
-    """One query token per sequence: q (B, hq, D) -> float32 (B, hq, D)."""
+def _plans(batch: PagedBatch, replan, by: str) -> bool:
+    """Whether this call makes the plan: as asked, or when the batch was
+    (re)loaded or its plan is the other entry point's."""
+    return batch.needs_plan or batch._planned_by != by if replan is None else bool(replan)
+
+
+def _attend_scored(cache, layer: int, q, batch: PagedBatch, out, replan, out_dtype):
+    """``cx_paged_attend``: score modifiers, 16-bit outputs, strided query rows."""
+    dev = cache.device
+    qt = rows_on_device(q, dev)
+    hq, d = batch.n_q_heads, cache.head_dim
+    expect = (batch.total_q, hq, d)
+    if tuple(qt.shape) != expect:
+        raise ValueError(f"q must have shape {expect}, got {tuple(qt.shape)}")
+    if not qt.is_contiguous() and (qt.stride(1) != d or qt.stride(0) < hq * d):
+        qt = qt.contiguous()
+    if out is None:
+        out = torch.empty(expect, dtype=out_dtype, device=dev)
+    elif tuple(out.shape) != expect or out.dtype != out_dtype or not out.is_contiguous() \
+            or not _lib.same_device(out.device, dev):
+        raise ValueError(f"out must be a contiguous {out_dtype} tensor of shape {expect} "
+                         f"on {dev}")
+    mods = _lib.CxAttnMods(batch.softcap or 0.0, _lib.cx_dtype(out_dtype),
+                           _lib.ptr(batch.alibi_slopes), _lib.ptr(batch.prefix_lens),
+                           0 if qt.is_contiguous() else qt.stride(0))
+    do_plan = _plans(batch, replan, "scored")
+    with _lib.on_device(dev):
+        _lib.check(_lib.lib().cx_paged_attend(
+            cache.cx_pool(), int(layer), batch.c_struct(), mods, qt.data_ptr(),
+            _lib.cx_dtype(qt.dtype), out.data_ptr(), batch.workspace.data_ptr(),
+            batch.workspace.numel(), int(do_plan), _lib.stream_ptr(dev)), "cx_paged_attend")
+    if do_plan:
+        batch.needs_plan = False
+        batch._planned_by = "scored"
+    return out
+
+
+def decode_batch(cache, layer: int, q, batch: PagedBatch, out=None, replan=None,
+                 out_dtype=None):
+    """One query token per sequence: q (B, hq, D) -> (B, hq, D), float32 unless
+    ``out`` or ``out_dtype`` says bfloat16 or float16."""
     if batch.verify:
         raise ValueError("decode_batch needs a PagedBatch built without q_lens")
-    return _attend(cache, layer, q, batch, out, replan, "cx_paged_decode")
+    return _attend(cache, layer, q, batch, out, replan, out_dtype, "cx_paged_decode")
 
 
-def verify_batch(cache, layer: int, q, batch: PagedBatch, out=None, replan=None):
+def verify_batch(cache, layer: int, q, batch: PagedBatch, out=None, replan=None,
+                 out_dtype=None):
     """q_lens[b] query tokens per sequence (speculative verify / prefill chunk):
-    q (sum q_lens, hq, D) -> float32 (sum q_lens, hq, D)."""
+    q (sum q_lens, hq, D) -> (sum q_lens, hq, D), float32 unless ``out`` or
+    ``out_dtype`` says bfloat16 or float16."""
     if not batch.verify:
         raise ValueError("verify_batch needs a PagedBatch built with q_lens")
-    return _attend(cache, layer, q, batch, out, replan, "cx_paged_verify")
+    return _attend(cache, layer, q, batch, out, replan, out_dtype, "cx_paged_verify")

@@ -46,6 +46,8 @@ struct GenericParams {
     int64_t table_stride;
     const int32_t* ctx_lens;
     const int32_t* q_start;  // NULL: one query per sequence
+    cx_attn_mods mod;        // read by the MOD instantiations only
+    void* mod_out;           // their output, of mod.out_dtype
 };
 
 constexpr int kGenRows = 8;     // packed rows per CTA
@@ -78,7 +80,9 @@ struct GenSmem {
     }
 };
 
-template <typename QT, typename KT, bool PAGED>
+// MOD (paged only): tanh cap, distance bias, visible prefix, strided queries and
+// output type of cx_paged_attend.
+template <typename QT, typename KT, bool PAGED, bool MOD = false>
 __global__ void __launch_bounds__(kGenWarps * 32) attn_generic_kernel(GenericParams p) {
     extern __shared__ float gsm[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -119,11 +123,16 @@ __global__ void __launch_bounds__(kGenWarps * 32) attn_generic_kernel(GenericPar
         float v = 0.f;
         if (r < nr) {
             const int64_t R = r0 + r, i = R / G, h = kh * G + R % G;
-            const int64_t qoff = PAGED ? ((q0 + i) * p.hq + h) * p.d
+            const int64_t qoff = MOD     ? (q0 + i) * p.mod.q_stride + h * p.d
+                                 : PAGED ? ((q0 + i) * p.hq + h) * p.d
                                        : ((b * p.hq + h) * sq + i) * p.d;
             v = Conv<QT>::to_f(qb[qoff + d]);
         }
         s_q[r * L.qs + d] = v;
+    }
+    int64_t pre = 0;                                   // keys every row sees
+    if constexpr (MOD) {
+        if (p.mod.prefix_lens) pre = min(max((int64_t)p.mod.prefix_lens[b], (int64_t)0), sk);
     }
     // key range over all rows of the CTA: [lo_all, hi_all]
     int64_t lo_all = sk, hi_all = -1;
@@ -137,6 +146,15 @@ __global__ void __launch_bounds__(kGenWarps * 32) attn_generic_kernel(GenericPar
         if (hi >= lo) {
             lo_all = lo < lo_all ? lo : lo_all;
             hi_all = hi > hi_all ? hi : hi_all;
+        }
+    }
+    // with a prefix the range starts at 0; tiles between it and the window are
+    // skipped below
+    const int64_t lo_run = lo_all;
+    if constexpr (MOD) {
+        if (pre > 0) {
+            lo_all = 0;
+            hi_all = hi_all > pre - 1 ? hi_all : pre - 1;
         }
     }
     __syncthreads();
@@ -165,6 +183,9 @@ __global__ void __launch_bounds__(kGenWarps * 32) attn_generic_kernel(GenericPar
     const int64_t t_end = hi_all >= lo_all ? hi_all / kGenKeys + 1 : 0;
     for (int64_t t = t_first + warp; t < t_end; t += kGenWarps) {
         const int64_t k0 = t * kGenKeys;
+        if constexpr (MOD) {
+            if (k0 >= pre && k0 + kGenKeys <= lo_run) continue;
+        }
         // ---- stage K and V of keys k0 .. k0 + 15 (fp32; keys outside [0, sk)
         // or in a bad block: zeros, and marked invalid).  Lane jj < 16 finds
         // key k0 + jj's row offset (one table lookup a key); the rows are then
@@ -271,7 +292,15 @@ __global__ void __launch_bounds__(kGenWarps * 32) attn_generic_kernel(GenericPar
             bool ok = r < nr && ((valid >> j) & 1u);
             if (ok) {
                 const int64_t iq = (r0 + r) / G, pos = sk - sq + iq;
-                if (p.mask_kind == 1)
+                if constexpr (MOD) {
+                    ok = key < pre || (key <= pos && (p.window <= 0 || key > pos - p.window));
+                    if (p.mod.softcap > 0.f)
+                        sc = p.mod.softcap * tanhf(sc / p.mod.softcap);
+                    if (p.mod.alibi_slopes) {
+                        const int64_t dist = pos > key ? pos - key : key - pos;
+                        sc -= p.mod.alibi_slopes[kh * G + (r0 + r) % G] * (float)dist;
+                    }
+                } else if (p.mask_kind == 1)
                     ok = key <= pos && (p.window <= 0 || key > pos - p.window);
                 else if (p.mask_kind == 2)
                     ok = p.mask[iq * sk + key] != 0;
@@ -324,7 +353,10 @@ __global__ void __launch_bounds__(kGenWarps * 32) attn_generic_kernel(GenericPar
             for (int r = 0; r < kGenRows; ++r) {
                 const float pr = s_p[r * kGenKeys + jj];
 #pragma unroll
-                for (int e = 0; e < kGenMaxE; ++e) acc[r][e] = fmaf(pr, vv[e], acc[r][e]);
+                for (int e = 0; e < kGenMaxE; ++e) {
+                    // MOD: a key the row does not see adds nothing, whatever it holds
+                    if (!MOD || pr != 0.f) acc[r][e] = fmaf(pr, vv[e], acc[r][e]);
+                }
             }
         }
         __syncwarp();
@@ -374,28 +406,31 @@ __global__ void __launch_bounds__(kGenWarps * 32) attn_generic_kernel(GenericPar
         }
         const int64_t R = r0 + r, i = R / G, h = kh * G + R % G;
         const int64_t ooff = PAGED ? ((q0 + i) * p.hq + h) * p.dv : ((b * p.hq + h) * sq + i) * p.dv;
-        p.out[ooff + d] = Lsum > 0.f ? O / Lsum : 0.f;
+        if constexpr (MOD)
+            store_as(p.mod_out, p.mod.out_dtype, ooff + d, Lsum > 0.f ? O / Lsum : 0.f);
+        else
+            p.out[ooff + d] = Lsum > 0.f ? O / Lsum : 0.f;
     }
 }
 
-template <bool PAGED, typename QT>
+template <bool PAGED, typename QT, bool MOD>
 static int launch_generic_kv(int32_t kvdt, const GenericParams& p, dim3 grid, size_t smem,
                              cudaStream_t st) {
     switch (kvdt) {
         case CX_F32: {
-            auto k = attn_generic_kernel<QT, float, PAGED>;
+            auto k = attn_generic_kernel<QT, float, PAGED, MOD>;
             CX_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
             k<<<grid, kGenWarps * 32, smem, st>>>(p);
             break;
         }
         case CX_BF16: {
-            auto k = attn_generic_kernel<QT, __nv_bfloat16, PAGED>;
+            auto k = attn_generic_kernel<QT, __nv_bfloat16, PAGED, MOD>;
             CX_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
             k<<<grid, kGenWarps * 32, smem, st>>>(p);
             break;
         }
         case CX_F16: {
-            auto k = attn_generic_kernel<QT, __half, PAGED>;
+            auto k = attn_generic_kernel<QT, __half, PAGED, MOD>;
             CX_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
             k<<<grid, kGenWarps * 32, smem, st>>>(p);
             break;
@@ -405,7 +440,7 @@ static int launch_generic_kv(int32_t kvdt, const GenericParams& p, dim3 grid, si
     return check_launch("attn_generic_kernel");
 }
 
-template <bool PAGED>
+template <bool PAGED, bool MOD = false>
 static int launch_generic(int32_t qdt, int32_t kvdt, const GenericParams& p, cudaStream_t st) {
     const int64_t G = p.hq / p.hk;
     const int64_t rows = G * p.max_q;
@@ -416,9 +451,9 @@ static int launch_generic(int32_t qdt, int32_t kvdt, const GenericParams& p, cud
     const size_t smem = GenSmem::of(p.d, p.dv).bytes(p.dv);
     dim3 grid((unsigned)(p.batch * p.hk), (unsigned)gy);
     switch (qdt) {
-        case CX_F32: return launch_generic_kv<PAGED, float>(kvdt, p, grid, smem, st);
-        case CX_BF16: return launch_generic_kv<PAGED, __nv_bfloat16>(kvdt, p, grid, smem, st);
-        case CX_F16: return launch_generic_kv<PAGED, __half>(kvdt, p, grid, smem, st);
+        case CX_F32: return launch_generic_kv<PAGED, float, MOD>(kvdt, p, grid, smem, st);
+        case CX_BF16: return launch_generic_kv<PAGED, __nv_bfloat16, MOD>(kvdt, p, grid, smem, st);
+        case CX_F16: return launch_generic_kv<PAGED, __half, MOD>(kvdt, p, grid, smem, st);
         default: return fail(CX_ERR_DTYPE, "attention: unknown query dtype");
     }
 }

@@ -68,6 +68,16 @@ template <> struct Conv<__half> {
     __device__ __forceinline__ static __half from_f(float x) { return __float2half_rn(x); }
 };
 
+// Element `i` of an array whose element type is known at run time only.
+__device__ __forceinline__ void store_as(void* p, int32_t dtype, int64_t i, float x) {
+    if (dtype == CX_F32)
+        static_cast<float*>(p)[i] = x;
+    else if (dtype == CX_BF16)
+        static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
+    else
+        static_cast<__half*>(p)[i] = __float2half_rn(x);
+}
+
 // ---- shared-memory / PTX helpers -----------------------------------------
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));

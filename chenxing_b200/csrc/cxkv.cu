@@ -3,8 +3,10 @@
 // relocatable device code).
 #include "capi.cuh"
 #include "kv_ops.cuh"
+#include "kv_norm_rope.cuh"
 #include "attn_generic.cuh"
 #include "attn_paged_mma.cuh"
+#include "attn_scored.cuh"
 
 // ---------------------------------------------------------------------------
 // Paged decode that allocates nothing.

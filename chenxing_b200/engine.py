@@ -79,7 +79,8 @@ class BatchedKVEngine:
 
     def __init__(self, cache: RadixPagedKVCache, *, n_q_heads: int, window: int | None = None,
                  scale: float | None = None, free_private_blocks: bool = False,
-                 publish_mode: str = "reference") -> None:
+                 publish_mode: str = "reference", softcap: float | None = None,
+                 alibi_slopes=None) -> None:
         if publish_mode not in ("reference", "suffix"):
             raise ValueError("publish_mode must be 'reference' or 'suffix'")
         self.cache = cache
@@ -87,6 +88,8 @@ class BatchedKVEngine:
         self.n_q_heads = int(n_q_heads)
         self.window = window
         self.scale = scale
+        self.softcap = softcap                    # score modifiers of PagedBatch
+        self.alibi_slopes = alibi_slopes
         self.free_private_blocks = free_private_blocks
         self.seqs: dict = {}
         self._alias_refs: Counter = Counter()     # block id -> live sequences aliasing it
@@ -208,7 +211,7 @@ class BatchedKVEngine:
     # one step
     # ------------------------------------------------------------------ #
     def plan(self, seq_ids, q_lens=None, *, verify: bool | None = None,
-             attend: bool = True) -> StepPlan:
+             attend: bool = True, prefix_lens=None) -> StepPlan:
         """Host metadata for one step: ``q_lens[i]`` new positions for
         sequence ``seq_ids[i]`` starting at its ``n_tokens``.  Grows tables like
         ``LLMEngine._ensure_capacity`` (engine.py:74-85, LRU eviction through
@@ -216,7 +219,9 @@ class BatchedKVEngine:
         preemption policy), privatises aliased blocks about to be written,
         and loads the batch's slots (and, with ``attend``, tables and
         lengths) onto the device.  ``attend=False`` is for steps that only
-        write K/V (a prompt whose attention the caller does elsewhere)."""
+        write K/V (a prompt whose attention the caller does elsewhere).
+        ``prefix_lens``: per sequence, the leading tokens that every query row
+        sees (``PagedBatch``)."""
         p = self.plan_host(seq_ids, q_lens)
         c = self.cache
         dev = c.device
@@ -228,7 +233,8 @@ class BatchedKVEngine:
             p.batch = PagedBatch(c, [s.block_table for s in p.seqs], p.n_past + p.q_lens,
                                  n_q_heads=self.n_q_heads,
                                  q_lens=p.q_lens if is_verify else None,
-                                 window=self.window, scale=self.scale)
+                                 window=self.window, scale=self.scale, softcap=self.softcap,
+                                 alibi_slopes=self.alibi_slopes, prefix_lens=prefix_lens)
         if p.cow_host:
             arr = np.asarray(p.cow_host, dtype=np.int32).T.copy()
             p.cow = tuple(upload(a, dev) for a in arr)
@@ -281,12 +287,15 @@ class BatchedKVEngine:
         plan.appended.add(int(layer))
 
     def append_rope(self, plan: StepPlan, layer: int, k, v, rope, q=None,
-                    q_out_dtype=torch.bfloat16):
+                    q_out_dtype=torch.bfloat16, *, q_weight=None, k_weight=None,
+                    eps: float = 1e-6):
         """``append`` with RoPE fused in: K rotated at each token's absolute
         position (its sequence's committed length + index in the step), V
         copied, and Q rotated into the returned tensor (transformer.py:84-87).
         The plan's copy-on-write copies run once, for every layer, before the
-        first such call."""
+        first such call.  With ``q_weight`` / ``k_weight``, or tables of part
+        of the head, the heads are RMS-normed and rotated by
+        ``cache.append_norm_rope``."""
         if plan.cow_host and not plan.cow_done:
             for src, dst, n in plan.cow_host:          # all layers at once
                 if n > 0:
@@ -297,22 +306,28 @@ class BatchedKVEngine:
                                   for n0, n in zip(plan.n_past, plan.q_lens)]) \
                 if len(plan.q_lens) else np.zeros(0, dtype=np.int64)
             plan.positions = upload(pos, self.cache.device)
-        qo = self.cache.append_rope(layer, k, v, plan.slots, plan.positions, rope, q,
-                                    q_out_dtype)
+        if q_weight is not None or k_weight is not None or rope.head_dim != self.cache.head_dim:
+            qo = self.cache.append_norm_rope(layer, k, v, plan.slots, plan.positions, rope, q,
+                                             q_weight=q_weight, k_weight=k_weight, eps=eps,
+                                             q_out_dtype=q_out_dtype)
+        else:
+            qo = self.cache.append_rope(layer, k, v, plan.slots, plan.positions, rope, q,
+                                        q_out_dtype)
         plan.appended.add(int(layer))
         return qo
 
-    def attend(self, plan: StepPlan, layer: int, q, out=None):
+    def attend(self, plan: StepPlan, layer: int, q, out=None, out_dtype=None):
         """Paged attention of the step's query rows (sum q_lens, Hq, D) over
-        every committed position plus the step's own; float32 output."""
+        every committed position plus the step's own; float32 output unless
+        ``out`` or ``out_dtype`` says otherwise."""
         if plan.batch is None:
             raise RuntimeError("plan(..., attend=False) has no attention batch")
         if int(layer) not in plan.appended:
             raise RuntimeError("attend() before append() for this layer: the step's own "
                                "keys would be missing")
         if plan.batch.verify:
-            return self.cache.verify_batch(layer, q, plan.batch, out)
-        return self.cache.decode_batch(layer, q, plan.batch, out)
+            return self.cache.verify_batch(layer, q, plan.batch, out, out_dtype=out_dtype)
+        return self.cache.decode_batch(layer, q, plan.batch, out, out_dtype=out_dtype)
 
     def commit(self, plan: StepPlan) -> None:
         """``forward_ids``'s ``seq.n_tokens += len(new_ids)`` (engine.py:127)."""

@@ -10,6 +10,8 @@ libcxkv kernel:
 * ``write_layer``  -> ``cx_kv_append``  (slot-mapped scatter, radix_kv.py:113-128)
 * ``append_rope``  -> ``cx_kv_append_rope`` (apply_rope on Q and K fused into the
   scatter, transformer.py:84-87)
+* ``append_norm_rope`` -> ``cx_kv_append_norm_rope`` (per-head RMS norm of Q and
+  K, partial rotation and the scatter in one launch)
 * ``read_layer``   -> ``cx_kv_gather``  (radix_kv.py:130-144)
 * ``copy_blocks`` / ``cow_tail`` / ``compact`` -> ``cx_block_copy`` (no reference
   counterpart)
@@ -31,7 +33,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._arrays import to_device, to_numpy, torch_dtype, upload
+from ._arrays import rows_on_device, to_device, to_numpy, torch_dtype, upload
 
 __all__ = ["RadixPagedKVCache", "RadixIndex", "PrefixHit", "OutOfKVCacheError"]
 
@@ -627,12 +629,75 @@ class RadixPagedKVCache(RadixIndex):
             "cx_kv_append_rope")
         return qo
 
-    def decode_batch(self, layer: int, q, batch, out=None, replan=None):
+    def append_norm_rope(self, layer: int, k, v, slot_mapping, positions, rope, q=None, *,
+                         q_weight=None, k_weight=None, eps: float = 1e-6, q_out_dtype=None):
+        """RMS norm of every query and key head, rotation of its leading dims and
+        the append, in one launch; returns Q (T, Hq, D) of ``q_out_dtype`` (the
+        rows' type by default), None without ``q``.
+
+        q (T, Hq, D), k and v (T, Hkv, D): one float type, any token and head
+        strides (slices of one projection are read in place).  A row ``x``
+        becomes ``x * rsqrt(mean(x^2) + eps) * weight``; a weight of None
+        leaves the query or key rows as they are.  ``rope.head_dim`` leading
+        dims are then rotated (all of them, or part of the head).  Everything
+        is fp32 and rounded once.  A negative slot stores K and V nowhere (Q is
+        still returned); the slots of one call must differ.  Weights: (D,),
+        float32 or the rows' type."""
+        qt = None if q is None else rows_on_device(q, self.device)
+        kt, vt = rows_on_device(k, self.device), rows_on_device(v, self.device)
+        if vt.dtype != kt.dtype or (qt is not None and qt.dtype != kt.dtype):
+            raise TypeError("q, k and v must have one element type")
+        T, D = int(kt.shape[0]), self.head_dim
+        shape = (T, self.n_kv_heads, D)
+        if tuple(kt.shape) != shape or tuple(vt.shape) != shape:
+            raise ValueError(f"k and v must have shape {shape}, got {tuple(kt.shape)} / "
+                             f"{tuple(vt.shape)}")
+        if qt is not None and (qt.dim() != 3 or qt.shape[0] != T or qt.shape[2] != D):
+            raise ValueError(f"q must be ({T}, Hq, {D}), got {tuple(qt.shape)}")
+        if rope.head_dim > D:
+            raise ValueError(f"RoPE tables of {rope.head_dim} dims for heads of {D}")
+        if not _lib.same_device(rope.device, self.device):
+            raise ValueError(f"RoPE tables on {rope.device}, the cache on {self.device}")
+        st = to_device(slot_mapping, self.device, float_only=False).to(torch.int64)
+        ps = to_device(positions, self.device, float_only=False).to(torch.int64)
+        if st.numel() != T or ps.numel() != T:
+            raise ValueError("slot_mapping and positions need one entry per token")
+
+        def weight(w, what):
+            if w is None:
+                return None
+            w = to_device(w, self.device)
+            if w.numel() != D:
+                raise ValueError(f"{what} must have {D} elements, got {w.numel()}")
+            return w if w.dtype in (torch.float32, kt.dtype) else w.float()
+
+        qw, kw = weight(q_weight, "q_weight"), weight(k_weight, "k_weight")
+        f32 = _lib.CX_F32
+        how = _lib.CxNormRope(_lib.ptr(qw), _lib.ptr(kw),
+                              f32 if qw is None else _lib.cx_dtype(qw.dtype),
+                              f32 if kw is None else _lib.cx_dtype(kw.dtype), float(eps),
+                              int(rope.interleaved), rope.cos.data_ptr(), rope.sin.data_ptr(),
+                              rope.rows, rope.head_dim)
+        qo, hq, qs = None, 0, (0, 0)
+        if qt is not None:
+            hq, qs = int(qt.shape[1]), qt.stride()
+            qo = torch.empty(qt.shape, dtype=q_out_dtype or kt.dtype, device=self.device)
+        ks, vs = kt.stride(), vt.stride()
+        rows = _lib.CxQkv(_lib.ptr(qt), kt.data_ptr(), vt.data_ptr(), qs[0], qs[1], ks[0], ks[1],
+                          vs[0], vs[1], T, hq, _lib.cx_dtype(kt.dtype), 0)
+        with _lib.on_device(self.device):
+            _lib.check(_lib.lib().cx_kv_append_norm_rope(
+                self._pool, int(layer), rows, st.data_ptr(), ps.data_ptr(), how, _lib.ptr(qo),
+                f32 if qo is None else _lib.cx_dtype(qo.dtype), _lib.stream_ptr(self.device)),
+                "cx_kv_append_norm_rope")
+        return qo
+
+    def decode_batch(self, layer: int, q, batch, out=None, replan=None, out_dtype=None):
         """Paged flash-decode of one query token per sequence of ``batch``."""
         from .batch import decode_batch
-        return decode_batch(self, layer, q, batch, out, replan)
+        return decode_batch(self, layer, q, batch, out, replan, out_dtype)
 
-    def verify_batch(self, layer: int, q, batch, out=None, replan=None):
+    def verify_batch(self, layer: int, q, batch, out=None, replan=None, out_dtype=None):
         """Paged multi-query attention (speculative verify / prefill chunk)."""
         from .batch import verify_batch
-        return verify_batch(self, layer, q, batch, out, replan)
+        return verify_batch(self, layer, q, batch, out, replan, out_dtype)

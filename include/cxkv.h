@@ -129,6 +129,53 @@ int cx_kv_append_rope(const cx_pool* pool, int64_t layer, const void* k_new, con
                       int64_t table_rows, int32_t interleaved, const void* q,
                       int64_t n_q_heads, void* q_out, int32_t q_out_dtype, void* stream);
 
+/* New rows of one step: q [n_tokens][n_q_heads][head_dim] (NULL with n_q_heads
+ * 0), k and v [n_tokens][n_kv_heads][head_dim], all of `dtype`, the innermost
+ * dimension contiguous.  Token and head strides are in elements, so the three
+ * may be slices of one projection's output. */
+typedef struct cx_qkv {
+    const void* q;
+    const void* k;
+    const void* v;
+    int64_t q_token_stride, q_head_stride;
+    int64_t k_token_stride, k_head_stride;
+    int64_t v_token_stride, v_head_stride;
+    int64_t n_tokens;
+    int64_t n_q_heads;
+    int32_t dtype;           /* CX_F32 / CX_BF16 / CX_F16 */
+    int32_t reserved;
+} cx_qkv;
+
+/* Per-head RMS norm and rotation of query and key rows.  A NULL weight leaves
+ * those rows unnormalised; weights are [head_dim], CX_F32 or the rows' type. */
+typedef struct cx_norm_rope {
+    const void* q_weight;
+    const void* k_weight;
+    int32_t q_weight_dtype;
+    int32_t k_weight_dtype;
+    float eps;
+    int32_t interleaved;     /* pairs (2j, 2j + 1), else (j, j + rot_dim / 2) */
+    const float* cos_table;  /* [table_rows][rot_dim] */
+    const float* sin_table;
+    int64_t table_rows;
+    int64_t rot_dim;         /* leading dims rotated: even, 2 .. head_dim */
+} cx_norm_rope;
+
+/* RMS norm of every query and key head, rotation of its leading rot_dim dims,
+ * and the append, in one launch (rms_norm, chenxing/core/tensor.py:36, before
+ * what cx_kv_append_rope replaces; the reference has no norm of single heads).
+ * A row x becomes x * rsqrt(mean(x^2) + eps) * weight; its first rot_dim dims
+ * are rotated at positions[t], the others are left; all in fp32, rounded once
+ * to the destination type.  K goes to slot_mapping[t] like cx_kv_append
+ * (negative slot = stored nowhere; the slots of one call must differ), V is
+ * copied, Q goes to q_out [n_tokens][n_q_heads][head_dim] (q_out_dtype)
+ * whatever its slot.  A position outside the table raises CX_DEV_BAD_POSITION
+ * and skips the token. */
+int cx_kv_append_norm_rope(const cx_pool* pool, int64_t layer, const cx_qkv* rows,
+                           const int64_t* slot_mapping, const int64_t* positions,
+                           const cx_norm_rope* how, void* q_out, int32_t q_out_dtype,
+                           void* stream);
+
 /* KV gather — replaces RadixPagedKVCache.read_layer
  * (chenxing/engine/radix_kv.py:130-144): k_out/v_out [n_tokens][n_kv_heads]
  * [head_dim] (pool dtype) receive the first n_tokens positions of the
@@ -223,6 +270,43 @@ void cx_set_wait_limit_ns(uint64_t ns);
 enum { CX_KERNEL_GENERIC = 0, CX_KERNEL_MMA = 1, CX_KERNEL_TCGEN05 = 2, CX_KERNEL_FMA = 3 };
 int cx_paged_kernel_kind(const cx_pool* pool, const cx_attn_batch* batch, int32_t q_dtype,
                          int32_t verify);
+
+/* What cx_paged_attend does to the scores and the output, beside the batch's
+ * scale and window (no counterpart in the reference). */
+typedef struct cx_attn_mods {
+    float softcap;               /* > 0: score s becomes softcap * tanh(s / softcap);  */
+                                 /* 0: scores are not capped                           */
+    int32_t out_dtype;           /* CX_F32 / CX_BF16 / CX_F16                          */
+    const float* alibi_slopes;   /* [n_q_heads] on the device, or NULL: the score of a */
+                                 /* key at j for a query at pos gets                   */
+                                 /* -slope[h] * |pos - j| after the cap (slopes >= 0)  */
+    const int32_t* prefix_lens;  /* [batch] on the device, or NULL: keys               */
+                                 /* j < prefix_lens[b] are seen by every query row,    */
+                                 /* past the causal limit and the window               */
+    int64_t q_stride;            /* elements between query tokens (0: contiguous);     */
+                                 /* the heads of a token are contiguous                */
+} cx_attn_mods;
+
+/* Paged attention with score modifiers: cx_paged_decode (batch->q_start NULL)
+ * or cx_paged_verify (q_start given) with
+ *     s    = scale * (q . k)
+ *     s    = softcap * tanh(s / softcap)          when softcap > 0
+ *     s    = s - slope[h] * |pos - j|             with alibi_slopes
+ *     seen = j < prefix  or  (j <= pos and (window <= 0 or j > pos - window))
+ * over keys j < ctx_lens[b].  out is [rows][n_q_heads][head_dim] of
+ * out_dtype, rounded once from the fp32 accumulators; a row that sees no key is
+ * zero.  What the pool holds at positions that no query row of a sequence sees
+ * (past the context in its last block, left of every row's window) does not
+ * reach the result, NaN and infinity included; at a position that only some
+ * rows see, V must be finite.  Workspace: cx_paged_attend_workspace_bytes,
+ * zero-filled once; a plan made by cx_paged_decode / cx_paged_verify does not
+ * serve this call, nor the other way round. */
+int cx_paged_attend(const cx_pool* pool, int64_t layer, const cx_attn_batch* batch,
+                    const cx_attn_mods* mods, const void* q, int32_t q_dtype, void* out,
+                    void* workspace, size_t workspace_bytes, int32_t replan, void* stream);
+size_t cx_paged_attend_workspace_bytes(const cx_pool* pool, const cx_attn_batch* batch);
+/* Which kernel cx_paged_attend runs (CX_KERNEL_*), as cx_paged_kernel_kind. */
+int cx_paged_attend_kind(const cx_pool* pool, const cx_attn_batch* batch, int32_t q_dtype);
 
 /* Dense attention — replaces flash_attention / naive_attention on contiguous
  * arrays (chenxing/core/attention.py:43-148): q [b][hq][sq][d],
