@@ -2,11 +2,12 @@
 
     python -m chenxing_b200.build
 
-The library is one translation unit (csrc/cxkv.cu includes the parts), linked
-against the static CUDA runtime, so it only needs the NVIDIA driver at run
-time.  Rebuilds unless the stamp file beside the library records the SHA-256
-of exactly the current sources, headers, nvcc flags and nvcc version (file
-times are not trusted: a library copied along with the tree keeps them).
+The library is two translation units (csrc/cxkv.cu and csrc/cxkv_scored.cu
+include the parts; compiled side by side), linked against the static CUDA
+runtime, so it only needs the NVIDIA driver at run time.  Rebuilds unless the
+stamp file beside the library records the SHA-256 of exactly the current
+sources, headers, nvcc flags and nvcc version (file times are not trusted: a
+library copied along with the tree keeps them).
 """
 from __future__ import annotations
 
@@ -16,13 +17,15 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libcxkv.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-shared", "-Xcompiler", "-fPIC,-O2",
-         "-Xptxas", "-v"]
+FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O2", "-Xptxas", "-v"]
+UNITS = ("cxkv.cu", "cxkv_scored.cu")
 
 
 def sources():
@@ -72,14 +75,26 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return LIB
     digest = content_hash()
     tmp = LIB + ".tmp"
-    cmd = [nvcc(), *ARCH, *FLAGS, "-I", os.path.join(ROOT, "include"),
-           os.path.join(HERE, "csrc", "cxkv.cu"), "-o", tmp]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        sys.stderr.write(res.stdout + res.stderr)
+
+    def nvcc_run(*args):
+        r = subprocess.run([nvcc(), *ARCH, *args], stdout=subprocess.PIPE,
+                           stderr=subprocess.STDOUT, text=True)
+        return r.returncode, r.stdout
+
+    with tempfile.TemporaryDirectory() as work, ThreadPoolExecutor(len(UNITS)) as pool:
+        objs = [os.path.join(work, u + ".o") for u in UNITS]
+        done = list(pool.map(
+            lambda u, o: nvcc_run(*FLAGS, "-I", os.path.join(ROOT, "include"), "-c",
+                                  os.path.join(HERE, "csrc", u), "-o", o), UNITS, objs))
+        if all(rc == 0 for rc, _ in done):
+            done.append(nvcc_run("-shared", *objs, "-o", tmp))
+    logs = "".join(log for _, log in done)
+    failed = any(rc != 0 for rc, _ in done)
+    if failed:
+        sys.stderr.write(logs)
         raise RuntimeError("nvcc failed to build libcxkv.so")
     if verbose:
-        sys.stderr.write(res.stderr)
+        sys.stderr.write(logs)
     os.replace(tmp, LIB)
     with open(STAMP, "w") as f:
         f.write(digest + "\n")

@@ -460,6 +460,7 @@ static int launch_generic(int32_t qdt, int32_t kvdt, const GenericParams& p, cud
 
 }  // namespace cx
 
+#ifdef CX_API_TU
 extern "C" int cx_attention_dense(const void* q, int32_t q_dtype, const void* k, const void* v,
                                   int32_t kv_dtype, int64_t b, int64_t hq, int64_t sq, int64_t hk,
                                   int64_t sk, int64_t d, int64_t dv, int32_t mask_kind,
@@ -496,3 +497,4 @@ extern "C" int cx_attention_dense(const void* q, int32_t q_dtype, const void* k,
     p.sk = sk;
     return launch_generic<false>(q_dtype, kv_dtype, p, as_stream(stream));
 }
+#endif  // CX_API_TU

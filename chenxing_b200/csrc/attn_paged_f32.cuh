@@ -68,7 +68,7 @@ struct F32Cfg {
     }
 };
 
-template <int D, int HG, int RT>
+template <int D, int HG, int RT, bool MOD = false>
 __global__ void __launch_bounds__(F32Cfg<D, HG, RT>::MAX_THREADS, 1)
     paged_attn_f32_kernel(const __grid_constant__ CUtensorMap tmk,
                           const __grid_constant__ CUtensorMap tmv, const MmaParams p) {
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(F32Cfg<D, HG, RT>::MAX_THREADS, 1)
         if (tid == 0 && blockIdx.x == 0) raise_flag(CX_DEV_BAD_QLEN);
         return;
     }
-    if (!plan_ok_zero_empty<D>(p)) return;
+    if (!plan_ok_zero_empty<D, MOD>(p)) return;
     const int W = p.plan[0], chunk = p.plan[1], P_eff = p.plan[2];
     if ((int)blockIdx.x >= P_eff) return;
     const int u0 = blockIdx.x * chunk;
@@ -114,10 +114,10 @@ __global__ void __launch_bounds__(F32Cfg<D, HG, RT>::MAX_THREADS, 1)
     }
     __syncthreads();
 
-    SegCursor cur;
+    SegCursorT<MOD> cur;
     cur.init(u0, u1, p);
     if (warp == NCW) {
-        produce_units<C::NBOX, 32, C::BOX, C::TILES, C::STAGE>(
+        produce_units<C::NBOX, 32, C::BOX, C::TILES, C::STAGE, MOD>(
             &tmk, &tmv, p, cur, HG, ring, full_bar, empty_bar, s_abort, s_bad, lane);
         return;
     }
@@ -144,6 +144,8 @@ __global__ void __launch_bounds__(F32Cfg<D, HG, RT>::MAX_THREADS, 1)
         const int64_t qs = p.q_start ? p.q_start[b] : b;
         const int rows_b = G * sq;
         const int pos0 = ctx - sq;  // position of query row 0
+        const int pre = MOD ? prefix_of(p, b, ctx) : 0;
+        const DeadTok dead{ctx, MOD && p.window > 0 ? pos0 - p.window + 1 : 0, pre};
 
         // stage the group's query rows (fp32, zero padding rows): tile
         // (hh2, mt2) row r is packed row mt2 * RT + r of head seg.g * HG + hh2
@@ -152,10 +154,16 @@ __global__ void __launch_bounds__(F32Cfg<D, HG, RT>::MAX_THREADS, 1)
             const int hh2 = tile % HG, R = (tile / HG) * RT + r;
             float v = 0.f;
             if (R < rows_b) {
-                const int64_t qi =
+                int64_t qi =
                     ((qs + R / G) * Hq + (int64_t)(seg.g * HG + hh2) * G + R % G) * D + d;
-                v = p.q_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.q)[qi])
-                             : static_cast<const float*>(p.q)[qi];
+                if constexpr (MOD)
+                    qi = (qs + R / G) * p.mod.q_stride +
+                         ((int64_t)(seg.g * HG + hh2) * G + R % G) * D + d;
+                if (MOD && p.mod.q_dtype == CX_F16)
+                    v = __half2float(static_cast<const __half*>(p.q)[qi]);
+                else
+                    v = p.q_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.q)[qi])
+                                 : static_cast<const float*>(p.q)[qi];
             }
             s_q[(size_t)tile * RT * C::QROW + r * C::QROW + d] = v;
         }
@@ -166,6 +174,16 @@ __global__ void __launch_bounds__(F32Cfg<D, HG, RT>::MAX_THREADS, 1)
         for (int i = 0; i < RPL; ++i) {
             const int R = mt * RT + rh + 2 * i;
             rpos[i] = R < rows_b ? pos0 + R / G : -1;
+        }
+        float slope[RPL];   // MOD: this lane's rows' slopes (base 2)
+        if constexpr (MOD) {
+#pragma unroll
+            for (int i = 0; i < RPL; ++i) {
+                const int R = mt * RT + rh + 2 * i;
+                slope[i] = p.mod.slopes ? p.mod.slopes[(int64_t)(seg.g * HG + hh) * G + R % G] *
+                                              1.4426950408889634f
+                                        : 0.f;
+            }
         }
         float o[RT][DPL];
         float m[RT];
@@ -210,16 +228,24 @@ __global__ void __launch_bounds__(F32Cfg<D, HG, RT>::MAX_THREADS, 1)
                         acc = fmaf(qv.w, kv.w, acc);
                     }
                 }
-                const int t0 = (seg.j0 + k) * kBlockTok;
-                const bool edge =
+                const int t0 = seg_block<MOD>(seg, k) * kBlockTok;
+                bool edge =
                     (t0 + kBlockTok - 1 > pos0) || (p.window > 0 && t0 <= ctx - 1 - p.window);
+                if constexpr (MOD) edge = edge && t0 + kBlockTok > pre;
                 float x[RPL], mx[RPL];
 #pragma unroll
                 for (int i = 0; i < RPL; ++i) {
                     x[i] = (sa[i] + sb[i]) * p.scale_log2;
+                    if constexpr (MOD) {
+                        if (p.mod.cap_log2 != 0.f)
+                            x[i] = p.mod.cap_log2 * tanhf((sa[i] + sb[i]) * p.mod.scale);
+                        if (p.mod.slopes)
+                            x[i] = fmaf(-slope[i], (float)abs(rpos[i] - (t0 + t)), x[i]);
+                    }
                     if (edge) {
                         const int tok = t0 + t;
-                        if (!(tok <= rpos[i] && (p.window <= 0 || tok > rpos[i] - p.window)))
+                        if (!((MOD && tok < pre) ||
+                              (tok <= rpos[i] && (p.window <= 0 || tok > rpos[i] - p.window))))
                             x[i] = -INFINITY;
                     }
                     float v = x[i];
@@ -264,6 +290,21 @@ __global__ void __launch_bounds__(F32Cfg<D, HG, RT>::MAX_THREADS, 1)
                 __syncwarp();
                 // ---- O += P V over the 16 keys of the unit ----
                 const unsigned char* vb = kb + C::TILES;
+                if constexpr (MOD) {
+                    if (dead.any(t0)) {
+                        unsigned char* vs = ring + (size_t)st * C::STAGE + C::TILES +
+                                            hh * (kBlockTok * 128);
+                        for (int u = 0; u < kBlockTok; ++u) {
+                            if (!dead(t0 + u)) continue;
+#pragma unroll
+                            for (int c = 0; c < C::NBOX; ++c)
+                                reinterpret_cast<uint32_t*>(vs + c * C::BOX + u * 128)[lane] = 0u;
+                        }
+                        __syncwarp();
+                        // before the producer's next copy into this stage
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    }
+                }
 #pragma unroll
                 for (int t4 = 0; t4 < kBlockTok; t4 += 4) {
                     float4 pr[RT];
@@ -328,8 +369,8 @@ __global__ void __launch_bounds__(F32Cfg<D, HG, RT>::MAX_THREADS, 1)
         }
         const int bg = b * p.n_groups + seg.g;
         float* slot = p.partials + (size_t)(blockIdx.x + bg) * slot_floats;
-        ks_merge<D, HG>(p, merge, slot, seg, qs, rows_b, ctid, NCT, KS);
-        if (!seg.whole) ticket_merge<D, HG>(p, seg, b, qs, rows_b, ctid, NCT, chunk, s_last);
+        ks_merge<D, HG, MOD>(p, merge, slot, seg, qs, rows_b, ctid, NCT, KS);
+        if (!seg.whole) ticket_merge<D, HG, MOD>(p, seg, b, qs, rows_b, ctid, NCT, chunk, s_last);
         named_bar_sync(1, NCT);
     }
 }

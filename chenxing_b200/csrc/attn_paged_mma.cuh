@@ -31,6 +31,10 @@
 // per-lane shared-memory slots (MmaCfg::QSM) instead of registers.  Key slices
 // (KS > 1) are merged through shared memory at the end of a range.  Every
 // wait is bounded and reports CX_DEV_WAIT_TIMEOUT instead of hanging.
+//
+// The MOD instantiations (cx_paged_attend) run the same units with the scores
+// capped and biased, a prefix of keys that every row sees, the pool's element
+// type E (bf16 or fp16), strided queries and an output of any type.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -45,14 +49,31 @@ namespace cx {
 constexpr int kBlockTok = 16;
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s per wait
 
+#ifdef CX_API_TU
 // Limit of the decode / verify pipeline waits (default kWaitLimitNs).  A test
 // shortens it (cx_set_wait_limit_ns) to make the waits run out on purpose and
 // check that the kernel returns with CX_DEV_WAIT_TIMEOUT raised.
 static std::atomic<unsigned long long> g_wait_limit_ns{kWaitLimitNs};
+unsigned long long wait_limit_ns() { return g_wait_limit_ns.load(std::memory_order_relaxed); }
+#endif
 constexpr int kPlanMagic = 0x43584b56;                       // "CXKV"
 constexpr int kMinUnitsPerCta = 4;
 constexpr int kConsumerWarps = 8;
 constexpr size_t kSmemBudget = 227 * 1024;
+
+// What the MOD instantiations of the decode / verify kernels need beside
+// MmaParams.  tanh(z) is taken as 1 - 2 / (1 + 2^(2 z log2 e)): two
+// special-function instructions, absolute error about 2^-22 (the score's error
+// is that times the cap).  The fp32 kernel calls tanhf.
+struct ScoreMod {
+    float scale;             // 16-bit pools: 2 log2(e) scale / cap; fp32 pool: scale / cap
+    float cap_log2;          // cap * log2(e); 0: no cap
+    const float* slopes;     // [hq] or NULL
+    const int32_t* prefix;   // [batch] or NULL
+    int64_t q_stride;        // elements between query tokens
+    void* out;
+    int32_t out_dtype, q_dtype;
+};
 
 struct MmaParams {
     const int32_t* tables;
@@ -74,7 +95,34 @@ struct MmaParams {
     int32_t* blk_lo;     // [batch] first block attended (sliding window)
     int32_t* counters;   // [batch * n_groups] merge tickets, zero between calls
     float* partials;     // [(P + batch*n_groups)][hg][rows][D + 2]
+    ScoreMod mod;        // MOD instantiations (and the plan: prefix blocks)
 };
+
+// Keys of sequence b that every query row sees (MOD with a prefix), at most ctx.
+__device__ __forceinline__ int prefix_of(const MmaParams& p, int b, int ctx) {
+    return p.mod.prefix ? min(max(p.mod.prefix[b], 0), ctx) : 0;
+}
+
+// Blocks of the prefix that end before the window's first block `lo`: they are
+// units of their own, the blocks between them and `lo` are skipped.
+__device__ __forceinline__ int prefix_blocks(int pre, int lo) {
+    return min((pre + kBlockTok - 1) / kBlockTok, lo);
+}
+
+template <bool MOD>
+__device__ __forceinline__ void put1(const MmaParams& p, int64_t i, float x) {
+    if constexpr (MOD)
+        store_as(p.mod.out, p.mod.out_dtype, i, x);
+    else
+        p.out[i] = x;
+}
+template <bool MOD>
+__device__ __forceinline__ void put2(const MmaParams& p, int64_t i, float x, float y) {
+    if constexpr (MOD)
+        store2_as(p.mod.out, p.mod.out_dtype, i, x, y);
+    else
+        *reinterpret_cast<float2*>(p.out + i) = make_float2(x, y);
+}
 
 // ---------------------------------------------------------------------------
 // plan: unit prefix sums and the chunking (one CTA of 1024 threads)
@@ -89,10 +137,11 @@ __device__ __forceinline__ int plan_units(const MmaParams& p, int b, int* lo_out
     const int lo = lo_tok / kBlockTok;
     const int hi = (ctx + kBlockTok - 1) / kBlockTok;
     *lo_out = lo;
-    return (ctx > 0 && hi > lo) ? (hi - lo) : 0;
+    const int npre = prefix_blocks(prefix_of(p, b, ctx), lo);
+    return (ctx > 0 && hi > lo) ? (hi - lo) + npre : 0;
 }
 
-__global__ void __launch_bounds__(1024) paged_plan_kernel(MmaParams p, int grid) {
+static __global__ void __launch_bounds__(1024) paged_plan_kernel(MmaParams p, int grid) {
     __shared__ long long s_warp[32];
     __shared__ long long s_total;
     const int t = threadIdx.x, B = p.batch;
@@ -165,13 +214,23 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(MmaParams p, int grid)
 struct Seg {
     int b, g, j0, cnt, nb;
     bool whole;
+    int pre_end, gap;   // MOD: the range's first pre_end units are prefix blocks, `gap` blocks
+                        // further left
 };
 
+// Block of the sequence that unit k of a range reads.
+template <bool MOD>
+__device__ __forceinline__ int seg_block(const Seg& s, int k) {
+    return MOD && k < s.pre_end ? s.j0 + k - s.gap : s.j0 + k;
+}
+
 // Walks the (sequence, head group) ranges covered by the CTA's unit interval.
-struct SegCursor {
+template <bool MOD>
+struct SegCursorT {
     int u, u_end, b, batch, ng;
     const int32_t* seq_start;
     const int32_t* blk_lo;
+    const MmaParams* par;
     __device__ void init(int u0, int u1, const MmaParams& p) {
         u = u0;
         u_end = u1;
@@ -179,6 +238,7 @@ struct SegCursor {
         ng = p.n_groups;
         seq_start = p.seq_start;
         blk_lo = p.blk_lo;
+        par = &p;
         int lo = 0, hi = batch;  // largest b with seq_start[b] <= u0
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
@@ -199,10 +259,19 @@ struct SegCursor {
         s.j0 = blk_lo[b] + jo;
         s.nb = nb;
         s.whole = (jo == 0 && s.cnt == nb);
+        if constexpr (MOD) {
+            const int cap = (int)(par->table_stride * kBlockTok);
+            const int ctx = min(max(par->ctx_lens[b], 0), cap);
+            const int npre = prefix_blocks(prefix_of(*par, b, ctx), blk_lo[b]);
+            s.pre_end = npre - jo;
+            s.gap = blk_lo[b] - npre;
+            s.j0 -= npre;
+        }
         u += s.cnt;
         return true;
     }
 };
+using SegCursor = SegCursorT<false>;
 
 // ---------------------------------------------------------------------------
 // TMA producer (the last warp of a decode / verify CTA), shared by the bf16
@@ -216,9 +285,9 @@ struct SegCursor {
 // stage is re-armed, and before returning the producer waits for its own
 // copies still in flight.
 // ---------------------------------------------------------------------------
-template <int NBOX, int BOX_COLS, int BOX_BYTES, int TILES, int STAGE>
+template <int NBOX, int BOX_COLS, int BOX_BYTES, int TILES, int STAGE, bool MOD = false>
 __device__ __forceinline__ void produce_units(const CUtensorMap* tmk, const CUtensorMap* tmv,
-                                              const MmaParams& p, SegCursor cur, int HG,
+                                              const MmaParams& p, SegCursorT<MOD> cur, int HG,
                                               unsigned char* ring, uint64_t* full_bar,
                                               uint64_t* empty_bar, volatile int* s_abort,
                                               volatile unsigned char* s_bad, int lane) {
@@ -233,7 +302,7 @@ __device__ __forceinline__ void produce_units(const CUtensorMap* tmk, const CUte
             const int n = min(32, seg.cnt - k0);
             int bid = -1;
             if (lane < n) {
-                const int jj = seg.j0 + k0 + lane;
+                const int jj = seg_block<MOD>(seg, k0 + lane);
                 bid = jj < p.table_stride ? bt[jj] : -1;
                 if (bid < 0 || bid >= p.n_blocks) {
                     raise_flag(CX_DEV_BAD_BLOCK);
@@ -300,7 +369,7 @@ __device__ __forceinline__ void produce_units(const CUtensorMap* tmk, const CUte
 // Merge the KS key slices of the CTA from shared memory (`merge`,
 // [KS][HG][p.rows][D + 2], filled by every consumer warp) into the final rows
 // (a range wholly inside this CTA) or into the CTA's workspace slot.
-template <int D, int HG>
+template <int D, int HG, bool MOD = false>
 __device__ __forceinline__ void ks_merge(const MmaParams& p, const float* merge, float* slot,
                                          const Seg& seg, int64_t qs, int rows_b, int ctid,
                                          int NCT, int KS) {
@@ -326,7 +395,7 @@ __device__ __forceinline__ void ks_merge(const MmaParams& p, const float* merge,
         }
         if (seg.whole) {
             const int64_t orow = (qs + R / G) * Hq + (int64_t)(seg.g * HG + eh) * G + R % G;
-            p.out[orow * D + d] = L > 0.f ? O / L : 0.f;
+            put1<MOD>(p, orow * D + d, L > 0.f ? O / L : 0.f);
         } else {
             float* r = slot + ((size_t)eh * p.rows + R) * (D + 2);
             r[d] = O;
@@ -341,7 +410,7 @@ __device__ __forceinline__ void ks_merge(const MmaParams& p, const float* merge,
 // A range cut by a chunk boundary: every CTA holding part of it takes an
 // atomic ticket after writing its slot; the last one merges all partials of
 // the range in one pass (log-sum-exp) and writes the final rows.  No waiting.
-template <int D, int HG>
+template <int D, int HG, bool MOD = false>
 __device__ __forceinline__ void ticket_merge(const MmaParams& p, const Seg& seg, int b,
                                              int64_t qs, int rows_b, int ctid, int NCT,
                                              int chunk, int* s_last) {
@@ -387,8 +456,7 @@ __device__ __forceinline__ void ticket_merge(const MmaParams& p, const Seg& seg,
         }
         const int64_t orow = (qs + R / G) * Hq + (int64_t)(seg.g * HG + eh) * G + R % G;
         const float inv = L > 0.f ? 1.f / L : 0.f;
-        *reinterpret_cast<float2*>(p.out + orow * D + d) =
-            L > 0.f ? make_float2(Ox * inv, Oy * inv) : make_float2(0.f, 0.f);
+        put2<MOD>(p, orow * D + d, L > 0.f ? Ox * inv : 0.f, L > 0.f ? Oy * inv : 0.f);
     }
     if (ctid == 0) p.counters[bg] = 0;
 }
@@ -396,7 +464,7 @@ __device__ __forceinline__ void ticket_merge(const MmaParams& p, const Seg& seg,
 // The plan must come from paged_plan_kernel for this batch shape (else the
 // flag is raised and the CTA returns false); sequences with no cached token
 // get zero rows (naive_attention semantics for rows with no key).
-template <int D>
+template <int D, bool MOD = false>
 __device__ __forceinline__ bool plan_ok_zero_empty(const MmaParams& p) {
     const int B = p.batch, Hq = p.hq, tid = threadIdx.x;
     if (p.plan[3] != kPlanMagic || p.plan[4] != B || p.plan[5] != p.n_groups) {
@@ -408,7 +476,7 @@ __device__ __forceinline__ bool plan_ok_zero_empty(const MmaParams& p) {
         const int sq = p.q_start ? p.q_start[b + 1] - p.q_start[b] : 1;
         const int64_t r0 = p.q_start ? p.q_start[b] : b;
         for (int64_t e = tid; e < (int64_t)sq * Hq * D; e += blockDim.x)
-            p.out[r0 * Hq * D + e] = 0.f;
+            put1<MOD>(p, r0 * Hq * D + e, 0.f);
     }
     return true;
 }
@@ -424,6 +492,11 @@ template <> struct QLoad<__nv_bfloat16> {
         return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(q + i));
     }
 };
+template <> struct QLoad<__half> {
+    __device__ __forceinline__ static float2 two(const __half* q, int64_t i) {
+        return __half22float2(*reinterpret_cast<const __half2*>(q + i));
+    }
+};
 
 // Rescale O only when a row max grows by more than 2^8 (see the consumer loop).
 constexpr float kMmaRescaleLog2 = 8.f;
@@ -435,6 +508,28 @@ __device__ __forceinline__ float ex2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+// 1 / x as one special-function-unit instruction (rcp.approx.ftz: 1 ulp;
+// 1 / inf = 0).
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// MOD: tokens of the 16 from t0 that no query row of the sequence sees — past
+// the context, or left of every row's window and past the prefix.  Their V rows
+// may hold anything, and 0 * NaN is NaN, so the warp that reads them writes
+// zeros over them first (every warp of a head writes the same zeros).
+struct DeadTok {
+    int ctx, lo, pre;   // lo: first key of the first row's window
+    __device__ __forceinline__ bool operator()(int tok) const {
+        return tok >= ctx || (tok < lo && tok >= pre);
+    }
+    __device__ __forceinline__ bool any(int t0) const {
+        return t0 + kBlockTok > ctx || (t0 < lo && t0 + kBlockTok > pre);
+    }
+};
 
 template <int D, int MT, int HG>
 struct MmaCfg {
@@ -483,7 +578,7 @@ struct MmaCfg {
     }
 };
 
-template <int D, int MT, int HG, typename QT>
+template <int D, int MT, int HG, typename QT, typename E = __nv_bfloat16, bool MOD = false>
 __global__ void __launch_bounds__(MmaCfg<D, MT, HG>::THREADS, 1)
     paged_attn_mma_kernel(const __grid_constant__ CUtensorMap tmk,
                           const __grid_constant__ CUtensorMap tmv, const MmaParams p) {
@@ -513,7 +608,7 @@ __global__ void __launch_bounds__(MmaCfg<D, MT, HG>::THREADS, 1)
         return;
     }
 
-    if (!plan_ok_zero_empty<D>(p)) return;
+    if (!plan_ok_zero_empty<D, MOD>(p)) return;
     const int W = p.plan[0], chunk = p.plan[1], P_eff = p.plan[2];
     if ((int)blockIdx.x >= P_eff) return;
     const int u0 = blockIdx.x * chunk;
@@ -531,12 +626,12 @@ __global__ void __launch_bounds__(MmaCfg<D, MT, HG>::THREADS, 1)
     }
     __syncthreads();
 
-    SegCursor cur;
+    SegCursorT<MOD> cur;
     cur.init(u0, u1, p);
     Seg seg;
 
     if (warp == C::NCW) {
-        produce_units<D / 64, 64, HG * C::HALF_BOX, C::TILES, C::STAGE>(
+        produce_units<D / 64, 64, HG * C::HALF_BOX, C::TILES, C::STAGE, MOD>(
             &tmk, &tmv, p, cur, HG, ring, full_bar, empty_bar, s_abort, s_bad, lane);
         return;
     }
@@ -567,13 +662,13 @@ __global__ void __launch_bounds__(MmaCfg<D, MT, HG>::THREADS, 1)
     // slower, and two instantiations made it spill.
     bool any_bad = true;
     if constexpr (MT > 1) {
-        SegCursor c2 = cur;
+        SegCursorT<MOD> c2 = cur;
         Seg s2;
         bool bad = false;
         while (c2.next(s2)) {
             const int32_t* bt = p.tables + (int64_t)s2.b * p.table_stride;
             for (int k = warp * 32 + lane; k < s2.cnt; k += C::NCW * 32) {
-                const int jj = s2.j0 + k;
+                const int jj = seg_block<MOD>(s2, k);
                 const int bid = jj < p.table_stride ? bt[jj] : -1;
                 bad |= bid < 0 || bid >= p.n_blocks;
             }
@@ -595,6 +690,30 @@ __global__ void __launch_bounds__(MmaCfg<D, MT, HG>::THREADS, 1)
         const int pos0 = ctx - sq;  // position of query row 0
         const int rpos0 = R0 < rows_b ? pos0 + R0 / G : -1;
         const int rpos1 = R1 < rows_b ? pos0 + R1 / G : -1;
+        // MOD: the prefix, the tokens no row sees, this lane's rows' slopes (base 2)
+        const int pre = MOD ? prefix_of(p, b, ctx) : 0;
+        const DeadTok dead{ctx, MOD && p.window > 0 ? pos0 - p.window + 1 : 0, pre};
+        float slope0 = 0.f, slope1 = 0.f;
+        if constexpr (MOD) {
+            if (p.mod.slopes) {
+                slope0 = p.mod.slopes[(int64_t)h * G + R0 % G] * 1.4426950408889634f;
+                slope1 = p.mod.slopes[(int64_t)h * G + R1 % G] * 1.4426950408889634f;
+            }
+        }
+        // element offset of packed row R's queries
+        auto q_row = [&](int R) {
+            if constexpr (MOD)
+                return (qs + R / G) * p.mod.q_stride + ((int64_t)h * G + R % G) * D;
+            else
+                return ((qs + R / G) * Hq + (int64_t)h * G + R % G) * D;
+        };
+        auto q_two = [&](int64_t i) {
+            if constexpr (MOD) {
+                if (p.mod.q_dtype == CX_F32)
+                    return QLoad<float>::two(static_cast<const float*>(p.q), i);
+            }
+            return QLoad<QT>::two(qbase, i);
+        };
 
         // Q fragments (bf16, A operand of m16n8k16), zero for padding rows
         uint32_t qa[C::KSTEP][4];
@@ -603,19 +722,19 @@ __global__ void __launch_bounds__(MmaCfg<D, MT, HG>::THREADS, 1)
             float2 a = make_float2(0.f, 0.f), bq = a, c = a, d = a;
             const int col = kk * 16 + qc;
             if (R0 < rows_b) {
-                const int64_t row = ((qs + R0 / G) * Hq + (int64_t)h * G + R0 % G) * D;
-                a = QLoad<QT>::two(qbase, row + col);
-                c = QLoad<QT>::two(qbase, row + col + 8);
+                const int64_t row = q_row(R0);
+                a = q_two(row + col);
+                c = q_two(row + col + 8);
             }
             if (R1 < rows_b) {
-                const int64_t row = ((qs + R1 / G) * Hq + (int64_t)h * G + R1 % G) * D;
-                bq = QLoad<QT>::two(qbase, row + col);
-                d = QLoad<QT>::two(qbase, row + col + 8);
+                const int64_t row = q_row(R1);
+                bq = q_two(row + col);
+                d = q_two(row + col + 8);
             }
-            qa[kk][0] = pack_bf16(a.x, a.y);
-            qa[kk][1] = pack_bf16(bq.x, bq.y);
-            qa[kk][2] = pack_bf16(c.x, c.y);
-            qa[kk][3] = pack_bf16(d.x, d.y);
+            qa[kk][0] = Half16<E>::pack(a.x, a.y);
+            qa[kk][1] = Half16<E>::pack(bq.x, bq.y);
+            qa[kk][2] = Half16<E>::pack(c.x, c.y);
+            qa[kk][3] = Half16<E>::pack(d.x, d.y);
         }
         if constexpr (C::QSM) {
             // each lane writes and later reads only its own slots
@@ -689,11 +808,11 @@ __global__ void __launch_bounds__(MmaCfg<D, MT, HG>::THREADS, 1)
                             qk[3] = qa[kk][3];
                         }
                         if (kk & 1) {
-                            mma_bf16_16816(sb[0], qk, f[0], f[1]);
-                            mma_bf16_16816(sb[1], qk, f[2], f[3]);
+                            Half16<E>::mma(sb[0], qk, f[0], f[1]);
+                            Half16<E>::mma(sb[1], qk, f[2], f[3]);
                         } else {
-                            mma_bf16_16816(sa[0], qk, f[0], f[1]);
-                            mma_bf16_16816(sa[1], qk, f[2], f[3]);
+                            Half16<E>::mma(sa[0], qk, f[0], f[1]);
+                            Half16<E>::mma(sa[1], qk, f[2], f[3]);
                         }
                     }
 #pragma unroll
@@ -701,9 +820,36 @@ __global__ void __launch_bounds__(MmaCfg<D, MT, HG>::THREADS, 1)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             x[u][n][e] = (sa[n][e] + sb[n][e]) * p.scale_log2;
-                    const int t0 = (seg.j0 + k + u * KS) * kBlockTok;
-                    const bool edge = (t0 + kBlockTok - 1 > pos0) ||
-                                      (p.window > 0 && t0 <= ctx - 1 - p.window);
+                    const int t0 = seg_block<MOD>(seg, k + u * KS) * kBlockTok;
+                    bool edge = (t0 + kBlockTok - 1 > pos0) ||
+                                (p.window > 0 && t0 <= ctx - 1 - p.window);
+                    if constexpr (MOD) {
+                        edge = edge && t0 + kBlockTok > pre;
+                        if (p.mod.cap_log2 != 0.f) {
+#pragma unroll
+                            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    x[u][n][e] = fmaf(
+                                        -2.f * p.mod.cap_log2,
+                                        rcp_approx(1.f + ex2_approx((sa[n][e] + sb[n][e]) *
+                                                                    p.mod.scale)),
+                                        p.mod.cap_log2);
+                        }
+                        if (p.mod.slopes) {
+#pragma unroll
+                            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    // the distance is exact in fp32, so near keys, whose
+                                    // weights count, lose nothing in long contexts
+                                    const int tok = t0 + n * 8 + qc + (e & 1);
+                                    const int dist = abs((e < 2 ? rpos0 : rpos1) - tok);
+                                    x[u][n][e] = fmaf(-(e < 2 ? slope0 : slope1), (float)dist,
+                                                      x[u][n][e]);
+                                }
+                        }
+                    }
                     if (edge) {
 #pragma unroll
                         for (int n = 0; n < 2; ++n)
@@ -712,7 +858,8 @@ __global__ void __launch_bounds__(MmaCfg<D, MT, HG>::THREADS, 1)
                                 const int tok = t0 + n * 8 + qc + (e & 1);
                                 const int rp = (e < 2) ? rpos0 : rpos1;
                                 const bool ok_t =
-                                    tok <= rp && (p.window <= 0 || tok > rp - p.window);
+                                    (MOD && tok < pre) ||
+                                    (tok <= rp && (p.window <= 0 || tok > rp - p.window));
                                 if (!ok_t) x[u][n][e] = -INFINITY;
                             }
                     }
@@ -772,17 +919,34 @@ __global__ void __launch_bounds__(MmaCfg<D, MT, HG>::THREADS, 1)
                 for (int u = 0; u < U; ++u) {
                     if ((u > 0 && !two) || bad[u]) continue;
                     const uint32_t vb = smem_addr(ring + (size_t)su[u] * C::STAGE) + C::TILES;
+                    if constexpr (MOD) {
+                        const int t0 = seg_block<MOD>(seg, k + u * KS) * kBlockTok;
+                        if (dead.any(t0)) {
+                            unsigned char* vs = ring + (size_t)su[u] * C::STAGE + C::TILES +
+                                                hh * C::HALF_BOX;
+                            for (int t = 0; t < kBlockTok; ++t) {
+                                if (!dead(t0 + t)) continue;
+#pragma unroll
+                                for (int c = 0; c < D / 64; ++c)
+                                    reinterpret_cast<uint32_t*>(vs + c * (HG * C::HALF_BOX) +
+                                                                t * 128)[lane] = 0u;
+                            }
+                            __syncwarp();
+                            // before the producer's next copy into this stage
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        }
+                    }
                     uint32_t pa[4];
-                    pa[0] = pack_bf16(pr[u][0][0], pr[u][0][1]);
-                    pa[1] = pack_bf16(pr[u][0][2], pr[u][0][3]);
-                    pa[2] = pack_bf16(pr[u][1][0], pr[u][1][1]);
-                    pa[3] = pack_bf16(pr[u][1][2], pr[u][1][3]);
+                    pa[0] = Half16<E>::pack(pr[u][0][0], pr[u][0][1]);
+                    pa[1] = Half16<E>::pack(pr[u][0][2], pr[u][0][3]);
+                    pa[2] = Half16<E>::pack(pr[u][1][0], pr[u][1][1]);
+                    pa[3] = Half16<E>::pack(pr[u][1][2], pr[u][1][3]);
 #pragma unroll
                     for (int np = 0; np < C::KSTEP; ++np) {
                         uint32_t f[4];
                         ldmatrix_x4_trans(f, vb + C::swz(hh, v_tok, np * 16 + v_dsub));
-                        mma_bf16_16816(o[2 * np], pa, f[0], f[1]);
-                        mma_bf16_16816(o[2 * np + 1], pa, f[2], f[3]);
+                        Half16<E>::mma(o[2 * np], pa, f[0], f[1]);
+                        Half16<E>::mma(o[2 * np + 1], pa, f[2], f[3]);
                     }
                 }
             }
@@ -820,12 +984,10 @@ __global__ void __launch_bounds__(MmaCfg<D, MT, HG>::THREADS, 1)
                 if (seg.whole) {
                     const float inv = ll > 0.f ? 1.f / ll : 0.f;
                     const int64_t orow = (qs + R / G) * Hq + (int64_t)h * G + R % G;
-                    float* dst = p.out + orow * D;
 #pragma unroll
-                    for (int n = 0; n < C::NT; ++n) {
-                        *reinterpret_cast<float2*>(dst + n * 8 + qc) =
-                            make_float2(o[n][2 * half] * inv, o[n][2 * half + 1] * inv);
-                    }
+                    for (int n = 0; n < C::NT; ++n)
+                        put2<MOD>(p, orow * D + n * 8 + qc, o[n][2 * half] * inv,
+                                  o[n][2 * half + 1] * inv);
                 } else {
                     float* r = slot + ((size_t)hh * p.rows + R) * (D + 2);
 #pragma unroll
@@ -858,10 +1020,10 @@ __global__ void __launch_bounds__(MmaCfg<D, MT, HG>::THREADS, 1)
                     }
                 }
             }
-            ks_merge<D, HG>(p, merge, slot, seg, qs, rows_b, ctid, NCT, KS);
+            ks_merge<D, HG, MOD>(p, merge, slot, seg, qs, rows_b, ctid, NCT, KS);
         }
         if (!seg.whole)
-            ticket_merge<D, HG>(p, seg, b, qs, rows_b, ctid, NCT, chunk, s_last);
+            ticket_merge<D, HG, MOD>(p, seg, b, qs, rows_b, ctid, NCT, chunk, s_last);
         named_bar_sync(1, NCT);
     }
 }
@@ -870,8 +1032,10 @@ __global__ void __launch_bounds__(MmaCfg<D, MT, HG>::THREADS, 1)
 
 #include "attn_paged_f32.cuh"
 #include "attn_prefill_tc.cuh"
+#ifdef CX_API_TU
 #include "attn_prefill_tc128.cuh"
 #include "attn_prefill_tc256.cuh"
+#endif
 
 namespace cx {
 
@@ -892,13 +1056,16 @@ static PFN_cuTensorMapEncodeTiled_v12000 tmap_encoder() {
     return fn;
 }
 
-// 3-D view of a bf16 or fp32 pool: (head_dim, 16 slots, layers*blocks*heads
+// 3-D view of a bf16, fp16 or fp32 pool: (head_dim, 16 slots, layers*blocks*heads
 // tiles), box of one 128-byte column (64 bf16 or 32 fp32 values) x 16 x hg
 // (hg consecutive heads of one block) with 128-byte swizzle.
 static int make_pool_tmap(CUtensorMap* m, void* base, const cx_pool* p, int hg) {
     auto enc = tmap_encoder();
     if (!enc) return fail(CX_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
     const bool f32 = p->dtype == CX_F32;
+    const CUtensorMapDataType type = f32                  ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : p->dtype == CX_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                          : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     const cuuint64_t e = f32 ? 4 : 2;
     const cuuint64_t dims[3] = {(cuuint64_t)p->head_dim, (cuuint64_t)p->block_size,
                                 (cuuint64_t)(p->n_layers * p->n_blocks * p->n_kv_heads)};
@@ -906,8 +1073,7 @@ static int make_pool_tmap(CUtensorMap* m, void* base, const cx_pool* p, int hg) 
                                    (cuuint64_t)(p->block_size * p->head_dim * e)};
     const cuuint32_t box[3] = {(cuuint32_t)(128 / e), (cuuint32_t)p->block_size, (cuuint32_t)hg};
     const cuuint32_t estr[3] = {1, 1, 1};
-    CUresult r = enc(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                     3, base, dims, strides, box, estr,
+    CUresult r = enc(m, type, 3, base, dims, strides, box, estr,
                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(CX_ERR_CUDA, "cuTensorMapEncodeTiled failed");
@@ -980,11 +1146,11 @@ static WsLayout ws_layout(int64_t batch, const MmaShape& sh, int64_t rows, int64
     return w;
 }
 
-template <int D, int MT, int HG, typename QT>
+template <int D, int MT, int HG, typename QT, typename E, bool MOD>
 static int launch_mma_cfg(const CUtensorMap& tk, const CUtensorMap& tv, MmaParams p,
                           cudaStream_t st, int grid) {
     using C = MmaCfg<D, MT, HG>;
-    auto kern = paged_attn_mma_kernel<D, MT, HG, QT>;
+    auto kern = paged_attn_mma_kernel<D, MT, HG, QT, E, MOD>;
     p.stages = C::stages_for(p.rows);
     p.stage_bytes = C::STAGE;
     if (p.stages < 2 || p.stages % C::KS != 0 || (C::U == 2 && p.stages < 2 * C::KS))
@@ -995,12 +1161,16 @@ static int launch_mma_cfg(const CUtensorMap& tk, const CUtensorMap& tv, MmaParam
     return check_launch("paged_attn_mma_kernel");
 }
 
-template <int D, typename QT>
+template <int D, typename QT, typename E = __nv_bfloat16, bool MOD = false>
 static int launch_mma_d(const MmaShape& sh, const CUtensorMap& tk, const CUtensorMap& tv,
                         const MmaParams& p, cudaStream_t st, int grid) {
 #define CX_CASE(MT_, HG_) \
-    if (sh.mt == MT_ && sh.hg == HG_) return launch_mma_cfg<D, MT_, HG_, QT>(tk, tv, p, st, grid);
-    CX_CASE(1, 8) CX_CASE(1, 4) CX_CASE(1, 2) CX_CASE(1, 1)
+    if (sh.mt == MT_ && sh.hg == HG_)        \
+        return launch_mma_cfg<D, MT_, HG_, QT, E, MOD>(tk, tv, p, st, grid);
+    if constexpr (!MOD) {
+        CX_CASE(1, 8)
+    }
+    CX_CASE(1, 4) CX_CASE(1, 2) CX_CASE(1, 1)
     CX_CASE(2, 4) CX_CASE(2, 2) CX_CASE(2, 1)
     CX_CASE(3, 4) CX_CASE(3, 2) CX_CASE(3, 1)
     CX_CASE(4, 2) CX_CASE(4, 1)
@@ -1008,11 +1178,11 @@ static int launch_mma_d(const MmaShape& sh, const CUtensorMap& tk, const CUtenso
     return fail(CX_ERR_UNSUPPORTED, "paged attention: no kernel for this row/head shape");
 }
 
-template <int D, int HG, int RT>
+template <int D, int HG, int RT, bool MOD>
 static int launch_f32_cfg(const CUtensorMap& tk, const CUtensorMap& tv, MmaParams p,
                           cudaStream_t st, int grid) {
     using C = F32Cfg<D, HG, RT>;
-    auto kern = paged_attn_f32_kernel<D, HG, RT>;
+    auto kern = paged_attn_f32_kernel<D, HG, RT, MOD>;
     // key slices: the ring length must be a multiple of them (each stage is
     // always consumed by the same slice).  Take the most consumer warps whose
     // ring still holds at least 4 stages and 3/4 of the longest ring: one warp
@@ -1045,12 +1215,12 @@ static int launch_f32_cfg(const CUtensorMap& tk, const CUtensorMap& tv, MmaParam
     return check_launch("paged_attn_f32_kernel");
 }
 
-template <int D>
+template <int D, bool MOD = false>
 static int launch_f32_d(const MmaShape& sh, const CUtensorMap& tk, const CUtensorMap& tv,
                         const MmaParams& p, cudaStream_t st, int grid) {
     const int rt = f32_rt(p.rows);
 #define CX_CASE(HG_, RT_) \
-    if (sh.hg == HG_ && rt == RT_) return launch_f32_cfg<D, HG_, RT_>(tk, tv, p, st, grid);
+    if (sh.hg == HG_ && rt == RT_) return launch_f32_cfg<D, HG_, RT_, MOD>(tk, tv, p, st, grid);
     CX_CASE(1, 4) CX_CASE(1, 8) CX_CASE(1, 16)
     CX_CASE(2, 4) CX_CASE(2, 8) CX_CASE(2, 16)
     if constexpr (D == 64) {
@@ -1086,6 +1256,7 @@ static bool mma_eligible(const cx_pool* pool, const cx_attn_batch* b, int32_t q_
 
 static int grid_size() { return num_sms(); }
 
+#ifdef CX_API_TU
 // Scratch bytes a decode (verify = false) or verify call will use: the plan /
 // split-K workspace of the mma.sync and fp32 FMA kernels; none for the
 // tcgen05 and generic kernels.  Same kernel choice as paged_attention.
@@ -1230,7 +1401,7 @@ static int paged_attention(const cx_pool* pool, int64_t layer, const cx_attn_bat
     p.layer = (int)layer;
     p.window = b.window > 0 ? (int)b.window : 0;
     p.scale_log2 = scale * 1.4426950408889634f;
-    p.wait_ns = g_wait_limit_ns.load(std::memory_order_relaxed);
+    p.wait_ns = wait_limit_ns();
     p.q = q;
     p.out = out;
     p.plan = reinterpret_cast<int32_t*>(w + wl.plan);
@@ -1259,8 +1430,11 @@ static int paged_attention(const cx_pool* pool, int64_t layer, const cx_attn_bat
                              : launch_mma_d<64, __nv_bfloat16>(sh, tk, tv, p, st, grid);
 }
 
+#endif  // CX_API_TU
+
 }  // namespace cx
 
+#ifdef CX_API_TU
 extern "C" {
 
 size_t cx_paged_workspace_bytes(const cx_pool* pool, const cx_attn_batch* b) {
@@ -1303,3 +1477,4 @@ int cx_paged_verify(const cx_pool* pool, int64_t layer, const cx_attn_batch* bat
 }
 
 }  // extern "C"
+#endif  // CX_API_TU

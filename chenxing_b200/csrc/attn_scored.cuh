@@ -6,6 +6,108 @@
 
 namespace cx {
 
+// Whether the split-K kernels take this pool and batch shape: 16-token blocks,
+// heads of 64 or 128, up to 64 packed rows (query tokens x GQA group).
+static bool split_shape(const cx_pool* pool, const cx_attn_batch* b) {
+    const int64_t rows = b->n_q_heads / pool->n_kv_heads * b->max_q_len;
+    const int64_t tiles = pool->n_layers * pool->n_blocks * pool->n_kv_heads;
+    const uintptr_t a = reinterpret_cast<uintptr_t>(pool->k) | reinterpret_cast<uintptr_t>(pool->v);
+    return (a & 15) == 0 && pool->block_size == kBlockTok && tiles < (1ll << 31) &&
+           (pool->head_dim == 64 || pool->head_dim == 128) && b->batch < (1 << 24) &&
+           pool->n_kv_heads * b->batch < (1 << 24) && rows >= 1 && rows <= 64;
+}
+
+// The kernel of a call.  `vec`: q, its token stride and out are 16-byte aligned.
+// 16-bit pools take queries of their own type or fp32, fp32 pools any type.
+static int attend_kind(const cx_pool* pool, const cx_attn_batch* b, int32_t q_dtype, bool vec) {
+    if (!vec || !split_shape(pool, b)) return CX_KERNEL_GENERIC;
+    if (pool->dtype == CX_F32) return CX_KERNEL_FMA;
+    return q_dtype == CX_F32 || q_dtype == pool->dtype ? CX_KERNEL_MMA : CX_KERNEL_GENERIC;
+}
+
+static size_t attend_workspace(const cx_pool* pool, const cx_attn_batch* b) {
+    const int64_t rows = b->n_q_heads / pool->n_kv_heads * b->max_q_len;
+    return ws_layout(b->batch, unit_shape(pool, rows), rows, pool->head_dim, grid_size()).total;
+}
+
+// The split-K kernels (attn_paged_mma.cuh, attn_paged_f32.cuh) with MOD.
+static int attend_split(const cx_pool* pool, int64_t layer, const cx_attn_batch& b,
+                        const cx_attn_mods& m, float scale, const void* q, int32_t q_dtype,
+                        void* out, void* ws, size_t ws_bytes, int32_t replan, bool plan_only,
+                        cudaStream_t st) {
+    const int64_t G = b.n_q_heads / pool->n_kv_heads, rows = G * b.max_q_len;
+    const MmaShape sh = unit_shape(pool, rows);
+    const int grid = grid_size();
+    const WsLayout wl = ws_layout(b.batch, sh, rows, pool->head_dim, grid);
+    if (!ws || ws_bytes < wl.total || (reinterpret_cast<uintptr_t>(ws) & 255) != 0)
+        return fail(CX_ERR_WORKSPACE,
+                    "cx_paged_attend: workspace missing, too small or not 256-byte aligned");
+    char* w = static_cast<char*>(ws);
+    MmaParams p{};
+    p.tables = b.block_tables;
+    p.table_stride = b.table_stride;
+    p.ctx_lens = b.ctx_lens;
+    p.q_start = b.q_start;
+    p.batch = (int)b.batch;
+    p.hk = (int)pool->n_kv_heads;
+    p.hq = (int)b.n_q_heads;
+    p.group = (int)G;
+    p.max_q = (int)b.max_q_len;
+    p.rows = (int)rows;
+    p.hg = sh.hg;
+    p.n_groups = sh.n_groups;
+    p.mt = sh.mt;
+    p.q_bf16 = q_dtype == CX_BF16;
+    p.n_blocks = (int)pool->n_blocks;
+    p.layer = (int)layer;
+    p.window = b.window > 0 ? (int)b.window : 0;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    p.wait_ns = wait_limit_ns();
+    p.q = q;
+    p.plan = reinterpret_cast<int32_t*>(w + wl.plan);
+    p.seq_start = reinterpret_cast<int32_t*>(w + wl.seq);
+    p.blk_lo = reinterpret_cast<int32_t*>(w + wl.lo);
+    p.counters = reinterpret_cast<int32_t*>(w + wl.cnt);
+    p.partials = reinterpret_cast<float*>(w + wl.part);
+    p.mod.slopes = m.alibi_slopes;
+    p.mod.prefix = m.prefix_lens;
+    p.mod.q_stride = m.q_stride;
+    p.mod.out = out;
+    p.mod.out_dtype = m.out_dtype;
+    p.mod.q_dtype = q_dtype;
+    if (m.softcap > 0.f) {
+        p.mod.cap_log2 = m.softcap * 1.4426950408889634f;
+        p.mod.scale = scale / m.softcap * (pool->dtype == CX_F32 ? 1.f : 2.8853900817779268f);
+    }
+    if (replan) {
+        paged_plan_kernel<<<1, 1024, 0, st>>>(p, grid);
+        const int rc = check_launch("paged_plan_kernel");
+        if (rc) return rc;
+    }
+    if (plan_only) return CX_OK;
+    CUtensorMap tk, tv;
+    int rc = make_pool_tmap(&tk, pool->k, pool, sh.hg);
+    if (rc) return rc;
+    rc = make_pool_tmap(&tv, pool->v, pool, sh.hg);
+    if (rc) return rc;
+    const bool d128 = pool->head_dim == 128;
+    switch (pool->dtype) {
+        case CX_F32:
+            return d128 ? launch_f32_d<128, true>(sh, tk, tv, p, st, grid)
+                        : launch_f32_d<64, true>(sh, tk, tv, p, st, grid);
+        case CX_BF16: {
+            using E = __nv_bfloat16;
+            return d128 ? launch_mma_d<128, E, E, true>(sh, tk, tv, p, st, grid)
+                        : launch_mma_d<64, E, E, true>(sh, tk, tv, p, st, grid);
+        }
+        default: {
+            using E = __half;
+            return d128 ? launch_mma_d<128, E, E, true>(sh, tk, tv, p, st, grid)
+                        : launch_mma_d<64, E, E, true>(sh, tk, tv, p, st, grid);
+        }
+    }
+}
+
 static int attend_scored(const cx_pool* pool, int64_t layer, const cx_attn_batch* bt,
                          const cx_attn_mods* mods, const void* q, int32_t q_dtype, void* out,
                          void* ws, size_t ws_bytes, int32_t replan, void* stream) {
@@ -33,30 +135,48 @@ static int attend_scored(const cx_pool* pool, int64_t layer, const cx_attn_batch
     const float scale = isnan(bt->scale) ? 1.0f / sqrtf((float)pool->head_dim) : bt->scale;
     cx_attn_mods m = *mods;
     if (m.q_stride == 0) m.q_stride = row;
+    cx_attn_batch b = *bt;
+    if (!b.q_start) b.max_q_len = 1;
+    if (b.window > (1ll << 30)) b.window = 1ll << 30;    // above any context
+    if (b.table_stride > (1ll << 26) || pool->n_blocks > INT32_MAX || b.max_q_len >= (1 << 24))
+        return fail(CX_ERR_UNSUPPORTED, "cx_paged_attend: pool, table or max_q_len too large");
+    const uintptr_t al = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) |
+                         static_cast<uintptr_t>(m.q_stride * elem_bytes(q_dtype));
+    cudaStream_t st = as_stream(stream);
+    const int kind = attend_kind(pool, &b, q_dtype, (al & 15) == 0);
+    if (kind == CX_KERNEL_MMA || kind == CX_KERNEL_FMA)
+        return attend_split(pool, layer, b, m, scale, q, q_dtype, out, ws, ws_bytes, replan,
+                            false, st);
+    // a later layer of the step may have queries that the split-K kernels take:
+    // the plan it then reads is made now
+    if (replan && split_shape(pool, &b) && ws) {
+        rc = attend_split(pool, layer, b, m, scale, q, q_dtype, out, ws, ws_bytes, 1, true, st);
+        if (rc) return rc;
+    }
 
     GenericParams g{};
     g.q = q;
     g.mod_out = out;
     g.mod = m;
-    g.batch = bt->batch;
-    g.hq = bt->n_q_heads;
+    g.batch = b.batch;
+    g.hq = b.n_q_heads;
     g.hk = pool->n_kv_heads;
     g.d = g.dv = pool->head_dim;
-    g.max_q = bt->q_start ? bt->max_q_len : 1;
+    g.max_q = b.max_q_len;
     g.scale = scale;
     g.mask_kind = 1;
-    g.window = bt->window;
+    g.window = b.window;
     g.kp = pool->k;
     g.vp = pool->v;
     g.n_layers = pool->n_layers;
     g.n_blocks = pool->n_blocks;
     g.block_size = pool->block_size;
     g.layer = layer;
-    g.tables = bt->block_tables;
-    g.table_stride = bt->table_stride;
-    g.ctx_lens = bt->ctx_lens;
-    g.q_start = bt->q_start;
-    return launch_generic<true, true>(q_dtype, pool->dtype, g, as_stream(stream));
+    g.tables = b.block_tables;
+    g.table_stride = b.table_stride;
+    g.ctx_lens = b.ctx_lens;
+    g.q_start = b.q_start;
+    return launch_generic<true, true>(q_dtype, pool->dtype, g, st);
 }
 
 }  // namespace cx
@@ -71,11 +191,18 @@ int cx_paged_attend(const cx_pool* pool, int64_t layer, const cx_attn_batch* bat
 }
 
 size_t cx_paged_attend_workspace_bytes(const cx_pool* pool, const cx_attn_batch* batch) {
-    return cx_paged_workspace_bytes(pool, batch);
+    if (!pool || !batch || pool->n_kv_heads <= 0 || batch->n_q_heads <= 0 || batch->batch < 0)
+        return 0;
+    cx_attn_batch b = *batch;
+    if (!b.q_start || b.max_q_len < 1) b.max_q_len = 1;
+    return cx::attend_workspace(pool, &b);
 }
 
-int cx_paged_attend_kind(const cx_pool*, const cx_attn_batch*, int32_t) {
-    return CX_KERNEL_GENERIC;
+int cx_paged_attend_kind(const cx_pool* pool, const cx_attn_batch* batch, int32_t q_dtype) {
+    if (!pool || !batch || pool->n_kv_heads <= 0) return CX_KERNEL_GENERIC;
+    cx_attn_batch b = *batch;
+    if (!b.q_start || b.max_q_len < 1) b.max_q_len = 1;
+    return cx::attend_kind(pool, &b, q_dtype, true);
 }
 
 }  // extern "C"

@@ -48,17 +48,11 @@ const char* cx_last_error(void) { return cx::t_last_error.c_str(); }
 int cx_device_error(void* stream, int clear, uint32_t* flags) {
     if (!flags) return cx::fail(CX_ERR_SHAPE, "cx_device_error: flags is NULL");
     cudaStream_t s = cx::as_stream(stream);
-    unsigned int v = 0;
-    CX_CUDA_CHECK(cudaMemcpyFromSymbolAsync(&v, cx::g_dev_flags, sizeof(v), 0,
-                                            cudaMemcpyDeviceToHost, s));
-    CX_CUDA_CHECK(cudaStreamSynchronize(s));
-    if (clear) {
-        unsigned int z = 0;
-        CX_CUDA_CHECK(cudaMemcpyToSymbolAsync(cx::g_dev_flags, &z, sizeof(z), 0,
-                                              cudaMemcpyHostToDevice, s));
-        CX_CUDA_CHECK(cudaStreamSynchronize(s));
-    }
-    *flags = v;
+    unsigned int v = 0, w = 0;
+    int rc = cx::read_dev_flags(s, clear, &v);
+    if (rc == CX_OK) rc = cx::read_dev_flags_scored(s, clear, &w);
+    if (rc != CX_OK) return rc;
+    *flags = v | w;
     return CX_OK;
 }
 

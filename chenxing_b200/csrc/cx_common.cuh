@@ -44,10 +44,40 @@ inline int elem_bytes(int32_t dt) {
 
 int num_sms();  // SM count of the current device (cached per device)
 
+// Limit of the decode / verify pipeline waits of later launches, ns
+// (cx_set_wait_limit_ns).
+unsigned long long wait_limit_ns();
+
+static inline int check_pool(const cx_pool* p) {
+    if (!p) return fail(CX_ERR_SHAPE, "pool is NULL");
+    if (!p->k || !p->v) return fail(CX_ERR_SHAPE, "pool buffers are NULL");
+    if (p->n_layers <= 0 || p->n_blocks <= 0 || p->block_size <= 0 || p->n_kv_heads <= 0 ||
+        p->head_dim <= 0)
+        return fail(CX_ERR_SHAPE, "pool sizes must be positive");
+    if (elem_bytes(p->dtype) == 0) return fail(CX_ERR_DTYPE, "unknown pool dtype");
+    return CX_OK;
+}
+
 // ---- device-side error flags ---------------------------------------------
-// The whole library is one translation unit (cxkv.cu), so this definition
-// is the only one.
-__device__ unsigned int g_dev_flags = 0;
+// One word per translation unit (cxkv.cu, cxkv_scored.cu: no relocatable
+// device code); cx_device_error reads and clears both.
+static __device__ unsigned int g_dev_flags = 0;
+
+// Reads this translation unit's word on `s` and clears it when asked.
+static int read_dev_flags(cudaStream_t s, int clear, unsigned int* v) {
+    CX_CUDA_CHECK(cudaMemcpyFromSymbolAsync(v, g_dev_flags, sizeof(*v), 0,
+                                            cudaMemcpyDeviceToHost, s));
+    CX_CUDA_CHECK(cudaStreamSynchronize(s));
+    if (clear) {
+        unsigned int z = 0;
+        CX_CUDA_CHECK(cudaMemcpyToSymbolAsync(g_dev_flags, &z, sizeof(z), 0,
+                                              cudaMemcpyHostToDevice, s));
+        CX_CUDA_CHECK(cudaStreamSynchronize(s));
+    }
+    return CX_OK;
+}
+
+int read_dev_flags_scored(cudaStream_t s, int clear, unsigned int* v);  // cxkv_scored.cu
 
 __device__ __forceinline__ void raise_flag(unsigned int bit) {
     atomicOr(&g_dev_flags, bit);
@@ -76,6 +106,17 @@ __device__ __forceinline__ void store_as(void* p, int32_t dtype, int64_t i, floa
         static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
     else
         static_cast<__half*>(p)[i] = __float2half_rn(x);
+}
+
+// Elements `i`, `i + 1` (i even, the array 8-byte aligned) of such an array.
+__device__ __forceinline__ void store2_as(void* p, int32_t dtype, int64_t i, float x, float y) {
+    if (dtype == CX_F32)
+        *reinterpret_cast<float2*>(static_cast<float*>(p) + i) = make_float2(x, y);
+    else if (dtype == CX_BF16)
+        *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(p) + i) =
+            __floats2bfloat162_rn(x, y);
+    else
+        *reinterpret_cast<__half2*>(static_cast<__half*>(p) + i) = __floats2half2_rn(x, y);
 }
 
 // ---- shared-memory / PTX helpers -----------------------------------------
@@ -184,10 +225,40 @@ __device__ __forceinline__ void mma_bf16_16816(float (&d)[4], const uint32_t (&a
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The same on fp16 operands.
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                              uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+        "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
 }
+
+// Two fp32 values as a 16-bit pair of type E, and the mma of that type.
+template <typename E> struct Half16;
+template <> struct Half16<__nv_bfloat16> {
+    __device__ __forceinline__ static uint32_t pack(float lo, float hi) { return pack_bf16(lo, hi); }
+    __device__ __forceinline__ static void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                               uint32_t b1) {
+        mma_bf16_16816(d, a, b0, b1);
+    }
+};
+template <> struct Half16<__half> {
+    __device__ __forceinline__ static uint32_t pack(float lo, float hi) {
+        const __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    __device__ __forceinline__ static void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                               uint32_t b1) {
+        mma_f16_16816(d, a, b0, b1);
+    }
+};
 
 __device__ __forceinline__ void named_bar_sync(int id, int threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");

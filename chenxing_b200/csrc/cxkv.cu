@@ -1,12 +1,11 @@
-// libcxkv.so — single translation unit of the C ABI declared in
-// include/cxkv.h (one TU so every kernel shares the device flag word without
-// relocatable device code).
+// libcxkv.so — main translation unit of the C ABI declared in include/cxkv.h
+// (cxkv_scored.cu has the attention with score modifiers).
+#define CX_API_TU 1
 #include "capi.cuh"
 #include "kv_ops.cuh"
 #include "kv_norm_rope.cuh"
 #include "attn_generic.cuh"
 #include "attn_paged_mma.cuh"
-#include "attn_scored.cuh"
 
 // ---------------------------------------------------------------------------
 // Paged decode that allocates nothing.

@@ -581,16 +581,6 @@ __global__ void __launch_bounds__(256) kv_gather_vec_kernel(
     }
 }
 
-static int check_pool(const cx_pool* p) {
-    if (!p) return fail(CX_ERR_SHAPE, "pool is NULL");
-    if (!p->k || !p->v) return fail(CX_ERR_SHAPE, "pool buffers are NULL");
-    if (p->n_layers <= 0 || p->n_blocks <= 0 || p->block_size <= 0 || p->n_kv_heads <= 0 ||
-        p->head_dim <= 0)
-        return fail(CX_ERR_SHAPE, "pool sizes must be positive");
-    if (elem_bytes(p->dtype) == 0) return fail(CX_ERR_DTYPE, "unknown pool dtype");
-    return CX_OK;
-}
-
 static int grid_for(int64_t work_items, int per_block) {
     int64_t b = (work_items + per_block - 1) / per_block;
     int64_t cap = (int64_t)num_sms() * 16;

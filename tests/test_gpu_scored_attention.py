@@ -144,6 +144,30 @@ def test_one_batch_through_both_entry_points():
         c.check(c.run(batch, out_dtype=dt))
 
 
+def test_plan_of_a_generic_call_serves_the_next_layer():
+    """The first layer's queries are off 16 bytes (generic kernel), the second's
+    are not: its split-K kernel finds the step's plan."""
+    c = _case("cap", 8, [100, 513, 40], hk=2, d=64, dtype=BF)
+    odd = torch.zeros(3 * 8 * 64 + 1, dtype=BF, device="cuda")[1:].view(3, 8, 64)
+    odd.copy_(c.q_dev)
+    batch = c.batch()
+    c.check(c.cache.decode_batch(0, odd, batch, out_dtype=BF))
+    assert not batch.needs_plan
+    c.check(c.run(batch, out_dtype=BF))
+
+
+KIND = {"decode": None, "chain": [3, 5], "chunk": [40, 70]}
+
+
+@pytest.mark.parametrize("shape,dtype,d,kind", [
+    ("decode", BF, 64, "mma"), ("decode", F16, 128, "mma"), ("chain", F16, 64, "mma"),
+    ("decode", F32, 64, "fma"), ("chain", F32, 128, "fma"), ("decode", BF, 96, "generic"),
+    ("chunk", F32, 64, "generic")])
+def test_kernel_choice(shape, dtype, d, kind):
+    c = _case("cap", 8, [70, 300], hk=2, d=d, dtype=dtype, q_lens=KIND[shape])
+    assert c.batch().kernel_kind(dtype) == kind
+
+
 def test_out_argument_and_untouched_rows():
     c = _case("cap", 8, [70, 300], hk=2, d=64, dtype=BF, q_lens=[3, 2])
     buf = torch.full((9, 8, 64), 7.0, dtype=BF, device="cuda")
