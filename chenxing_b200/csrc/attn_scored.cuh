@@ -1,32 +1,78 @@
-// Paged attention with score modifiers (cx_paged_attend): argument checks and
-// the choice of the kernel.
+// Paged attention with score modifiers (cx_paged_attend): argument checks, the
+// choice of the kernel and its launch.
 #pragma once
 
-#include "cx_common.cuh"  // unity build: included from cxkv.cu after the kernels
+#include <algorithm>
+
+#include "cx_common.cuh"  // unity build: included from cxkv_scored.cu after the kernels
+#include "attn_scored_tc.cuh"
 
 namespace cx {
 
-// Whether the split-K kernels take this pool and batch shape: 16-token blocks,
-// heads of 64 or 128, up to 64 packed rows (query tokens x GQA group).
-static bool split_shape(const cx_pool* pool, const cx_attn_batch* b) {
-    const int64_t rows = b->n_q_heads / pool->n_kv_heads * b->max_q_len;
+// What every TMA kernel needs of the pool and the batch: 16-token blocks, heads
+// of 64 or 128, 16-byte alignment, indexes that fit 32 bits.
+static bool tma_shape(const cx_pool* pool, const cx_attn_batch* b) {
     const int64_t tiles = pool->n_layers * pool->n_blocks * pool->n_kv_heads;
     const uintptr_t a = reinterpret_cast<uintptr_t>(pool->k) | reinterpret_cast<uintptr_t>(pool->v);
     return (a & 15) == 0 && pool->block_size == kBlockTok && tiles < (1ll << 31) &&
            (pool->head_dim == 64 || pool->head_dim == 128) && b->batch < (1 << 24) &&
-           pool->n_kv_heads * b->batch < (1 << 24) && rows >= 1 && rows <= 64;
+           pool->n_kv_heads * b->batch < (1 << 24);
+}
+
+// The tcgen05 kernel: 16-bit pools from 64 packed rows (query tokens x GQA
+// group) of more than one token, and groups that the split-K kernels' 64 rows
+// do not hold.
+static bool tc_shape(const cx_pool* pool, const cx_attn_batch* b) {
+    const int64_t G = b->n_q_heads / pool->n_kv_heads, rows = G * b->max_q_len;
+    return pool->dtype != CX_F32 && tma_shape(pool, b) && G <= kTcRows &&
+           (rows > 64 || (rows == 64 && b->max_q_len > 1));
+}
+
+// The split-K kernels: up to 64 packed rows.
+static bool split_shape(const cx_pool* pool, const cx_attn_batch* b) {
+    const int64_t rows = b->n_q_heads / pool->n_kv_heads * b->max_q_len;
+    return tma_shape(pool, b) && rows >= 1 && rows <= 64 && !tc_shape(pool, b);
 }
 
 // The kernel of a call.  `vec`: q, its token stride and out are 16-byte aligned.
 // 16-bit pools take queries of their own type or fp32, fp32 pools any type.
 static int attend_kind(const cx_pool* pool, const cx_attn_batch* b, int32_t q_dtype, bool vec) {
-    if (!vec || !split_shape(pool, b)) return CX_KERNEL_GENERIC;
-    if (pool->dtype == CX_F32) return CX_KERNEL_FMA;
-    return q_dtype == CX_F32 || q_dtype == pool->dtype ? CX_KERNEL_MMA : CX_KERNEL_GENERIC;
+    if (!vec) return CX_KERNEL_GENERIC;
+    if (pool->dtype == CX_F32) return split_shape(pool, b) ? CX_KERNEL_FMA : CX_KERNEL_GENERIC;
+    if (q_dtype != CX_F32 && q_dtype != pool->dtype) return CX_KERNEL_GENERIC;
+    return tc_shape(pool, b)      ? CX_KERNEL_TCGEN05
+           : split_shape(pool, b) ? CX_KERNEL_MMA
+                                  : CX_KERNEL_GENERIC;
+}
+
+// CTAs of the tcgen05 kernel, and over how many the key tiles of each are split
+// when they are fewer than half the SMs: at least 4 tiles (512 keys) a part.
+// The host knows the contexts by the width of the tables only.
+static void tc_grid(const cx_pool* pool, const cx_attn_batch* b, int* tpt, int64_t* n_ctiles,
+                    int* n_split) {
+    const int64_t G = b->n_q_heads / pool->n_kv_heads;
+    *tpt = (int)(kTcRows / G);
+    *n_ctiles = (b->max_q_len + 2 * *tpt - 1) / (2 * *tpt);
+    const int64_t ctas = *n_ctiles * b->batch * pool->n_kv_heads, sms = grid_size();
+    int64_t keys = b->table_stride * kBlockTok;
+    if (b->window > 0) keys = std::min(keys, b->window + 2 * *tpt + kScKeys);
+    const int64_t tiles = (keys + kScKeys - 1) / kScKeys;
+    int64_t s = 1;
+    if (ctas > 0 && 2 * ctas <= sms) s = std::min(sms / ctas, tiles / 4);
+    *n_split = (int)std::max<int64_t>(1, s);
 }
 
 static size_t attend_workspace(const cx_pool* pool, const cx_attn_batch* b) {
     const int64_t rows = b->n_q_heads / pool->n_kv_heads * b->max_q_len;
+    if (tc_shape(pool, b)) {
+        int tpt, n_split;
+        int64_t n_ctiles;
+        tc_grid(pool, b, &tpt, &n_ctiles, &n_split);
+        return n_split == 1 ? 256
+                            : (size_t)(n_ctiles * b->batch * pool->n_kv_heads) * n_split * 256 *
+                                  (pool->head_dim + 2) * 4;
+    }
+    if (!split_shape(pool, b)) return 256;
     return ws_layout(b->batch, unit_shape(pool, rows), rows, pool->head_dim, grid_size()).total;
 }
 
@@ -108,6 +154,54 @@ static int attend_split(const cx_pool* pool, int64_t layer, const cx_attn_batch&
     }
 }
 
+// The tcgen05 kernel (attn_scored_tc.cuh).
+static int attend_tc(const cx_pool* pool, int64_t layer, const cx_attn_batch& b,
+                     const cx_attn_mods& m, float scale, const void* q, int32_t q_dtype, void* out,
+                     void* ws, size_t ws_bytes, cudaStream_t st) {
+    ScoredTcParams p{};
+    int64_t n_ctiles = 0;
+    tc_grid(pool, &b, &p.tpt, &n_ctiles, &p.n_split);
+    if (n_ctiles > (1 << 24)) return fail(CX_ERR_UNSUPPORTED, "cx_paged_attend: grid too large");
+    if (p.n_split > 1 && (!ws || ws_bytes < attend_workspace(pool, &b) ||
+                          (reinterpret_cast<uintptr_t>(ws) & 255) != 0))
+        return fail(CX_ERR_WORKSPACE,
+                    "cx_paged_attend: workspace missing, too small or not 256-byte aligned");
+    p.tables = b.block_tables;
+    p.table_stride = b.table_stride;
+    p.ctx_lens = b.ctx_lens;
+    p.q_start = b.q_start;
+    p.slopes = m.alibi_slopes;
+    p.prefix = m.prefix_lens;
+    p.q = q;
+    p.out = out;
+    p.part = static_cast<float*>(ws);
+    p.q_stride = m.q_stride;
+    p.batch = (int)b.batch;
+    p.hk = (int)pool->n_kv_heads;
+    p.hq = (int)b.n_q_heads;
+    p.group = p.hq / p.hk;
+    p.n_ctiles = (int)n_ctiles;
+    p.n_blocks = (int)pool->n_blocks;
+    p.layer = (int)layer;
+    p.window = b.window > 0 ? (int)b.window : 0;
+    p.q_dtype = q_dtype;
+    p.out_dtype = m.out_dtype;
+    p.scale_log2 = fabsf(scale) * 1.4426950408889634f;
+    p.z_scale = m.softcap > 0.f ? fabsf(scale) / m.softcap : 0.f;
+    p.cap_log2 = m.softcap * 1.4426950408889634f;
+    p.neg = scale < 0.f;
+    CUtensorMap tk, tv;
+    int rc = make_pool_tmap(&tk, pool->k, pool, 1);
+    if (rc) return rc;
+    rc = make_pool_tmap(&tv, pool->v, pool, 1);
+    if (rc) return rc;
+    if (pool->dtype == CX_BF16)
+        return pool->head_dim == 128 ? launch_scored_tc<128, __nv_bfloat16>(tk, tv, p, st)
+                                     : launch_scored_tc<64, __nv_bfloat16>(tk, tv, p, st);
+    return pool->head_dim == 128 ? launch_scored_tc<128, __half>(tk, tv, p, st)
+                                 : launch_scored_tc<64, __half>(tk, tv, p, st);
+}
+
 static int attend_scored(const cx_pool* pool, int64_t layer, const cx_attn_batch* bt,
                          const cx_attn_mods* mods, const void* q, int32_t q_dtype, void* out,
                          void* ws, size_t ws_bytes, int32_t replan, void* stream) {
@@ -147,6 +241,8 @@ static int attend_scored(const cx_pool* pool, int64_t layer, const cx_attn_batch
     if (kind == CX_KERNEL_MMA || kind == CX_KERNEL_FMA)
         return attend_split(pool, layer, b, m, scale, q, q_dtype, out, ws, ws_bytes, replan,
                             false, st);
+    if (kind == CX_KERNEL_TCGEN05)
+        return attend_tc(pool, layer, b, m, scale, q, q_dtype, out, ws, ws_bytes, st);
     // a later layer of the step may have queries that the split-K kernels take:
     // the plan it then reads is made now
     if (replan && split_shape(pool, &b) && ws) {

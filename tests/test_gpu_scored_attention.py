@@ -94,6 +94,30 @@ def test_type_mixes(dtype, out_dtype, q_dtype, q_lens):
     c.check(c.run(out_dtype=out_dtype))
 
 
+@pytest.mark.parametrize("mods", ["cap", "alibi", "window-prefix-cap", "prefix"])
+@pytest.mark.parametrize("hq,hk,d,dtype,q_lens,ctx", [
+    (4, 1, 128, BF, [33], [5000]),                    # one tile, its keys over many CTAs
+    (2, 2, 64, F16, [300, 70], [4100, 70]),           # two sequences, one too short to split
+    (96, 1, 64, BF, None, [3000, 1, 0]),              # one token of 96 heads on one KV head
+    (5, 1, 128, F16, [1, 60, 0], [2500, 900, 40]),
+])
+def test_key_tiles_split_over_ctas(mods, hq, hk, d, dtype, q_lens, ctx):
+    c = _case(mods, hq, ctx, q_lens=q_lens, hk=hk, d=d, dtype=dtype, seed=7)
+    batch = c.batch()
+    assert batch.kernel_kind(dtype) == "tcgen05"
+    a = c.run(batch, out_dtype=dtype)
+    c.check(a)
+    assert torch.equal(a, c.run(batch, out_dtype=dtype))
+
+
+@pytest.mark.parametrize("q_scale", [1.0, 12.0])
+def test_scores_on_both_sides_of_the_polynomial(q_scale):
+    """|z| = |score| / cap below 0.8 for every key, and beyond it for most."""
+    c = _case("plain", 8, [700, 640], hk=4, d=128, dtype=F16, q_lens=[300, 90], softcap=12.0,
+              q_scale=q_scale)
+    c.check(c.run(out_dtype=F16))
+
+
 @pytest.mark.parametrize("q_lens", [None, [3, 5], [3, 80]])
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_query_heads_of_a_fused_projection(dtype, q_lens):
@@ -162,7 +186,7 @@ KIND = {"decode": None, "chain": [3, 5], "chunk": [40, 70]}
 @pytest.mark.parametrize("shape,dtype,d,kind", [
     ("decode", BF, 64, "mma"), ("decode", F16, 128, "mma"), ("chain", F16, 64, "mma"),
     ("decode", F32, 64, "fma"), ("chain", F32, 128, "fma"), ("decode", BF, 96, "generic"),
-    ("chunk", F32, 64, "generic")])
+    ("chunk", F32, 64, "generic"), ("chunk", BF, 128, "tcgen05"), ("chunk", F16, 64, "tcgen05")])
 def test_kernel_choice(shape, dtype, d, kind):
     c = _case("cap", 8, [70, 300], hk=2, d=d, dtype=dtype, q_lens=KIND[shape])
     assert c.batch().kernel_kind(dtype) == kind
