@@ -170,7 +170,10 @@ def _prepare_append(case, seed):
     s["vp"] = torch.zeros(nb * BLOCK + 1, hk, d, dtype=dt, device=DEV)
     if own:                 # the program's cache and rotation tables
         from chenxing_b200 import RadixPagedKVCache, RopeTables
-        s["cache"] = RadixPagedKVCache(nb, BLOCK, 1, hk, d, dtype=dt, host_io=False)
+        # one block of all the slots, so that the pools seen token by token are views (the
+        # slots are scattered rows either way)
+        s["cache"] = RadixPagedKVCache(1, nb * BLOCK, 1, hk, d, dtype=dt, host_io=False)
+        s["pools"] = s["cache"].k_pool[0, 0], s["cache"].v_pool[0, 0]
         s["rope"] = RopeTables(case["max_pos"], rot, interleaved=case["inter"],
                                tables=(s["cos"].cpu().numpy(), s["sin"].cpu().numpy()))
     return s
@@ -230,7 +233,7 @@ def _own(s):
     if case["op"] == "append":
         q_out = cache.append_norm_rope(0, s["k"], s["v"], s["slots"], s["positions"], s["rope"],
                                        s["q"], q_weight=s["qw"], k_weight=s["kw"], eps=EPS)
-        return q_out, cache.k_pool[0].flatten(0, 1), cache.v_pool[0].flatten(0, 1)
+        return (q_out, *s["pools"])
     call = cache.decode_batch if case["op"] == "decode" else cache.verify_batch
     return call(0, s["q"], s["batch"], out_dtype=DTYPES[case["dtype"]])
 
