@@ -81,6 +81,14 @@ def rows_on_device(x, device: torch.device) -> torch.Tensor:
     return to_device(x, device)
 
 
+def index_on_device(x, device: torch.device) -> torch.Tensor:
+    """Slots or positions as a contiguous int64 tensor on ``device``."""
+    if isinstance(x, torch.Tensor) and x.is_cuda and x.dtype == torch.int64 \
+            and x.device == device and x.is_contiguous():
+        return x
+    return to_device(x, device, float_only=False).to(torch.int64)
+
+
 def upload(a, device: torch.device) -> torch.Tensor:
     """Host metadata (NumPy) -> device without synchronising the stream: the
     array is staged in pinned memory and copied with ``non_blocking`` on the

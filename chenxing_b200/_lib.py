@@ -201,6 +201,16 @@ def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def raw_stream(device: torch.device) -> int:
+    """``stream_ptr`` without building a Stream object (0.1 instead of 2.2 us)."""
+    if _RAW_STREAM is None or device.index is None:
+        return stream_ptr(device)
+    return _RAW_STREAM(device.index)
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

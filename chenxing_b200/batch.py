@@ -258,7 +258,7 @@ def _attend_scored(cache, layer: int, q, batch: PagedBatch, out, replan, out_dty
     if not qt.is_contiguous() and (qt.stride(1) != d or qt.stride(0) < hq * d):
         qt = qt.contiguous()
     if out is None:
-        out = torch.empty(expect, dtype=out_dtype, device=dev)
+        out = qt.new_empty(expect, dtype=out_dtype)
     elif tuple(out.shape) != expect or out.dtype != out_dtype or not out.is_contiguous() \
             or not _lib.same_device(out.device, dev):
         raise ValueError(f"out must be a contiguous {out_dtype} tensor of shape {expect} "
@@ -271,7 +271,7 @@ def _attend_scored(cache, layer: int, q, batch: PagedBatch, out, replan, out_dty
         _lib.check(_lib.lib().cx_paged_attend(
             cache.cx_pool(), int(layer), batch.c_struct(), mods, qt.data_ptr(),
             _lib.cx_dtype(qt.dtype), out.data_ptr(), batch.workspace.data_ptr(),
-            batch.workspace.numel(), int(do_plan), _lib.stream_ptr(dev)), "cx_paged_attend")
+            batch.workspace.numel(), int(do_plan), _lib.raw_stream(dev)), "cx_paged_attend")
     if do_plan:
         batch.needs_plan = False
         batch._planned_by = "scored"

@@ -119,6 +119,31 @@ __device__ __forceinline__ void store2_as(void* p, int32_t dtype, int64_t i, flo
         *reinterpret_cast<__half2*>(static_cast<__half*>(p) + i) = __floats2half2_rn(x, y);
 }
 
+// ---- packed fp32 pairs ------------------------------------------------------
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 f2_of(float lo, float hi) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void f2_get(f2 v, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ f2 f2_fma(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f2 f2_mul(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 f2_add(f2 a, f2 b) {
+    f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 // ---- shared-memory / PTX helpers -----------------------------------------
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -244,6 +269,9 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 template <typename E> struct Half16;
 template <> struct Half16<__nv_bfloat16> {
     __device__ __forceinline__ static uint32_t pack(float lo, float hi) { return pack_bf16(lo, hi); }
+    __device__ __forceinline__ static f2 unpack(uint32_t u) {
+        return f2_of(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    }
     __device__ __forceinline__ static void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                                uint32_t b1) {
         mma_bf16_16816(d, a, b0, b1);
@@ -253,6 +281,10 @@ template <> struct Half16<__half> {
     __device__ __forceinline__ static uint32_t pack(float lo, float hi) {
         const __half2 v = __floats2half2_rn(lo, hi);
         return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    __device__ __forceinline__ static f2 unpack(uint32_t u) {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&u));
+        return f2_of(v.x, v.y);
     }
     __device__ __forceinline__ static void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                                uint32_t b1) {

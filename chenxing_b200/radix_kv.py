@@ -33,7 +33,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._arrays import rows_on_device, to_device, to_numpy, torch_dtype, upload
+from ._arrays import index_on_device, rows_on_device, to_device, to_numpy, torch_dtype, upload
 
 __all__ = ["RadixPagedKVCache", "RadixIndex", "PrefixHit", "OutOfKVCacheError"]
 
@@ -643,54 +643,59 @@ class RadixPagedKVCache(RadixIndex):
         is fp32 and rounded once.  A negative slot stores K and V nowhere (Q is
         still returned); the slots of one call must differ.  Weights: (D,),
         float32 or the rows' type."""
-        qt = None if q is None else rows_on_device(q, self.device)
-        kt, vt = rows_on_device(k, self.device), rows_on_device(v, self.device)
-        if vt.dtype != kt.dtype or (qt is not None and qt.dtype != kt.dtype):
+        dev, D = self.device, self.head_dim
+        kt, vt = rows_on_device(k, dev), rows_on_device(v, dev)
+        dt, T = kt.dtype, kt.shape[0]
+        if kt.shape != (T, self.n_kv_heads, D) or vt.shape != kt.shape:
+            raise ValueError(f"k and v must have shape {(T, self.n_kv_heads, D)}, got "
+                             f"{tuple(kt.shape)} / {tuple(vt.shape)}")
+        qt = qo = None
+        hq, qs, q_code = 0, (0, 0), _lib.CX_F32
+        if q is not None:
+            qt = rows_on_device(q, dev)
+            if qt.dim() != 3 or qt.shape[0] != T or qt.shape[2] != D:
+                raise ValueError(f"q must be ({T}, Hq, {D}), got {tuple(qt.shape)}")
+            hq, qs = qt.shape[1], qt.stride()
+        if vt.dtype != dt or (qt is not None and qt.dtype != dt):
             raise TypeError("q, k and v must have one element type")
-        T, D = int(kt.shape[0]), self.head_dim
-        shape = (T, self.n_kv_heads, D)
-        if tuple(kt.shape) != shape or tuple(vt.shape) != shape:
-            raise ValueError(f"k and v must have shape {shape}, got {tuple(kt.shape)} / "
-                             f"{tuple(vt.shape)}")
-        if qt is not None and (qt.dim() != 3 or qt.shape[0] != T or qt.shape[2] != D):
-            raise ValueError(f"q must be ({T}, Hq, {D}), got {tuple(qt.shape)}")
         if rope.head_dim > D:
             raise ValueError(f"RoPE tables of {rope.head_dim} dims for heads of {D}")
-        if not _lib.same_device(rope.device, self.device):
-            raise ValueError(f"RoPE tables on {rope.device}, the cache on {self.device}")
-        st = to_device(slot_mapping, self.device, float_only=False).to(torch.int64)
-        ps = to_device(positions, self.device, float_only=False).to(torch.int64)
+        if rope.device != dev and not _lib.same_device(rope.device, dev):
+            raise ValueError(f"RoPE tables on {rope.device}, the cache on {dev}")
+        st, ps = index_on_device(slot_mapping, dev), index_on_device(positions, dev)
         if st.numel() != T or ps.numel() != T:
             raise ValueError("slot_mapping and positions need one entry per token")
-
-        def weight(w, what):
-            if w is None:
-                return None
-            w = to_device(w, self.device)
-            if w.numel() != D:
-                raise ValueError(f"{what} must have {D} elements, got {w.numel()}")
-            return w if w.dtype in (torch.float32, kt.dtype) else w.float()
-
-        qw, kw = weight(q_weight, "q_weight"), weight(k_weight, "k_weight")
-        f32 = _lib.CX_F32
-        how = _lib.CxNormRope(_lib.ptr(qw), _lib.ptr(kw),
-                              f32 if qw is None else _lib.cx_dtype(qw.dtype),
-                              f32 if kw is None else _lib.cx_dtype(kw.dtype), float(eps),
-                              int(rope.interleaved), rope.cos.data_ptr(), rope.sin.data_ptr(),
-                              rope.rows, rope.head_dim)
-        qo, hq, qs = None, 0, (0, 0)
+        code = _lib.cx_dtype(dt)
+        qw, qw_code = self._norm_weight(q_weight, "q_weight", dt, code)
+        kw, kw_code = self._norm_weight(k_weight, "k_weight", dt, code)
         if qt is not None:
-            hq, qs = int(qt.shape[1]), qt.stride()
-            qo = torch.empty(qt.shape, dtype=q_out_dtype or kt.dtype, device=self.device)
+            qo = qt.new_empty(qt.shape, dtype=q_out_dtype or dt)
+            q_code = _lib.cx_dtype(qo.dtype)
         ks, vs = kt.stride(), vt.stride()
         rows = _lib.CxQkv(_lib.ptr(qt), kt.data_ptr(), vt.data_ptr(), qs[0], qs[1], ks[0], ks[1],
-                          vs[0], vs[1], T, hq, _lib.cx_dtype(kt.dtype), 0)
-        with _lib.on_device(self.device):
+                          vs[0], vs[1], T, hq, code, 0)
+        how = _lib.CxNormRope(_lib.ptr(qw), _lib.ptr(kw), qw_code, kw_code, eps,
+                              rope.interleaved, rope.cos.data_ptr(), rope.sin.data_ptr(),
+                              rope.rows, rope.head_dim)
+        with _lib.on_device(dev):
             _lib.check(_lib.lib().cx_kv_append_norm_rope(
-                self._pool, int(layer), rows, st.data_ptr(), ps.data_ptr(), how, _lib.ptr(qo),
-                f32 if qo is None else _lib.cx_dtype(qo.dtype), _lib.stream_ptr(self.device)),
-                "cx_kv_append_norm_rope")
+                self._pool, layer, rows, st.data_ptr(), ps.data_ptr(), how, _lib.ptr(qo),
+                q_code, _lib.raw_stream(dev)), "cx_kv_append_norm_rope")
         return qo
+
+    def _norm_weight(self, w, what: str, dt: torch.dtype, code: int):
+        """A (head_dim,) weight on the device as float32 or the rows' type, and
+        its type code."""
+        if w is None:
+            return None, _lib.CX_F32
+        if not (isinstance(w, torch.Tensor) and w.is_cuda and w.device == self.device
+                and w.is_contiguous()):
+            w = to_device(w, self.device)
+        if w.numel() != self.head_dim:
+            raise ValueError(f"{what} must have {self.head_dim} elements, got {w.numel()}")
+        if w.dtype == dt:
+            return w, code
+        return (w if w.dtype == torch.float32 else w.float()), _lib.CX_F32
 
     def decode_batch(self, layer: int, q, batch, out=None, replan=None, out_dtype=None):
         """Paged flash-decode of one query token per sequence of ``batch``."""

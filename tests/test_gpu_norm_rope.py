@@ -146,6 +146,16 @@ def test_token_and_head_counts(T, hq, hk):
     r.check(r.call())
 
 
+@pytest.mark.parametrize("T,d,rot,dtype,pool,hq,hk", [
+    (1400, 128, 128, BF, BF, 32, 8), (3000, 64, 16, F32, F32, 17, 3),
+    (2600, 96, 24, F16, F16, 24, 4), (2000, 256, 128, F32, BF, 4, 2), (3000, 80, 40, BF, BF, 24, 4)])
+@pytest.mark.parametrize("inter", [False, True])
+def test_staged_form_for_much_data(T, d, rot, dtype, pool, hq, hk, inter):
+    """From 14 MB of rows a CTA copies several tokens ahead into shared memory."""
+    r = Rows(T, hq, hk, d, rot, dtype=dtype, pool=pool, inter=inter, seed=d, skip=range(0, T, 7))
+    r.check(r.call(q_out_dtype=pool))
+
+
 @pytest.mark.parametrize("layout", ["fused", "heads-first", "odd", "contiguous"])
 @pytest.mark.parametrize("dtype", [BF, F16, F32])
 @pytest.mark.parametrize("norm", ["qk", "q", "k", ""])
@@ -219,13 +229,18 @@ def test_bad_position_and_slot_are_skipped_and_flagged():
     assert _lib.device_flags(clear=True) == 1
     r.slots[2] = -1
     r.check(out)
-    r = Rows(6, 2, 2, 64, 64)
-    r.pos[3] = 600
-    r.call()
-    assert _lib.device_flags(clear=True) == 32
-    at = int(r.slots[3])
-    assert (r.cache.k_pool[0, at // 16, at % 16] == 3).all()
-    assert (r.cache.v_pool[0, at // 16, at % 16] == 5).all()
+    for T, hq, bad in ((6, 2, 3), (3000, 40, 2500)):
+        r = Rows(T, hq, 2, 64, 64)
+        r.pos[bad] = 600
+        out = r.call()
+        assert _lib.device_flags(clear=True) == 32
+        at = int(r.slots[bad])
+        assert (r.cache.k_pool[0, at // 16, at % 16] == 3).all()
+        assert (r.cache.v_pool[0, at // 16, at % 16] == 5).all()
+        r.pos[bad], r.slots[bad] = 0, -1        # all other rows are right
+        want, _ = r.turned(r.q, r.qw, BF)
+        out[bad] = want[bad].to(BF).cuda()
+        r.check(out)
 
 
 def test_numpy_rows():
