@@ -123,7 +123,9 @@ static int attend_split(const cx_pool* pool, int64_t layer, const cx_attn_batch&
     p.mod.q_dtype = q_dtype;
     if (m.softcap > 0.f) {
         p.mod.cap_log2 = m.softcap * 1.4426950408889634f;
-        p.mod.scale = scale / m.softcap * (pool->dtype == CX_F32 ? 1.f : 2.8853900817779268f);
+        p.mod.scale = scale / m.softcap;
+        const float c[5] = {kTanhC0, kTanhC1, kTanhC2, kTanhC3, kTanhC4};
+        for (int i = 0; i < 5; ++i) p.mod.c[i] = p.mod.cap_log2 * c[i];
     }
     if (replan) {
         paged_plan_kernel<<<1, 1024, 0, st>>>(p, grid);

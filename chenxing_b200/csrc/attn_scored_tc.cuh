@@ -98,12 +98,6 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
     return r;
 }
 
-// tanh over |z| <= kTanhMax: z * P(z^2), coefficients from z^0 up.
-constexpr float kTanhMax = 0.8f;
-constexpr float kTanhC0 = 0.9999951345111643f, kTanhC1 = -0.3331742660309651f,
-                kTanhC2 = 0.13186219564770923f, kTanhC3 = -0.048261313435940166f,
-                kTanhC4 = 0.011464653557922883f;
-
 // cap * log2(e) * tanh(z) for any z.
 __device__ __forceinline__ float cap_any(float z, float cap_log2) {
     return fmaf(-2.f * cap_log2, rcp_approx(1.f + ex2_sfu(z * 2.8853900817779268f)), cap_log2);
