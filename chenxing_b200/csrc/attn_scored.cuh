@@ -192,6 +192,21 @@ static int attend_tc(const cx_pool* pool, int64_t layer, const cx_attn_batch& b,
     p.z_scale = m.softcap > 0.f ? fabsf(scale) / m.softcap : 0.f;
     p.cap_log2 = m.softcap * 1.4426950408889634f;
     p.neg = scale < 0.f;
+    if (m.softcap > 0.f && p.z_scale > 0.f) {
+        // in double: z_scale^9 may be small, but its product with the score is not.
+        // A coefficient below fp32's normal range (caps beyond some thousands) leaves
+        // every score to the other form (s4_max = s5_max = 0).
+        double zk = p.z_scale;
+        const double z2 = (double)p.z_scale * p.z_scale;
+        bool fits = true;
+        for (int i = 0; i < 5; ++i, zk *= z2) {
+            p.c5[i] = (float)(p.cap_log2 * kTanh5[i] * zk);
+            if (i < 4) p.c4[i] = (float)(p.cap_log2 * kTanh4[i] * zk);
+            fits = fits && fabs(p.cap_log2 * kTanh5[i] * zk) > 1e-36;
+        }
+        p.s4_max = fits ? kTanh4Max / p.z_scale : 0.f;
+        p.s5_max = fits ? kTanhMax / p.z_scale : 0.f;
+    }
     CUtensorMap tk, tv;
     int rc = make_pool_tmap(&tk, pool->k, pool, 1);
     if (rc) return rc;

@@ -43,7 +43,8 @@ def build_rope_cache(seq_len: int, head_dim: int, base: float = 10000.0, *,
 
 
 class RopeTables:
-    """Device-resident cos / sin tables of one model's RoPE configuration."""
+    """Device-resident cos / sin tables of one model's RoPE configuration.
+    ``tables``: (cos, sin) of one's own, NumPy arrays or torch tensors."""
 
     def __init__(self, max_positions: int, head_dim: int, base: float = 10000.0, *,
                  scaling_factor: float = 1.0, original_max_pos: int = 4096,
@@ -55,11 +56,13 @@ class RopeTables:
                                       scaling_factor=scaling_factor,
                                       original_max_pos=original_max_pos,
                                       beta_fast=beta_fast, beta_slow=beta_slow)
-        cos, sin = (np.ascontiguousarray(t, dtype=np.float32) for t in tables)
+        cos, sin = (t.detach().to(self.device, torch.float32).contiguous()
+                    if isinstance(t, torch.Tensor) else np.ascontiguousarray(t, dtype=np.float32)
+                    for t in tables)
         if cos.shape != sin.shape or cos.ndim != 2 or cos.shape[1] != head_dim:
             raise ValueError("cos / sin tables must both be (positions, head_dim)")
         self.head_dim = int(head_dim)
         self.rows = int(cos.shape[0])
         self.interleaved = bool(interleaved)
-        self.cos = torch.from_numpy(cos).to(self.device)
-        self.sin = torch.from_numpy(sin).to(self.device)
+        self.cos, self.sin = (t if isinstance(t, torch.Tensor)
+                              else torch.from_numpy(t).to(self.device) for t in (cos, sin))

@@ -217,8 +217,12 @@ def test_scaled_tables_for_long_contexts():
     from chenxing_b200 import RopeTables
     r = Rows(30, 4, 2, 128, 64, dtype=F32, max_pos=20000)
     r.cos, r.sin = tables(20000, 64, scaling_factor=8.0, original_max_pos=2048)
-    r.rope = RopeTables(20000, 64, tables=(r.cos, r.sin))
-    r.check(r.call())
+    for dev in ("numpy", "cpu", "cuda"):
+        tabs = [x if dev == "numpy" else torch.from_numpy(x).to(dev) for x in (r.cos, r.sin)]
+        r.rope = RopeTables(20000, 64, tables=tabs)
+        r.check(r.call())
+    with pytest.raises(ValueError):
+        RopeTables(20000, 32, tables=tabs)
 
 
 def test_bad_position_and_slot_are_skipped_and_flagged():
