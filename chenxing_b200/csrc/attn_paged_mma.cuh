@@ -792,10 +792,13 @@ __global__ void __launch_bounds__(MmaCfg<D, MT, HG>::THREADS, 1)
                 bool bad[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u) bad[u] = BAD && (u == 0 || two) && s_bad[su[u]] != 0;
+                // FAST (MOD): every unit is there and good, and every row sees all its keys
+                auto work = [&](auto fast_tag) {
+                constexpr bool FAST = decltype(fast_tag)::value;
                 float x[U][2][4];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    if ((u > 0 && !two) || bad[u]) {
+                    if (!FAST && ((u > 0 && !two) || bad[u])) {
 #pragma unroll
                         for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -832,8 +835,8 @@ __global__ void __launch_bounds__(MmaCfg<D, MT, HG>::THREADS, 1)
                         for (int e = 0; e < 4; ++e)
                             x[u][n][e] = (sa[n][e] + sb[n][e]) * p.scale_log2;
                     const int t0 = seg_block<MOD>(seg, k + u * KS) * kBlockTok;
-                    bool edge = (t0 + kBlockTok - 1 > pos0) ||
-                                (p.window > 0 && t0 <= ctx - 1 - p.window);
+                    bool edge = !FAST && ((t0 + kBlockTok - 1 > pos0) ||
+                                          (p.window > 0 && t0 <= ctx - 1 - p.window));
                     if constexpr (MOD) {
                         edge = edge && t0 + kBlockTok > pre;
                         if (p.mod.cap_log2 != 0.f) {
@@ -908,8 +911,9 @@ __global__ void __launch_bounds__(MmaCfg<D, MT, HG>::THREADS, 1)
                 // max exceeds it by more than 2^8 (p <= 256 meanwhile; the
                 // final division, and the split-K merge, which uses each
                 // partial's own m, make a stale max exact)
-                const bool g0 = mx0 > m0 + kMmaRescaleLog2 || (m0 == -INFINITY && mx0 > -INFINITY);
-                const bool g1 = mx1 > m1 + kMmaRescaleLog2 || (m1 == -INFINITY && mx1 > -INFINITY);
+                constexpr float kGrow = MOD ? Half16<E>::kGrowLog2 : kMmaRescaleLog2;
+                const bool g0 = mx0 > m0 + kGrow || (m0 == -INFINITY && mx0 > -INFINITY);
+                const bool g1 = mx1 > m1 + kGrow || (m1 == -INFINITY && mx1 > -INFINITY);
                 const float mn0 = g0 ? mx0 : m0, mn1 = g1 ? mx1 : m1;
                 const float base0 = mn0 == -INFINITY ? 0.f : mn0;
                 const float base1 = mn1 == -INFINITY ? 0.f : mn1;
@@ -945,9 +949,9 @@ __global__ void __launch_bounds__(MmaCfg<D, MT, HG>::THREADS, 1)
                 }
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    if ((u > 0 && !two) || bad[u]) continue;
+                    if (!FAST && ((u > 0 && !two) || bad[u])) continue;
                     const uint32_t vb = smem_addr(ring + (size_t)su[u] * C::STAGE) + C::TILES;
-                    if constexpr (MOD) {
+                    if constexpr (MOD && !FAST) {
                         const int t0 = seg_block<MOD>(seg, k + u * KS) * kBlockTok;
                         if (dead.any(t0)) {
                             unsigned char* vs = ring + (size_t)su[u] * C::STAGE + C::TILES +
@@ -976,6 +980,24 @@ __global__ void __launch_bounds__(MmaCfg<D, MT, HG>::THREADS, 1)
                         Half16<E>::mma(o[2 * np], pa, f[0], f[1]);
                         Half16<E>::mma(o[2 * np + 1], pa, f[2], f[3]);
                     }
+                }
+                };
+                if constexpr (MOD) {
+                    bool fast = true;
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const int t0 = seg_block<MOD>(seg, k + u * KS) * kBlockTok;
+                        fast = fast && !bad[u] &&
+                               (t0 + kBlockTok <= pre ||
+                                (t0 + kBlockTok - 1 <= pos0 &&
+                                 (p.window <= 0 || t0 > ctx - 1 - p.window)));
+                    }
+                    if (fast && (U == 1 || two))
+                        work(std::true_type{});
+                    else
+                        work(std::false_type{});
+                } else {
+                    work(std::false_type{});
                 }
             }
             __syncwarp();

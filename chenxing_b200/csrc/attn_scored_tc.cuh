@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
             const int w_hi = __shfl_sync(0xffffffffu, pos, 31);
             // growth of a row maximum that makes its reference follow (base 2): what P's
             // type holds above 1 (bf16 as much as the fp32 sums, fp16 below 2^16)
-            constexpr float kRescale = std::is_same<E, __nv_bfloat16>::value ? 60.f : 15.f;
+            constexpr float kRescale = Half16<E>::kGrowLog2;
             float m = -INFINITY, l = 0.f;
             // `ok` turns false (warp-uniformly) when a bounded wait gives up; the warp
             // then skips its waits and TMEM work but keeps meeting the other half's
