@@ -149,21 +149,38 @@ __global__ void __launch_bounds__(F32Cfg<D, HG, RT>::MAX_THREADS, 1)
 
         // stage the group's query rows (fp32, zero padding rows): tile
         // (hh2, mt2) row r is packed row mt2 * RT + r of head seg.g * HG + hh2
+        if constexpr (MOD) {
+            // a warp per row, two columns a lane
+            for (int row = ctid >> 5; row < HG * MT * RT; row += NCT >> 5) {
+                const int r = row % RT, tile = row / RT, hh2 = tile % HG, R = (tile / HG) * RT + r;
+                float* dst = s_q + (size_t)tile * RT * C::QROW + r * C::QROW;
+                const int tok = R / G;
+                const int64_t q0 = (qs + tok) * p.mod.q_stride +
+                                   ((int64_t)(seg.g * HG + hh2) * G + (R - tok * G)) * D;
+#pragma unroll
+                for (int k = 0; k < D / 64; ++k) {
+                    const int d = k * 64 + 2 * lane;
+                    float2 v = make_float2(0.f, 0.f);
+                    if (R < rows_b)
+                        v = p.mod.q_dtype == CX_F32
+                                ? QLoad<float>::two(static_cast<const float*>(p.q), q0 + d)
+                            : p.mod.q_dtype == CX_F16
+                                ? QLoad<__half>::two(static_cast<const __half*>(p.q), q0 + d)
+                                : QLoad<__nv_bfloat16>::two(
+                                      static_cast<const __nv_bfloat16*>(p.q), q0 + d);
+                    *reinterpret_cast<float2*>(dst + d) = v;
+                }
+            }
+        } else
         for (int e = ctid; e < HG * MT * RT * D; e += NCT) {
             const int d = e % D, r = (e / D) % RT, tile = e / (D * RT);
             const int hh2 = tile % HG, R = (tile / HG) * RT + r;
             float v = 0.f;
             if (R < rows_b) {
-                int64_t qi =
+                const int64_t qi =
                     ((qs + R / G) * Hq + (int64_t)(seg.g * HG + hh2) * G + R % G) * D + d;
-                if constexpr (MOD)
-                    qi = (qs + R / G) * p.mod.q_stride +
-                         ((int64_t)(seg.g * HG + hh2) * G + R % G) * D + d;
-                if (MOD && p.mod.q_dtype == CX_F16)
-                    v = __half2float(static_cast<const __half*>(p.q)[qi]);
-                else
-                    v = p.q_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.q)[qi])
-                                 : static_cast<const float*>(p.q)[qi];
+                v = p.q_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.q)[qi])
+                             : static_cast<const float*>(p.q)[qi];
             }
             s_q[(size_t)tile * RT * C::QROW + r * C::QROW + d] = v;
         }
@@ -214,7 +231,10 @@ __global__ void __launch_bounds__(F32Cfg<D, HG, RT>::MAX_THREADS, 1)
                 float sa[RPL], sb[RPL];
 #pragma unroll
                 for (int i = 0; i < RPL; ++i) sa[i] = sb[i] = 0.f;
-#pragma unroll
+                // (MOD: a quarter of the code; a short chain's few units wait for
+                // instructions more than for anything else)
+                constexpr int kChunkUnroll = MOD ? 4 : D / 4;
+#pragma unroll kChunkUnroll
                 for (int c = 0; c < D / 4; ++c) {
                     const float4 kv = *reinterpret_cast<const float4*>(kb + C::off(hh, t, c));
 #pragma unroll
@@ -305,7 +325,8 @@ __global__ void __launch_bounds__(F32Cfg<D, HG, RT>::MAX_THREADS, 1)
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     }
                 }
-#pragma unroll
+                constexpr int kTokUnroll = MOD ? 1 : kBlockTok / 4;
+#pragma unroll kTokUnroll
                 for (int t4 = 0; t4 < kBlockTok; t4 += 4) {
                     float4 pr[RT];
 #pragma unroll

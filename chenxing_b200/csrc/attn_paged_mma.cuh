@@ -386,6 +386,54 @@ __device__ __forceinline__ void ks_merge(const MmaParams& p, const float* merge,
                                          int NCT, int KS) {
     const int G = p.group, Hq = p.hq;
     named_bar_sync(1, NCT);
+    if constexpr (MOD) {
+        // a warp per row, so that the row's indexes and weights are worked out once
+        // and not for every element (a third of a short chain's instructions)
+        const int lane = ctid & 31;
+        for (int pr = ctid >> 5; pr < HG * rows_b; pr += NCT >> 5) {
+            const int eh = pr / rows_b, R = pr - eh * rows_b;
+            const float* row0 = merge + ((size_t)eh * p.rows + R) * (D + 2);
+            const size_t step = (size_t)HG * p.rows * (D + 2);
+            float M = -INFINITY;
+            for (int s2 = 0; s2 < KS; ++s2) M = fmaxf(M, row0[s2 * step + D]);
+            float L = 0.f, o[D / 32];
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k) o[k] = 0.f;
+            if (M != -INFINITY) {
+                for (int s2 = 0; s2 < KS; ++s2) {
+                    const float* r = row0 + s2 * step;
+                    const float wgt = exp2f(r[D] - M);
+                    L += r[D + 1] * wgt;
+#pragma unroll
+                    for (int k = 0; k < D / 64; ++k) {
+                        const float2 v =
+                            *reinterpret_cast<const float2*>(r + k * 64 + 2 * lane);
+                        o[2 * k] += v.x * wgt;
+                        o[2 * k + 1] += v.y * wgt;
+                    }
+                }
+            }
+            if (seg.whole) {
+                const int64_t orow = (qs + R / G) * Hq + (int64_t)(seg.g * HG + eh) * G + R % G;
+                const float inv = L > 0.f ? 1.f / L : 0.f;
+#pragma unroll
+                for (int k = 0; k < D / 64; ++k)
+                    put2<MOD>(p, orow * D + k * 64 + 2 * lane, o[2 * k] * inv,
+                              o[2 * k + 1] * inv);
+            } else {
+                float* r = slot + ((size_t)eh * p.rows + R) * (D + 2);
+#pragma unroll
+                for (int k = 0; k < D / 64; ++k)
+                    *reinterpret_cast<float2*>(r + k * 64 + 2 * lane) =
+                        make_float2(o[2 * k], o[2 * k + 1]);
+                if (lane == 0) {
+                    r[D] = M;
+                    r[D + 1] = L;
+                }
+            }
+        }
+        return;
+    }
     for (int e = ctid; e < HG * rows_b * D; e += NCT) {
         const int d = e % D;
         const int R = (e / D) % rows_b;
@@ -441,6 +489,86 @@ __device__ __forceinline__ void ticket_merge(const MmaParams& p, const Seg& seg,
     if (!last) return;
     __threadfence();
     const int pf = (last - 1) & 0xffff, pl = (last - 1) >> 16;
+    if constexpr (MOD) {
+        // A warp takes up to NR rows at a time.  Lanes load the references and
+        // denominators of 32 partials at once; with every weight known, the partials'
+        // columns are loads that wait for nothing.  Taken one partial after the other,
+        // as below, this merge was 40 of the 65 us of 8 short fp32 chains.
+        constexpr int NR = 2;
+        const int lane = ctid & 31, n = pl - pf + 1, stride = NCT >> 5;
+        const int n_rows = HG * rows_b;
+        for (int pr = ctid >> 5; pr < n_rows; pr += NR * stride) {
+            const float* r0[NR];
+            float M[NR], L[NR], o[NR][D / 32];
+#pragma unroll
+            for (int u = 0; u < NR; ++u) {
+                const int q = min(pr + u * stride, n_rows - 1);
+                const int eh = q / rows_b;
+                r0[u] = p.partials + (size_t)(pf + bg) * slot_floats +
+                        ((size_t)eh * p.rows + (q - eh * rows_b)) * (D + 2);
+                M[u] = -INFINITY;
+                L[u] = 0.f;
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k) o[u][k] = 0.f;
+            }
+            for (int p0 = 0; p0 < n; p0 += 32) {
+                const int np = min(32, n - p0);
+                float w[NR];
+#pragma unroll
+                for (int u = 0; u < NR; ++u) {
+                    const float* r = r0[u] + (size_t)(p0 + lane) * slot_floats;
+                    const bool on = lane < np && pr + u * stride < n_rows;
+                    const float m = on ? __ldcg(r + D) : -INFINITY;
+                    const float l = on ? __ldcg(r + D + 1) : 0.f;
+                    float Mn = m;
+#pragma unroll
+                    for (int s2 = 16; s2; s2 >>= 1)
+                        Mn = fmaxf(Mn, __shfl_xor_sync(0xffffffffu, Mn, s2));
+                    Mn = fmaxf(Mn, M[u]);
+                    // (a partial that saw no key: weight 0, its columns are 0)
+                    const float base = Mn == -INFINITY ? 0.f : Mn;
+                    const float a = exp2f(M[u] - base);
+                    w[u] = exp2f(m - base);
+                    float ls = l * w[u];
+#pragma unroll
+                    for (int s2 = 16; s2; s2 >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, s2);
+                    L[u] = L[u] * a + ls;
+#pragma unroll
+                    for (int k = 0; k < D / 32; ++k) o[u][k] *= a;
+                    M[u] = Mn;
+                }
+#pragma unroll 4
+                for (int pp = 0; pp < np; ++pp) {
+#pragma unroll
+                    for (int u = 0; u < NR; ++u) {
+                        if (pr + u * stride >= n_rows) continue;
+                        const float* r = r0[u] + (size_t)(p0 + pp) * slot_floats + 2 * lane;
+                        const float wp = __shfl_sync(0xffffffffu, w[u], pp);
+#pragma unroll
+                        for (int k = 0; k < D / 64; ++k) {
+                            const float2 v = __ldcg(reinterpret_cast<const float2*>(r + k * 64));
+                            o[u][2 * k] = fmaf(v.x, wp, o[u][2 * k]);
+                            o[u][2 * k + 1] = fmaf(v.y, wp, o[u][2 * k + 1]);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < NR; ++u) {
+                const int q = pr + u * stride;
+                if (q >= n_rows) continue;
+                const int eh = q / rows_b, R = q - eh * rows_b;
+                const int64_t orow = (qs + R / G) * Hq + (int64_t)(seg.g * HG + eh) * G + R % G;
+                const float inv = L[u] > 0.f ? 1.f / L[u] : 0.f;
+#pragma unroll
+                for (int k = 0; k < D / 64; ++k)
+                    put2<MOD>(p, orow * D + k * 64 + 2 * lane, o[u][2 * k] * inv,
+                              o[u][2 * k + 1] * inv);
+            }
+        }
+        if (ctid == 0) p.counters[bg] = 0;
+        return;
+    }
     // one pass over the partials, two columns per thread: the loads of every
     // partial are independent of the running merge, so they overlap instead
     // of costing an L2 round trip each
