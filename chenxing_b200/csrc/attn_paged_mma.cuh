@@ -296,12 +296,15 @@ using SegCursor = SegCursorT<false>;
 // stage is re-armed, and before returning the producer waits for its own
 // copies still in flight.
 // ---------------------------------------------------------------------------
-template <int NBOX, int BOX_COLS, int BOX_BYTES, int TILES, int STAGE, bool MOD = false>
+// With NP > 1 producer warps, warp `pw` issues units pw, pw + NP, ...
+template <int NBOX, int BOX_COLS, int BOX_BYTES, int TILES, int STAGE, bool MOD = false,
+          int NP = 1>
 __device__ __forceinline__ void produce_units(const CUtensorMap* tmk, const CUtensorMap* tmv,
                                               const MmaParams& p, SegCursorT<MOD> cur, int HG,
                                               unsigned char* ring, uint64_t* full_bar,
                                               uint64_t* empty_bar, volatile int* s_abort,
-                                              volatile unsigned char* s_bad, int lane) {
+                                              volatile unsigned char* s_bad, int lane,
+                                              int pw = 0) {
     const int STAGES = p.stages;
     Seg seg;
     int i = 0, issued = 0;
@@ -322,7 +325,7 @@ __device__ __forceinline__ void produce_units(const CUtensorMap* tmk, const CUte
             }
             for (int k = 0; k < n; ++k, ++i) {
                 const int bk = __shfl_sync(0xffffffffu, bid, k);
-                if (lane == 0 && !aborted) {
+                if (lane == 0 && !aborted && (NP == 1 || i % NP == pw)) {
                     const int s = i % STAGES;
                     const uint32_t par = ((i / STAGES) & 1) ^ 1;
                     if (!mbar_wait_bounded(&empty_bar[s], par, s_abort, p.wait_ns)) {
@@ -351,7 +354,7 @@ __device__ __forceinline__ void produce_units(const CUtensorMap* tmk, const CUte
                         s_bad[s] = 1;
                         mbar_arrive(&full_bar[s]);
                     }
-                    if (!aborted) ++issued;
+                    if (!aborted) issued = NP == 1 ? issued + 1 : i + 1;
                 }
                 __syncwarp();
             }
@@ -363,6 +366,7 @@ __device__ __forceinline__ void produce_units(const CUtensorMap* tmk, const CUte
     if (lane == 0) {
         const int first = issued > STAGES ? issued - STAGES : 0;
         for (int t = first; t < issued; ++t) {
+            if (NP > 1 && t % NP != pw) continue;
             if (!mbar_wait_bounded(&full_bar[t % STAGES], (t / STAGES) & 1, nullptr,
                                    kWaitLimitNs)) {
                 raise_flag(CX_DEV_WAIT_TIMEOUT);
@@ -675,6 +679,13 @@ struct MmaCfg {
     static constexpr int KS = (HG * MT >= kConsumerWarps) ? 1 : kConsumerWarps / (HG * MT);
     static constexpr int NCW = HG * MT * KS;           // consumer warps
     static constexpr int THREADS = (NCW + 1) * 32;     // + producer warp
+    // MOD with one or two heads a unit: four producer warps, units in turn.  A unit
+    // is then 4 to 16 KB, and one thread needs about 800 cycles for each, whatever
+    // its boxes (32 long sequences on one KV head of 128, bf16: 162 us; a warp each
+    // for K and V 138, four warps 82).  Three and four row tiles are bound by the
+    // consumers and keep one.
+    static constexpr int PRODUCERS_MOD = HG <= 2 && MT <= 2 ? 4 : 1;
+    static constexpr int THREADS_MOD = (NCW + PRODUCERS_MOD) * 32;
     // Q fragments in shared memory (one 16-byte slot per lane and k-step,
     // reloaded per block) instead of registers: lets 12 consumer warps (13
     // warps, 128 registers a thread) run without spilling, and frees the
@@ -718,7 +729,8 @@ struct MmaCfg {
 };
 
 template <int D, int MT, int HG, typename QT, typename E = __nv_bfloat16, bool MOD = false>
-__global__ void __launch_bounds__(MmaCfg<D, MT, HG>::THREADS, 1)
+__global__ void __launch_bounds__(MOD ? MmaCfg<D, MT, HG>::THREADS_MOD
+                                      : MmaCfg<D, MT, HG>::THREADS, 1)
     paged_attn_mma_kernel(const __grid_constant__ CUtensorMap tmk,
                           const __grid_constant__ CUtensorMap tmv, const MmaParams p) {
     using C = MmaCfg<D, MT, HG>;
@@ -769,7 +781,14 @@ __global__ void __launch_bounds__(MmaCfg<D, MT, HG>::THREADS, 1)
     cur.init(u0, u1, p);
     Seg seg;
 
-    if (warp == C::NCW) {
+    if constexpr (MOD && C::PRODUCERS_MOD > 1) {
+        if (warp >= C::NCW) {
+            produce_units<D / 64, 64, HG * C::HALF_BOX, C::TILES, C::STAGE, MOD, C::PRODUCERS_MOD>(
+                &tmk, &tmv, p, cur, HG, ring, full_bar, empty_bar, s_abort, s_bad, lane,
+                warp - C::NCW);
+            return;
+        }
+    } else if (warp == C::NCW) {
         produce_units<D / 64, 64, HG * C::HALF_BOX, C::TILES, C::STAGE, MOD>(
             &tmk, &tmv, p, cur, HG, ring, full_bar, empty_bar, s_abort, s_bad, lane);
         return;
@@ -1335,7 +1354,7 @@ static int launch_mma_cfg(const CUtensorMap& tk, const CUtensorMap& tv, MmaParam
         return fail(CX_ERR_UNSUPPORTED, "paged attention: shared memory too small");
     const size_t smem = C::smem_bytes(p.rows, p.stages);
     CX_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    kern<<<grid, C::THREADS, smem, st>>>(tk, tv, p);
+    kern<<<grid, MOD ? C::THREADS_MOD : C::THREADS, smem, st>>>(tk, tv, p);
     return check_launch("paged_attn_mma_kernel");
 }
 
