@@ -36,6 +36,10 @@ struct F32Cfg {
     static constexpr bool WIDE = RT == 16 || (RT == 8 && D == 128);
     static constexpr int MAX_CONSUMERS = WIDE ? 7 : kConsumerWarps;
     static constexpr int MAX_THREADS = (MAX_CONSUMERS + 1) * 32;
+    // MOD: two producer warps where the registers allow (the 16-bit kernel's reason;
+    // two, since the ring is a multiple of them and of the key slices)
+    static constexpr int PRODUCERS_MOD = WIDE ? 1 : 2;
+    static constexpr int MAX_THREADS_MOD = (MAX_CONSUMERS + PRODUCERS_MOD) * 32;
     static constexpr int RPL = RT / 2;                  // rows per lane in the S phase
     static constexpr int BOX = HG * kBlockTok * 128;    // one 32-column box of HG heads
     static constexpr int NBOX = D / 32;
@@ -69,7 +73,8 @@ struct F32Cfg {
 };
 
 template <int D, int HG, int RT, bool MOD = false>
-__global__ void __launch_bounds__(F32Cfg<D, HG, RT>::MAX_THREADS, 1)
+__global__ void __launch_bounds__(MOD ? F32Cfg<D, HG, RT>::MAX_THREADS_MOD
+                                      : F32Cfg<D, HG, RT>::MAX_THREADS, 1)
     paged_attn_f32_kernel(const __grid_constant__ CUtensorMap tmk,
                           const __grid_constant__ CUtensorMap tmv, const MmaParams p) {
     using C = F32Cfg<D, HG, RT>;
@@ -93,7 +98,8 @@ __global__ void __launch_bounds__(F32Cfg<D, HG, RT>::MAX_THREADS, 1)
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int Hq = p.hq, G = p.group;
-    if (STAGES < 1 || KS < 1 || STAGES % KS != 0 || (int)blockDim.x != (NCW + 1) * 32) {
+    if (STAGES < 1 || KS < 1 || STAGES % KS != 0 ||
+        (MOD && STAGES % C::PRODUCERS_MOD != 0) || (int)blockDim.x != (NCW + (MOD ? C::PRODUCERS_MOD : 1)) * 32) {
         if (tid == 0 && blockIdx.x == 0) raise_flag(CX_DEV_BAD_QLEN);
         return;
     }
@@ -116,7 +122,14 @@ __global__ void __launch_bounds__(F32Cfg<D, HG, RT>::MAX_THREADS, 1)
 
     SegCursorT<MOD> cur;
     cur.init(u0, u1, p);
-    if (warp == NCW) {
+    if constexpr (MOD && C::PRODUCERS_MOD > 1) {
+        if (warp >= NCW) {
+            produce_units<C::NBOX, 32, C::BOX, C::TILES, C::STAGE, MOD, C::PRODUCERS_MOD>(
+                &tmk, &tmv, p, cur, HG, ring, full_bar, empty_bar, s_abort, s_bad, lane,
+                warp - NCW);
+            return;
+        }
+    } else if (warp == NCW) {
         produce_units<C::NBOX, 32, C::BOX, C::TILES, C::STAGE, MOD>(
             &tmk, &tmv, p, cur, HG, ring, full_bar, empty_bar, s_abort, s_bad, lane);
         return;

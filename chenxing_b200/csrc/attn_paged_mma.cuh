@@ -296,7 +296,10 @@ using SegCursor = SegCursorT<false>;
 // stage is re-armed, and before returning the producer waits for its own
 // copies still in flight.
 // ---------------------------------------------------------------------------
-// With NP > 1 producer warps, warp `pw` issues units pw, pw + NP, ...
+// With NP > 1 producer warps, warp `pw` issues units pw, pw + NP, ...; the ring
+// length must be a multiple of NP, so that each stage always has the same
+// producer: a wait on a stage's parity tells its fills apart only for the warp
+// that issued the one before.
 template <int NBOX, int BOX_COLS, int BOX_BYTES, int TILES, int STAGE, bool MOD = false,
           int NP = 1>
 __device__ __forceinline__ void produce_units(const CUtensorMap* tmk, const CUtensorMap* tmv,
@@ -679,13 +682,6 @@ struct MmaCfg {
     static constexpr int KS = (HG * MT >= kConsumerWarps) ? 1 : kConsumerWarps / (HG * MT);
     static constexpr int NCW = HG * MT * KS;           // consumer warps
     static constexpr int THREADS = (NCW + 1) * 32;     // + producer warp
-    // MOD with one or two heads a unit: four producer warps, units in turn.  A unit
-    // is then 4 to 16 KB, and one thread needs about 800 cycles for each, whatever
-    // its boxes (32 long sequences on one KV head of 128, bf16: 162 us; a warp each
-    // for K and V 138, four warps 82).  Three and four row tiles are bound by the
-    // consumers and keep one.
-    static constexpr int PRODUCERS_MOD = HG <= 2 && MT <= 2 ? 4 : 1;
-    static constexpr int THREADS_MOD = (NCW + PRODUCERS_MOD) * 32;
     // Q fragments in shared memory (one 16-byte slot per lane and k-step,
     // reloaded per block) instead of registers: lets 12 consumer warps (13
     // warps, 128 registers a thread) run without spilling, and frees the
@@ -700,6 +696,12 @@ struct MmaCfg {
     static constexpr int HALF_BOX = kBlockTok * 128;   // one head, 16 rows x 128 B
     static constexpr int TILES = HG * kBlockTok * D * 2;  // K (or V) bytes of a unit
     static constexpr int STAGE = 2 * TILES;
+    // MOD with units of up to 16 KB: four producer warps, units in turn.  One thread
+    // needs about 800 cycles for a unit, whatever its boxes (32 long sequences on one
+    // KV head of 128, bf16: 162 us; a warp each for K and V 138, four warps 82).
+    // Three and four row tiles are bound by the consumers and keep one.
+    static constexpr int PRODUCERS_MOD = STAGE <= 16384 && MT <= 2 ? 4 : 1;
+    static constexpr int THREADS_MOD = (NCW + PRODUCERS_MOD) * 32;
     static constexpr int NT = D / 8;     // n-tiles of the output
     static constexpr int KSTEP = D / 16;
     // byte offset of (head hh, token t, dim d [multiple of 8]) inside a K or V
@@ -754,7 +756,8 @@ __global__ void __launch_bounds__(MOD ? MmaCfg<D, MT, HG>::THREADS_MOD
     // A warp taking two units holds the first while it waits for the second
     // (KS units later); the producer can fill that one only if the ring has
     // more than KS stages.
-    if (STAGES < 2 || STAGES % KS != 0 || (C::U == 2 && STAGES < 2 * KS)) {
+    if (STAGES < 2 || STAGES % KS != 0 || (C::U == 2 && STAGES < 2 * KS) ||
+        (MOD && STAGES % C::PRODUCERS_MOD != 0)) {
         if (tid == 0 && blockIdx.x == 0) raise_flag(CX_DEV_BAD_QLEN);
         return;
     }
@@ -1349,6 +1352,10 @@ static int launch_mma_cfg(const CUtensorMap& tk, const CUtensorMap& tv, MmaParam
     using C = MmaCfg<D, MT, HG>;
     auto kern = paged_attn_mma_kernel<D, MT, HG, QT, E, MOD>;
     p.stages = C::stages_for(p.rows);
+    if constexpr (MOD) {                   // (both are powers of two)
+        constexpr int m = C::KS > C::PRODUCERS_MOD ? C::KS : C::PRODUCERS_MOD;
+        p.stages = p.stages / m * m;
+    }
     p.stage_bytes = C::STAGE;
     if (p.stages < 2 || p.stages % C::KS != 0 || (C::U == 2 && p.stages < 2 * C::KS))
         return fail(CX_ERR_UNSUPPORTED, "paged attention: shared memory too small");
@@ -1390,7 +1397,9 @@ static int launch_f32_cfg(const CUtensorMap& tk, const CUtensorMap& tv, MmaParam
     int stg_of[kConsumerWarps + 1] = {};
     int longest = 0;
     for (int ks = 1; ks <= max_ks; ++ks) {
-        stg_of[ks] = (C::raw_stages(p.rows, p.mt, ks) / ks) * ks;
+        // (with two producers, a multiple of 2 as well)
+        const int m = MOD && C::PRODUCERS_MOD == 2 && ks % 2 ? 2 * ks : ks;
+        stg_of[ks] = (C::raw_stages(p.rows, p.mt, ks) / m) * m;
         longest = stg_of[ks] > longest ? stg_of[ks] : longest;
     }
     int best_ks = 0, best_st = 0;
@@ -1406,7 +1415,7 @@ static int launch_f32_cfg(const CUtensorMap& tk, const CUtensorMap& tv, MmaParam
     p.stages = best_st;
     p.stage_bytes = C::STAGE;
     const size_t smem = C::smem_bytes(p.rows, p.mt, p.ks, p.stages);
-    const int threads = (HG * p.mt * p.ks + 1) * 32;
+    const int threads = (HG * p.mt * p.ks + (MOD ? C::PRODUCERS_MOD : 1)) * 32;
     CX_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     kern<<<grid, threads, smem, st>>>(tk, tv, p);
     return check_launch("paged_attn_f32_kernel");

@@ -149,6 +149,23 @@ def test_long_context_is_split_and_joined():
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("hq,hk,d,dtype,q", [
+    (8, 2, 64, BF, 7), (8, 2, 64, F16, 5), (4, 4, 64, BF, 20), (4, 1, 128, BF, 1), (8, 2, 128, F16, 6),
+    (8, 1, 64, BF, 1), (4, 2, 128, F32, 1), (4, 1, 128, F32, 2), (8, 8, 64, F32, 1),
+    (4, 2, 64, F32, 3), (12, 4, 128, F32, 4)])
+def test_rings_that_wrap_many_times(hq, hk, d, dtype, q):
+    """Contexts of several hundred blocks a CTA: every ring length goes round often
+    under all its producer warps (their number divides it), twice the same bits."""
+    ctx = [30000, 33, 9001, 25000]
+    c = _case("plain", hq, ctx, hk=hk, d=d, dtype=dtype, q_lens=None if q == 1 else [q] * 4,
+              softcap=30.0)
+    batch = c.batch()
+    a = c.run(batch, out_dtype=dtype)
+    c.check(a)
+    for _ in range(3):
+        assert torch.equal(a, c.run(batch, out_dtype=dtype))
+
+
 @pytest.mark.parametrize("hq,hk,d,q_lens", [(8, 2, 128, None), (32, 8, 64, [5, 3]),
                                             (8, 2, 128, [64, 100])])
 def test_no_modifier_matches_the_plain_entry_point(hq, hk, d, q_lens):
