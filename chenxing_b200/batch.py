@@ -263,6 +263,8 @@ def _attend_scored(cache, layer: int, q, batch: PagedBatch, out, replan, out_dty
             or not _lib.same_device(out.device, dev):
         raise ValueError(f"out must be a contiguous {out_dtype} tensor of shape {expect} "
                          f"on {dev}")
+    if batch.total_q == 0:               # no query row at all
+        return out
     mods = _lib.CxAttnMods(batch.softcap or 0.0, _lib.cx_dtype(out_dtype),
                            _lib.ptr(batch.alibi_slopes), _lib.ptr(batch.prefix_lens),
                            0 if qt.is_contiguous() else qt.stride(0))

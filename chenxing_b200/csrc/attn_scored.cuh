@@ -193,19 +193,26 @@ static int attend_tc(const cx_pool* pool, int64_t layer, const cx_attn_batch& b,
     p.cap_log2 = m.softcap * 1.4426950408889634f;
     p.neg = scale < 0.f;
     if (m.softcap > 0.f && p.z_scale > 0.f) {
-        // in double: z_scale^9 may be small, but its product with the score is not.
-        // A coefficient below fp32's normal range (caps beyond some thousands) leaves
-        // every score to the other form (s4_max = s5_max = 0).
-        double zk = p.z_scale;
-        const double z2 = (double)p.z_scale * p.z_scale;
-        bool fits = true;
+        // In double: z_scale^9 may be small, but its product with the score is not.
+        // Where a coefficient falls below fp32's normal range (caps beyond some
+        // thousands), |z| <= 0.05, so that what it loses (the z^9 term is below 3e-14
+        // there) does not count; where one is too large (caps below 1e-5) all are 0
+        // and every score but 0 takes the other form.
+        const double z1 = p.z_scale, z2 = z1 * z1;
+        double zk = z1, least = 1, most = 0;
+        for (int i = 0; i < 5; ++i, zk *= z2) {
+            const double c = fabs(p.cap_log2 * kTanh5[i] * zk);
+            least = std::min(least, c);
+            most = std::max(most, c);
+        }
+        zk = most < 1e30 ? z1 : 0;
         for (int i = 0; i < 5; ++i, zk *= z2) {
             p.c5[i] = (float)(p.cap_log2 * kTanh5[i] * zk);
             if (i < 4) p.c4[i] = (float)(p.cap_log2 * kTanh4[i] * zk);
-            fits = fits && fabs(p.cap_log2 * kTanh5[i] * zk) > 1e-36;
         }
-        p.s4_max = fits ? kTanh4Max / p.z_scale : 0.f;
-        p.s5_max = fits ? kTanhMax / p.z_scale : 0.f;
+        const bool small = least < 1e-36;
+        p.s4_max = most >= 1e30 ? 0.f : (small ? 0.05f : kTanh4Max) / p.z_scale;
+        p.s5_max = most >= 1e30 ? 0.f : (small ? 0.05f : kTanhMax) / p.z_scale;
     }
     CUtensorMap tk, tv;
     int rc = make_pool_tmap(&tk, pool->k, pool, 1);

@@ -110,6 +110,44 @@ def test_key_tiles_split_over_ctas(mods, hq, hk, d, dtype, q_lens, ctx):
     assert torch.equal(a, c.run(batch, out_dtype=dtype))
 
 
+@pytest.mark.parametrize("softcap", [3e-6, 1e-3, 0.3, 3e3, 1e5])
+@pytest.mark.parametrize("q_lens", [None, [40, 60]])
+def test_extreme_caps(softcap, q_lens):
+    """Coefficients beyond fp32's range on either side, rows of zero scores."""
+    c = _case("plain", 8, [70, 300], hk=2, d=128, dtype=BF, q_lens=q_lens, softcap=softcap)
+    c.check(c.run(out_dtype=BF))
+    c.q_dev.zero_()
+    c.q.zero_()
+    c.check(c.run(out_dtype=BF))
+
+
+@pytest.mark.parametrize("hq,hk,ctx", [(8, 2, [120000, 300, 80000]), (32, 8, [50000, 300, 20000])])
+def test_wait_timeout_returns_and_flags(hq, hk, ctx):
+    """Pipeline waits that run out (more K and V than L2 holds, a limit of a few
+    ns; four producer warps and one): the call returns with the flag raised, and
+    the next one has the bits of the one before."""
+    from chenxing_b200 import _lib
+    c = _case("cap", hq, ctx, hk=hk, d=128, dtype=BF)
+    batch = c.batch()
+    ref = c.run(batch, out_dtype=BF)
+    lib = _lib.lib()
+    try:
+        lib.cx_set_wait_limit_ns(5)
+        c.run(batch, out_dtype=BF)
+        flags = _lib.device_flags(clear=True)
+    finally:
+        lib.cx_set_wait_limit_ns(0)
+    assert flags & 8, f"expected a wait timeout, flags = {_lib.describe_flags(flags)}"
+    batch.needs_plan = True
+    assert torch.equal(c.run(batch, out_dtype=BF), ref)
+    assert _lib.device_flags(clear=True) == 0
+
+
+def test_no_query_row():
+    c = _case("cap", 8, [70, 300], hk=2, d=64, dtype=BF, q_lens=[0, 0])
+    assert c.run(out_dtype=BF).shape == (0, 8, 64)
+
+
 @pytest.mark.parametrize("q_scale", [1.0, 12.0])
 def test_scores_on_both_sides_of_the_polynomial(q_scale):
     """|z| = |score| / cap below 0.8 for every key, and beyond it for most."""
