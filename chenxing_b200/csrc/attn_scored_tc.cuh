@@ -543,11 +543,14 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
                                     }
                                     e0 = ex2_sfu(e0);
                                     e1 = ex2_sfu(e1);
+                                    // (the sum of what the PV product gets: numerator and
+                                    // denominator round alike)
+                                    const uint32_t u = Half16<E>::pack(e0, e1);
                                     if (k & 1)
-                                        sum1 = f2_add(sum1, f2_of(e0, e1));
+                                        sum1 = f2_add(sum1, Half16<E>::unpack(u));
                                     else
-                                        sum0 = f2_add(sum0, f2_of(e0, e1));
-                                    pk[ch * 16 + k] = Half16<E>::pack(e0, e1);
+                                        sum0 = f2_add(sum0, Half16<E>::unpack(u));
+                                    pk[ch * 16 + k] = u;
                                 }
                                 mt = max3(mt, a0, a1);
                                 if (PLAIN && CAP) largest = max3(largest, n0, n1);

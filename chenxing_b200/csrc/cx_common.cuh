@@ -271,6 +271,7 @@ template <> struct Half16<__nv_bfloat16> {
     // How far a row maximum may outgrow its softmax reference (base 2) before the
     // reference follows: 2^x of that still fits the type (and the fp32 sums).
     static constexpr float kGrowLog2 = 60.f;
+    static constexpr uint32_t kOnes = 0x3f803f80u;   // a pair of ones
     __device__ __forceinline__ static uint32_t pack(float lo, float hi) { return pack_bf16(lo, hi); }
     __device__ __forceinline__ static f2 unpack(uint32_t u) {
         return f2_of(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
@@ -282,6 +283,7 @@ template <> struct Half16<__nv_bfloat16> {
 };
 template <> struct Half16<__half> {
     static constexpr float kGrowLog2 = 15.f;
+    static constexpr uint32_t kOnes = 0x3c003c00u;
     __device__ __forceinline__ static uint32_t pack(float lo, float hi) {
         const __half2 v = __floats2half2_rn(lo, hi);
         return *reinterpret_cast<const uint32_t*>(&v);
