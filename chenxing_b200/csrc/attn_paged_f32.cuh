@@ -103,6 +103,9 @@ __global__ void __launch_bounds__(MOD ? F32Cfg<D, HG, RT>::MAX_THREADS_MOD
         if (tid == 0 && blockIdx.x == 0) raise_flag(CX_DEV_BAD_QLEN);
         return;
     }
+    if constexpr (MOD) {
+        if (p.mod.join_min) asm volatile("griddepcontrol.launch_dependents;");
+    }
     if (!plan_ok_zero_empty<D, MOD>(p)) return;
     const int W = p.plan[0], chunk = p.plan[1], P_eff = p.plan[2];
     if ((int)blockIdx.x >= P_eff) return;

@@ -84,6 +84,8 @@ struct ScoreMod {
     int64_t q_stride;        // elements between query tokens
     void* out;
     int32_t out_dtype, q_dtype;
+    int32_t join_min;        // ranges cut into more partials are joined by paged_join_kernel;
+                             // 0: none
 };
 
 struct MmaParams {
@@ -473,6 +475,12 @@ __device__ __forceinline__ void ks_merge(const MmaParams& p, const float* merge,
     }
 }
 
+// First chunk that holds part of range (b, g), and how many do.
+__device__ __forceinline__ int2 range_chunks(const MmaParams& p, int b, int g, int nb, int chunk) {
+    const int first = p.seq_start[b] + g * nb, pf = first / chunk;
+    return make_int2(pf, (first + nb - 1) / chunk - pf + 1);
+}
+
 // A range cut by a chunk boundary: every CTA holding part of it takes an
 // atomic ticket after writing its slot; the last one merges all partials of
 // the range in one pass (log-sum-exp) and writes the final rows.  No waiting.
@@ -480,6 +488,9 @@ template <int D, int HG, bool MOD = false>
 __device__ __forceinline__ void ticket_merge(const MmaParams& p, const Seg& seg, int b,
                                              int64_t qs, int rows_b, int ctid, int NCT,
                                              int chunk, int* s_last) {
+    if constexpr (MOD) {                 // left to paged_join_kernel
+        if (p.mod.join_min && range_chunks(p, b, seg.g, seg.nb, chunk).y > p.mod.join_min) return;
+    }
     const int G = p.group, Hq = p.hq;
     const int bg = b * p.n_groups + seg.g;
     const size_t slot_floats = (size_t)HG * p.rows * (D + 2);
@@ -627,6 +638,105 @@ __device__ __forceinline__ bool plan_ok_zero_empty(const MmaParams& p) {
     return true;
 }
 
+// Joins the partials of the ranges that ticket_merge leaves (MOD): one CTA per
+// (range, row), its warps take every eighth partial.  The last CTA of a range alone
+// joins it at some 16 GB/s (a row's partials are round trips to L2, and a warp has
+// rows to take one after the other): 473 of the 505 us of one chain of 6 rows over
+// 15,000 bf16 keys, 16 query heads over 4, which takes 34 us with this kernel, and a
+// single token over 60,000 keys 39 instead of 110.
+template <int D>
+__global__ void __launch_bounds__(256) paged_join_kernel(const MmaParams p) {
+    __shared__ float s_o[8][D], s_m[8], s_l[8];
+    // (launched while the split kernel's last CTAs still run: 2 us less a call)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (p.plan[3] != kPlanMagic || p.plan[4] != p.batch || p.plan[5] != p.n_groups) return;
+    // A range in more than join_min chunks has join_min - 1 or more whole ones, so that
+    // one of them is a multiple of that: the CTAs of the first such find the range.
+    const int step = p.mod.join_min - 1, c = ((int)blockIdx.x + 1) * step, chunk = p.plan[1];
+    if (c >= p.plan[2]) return;
+    int b = 0, hi = p.batch - 1;         // largest b with seq_start[b] <= the chunk's start
+    while (b < hi) {
+        const int mid = (b + hi + 1) >> 1;
+        if (p.seq_start[mid] <= c * chunk) b = mid; else hi = mid - 1;
+    }
+    const int nb = (p.seq_start[b + 1] - p.seq_start[b]) / p.n_groups;
+    if (nb == 0) return;
+    const int g = (c * chunk - p.seq_start[b]) / nb, bg = b * p.n_groups + g;
+    const int2 ch = range_chunks(p, b, g, nb, chunk);
+    const int n = ch.y, G = p.group;
+    if (n <= p.mod.join_min || c != (ch.x / step + 1) * step) return;
+    const int sq = p.q_start ? min(max(p.q_start[b + 1] - p.q_start[b], 0), p.max_q) : 1;
+    const int64_t qs = p.q_start ? p.q_start[b] : b;
+    const int eh = blockIdx.y / p.rows, R = blockIdx.y - eh * p.rows;
+    if (R >= G * sq) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const size_t slot_floats = (size_t)p.hg * p.rows * (D + 2);
+    const float* row = p.partials + (size_t)(ch.x + bg) * slot_floats +
+                       ((size_t)eh * p.rows + R) * (D + 2);
+    float M = -INFINITY, L = 0.f, o[D / 32];
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) o[k] = 0.f;
+    for (int s0 = warp; s0 < n; s0 += 8 * 32) {
+        // lane i: reference and denominator of partial s0 + 8 i
+        const int np = min(32, (n - s0 + 7) / 8);
+        const float* r = row + (size_t)(s0 + 8 * lane) * slot_floats;
+        const float m = lane < np ? __ldcg(r + D) : -INFINITY;
+        const float l = lane < np ? __ldcg(r + D + 1) : 0.f;
+        float Mn = m;
+#pragma unroll
+        for (int s2 = 16; s2; s2 >>= 1) Mn = fmaxf(Mn, __shfl_xor_sync(0xffffffffu, Mn, s2));
+        Mn = fmaxf(Mn, M);
+        // (a partial that saw no key: weight 0, its columns are 0)
+        const float base = Mn == -INFINITY ? 0.f : Mn;
+        const float a = exp2f(M - base), w = exp2f(m - base);
+        float ls = l * w;
+#pragma unroll
+        for (int s2 = 16; s2; s2 >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, s2);
+        L = L * a + ls;
+        M = Mn;
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) o[k] *= a;
+#pragma unroll 8
+        for (int i = 0; i < np; ++i) {
+            const float* c = row + (size_t)(s0 + 8 * i) * slot_floats + 2 * lane;
+            const float wi = __shfl_sync(0xffffffffu, w, i);
+#pragma unroll
+            for (int k = 0; k < D / 64; ++k) {
+                const float2 v = __ldcg(reinterpret_cast<const float2*>(c + k * 64));
+                o[2 * k] = fmaf(v.x, wi, o[2 * k]);
+                o[2 * k + 1] = fmaf(v.y, wi, o[2 * k + 1]);
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < D / 64; ++k)
+        *reinterpret_cast<float2*>(&s_o[warp][k * 64 + 2 * lane]) =
+            make_float2(o[2 * k], o[2 * k + 1]);
+    if (lane == 0) {
+        s_m[warp] = M;
+        s_l[warp] = L;
+    }
+    __syncthreads();
+    const int d = 2 * threadIdx.x;
+    if (d >= D) return;
+    M = s_m[0];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) M = fmaxf(M, s_m[w]);
+    const float base = M == -INFINITY ? 0.f : M;
+    float x = 0.f, y = 0.f;
+    L = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+        const float wgt = exp2f(s_m[w] - base);
+        L += s_l[w] * wgt;
+        x += s_o[w][d] * wgt;
+        y += s_o[w][d + 1] * wgt;
+    }
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const int64_t orow = (qs + R / G) * p.hq + (int64_t)(g * p.hg + eh) * G + R % G;
+    put2<true>(p, orow * D + d, x * inv, y * inv);
+}
+
 template <typename QT> struct QLoad;
 template <> struct QLoad<float> {
     __device__ __forceinline__ static float2 two(const float* q, int64_t i) {
@@ -762,6 +872,9 @@ __global__ void __launch_bounds__(MOD ? MmaCfg<D, MT, HG>::THREADS_MOD
         return;
     }
 
+    if constexpr (MOD) {
+        if (p.mod.join_min) asm volatile("griddepcontrol.launch_dependents;");
+    }
     if (!plan_ok_zero_empty<D, MOD>(p)) return;
     const int W = p.plan[0], chunk = p.plan[1], P_eff = p.plan[2];
     if ((int)blockIdx.x >= P_eff) return;

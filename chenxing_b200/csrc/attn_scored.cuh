@@ -139,21 +139,48 @@ static int attend_split(const cx_pool* pool, int64_t layer, const cx_attn_batch&
     rc = make_pool_tmap(&tv, pool->v, pool, sh.hg);
     if (rc) return rc;
     const bool d128 = pool->head_dim == 128;
+    // Ranges cut into many partials are joined by a launch of their own where that
+    // pays: with few ranges each is cut often (one chain of 6 rows over 15,000 bf16 keys
+    // 505 -> 34 us, 8 fp32 chains of 4 over 600 48 -> 37; a call whose ranges are cut
+    // less pays 2 us).  Chains of 16-bit types have many rows to join, so that one long
+    // sequence among many short ones pays too: 128 chains of 5, one over 40,000 keys
+    // and the rest over 400, 227 -> 150 us, against 4 us more for 128 even ones (173 ->
+    // 178).  Single tokens and fp32 gain nothing there (141 -> 147 us).
+    if (2 * b.batch * sh.n_groups <= grid)
+        p.mod.join_min = 4;
+    else if (b.max_q_len > 1 && pool->dtype != CX_F32)
+        p.mod.join_min = 16;
     switch (pool->dtype) {
         case CX_F32:
-            return d128 ? launch_f32_d<128, true>(sh, tk, tv, p, st, grid)
-                        : launch_f32_d<64, true>(sh, tk, tv, p, st, grid);
+            rc = d128 ? launch_f32_d<128, true>(sh, tk, tv, p, st, grid)
+                      : launch_f32_d<64, true>(sh, tk, tv, p, st, grid);
+            break;
         case CX_BF16: {
             using E = __nv_bfloat16;
-            return d128 ? launch_mma_d<128, E, E, true>(sh, tk, tv, p, st, grid)
-                        : launch_mma_d<64, E, E, true>(sh, tk, tv, p, st, grid);
+            rc = d128 ? launch_mma_d<128, E, E, true>(sh, tk, tv, p, st, grid)
+                      : launch_mma_d<64, E, E, true>(sh, tk, tv, p, st, grid);
+            break;
         }
         default: {
             using E = __half;
-            return d128 ? launch_mma_d<128, E, E, true>(sh, tk, tv, p, st, grid)
-                        : launch_mma_d<64, E, E, true>(sh, tk, tv, p, st, grid);
+            rc = d128 ? launch_mma_d<128, E, E, true>(sh, tk, tv, p, st, grid)
+                      : launch_mma_d<64, E, E, true>(sh, tk, tv, p, st, grid);
         }
     }
+    if (rc || !p.mod.join_min) return rc;
+    const dim3 jg((grid - 1) / (p.mod.join_min - 1), sh.hg * p.rows);
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = jg;
+    cfg.blockDim = 256;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    CX_CUDA_CHECK(cudaLaunchKernelEx(&cfg, d128 ? paged_join_kernel<128> : paged_join_kernel<64>,
+                                     p));
+    return check_launch("paged_join_kernel");
 }
 
 // The tcgen05 kernel (attn_scored_tc.cuh).

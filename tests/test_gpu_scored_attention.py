@@ -204,6 +204,26 @@ def test_rings_that_wrap_many_times(hq, hk, d, dtype, q):
         assert torch.equal(a, c.run(batch, out_dtype=dtype))
 
 
+@pytest.mark.parametrize("mods", ["cap-alibi-window", "window-prefix-cap", "prefix", "alibi"])
+@pytest.mark.parametrize("hq,hk,d,dtype,ctx,q_lens", [
+    (16, 4, 128, BF, [6000], [6]),                          # one range over every CTA
+    (8, 8, 64, F16, [40, 4000, 0, 900], None),              # two head groups, an empty sequence
+    (4, 2, 128, F32, [33, 5000, 20], [2, 3, 0]),
+    (3, 1, 64, F32, [2500], None),
+    (8, 4, 64, F16, [40] * 40 + [9000] + [25] * 39, [3] * 80),   # more ranges than half the CTAs
+    (8, 1, 128, BF, [9000, 7000] + [70] * 98, [5, 1] + [2] * 98),
+])
+def test_ranges_cut_into_many_partials(mods, hq, hk, d, dtype, ctx, q_lens):
+    c = _case(mods, hq, ctx, q_lens=q_lens, hk=hk, d=d, dtype=dtype, seed=11)
+    batch = c.batch()
+    a = c.run(batch, out_dtype=dtype)
+    c.check(a)
+    b = a.clone().fill_(float("nan"))
+    for _ in range(2):
+        c.run(batch, out=b)
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("hq,hk,d,q_lens", [(8, 2, 128, None), (32, 8, 64, [5, 3]),
                                             (8, 2, 128, [64, 100])])
 def test_no_modifier_matches_the_plain_entry_point(hq, hk, d, q_lens):
