@@ -657,8 +657,11 @@ static int try_norm_rope_vec(const NormRopeParams& p, cudaStream_t st, bool stag
         // CTAs an SM holds by shared memory and by registers (at most 72 a thread)
         const int64_t per_sm =
             std::min<int64_t>(std::min(16, 65536 / (72 * threads)), 224 * 1024 / (smem + 1536));
+        // (V rows leave the stage in chunks of 2 V elements, 16 bytes at a time)
+        const bool v_off = (reinterpret_cast<uintptr_t>(p.vp) & 15) != 0;
         if (staged && D * s % 16 == 0 && rot % 4 == 0 && per_sm >= 2 && !not_bulk(p, s) &&
-            R * D * s >= 4096 && T * R * D * s >= (14ll << 20) && T >= 3ll * num_sms()) {
+            !v_off && R * D * s >= 4096 && T * R * D * s >= (14ll << 20) &&
+            T >= 3ll * num_sms()) {
             *done = true;
             auto kern = kv_append_norm_rope_tok_kernel<S, O, V>;
             CX_CUDA_CHECK(cudaFuncSetAttribute(

@@ -1,0 +1,43 @@
+"""Calls at the edges of the normalised append's and the scored attention's
+documented ranges (definitions and bounds: test_gpu_norm_rope, scored_cases)."""
+import pytest
+import torch
+
+from test_gpu_norm_rope import Rows
+
+pytestmark = pytest.mark.gpu
+BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(autouse=True)
+def _clean_flags():
+    from chenxing_b200 import _lib
+    _lib.device_flags(clear=True)
+    yield
+    flags = _lib.device_flags(clear=True)
+    assert flags == 0, f"device error flags raised: {_lib.describe_flags(flags)}"
+
+
+@pytest.mark.parametrize("off_k,off_v", [(0, 8), (8, 8), (8, 0)])
+@pytest.mark.parametrize("dtype,pool", [(BF, BF), (F32, F16)])
+def test_append_of_much_data_into_pools_off_16_bytes(off_k, off_v, dtype, pool):
+    """A pool of the caller's own (C interface) may start at any element."""
+    r = Rows(2100, 24, 8, 96, 96, dtype=dtype, pool=pool, seed=off_k + off_v)
+    pool_c, cache = r.cache._pool, r.cache
+    at = pool_c.k, pool_c.v
+    moved = []
+    try:
+        for name, off in (("k", off_k), ("v", off_v)):
+            was = getattr(cache, "_" + name)
+            buf = torch.zeros(was.numel() + 8, dtype=pool, device="cuda")
+            assert buf.data_ptr() % 16 == 0
+            part = buf[off // 2:][:was.numel()].view_as(was)
+            part.copy_(was)
+            setattr(pool_c, name, part.data_ptr())
+            moved.append((was, part, buf))
+        out = r.call(q_out_dtype=pool)
+        for was, part, _ in moved:
+            was.copy_(part)
+    finally:
+        pool_c.k, pool_c.v = at
+    r.check(out)
