@@ -566,8 +566,10 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
                     bool large = false;
                     if (plain) {
                         if (CAP) large = __any_sync(0xffffffffu, largest > p.s4_max);
+                        // (beyond its range the polynomial may be far above the cap: no
+                        // maximum of such scores becomes a reference)
                         if (ALIBI)
-                            mt += m_use;
+                            mt = large ? -INFINITY : mt + m_use;
                         else
                             mt = CAP ? cap_any(mt * p.z_scale, cl) : mt * p.scale_log2;
                     }

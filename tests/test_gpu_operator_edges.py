@@ -3,6 +3,7 @@ documented ranges (definitions and bounds: test_gpu_norm_rope, scored_cases)."""
 import pytest
 import torch
 
+from scored_cases import ScoredCase, alibi
 from test_gpu_norm_rope import Rows
 
 pytestmark = pytest.mark.gpu
@@ -41,3 +42,14 @@ def test_append_of_much_data_into_pools_off_16_bytes(off_k, off_v, dtype, pool):
     finally:
         pool_c.k, pool_c.v = at
     r.check(out)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("softcap,q_scale", [(10.0, 12.0), (30.0, 25.0)])
+def test_biased_scores_far_beyond_the_cap(softcap, q_scale, dtype):
+    """Raw scores of several caps on either side, with a distance bias, on tiles
+    that every row sees: the reference maximum follows capped scores only."""
+    c = ScoredCase(hq=8, hk=2, d=128, ctx=[900, 700, 333], q_lens=[64, 90, 40], dtype=dtype,
+                   softcap=softcap, slopes=alibi(8), q_scale=q_scale, seed=4)
+    assert c.batch().kernel_kind(dtype) == "tcgen05"
+    c.check(c.run(out_dtype=dtype))
