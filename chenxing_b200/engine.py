@@ -287,7 +287,7 @@ class BatchedKVEngine:
         plan.appended.add(int(layer))
 
     def append_rope(self, plan: StepPlan, layer: int, k, v, rope, q=None,
-                    q_out_dtype=torch.bfloat16, *, q_weight=None, k_weight=None,
+                    q_out_dtype=None, *, q_weight=None, k_weight=None,
                     eps: float = 1e-6):
         """``append`` with RoPE fused in: K rotated at each token's absolute
         position (its sequence's committed length + index in the step), V
@@ -295,7 +295,9 @@ class BatchedKVEngine:
         The plan's copy-on-write copies run once, for every layer, before the
         first such call.  With ``q_weight`` / ``k_weight``, or tables of part
         of the head, the heads are RMS-normed and rotated by
-        ``cache.append_norm_rope``."""
+        ``cache.append_norm_rope``.  Q is returned as bfloat16 from the plain
+        rotation and, from the other, in the pool's type, which the attention
+        over it takes as it is; ``q_out_dtype`` says otherwise."""
         if plan.cow_host and not plan.cow_done:
             for src, dst, n in plan.cow_host:          # all layers at once
                 if n > 0:
@@ -309,10 +311,10 @@ class BatchedKVEngine:
         if q_weight is not None or k_weight is not None or rope.head_dim != self.cache.head_dim:
             qo = self.cache.append_norm_rope(layer, k, v, plan.slots, plan.positions, rope, q,
                                              q_weight=q_weight, k_weight=k_weight, eps=eps,
-                                             q_out_dtype=q_out_dtype)
+                                             q_out_dtype=q_out_dtype or self.cache.torch_dtype)
         else:
             qo = self.cache.append_rope(layer, k, v, plan.slots, plan.positions, rope, q,
-                                        q_out_dtype)
+                                        q_out_dtype or torch.bfloat16)
         plan.appended.add(int(layer))
         return qo
 

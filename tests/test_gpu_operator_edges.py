@@ -53,3 +53,39 @@ def test_biased_scores_far_beyond_the_cap(softcap, q_scale, dtype):
                    softcap=softcap, slopes=alibi(8), q_scale=q_scale, seed=4)
     assert c.batch().kernel_kind(dtype) == "tcgen05"
     c.check(c.run(out_dtype=dtype))
+
+
+@pytest.mark.parametrize("dtype,rows,kinds", [
+    (BF, BF, ("mma", "tcgen05")), (F16, F16, ("mma", "tcgen05")), (F32, F32, ("fma", "generic")),
+    (BF, F32, ("mma", "tcgen05")), (F16, BF, ("mma", "tcgen05"))])
+def test_engine_step_keeps_the_pools_type(dtype, rows, kinds):
+    """Norms, append and attention over bf16, fp16 and fp32 pools: Q comes in the
+    pool's type, and the pool's kernel attends."""
+    from chenxing_b200 import BatchedKVEngine, RadixPagedKVCache, RopeTables
+    hq, hk, d, cap = 8, 2, 64, 15.0
+    cache = RadixPagedKVCache(64, 16, 1, hk, d, dtype=dtype, host_io=False)
+    eng = BatchedKVEngine(cache, n_q_heads=hq, softcap=cap)
+    rope = RopeTables(512, d)
+    gen = torch.Generator().manual_seed(6)
+    lens = [70, 33]
+    for i, n in enumerate(lens):
+        eng.add(i, list(range(1000 * i, 1000 * i + n)))
+    w = (1 + 0.2 * torch.randn(2, d, generator=gen)).to(rows).cuda()
+    for q_lens, kind in ((lens, kinds[1]), ([1, 1], kinds[0])):
+        plan = eng.plan([0, 1], q_lens)
+        x = torch.randn(sum(q_lens), hq + 2 * hk, d, generator=gen).to(rows).cuda()
+        q = eng.append_rope(plan, 0, x[:, hq:hq + hk], x[:, hq + hk:], rope, x[:, :hq],
+                            q_weight=w[0], k_weight=w[1])
+        assert q.dtype == dtype
+        assert plan.batch.kernel_kind(q.dtype) == kind
+        out = eng.attend(plan, 0, q, out_dtype=dtype)
+        c = object.__new__(ScoredCase)
+        c.hq, c.hk, c.d, c.dtype, c.q_dtype = hq, hk, d, dtype, dtype
+        c.softcap, c.window, c.slopes, c.prefix = cap, None, None, None
+        c.scale, c.q, c.q_lens = d ** -0.5, q.double().cpu(), q_lens
+        c.ctx = [int(s.n_tokens + n) for s, n in zip(plan.seqs, q_lens)]
+        kv = [cache.read_layer(s.block_table, n, 0) for s, n in zip(plan.seqs, c.ctx)]
+        c.k = [a.double().cpu() for a, _ in kv]
+        c.v = [b.double().cpu() for _, b in kv]
+        c.check(out)
+        eng.commit(plan)

@@ -1,0 +1,41 @@
+"""What the engine and the batch pass on to the normalised append and the scored
+attention, and what they refuse: host logic only (no GPU needed)."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from chenxing_b200 import BatchedKVEngine
+
+
+class CallsOnly:
+    """Stands in for a cache: notes which append an engine makes, and how."""
+
+    head_dim, torch_dtype = 64, torch.float16
+
+    def append_rope(self, layer, k, v, slots, positions, rope, q, q_out_dtype):
+        self.last = "append_rope", q_out_dtype
+
+    def append_norm_rope(self, layer, k, v, slots, positions, rope, q, *, q_weight, k_weight, eps,
+                         q_out_dtype):
+        self.last = "append_norm_rope", q_out_dtype
+
+
+def append(rot=64, **kw):
+    eng = object.__new__(BatchedKVEngine)
+    eng.cache = CallsOnly()
+    plan = SimpleNamespace(cow_host=[], cow_done=False, positions=torch.zeros(1), slots=None,
+                           appended=set())
+    eng.append_rope(plan, 0, None, None, SimpleNamespace(head_dim=rot), None, **kw)
+    return eng.cache.last
+
+
+@pytest.mark.parametrize("kw,want", [
+    (dict(), ("append_rope", torch.bfloat16)),
+    (dict(q_out_dtype=torch.float32), ("append_rope", torch.float32)),
+    (dict(q_weight=1), ("append_norm_rope", torch.float16)),    # the pool's type
+    (dict(k_weight=1), ("append_norm_rope", torch.float16)),
+    (dict(q_weight=1, rot=32), ("append_norm_rope", torch.float16)),
+    (dict(k_weight=1, q_out_dtype=torch.float32), ("append_norm_rope", torch.float32))])
+def test_engine_query_type(kw, want):
+    assert append(**kw) == want
