@@ -288,16 +288,19 @@ class BatchedKVEngine:
 
     def append_rope(self, plan: StepPlan, layer: int, k, v, rope, q=None,
                     q_out_dtype=None, *, q_weight=None, k_weight=None,
-                    eps: float = 1e-6):
+                    eps: float = 1e-6, rot_dim: int | None = None):
         """``append`` with RoPE fused in: K rotated at each token's absolute
         position (its sequence's committed length + index in the step), V
         copied, and Q rotated into the returned tensor (transformer.py:84-87).
         The plan's copy-on-write copies run once, for every layer, before the
-        first such call.  With ``q_weight`` / ``k_weight``, or tables of part
-        of the head, the heads are RMS-normed and rotated by
-        ``cache.append_norm_rope``.  Q is returned as bfloat16 from the plain
+        first such call.  With ``q_weight`` / ``k_weight`` the heads are
+        RMS-normed and rotated, by as many leading dims as the tables have, by
+        ``cache.append_norm_rope``; without weights, tables of part of the head
+        are refused unless ``rot_dim`` says that they are meant.  Q is returned as bfloat16 from the plain
         rotation and, from the other, in the pool's type, which the attention
         over it takes as it is; ``q_out_dtype`` says otherwise."""
+        if rot_dim is not None and rot_dim != rope.head_dim:
+            raise ValueError(f"rot_dim {rot_dim} with RoPE tables of {rope.head_dim} dims")
         if plan.cow_host and not plan.cow_done:
             for src, dst, n in plan.cow_host:          # all layers at once
                 if n > 0:
@@ -308,7 +311,7 @@ class BatchedKVEngine:
                                   for n0, n in zip(plan.n_past, plan.q_lens)]) \
                 if len(plan.q_lens) else np.zeros(0, dtype=np.int64)
             plan.positions = upload(pos, self.cache.device)
-        if q_weight is not None or k_weight is not None or rope.head_dim != self.cache.head_dim:
+        if q_weight is not None or k_weight is not None or rot_dim is not None:
             qo = self.cache.append_norm_rope(layer, k, v, plan.slots, plan.positions, rope, q,
                                              q_weight=q_weight, k_weight=k_weight, eps=eps,
                                              q_out_dtype=q_out_dtype or self.cache.torch_dtype)

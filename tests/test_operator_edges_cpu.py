@@ -14,6 +14,8 @@ class CallsOnly:
     head_dim, torch_dtype = 64, torch.float16
 
     def append_rope(self, layer, k, v, slots, positions, rope, q, q_out_dtype):
+        if rope.head_dim != self.head_dim:
+            raise ValueError("RoPE tables were built for another head_dim")
         self.last = "append_rope", q_out_dtype
 
     def append_norm_rope(self, layer, k, v, slots, positions, rope, q, *, q_weight, k_weight, eps,
@@ -39,3 +41,14 @@ def append(rot=64, **kw):
     (dict(k_weight=1, q_out_dtype=torch.float32), ("append_norm_rope", torch.float32))])
 def test_engine_query_type(kw, want):
     assert append(**kw) == want
+
+
+def test_engine_refuses_narrow_tables_unless_they_are_meant():
+    with pytest.raises(ValueError):
+        append(rot=32)
+    with pytest.raises(ValueError):
+        append(rot=32, rot_dim=16)
+    with pytest.raises(ValueError):
+        append(rot=32, rot_dim=16, q_weight=1)
+    assert append(rot=32, rot_dim=32)[0] == "append_norm_rope"
+    assert append(rot=64, rot_dim=64)[0] == "append_norm_rope"
