@@ -243,8 +243,15 @@ def _attend(cache, layer: int, q, batch: PagedBatch, out, replan, out_dtype, fn_
 
 def _plans(batch: PagedBatch, replan, by: str) -> bool:
     """Whether this call makes the plan: as asked, or when the batch was
-    (re)loaded or its plan is the other entry point's."""
-    return batch.needs_plan or batch._planned_by != by if replan is None else bool(replan)
+    (re)loaded or its plan is the other entry point's (which serves no call
+    of this one)."""
+    if replan is None:
+        return batch.needs_plan or batch._planned_by != by
+    if not replan and batch._planned_by not in (None, by):
+        raise ValueError("replan=False, but the batch's plan is that of calls "
+                         f"{'with' if by == 'plain' else 'without'} score modifiers or a "
+                         "16-bit output")
+    return bool(replan)
 
 
 def _attend_scored(cache, layer: int, q, batch: PagedBatch, out, replan, out_dtype):

@@ -109,7 +109,15 @@ struct MmaParams {
     int32_t* counters;   // [batch * n_groups] merge tickets, zero between calls
     float* partials;     // [(P + batch*n_groups)][hg][rows][D + 2]
     ScoreMod mod;        // MOD instantiations (and the plan: prefix blocks)
+    int32_t plan_kind;   // 0: cx_paged_decode / _verify; cx_paged_attend: 1, with a prefix 3
 };
+
+// Whether the workspace holds a plan of this call's shape, window and entry point
+// (a plan without the prefix lacks units, and so on).
+__device__ __forceinline__ bool plan_serves(const MmaParams& p) {
+    return p.plan[3] == kPlanMagic && p.plan[4] == p.batch && p.plan[5] == p.n_groups &&
+           p.plan[6] == p.window && p.plan[7] == p.plan_kind;
+}
 
 // Keys of sequence b that every query row sees (MOD with a prefix), at most ctx.
 __device__ __forceinline__ int prefix_of(const MmaParams& p, int b, int ctx) {
@@ -216,6 +224,8 @@ static __global__ void __launch_bounds__(1024) paged_plan_kernel(MmaParams p, in
         p.plan[2] = W > 0 ? (int)((W + chunk - 1) / chunk) : 0;
         p.plan[4] = B;
         p.plan[5] = p.n_groups;
+        p.plan[6] = p.window;
+        p.plan[7] = p.plan_kind;
         __threadfence();
         p.plan[3] = kPlanMagic;
     }
@@ -618,13 +628,13 @@ __device__ __forceinline__ void ticket_merge(const MmaParams& p, const Seg& seg,
     if (ctid == 0) p.counters[bg] = 0;
 }
 
-// The plan must come from paged_plan_kernel for this batch shape (else the
+// The plan must come from paged_plan_kernel for this call (plan_serves; else the
 // flag is raised and the CTA returns false); sequences with no cached token
 // get zero rows (naive_attention semantics for rows with no key).
 template <int D, bool MOD = false>
 __device__ __forceinline__ bool plan_ok_zero_empty(const MmaParams& p) {
     const int B = p.batch, Hq = p.hq, tid = threadIdx.x;
-    if (p.plan[3] != kPlanMagic || p.plan[4] != B || p.plan[5] != p.n_groups) {
+    if (!plan_serves(p)) {
         if (tid == 0 && blockIdx.x == 0) raise_flag(CX_DEV_BAD_QLEN);
         return false;
     }
@@ -649,7 +659,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const MmaParams p) {
     __shared__ float s_o[8][D], s_m[8], s_l[8];
     // (launched while the split kernel's last CTAs still run: 2 us less a call)
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (p.plan[3] != kPlanMagic || p.plan[4] != p.batch || p.plan[5] != p.n_groups) return;
+    if (!plan_serves(p)) return;
     // A range in more than join_min chunks has join_min - 1 or more whole ones, so that
     // one of them is a multiple of that: the CTAs of the first such find the range.
     const int step = p.mod.join_min - 1, c = ((int)blockIdx.x + 1) * step, chunk = p.plan[1];

@@ -117,6 +117,7 @@ static int attend_split(const cx_pool* pool, int64_t layer, const cx_attn_batch&
     p.partials = reinterpret_cast<float*>(w + wl.part);
     p.mod.slopes = m.alibi_slopes;
     p.mod.prefix = m.prefix_lens;
+    p.plan_kind = m.prefix_lens ? 3 : 1;
     p.mod.q_stride = m.q_stride;
     p.mod.out = out;
     p.mod.out_dtype = m.out_dtype;

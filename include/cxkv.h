@@ -300,7 +300,9 @@ typedef struct cx_attn_mods {
  * reach the result, NaN and infinity included; at a position that only some
  * rows see, V must be finite.  Workspace: cx_paged_attend_workspace_bytes,
  * zero-filled once; a plan made by cx_paged_decode / cx_paged_verify does not
- * serve this call, nor the other way round. */
+ * serve this call, nor the other way round, nor one for another window or made
+ * without the prefix (replan = 0 then raises CX_DEV_BAD_QLEN and leaves out as
+ * it was). */
 int cx_paged_attend(const cx_pool* pool, int64_t layer, const cx_attn_batch* batch,
                     const cx_attn_mods* mods, const void* q, int32_t q_dtype, void* out,
                     void* workspace, size_t workspace_bytes, int32_t replan, void* stream);

@@ -89,3 +89,41 @@ def test_engine_step_keeps_the_pools_type(dtype, rows, kinds):
         c.v = [b.double().cpu() for _, b in kv]
         c.check(out)
         eng.commit(plan)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_a_plan_of_another_call_is_refused_on_the_device(dtype):
+    """A plan of cx_paged_decode, of another window or without the prefix, given
+    to cx_paged_attend with replan = 0 (the C interface does not see whose it is)."""
+    from chenxing_b200 import _lib
+    c = ScoredCase(hq=8, hk=2, d=64, ctx=[700, 333], dtype=dtype, window=100, prefix=[40, 60],
+                   poison=False)
+    batch = c.batch()
+
+    def left(plan, out_dtype):
+        """Makes `batch` plan as ``plan`` says, then calls it without a plan."""
+        good, kept = batch._c, batch.prefix_lens
+        plan()
+        batch._c, batch.prefix_lens, batch._planned_by = good, kept, None
+        out = torch.full((2, 8, 64), 7.0, dtype=out_dtype, device="cuda")
+        c.run(batch, out=out, out_dtype=out_dtype, replan=False)
+        flags = _lib.device_flags(clear=True)
+        return flags, bool((out == 7).all())
+
+    def plain():
+        batch.prefix_lens = None
+        c.run(batch, out_dtype=F32, replan=True)
+
+    def no_prefix():
+        batch.prefix_lens = None
+        c.run(batch, out_dtype=BF, replan=True)
+
+    def other_window():
+        batch._c = _lib.CxAttnBatch.from_buffer_copy(batch._c)
+        batch._c.window = 50
+        c.run(batch, out_dtype=BF, replan=True)
+
+    for plan in (plain, no_prefix, other_window):
+        assert left(plan, BF) == (16, True), plan.__name__
+    batch.needs_plan = True
+    c.check(c.run(batch, out_dtype=dtype))

@@ -52,3 +52,17 @@ def test_engine_refuses_narrow_tables_unless_they_are_meant():
         append(rot=32, rot_dim=16, q_weight=1)
     assert append(rot=32, rot_dim=32)[0] == "append_norm_rope"
     assert append(rot=64, rot_dim=64)[0] == "append_norm_rope"
+
+
+def test_replan_false_needs_a_plan_of_the_same_entry_point():
+    from chenxing_b200.batch import _plans
+    b = SimpleNamespace(needs_plan=False, _planned_by="plain")
+    assert not _plans(b, None, "plain") and _plans(b, None, "scored")
+    assert not _plans(b, False, "plain") and _plans(b, True, "scored")
+    with pytest.raises(ValueError):
+        _plans(b, False, "scored")
+    b._planned_by = "scored"
+    with pytest.raises(ValueError):
+        _plans(b, False, "plain")
+    b._planned_by = None                     # never planned here: the device checks
+    assert not _plans(b, False, "plain")
