@@ -1193,7 +1193,8 @@ __global__ void __launch_bounds__(MOD ? MmaCfg<D, MT, HG>::THREADS_MOD
                 constexpr float kGrow = MOD ? Half16<E>::kGrowLog2 : kMmaRescaleLog2;
                 const bool g0 = mx0 > m0 + kGrow || (m0 == -INFINITY && mx0 > -INFINITY);
                 const bool g1 = mx1 > m1 + kGrow || (m1 == -INFINITY && mx1 > -INFINITY);
-                const float mn0 = g0 ? mx0 : m0, mn1 = g1 ? mx1 : m1;
+                constexpr float kLead = MOD ? Half16<E>::kLeadLog2 : 0.f;
+                const float mn0 = g0 ? mx0 + kLead : m0, mn1 = g1 ? mx1 + kLead : m1;
                 const float base0 = mn0 == -INFINITY ? 0.f : mn0;
                 const float base1 = mn1 == -INFINITY ? 0.f : mn1;
                 const float a0 = g0 ? exp2f(m0 - base0) : 1.f, a1 = g1 ? exp2f(m1 - base1) : 1.f;

@@ -385,9 +385,9 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
             // positions of this warp's first and last row
             const int w_lo = __shfl_sync(0xffffffffu, pos, 0);
             const int w_hi = __shfl_sync(0xffffffffu, pos, 31);
-            // growth of a row maximum that makes its reference follow (base 2): what P's
-            // type holds above 1 (bf16 as much as the fp32 sums, fp16 below 2^16)
-            constexpr float kRescale = Half16<E>::kGrowLog2;
+            // the reference of a row (base 2): kLead above the maximum it is set to, and
+            // following a maximum that is kRescale above it (Half16)
+            constexpr float kRescale = Half16<E>::kGrowLog2, kLead = Half16<E>::kLeadLog2;
             float m = -INFINITY, l = 0.f;
             // `ok` turns false (warp-uniformly) when a bounded wait gives up; the warp
             // then skips its waits and TMEM work but keeps meeting the other half's
@@ -583,8 +583,8 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
                     const float mr = both(mt, false);
                     float alpha = 1.f;
                     if (mr > m + kRescale || (m == -INFINITY && mr > -INFINITY)) {
-                        alpha = exp2f(m - mr);
-                        m = mr;
+                        alpha = exp2f(m - (mr + kLead));
+                        m = mr + kLead;
                     }
                     l *= alpha;
                     // O_w holds PV_w(0 .. i-1): S_w(i) was issued after PV_w(i-1)

@@ -268,9 +268,12 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 // Two fp32 values as a 16-bit pair of type E, and the mma of that type.
 template <typename E> struct Half16;
 template <> struct Half16<__nv_bfloat16> {
-    // How far a row maximum may outgrow its softmax reference (base 2) before the
-    // reference follows: 2^x of that still fits the type (and the fp32 sums).
-    static constexpr float kGrowLog2 = 60.f;
+    // A softmax reference (base 2) is set kLeadLog2 above its row's maximum and
+    // follows when the maximum is kGrowLog2 above it: it then follows once in 60
+    // powers of two, and no probability is above 2^8, so that their products with V
+    // overflow no earlier than those of a reference that stays near the maximum.
+    // (The price: a product with V below 2^-74 may fall below fp32's normal range.)
+    static constexpr float kGrowLog2 = 8.f, kLeadLog2 = 52.f;
     static constexpr uint32_t kOnes = 0x3f803f80u;   // a pair of ones
     __device__ __forceinline__ static uint32_t pack(float lo, float hi) { return pack_bf16(lo, hi); }
     __device__ __forceinline__ static f2 unpack(uint32_t u) {
@@ -282,7 +285,8 @@ template <> struct Half16<__nv_bfloat16> {
     }
 };
 template <> struct Half16<__half> {
-    static constexpr float kGrowLog2 = 15.f;
+    // fp16 holds 2^15 above the reference and loses bits 2^14 below it: no lead.
+    static constexpr float kGrowLog2 = 15.f, kLeadLog2 = 0.f;
     static constexpr uint32_t kOnes = 0x3c003c00u;
     __device__ __forceinline__ static uint32_t pack(float lo, float hi) {
         const __half2 v = __floats2half2_rn(lo, hi);

@@ -298,7 +298,9 @@ typedef struct cx_attn_mods {
  * zero.  What the pool holds at positions that no query row of a sequence sees
  * (past the context in its last block, left of every row's window) does not
  * reach the result, NaN and infinity included; at a position that only some
- * rows see, V must be finite.  Workspace: cx_paged_attend_workspace_bytes,
+ * rows see, V must be finite.  Sums are fp32 and their terms at most 2^8 |V|:
+ * |V| below 2^96 overflows in no context of up to 2^23 keys (bf16 pools keep
+ * their bits down to |V| of 2^-74).  Workspace: cx_paged_attend_workspace_bytes,
  * zero-filled once; a plan made by cx_paged_decode / cx_paged_verify does not
  * serve this call, nor the other way round, nor one for another window or made
  * without the prefix (replan = 0 then raises CX_DEV_BAD_QLEN and leaves out as

@@ -127,3 +127,27 @@ def test_a_plan_of_another_call_is_refused_on_the_device(dtype):
         assert left(plan, BF) == (16, True), plan.__name__
     batch.needs_plan = True
     c.check(c.run(batch, out_dtype=dtype))
+
+
+@pytest.mark.parametrize("size", [2.0 ** 90, 2.0 ** -60])
+@pytest.mark.parametrize("q_lens,ctx", [(None, 60000), ([5], 60000), ([60], 1300), ([2, 70], 2500)])
+def test_large_and_small_values_under_scores_that_jump(q_lens, ctx, size):
+    """Row maxima that grow by 50 powers of two between tiles, in either order of
+    the keys, times V far from 1: what is finite stays finite."""
+    hq, hk, d = 8, 2, 128
+    n = len(q_lens or [1])
+    c = ScoredCase(hq=hq, hk=hk, d=d, ctx=[ctx - 300 * b for b in range(n)], q_lens=q_lens,
+                   softcap=200.0, poison=False, q_scale=0.0)
+    c.q = (1.0 + 0.1 * torch.randn(c.q.shape, generator=torch.Generator().manual_seed(1))).to(BF)
+    c.q_dev = c.q.cuda()
+    c.q = c.q.double()
+    top = 50 * 0.6931 / (d * c.scale)          # adds 50 to a score in base 2
+    for b in range(n):
+        j = torch.arange(c.ctx[b])
+        k = c.k[b] * 0.05 + (top * ((j // 128) % 2))[:, None, None]
+        c.k[b] = k.to(BF).double()
+        c.v[b] = (c.v[b] * size).to(BF).double()
+        t = torch.tensor(c.tables[b])
+        c.cache.k_pool[0][t[j // 16].cuda(), (j % 16).cuda()] = c.k[b].to(BF).cuda()
+        c.cache.v_pool[0][t[j // 16].cuda(), (j % 16).cuda()] = c.v[b].to(BF).cuda()
+    c.check(c.run(out_dtype=BF))
