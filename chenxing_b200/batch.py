@@ -68,7 +68,7 @@ class PagedBatch:
     Score modifiers, none by default (the scaled score of a query at position
     ``pos`` and a key at ``j`` is ``s``):
 
-    * ``softcap``: ``s`` becomes ``softcap * tanh(s / softcap)``;
+    * ``softcap`` (1e-30 .. 1e30): ``s`` becomes ``softcap * tanh(s / softcap)``;
     * ``alibi_slopes`` (n_q_heads values >= 0): ``s -= slope[h] * |pos - j|``,
       after the cap;
     * ``prefix_lens`` (one per sequence): keys ``j < prefix_lens[b]`` are seen by
@@ -96,8 +96,8 @@ class PagedBatch:
         self.verify = q_lens is not None
         self.table_stride = table_stride
         self.softcap = None if softcap is None else float(softcap)
-        if softcap is not None and not (0 < self.softcap < math.inf):
-            raise ValueError("softcap must be positive and finite (or None)")
+        if softcap is not None and not (1e-30 <= self.softcap <= 1e30):
+            raise ValueError("softcap must be None or 1e-30 .. 1e30")
         self.alibi_slopes = None
         if alibi_slopes is not None:
             sl = alibi_slopes.detach().cpu().numpy() if isinstance(alibi_slopes, torch.Tensor) \

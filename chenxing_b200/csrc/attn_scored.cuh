@@ -267,8 +267,9 @@ static int attend_scored(const cx_pool* pool, int64_t layer, const cx_attn_batch
                     "cx_paged_attend: n_q_heads must be a multiple of n_kv_heads");
     if (bt->q_start && bt->max_q_len < 1)
         return fail(CX_ERR_SHAPE, "cx_paged_attend: max_q_len must be at least 1");
-    if (!(mods->softcap >= 0.f) || isinf(mods->softcap))
-        return fail(CX_ERR_SHAPE, "cx_paged_attend: softcap must be finite and >= 0");
+    // (caps near the ends of fp32's range: their products and quotients overflow)
+    if (!(mods->softcap == 0.f || (mods->softcap >= 1e-30f && mods->softcap <= 1e30f)))
+        return fail(CX_ERR_SHAPE, "cx_paged_attend: softcap must be 0 or 1e-30 .. 1e30");
     if (elem_bytes(mods->out_dtype) == 0 || elem_bytes(q_dtype) == 0)
         return fail(CX_ERR_DTYPE, "cx_paged_attend: unknown query or output type");
     if (pool->head_dim > 256) return fail(CX_ERR_UNSUPPORTED, "cx_paged_attend: head_dim > 256");
@@ -279,6 +280,8 @@ static int attend_scored(const cx_pool* pool, int64_t layer, const cx_attn_batch
     if (!bt->block_tables || !bt->ctx_lens || !q || !out || bt->table_stride <= 0)
         return fail(CX_ERR_SHAPE, "cx_paged_attend: NULL array or empty table");
     const float scale = isnan(bt->scale) ? 1.0f / sqrtf((float)pool->head_dim) : bt->scale;
+    if (mods->softcap > 0.f && !isfinite(scale / mods->softcap))
+        return fail(CX_ERR_SHAPE, "cx_paged_attend: scale / softcap must be finite");
     cx_attn_mods m = *mods;
     if (m.q_stride == 0) m.q_stride = row;
     cx_attn_batch b = *bt;

@@ -274,7 +274,8 @@ int cx_paged_kernel_kind(const cx_pool* pool, const cx_attn_batch* batch, int32_
 /* What cx_paged_attend does to the scores and the output, beside the batch's
  * scale and window (no counterpart in the reference). */
 typedef struct cx_attn_mods {
-    float softcap;               /* > 0: score s becomes softcap * tanh(s / softcap);  */
+    float softcap;               /* > 0: score s becomes softcap * tanh(s / softcap),  */
+                                 /* 1e-30 .. 1e30, scale / softcap finite;             */
                                  /* 0: scores are not capped                           */
     int32_t out_dtype;           /* CX_F32 / CX_BF16 / CX_F16                          */
     const float* alibi_slopes;   /* [n_q_heads] on the device, or NULL: the score of a */

@@ -151,3 +151,16 @@ def test_large_and_small_values_under_scores_that_jump(q_lens, ctx, size):
         c.cache.k_pool[0][t[j // 16].cuda(), (j % 16).cuda()] = c.k[b].to(BF).cuda()
         c.cache.v_pool[0][t[j // 16].cuda(), (j % 16).cuda()] = c.v[b].to(BF).cuda()
     c.check(c.run(out_dtype=BF))
+
+
+@pytest.mark.parametrize("softcap", [1e-30, 1e30])
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (F16, 64), (F32, 64), (BF, 96)])
+@pytest.mark.parametrize("q_lens", [None, [40, 60]])
+def test_smallest_and_largest_cap(softcap, dtype, d, q_lens):
+    """The mean of the visible V under the one, no cap at all under the other."""
+    c = ScoredCase(hq=8, hk=2, d=d, ctx=[70, 300], q_lens=q_lens, dtype=dtype, softcap=softcap)
+    batch = c.batch()
+    out = c.run(batch, out_dtype=dtype)
+    if softcap > 1:
+        c.softcap = None
+    c.check(out)

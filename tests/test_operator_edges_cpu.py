@@ -1,11 +1,13 @@
 """What the engine and the batch pass on to the normalised append and the scored
 attention, and what they refuse: host logic only (no GPU needed)."""
+import math
 from types import SimpleNamespace
 
 import pytest
 import torch
 
-from chenxing_b200 import BatchedKVEngine
+from chenxing_b200 import BatchedKVEngine, PagedBatch, _lib
+from test_scored_refusals_cpu import _attend, _cache
 
 
 class CallsOnly:
@@ -66,3 +68,22 @@ def test_replan_false_needs_a_plan_of_the_same_entry_point():
         _plans(b, False, "plain")
     b._planned_by = None                     # never planned here: the device checks
     assert not _plans(b, False, "plain")
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _lib.load_library()
+
+
+@pytest.mark.parametrize("softcap", [1e-50, 1e-40, 9e-31, 2e30, 3e38])
+def test_caps_outside_fp32_arithmetic_are_refused(lib, softcap):
+    """1e-50 is 0 in fp32, which would mean no cap."""
+    with pytest.raises(ValueError):
+        PagedBatch(_cache(), [[0, 1], [2]], [20, 5], n_q_heads=4, softcap=softcap)
+    if softcap > 1e-45:
+        assert _attend(lib, mods=dict(softcap=softcap)) == _lib.CX_ERR_SHAPE
+
+
+@pytest.mark.parametrize("scale", [1e9, -1e9, math.inf])
+def test_scale_over_cap_must_be_finite(lib, scale):
+    assert _attend(lib, batch=dict(scale=scale), mods=dict(softcap=1e-30)) == _lib.CX_ERR_SHAPE
