@@ -69,8 +69,8 @@ class PagedBatch:
     ``pos`` and a key at ``j`` is ``s``):
 
     * ``softcap`` (1e-30 .. 1e30): ``s`` becomes ``softcap * tanh(s / softcap)``;
-    * ``alibi_slopes`` (n_q_heads values >= 0): ``s -= slope[h] * |pos - j|``,
-      after the cap;
+    * ``alibi_slopes`` (n_q_heads values >= 0, times the longest context below
+      2^23): ``s -= slope[h] * |pos - j|``, after the cap;
     * ``prefix_lens`` (one per sequence): keys ``j < prefix_lens[b]`` are seen by
       every query row of the sequence, past the causal limit (a prompt whose
       first tokens see one another) and the window (tokens that a long stream
@@ -99,12 +99,14 @@ class PagedBatch:
         if softcap is not None and not (1e-30 <= self.softcap <= 1e30):
             raise ValueError("softcap must be None or 1e-30 .. 1e30")
         self.alibi_slopes = None
+        self._steepest = 0.0
         if alibi_slopes is not None:
-            sl = alibi_slopes.detach().cpu().numpy() if isinstance(alibi_slopes, torch.Tensor) \
-                else alibi_slopes
+            sl = alibi_slopes.detach().float().cpu().numpy() \
+                if isinstance(alibi_slopes, torch.Tensor) else alibi_slopes
             sl = np.asarray(sl, dtype=np.float32).reshape(-1)
             if sl.shape[0] != self.n_q_heads or not np.all(np.isfinite(sl)) or np.any(sl < 0):
                 raise ValueError(f"alibi_slopes must be {self.n_q_heads} finite values >= 0")
+            self._steepest = float(sl.max(initial=0.0))
             self.alibi_slopes = upload(sl, self.device)
         self.prefix_lens = None
         self.prefix_host = None
@@ -129,6 +131,11 @@ class PagedBatch:
             raise ValueError("a block table is longer than table_stride")
         if np.any(ctx < 0) or np.any(ctx > lens * bs):
             raise ValueError("context length outside [0, len(block_table) * block_size]")
+        # beside a bias of 2^23 fp32 loses half a unit of a score: more, and the
+        # probabilities of far keys overflow fp16
+        if self._steepest * int(ctx.max(initial=0)) >= 2 ** 23:
+            raise ValueError("the steepest of alibi_slopes times the longest context must be "
+                             "below 2**23")
         if prefix_lens is None:
             pre = self.prefix_host
             if pre is not None and pre.shape[0] != B:

@@ -280,7 +280,9 @@ typedef struct cx_attn_mods {
     int32_t out_dtype;           /* CX_F32 / CX_BF16 / CX_F16                          */
     const float* alibi_slopes;   /* [n_q_heads] on the device, or NULL: the score of a */
                                  /* key at j for a query at pos gets                   */
-                                 /* -slope[h] * |pos - j| after the cap (slopes >= 0)  */
+                                 /* -slope[h] * |pos - j| after the cap; slopes >= 0,  */
+                                 /* slope * context below 2^23 (beside larger biases   */
+                                 /* fp32 loses the scores)                             */
     const int32_t* prefix_lens;  /* [batch] on the device, or NULL: keys               */
                                  /* j < prefix_lens[b] are seen by every query row,    */
                                  /* past the causal limit and the window               */

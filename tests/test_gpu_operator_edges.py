@@ -164,3 +164,16 @@ def test_smallest_and_largest_cap(softcap, dtype, d, q_lens):
     if softcap > 1:
         c.softcap = None
     c.check(out)
+
+
+@pytest.mark.parametrize("hq,hk,d,dtype,q_lens,ctx", [
+    (4, 1, 128, BF, [33], 5000), (8, 2, 64, F16, [200], 3000), (96, 1, 64, BF, None, 3000),
+    (8, 2, 128, BF, None, 6000), (4, 2, 64, F32, [3], 5000), (4, 2, 96, BF, [5], 700)])
+def test_steepest_slopes(hq, hk, d, dtype, q_lens, ctx):
+    """A bias that leaves each row its own key alone: the output is that V row."""
+    steep = 2.0 ** 23 / (ctx + 1)
+    c = ScoredCase(hq=hq, hk=hk, d=d, ctx=[ctx], q_lens=q_lens, dtype=dtype,
+                   slopes=[steep / (1 + h % 3) for h in range(hq)])
+    out = c.run(out_dtype=dtype).cpu()
+    own = c.v[0][-len(out):].to(dtype).repeat_interleave(hq // hk, 1)
+    assert torch.equal(out, own)

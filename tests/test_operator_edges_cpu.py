@@ -87,3 +87,23 @@ def test_caps_outside_fp32_arithmetic_are_refused(lib, softcap):
 @pytest.mark.parametrize("scale", [1e9, -1e9, math.inf])
 def test_scale_over_cap_must_be_finite(lib, scale):
     assert _attend(lib, batch=dict(scale=scale), mods=dict(softcap=1e-30)) == _lib.CX_ERR_SHAPE
+
+
+def test_steep_slopes_are_refused_for_long_contexts(lib):
+    """fp32 loses half a unit of a score beside a bias of 2^23."""
+    def batch(slope):
+        return PagedBatch(_cache(), [[0, 1], [2]], [20, 5], n_q_heads=4,
+                          alibi_slopes=[0.5, slope, 0.0, 1.0])
+    for slope in (2.0 ** 23 / 20, 1e30):
+        with pytest.raises(ValueError):
+            batch(slope)
+    b = batch(2.0 ** 23 / 21)
+    with pytest.raises(ValueError):
+        b.advance()
+    assert b.ctx_host.tolist() == [20, 5]          # as it was
+
+
+def test_slopes_of_a_bf16_tensor(lib):
+    b = PagedBatch(_cache(), [[0]], [4], n_q_heads=2,
+                   alibi_slopes=torch.tensor([0.5, 0.25], dtype=torch.bfloat16))
+    assert b.alibi_slopes.tolist() == [0.5, 0.25]
