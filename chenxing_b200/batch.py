@@ -199,13 +199,15 @@ class PagedBatch:
             return int(np.sum(self.ctx_host - lo + pre))
         return int(self.ctx_host.sum())
 
-    def kernel_kind(self, q_dtype=torch.bfloat16) -> str:
-        """Which libcxkv kernel attends this batch: "generic", "mma" or "tcgen05"."""
-        if self.scored:
-            return _lib.KERNEL_KINDS[_lib.lib().cx_paged_attend_kind(
-                self.cache.cx_pool(), self._c, _lib.cx_dtype(q_dtype))]
-        k = _lib.lib().cx_paged_kernel_kind(self.cache.cx_pool(), self._c,
-                                            _lib.cx_dtype(q_dtype), int(self.verify))
+    def kernel_kind(self, q_dtype=torch.bfloat16, out_dtype=torch.float32) -> str:
+        """Which libcxkv kernel attends this batch for queries and outputs of these
+        types: "generic", "mma", "tcgen05" or "fma"."""
+        if self.takes_attend(out_dtype):
+            k = _lib.lib().cx_paged_attend_kind(self.cache.cx_pool(), self._c,
+                                                _lib.cx_dtype(q_dtype))
+        else:
+            k = _lib.lib().cx_paged_kernel_kind(self.cache.cx_pool(), self._c,
+                                                _lib.cx_dtype(q_dtype), int(self.verify))
         return _lib.KERNEL_KINDS[k]
 
     @property
@@ -213,6 +215,10 @@ class PagedBatch:
         """Whether the batch changes the scores or the visible keys."""
         return self.softcap is not None or self.alibi_slopes is not None \
             or self.prefix_lens is not None
+
+    def takes_attend(self, out_dtype) -> bool:
+        """Whether calls with this output type are ``cx_paged_attend``'s."""
+        return self.scored or out_dtype != torch.float32
 
     def c_struct(self) -> _lib.CxAttnBatch:
         return self._c
@@ -227,7 +233,7 @@ def _attend(cache, layer: int, q, batch: PagedBatch, out, replan, out_dtype, fn_
         raise ValueError("PagedBatch belongs to a different cache")
     if out_dtype is None:
         out_dtype = torch.float32 if out is None else out.dtype
-    if batch.scored or out_dtype != torch.float32:
+    if batch.takes_attend(out_dtype):
         return _attend_scored(cache, layer, q, batch, out, replan, out_dtype)
     qt = to_device(q, cache.device)
     expect = (batch.total_q, batch.n_q_heads, cache.head_dim)

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from chenxing_b200 import BatchedKVEngine, PagedBatch, _lib
-from test_scored_refusals_cpu import _attend, _cache
+from test_scored_refusals_cpu import _attend, _cache, _pool
 
 
 class CallsOnly:
@@ -107,3 +107,17 @@ def test_slopes_of_a_bf16_tensor(lib):
     b = PagedBatch(_cache(), [[0]], [4], n_q_heads=2,
                    alibi_slopes=torch.tensor([0.5, 0.25], dtype=torch.bfloat16))
     assert b.alibi_slopes.tolist() == [0.5, 0.25]
+
+
+def test_kernel_kind_knows_the_output_type(lib):
+    """A batch without modifiers changes the entry point with its output type."""
+    f16 = _cache()
+    f16.cx_pool = lambda: _pool(dtype=_lib.CX_F16)
+    b = PagedBatch(f16, [[0, 1], [2]], [20, 5], n_q_heads=4)
+    assert b.kernel_kind(torch.float16) == "generic"
+    assert b.kernel_kind(torch.float16, torch.float16) == "mma"
+    assert b.kernel_kind(torch.float16, out_dtype=torch.bfloat16) == "mma"
+    b = PagedBatch(f16, [[0, 1], [2]], [20, 5], n_q_heads=4, softcap=5.0)
+    assert b.kernel_kind(torch.float16) == b.kernel_kind(torch.float16, torch.float16) == "mma"
+    b = PagedBatch(_cache(), [[0, 1], [2]], [20, 5], n_q_heads=4)
+    assert b.kernel_kind() == b.kernel_kind(out_dtype=torch.float16) == "mma"
