@@ -1790,6 +1790,9 @@ size_t cx_paged_workspace_bytes(const cx_pool* pool, const cx_attn_batch* b) {
     if (!pool || !b || pool->n_kv_heads <= 0 || b->n_q_heads <= 0 || b->batch < 0) return 0;
     const int64_t G = b->n_q_heads / pool->n_kv_heads;
     const int64_t max_q = b->q_start ? (b->max_q_len > 0 ? b->max_q_len : 1) : 1;
+    // more than 64 packed rows: the tcgen05 and the generic kernel, which read none
+    // (4 sequences of 1024 rows, 32 / 8 heads of 128, would be 699 MB to fill)
+    if (G * max_q > 64) return 256;
     return ws_layout(b->batch, unit_shape(pool, G * max_q), G * max_q, pool->head_dim,
                      grid_size()).total;
 }

@@ -121,3 +121,18 @@ def test_kernel_kind_knows_the_output_type(lib):
     assert b.kernel_kind(torch.float16) == b.kernel_kind(torch.float16, torch.float16) == "mma"
     b = PagedBatch(_cache(), [[0, 1], [2]], [20, 5], n_q_heads=4)
     assert b.kernel_kind() == b.kernel_kind(out_dtype=torch.float16) == "mma"
+
+
+@pytest.mark.parametrize("dtype", [_lib.CX_BF16, _lib.CX_F16, _lib.CX_F32])
+def test_prompt_chunks_size_no_split_workspace(lib, dtype):
+    """Above 64 packed rows no kernel of either entry point reads a split-K plan."""
+    pool = _pool(dtype=dtype, n_kv_heads=8, head_dim=128)
+
+    def need(fn, max_q):
+        return fn(pool, _lib.CxAttnBatch(0x100, 512, 0x200, 0x300, 4, max_q, 32, 0.1, 0, 0))
+    assert need(lib.cx_paged_workspace_bytes, 1024) <= 1 << 20
+    assert need(lib.cx_paged_attend_workspace_bytes, 1024) <= 1 << 20
+    assert need(lib.cx_paged_workspace_bytes, 17) <= 1 << 20
+    rows = 4 * 8 * 15 * 4                    # partial rows of the batch's ranges at least
+    assert need(lib.cx_paged_workspace_bytes, 15) > rows * 130 * 4
+    assert need(lib.cx_paged_attend_workspace_bytes, 15) > rows * 130 * 4
