@@ -57,6 +57,12 @@ def slot_mapping(block_tables, starts, counts, block_size: int) -> np.ndarray:
     return ids[base + pos // bs] * bs + pos % bs
 
 
+def _same_start(a, b) -> bool:
+    """Whether two block tables may be one sequence's: equal as far as both go."""
+    n = min(len(a), len(b))
+    return list(a[:n]) == list(b[:n]) and (n > 0 or len(a) == len(b))
+
+
 class PagedBatch:
     """Device metadata + workspace for batched decode / verify on one cache.
 
@@ -118,7 +124,8 @@ class PagedBatch:
     # ------------------------------------------------------------------ #
     def set(self, block_tables, ctx_lens, q_lens=None, prefix_lens=None) -> None:
         """(Re)load tables and lengths; the next attention call re-plans.  Without
-        ``prefix_lens`` a batch that has some keeps them (for as many sequences)."""
+        ``prefix_lens`` a batch that has some keeps them, for the same sequences:
+        as many, and each table the one before, grown or cut."""
         bs = self.cache.block_size
         B = len(block_tables)
         ctx = np.asarray(ctx_lens, dtype=np.int64).reshape(-1)
@@ -140,6 +147,9 @@ class PagedBatch:
             pre = self.prefix_host
             if pre is not None and pre.shape[0] != B:
                 raise ValueError("prefix_lens must be given again for another batch size")
+            if pre is not None and any(not _same_start(a, t) for a, t in
+                                       zip(self.tables_host, block_tables)):
+                raise ValueError("prefix_lens must be given again for other sequences")
         else:
             pre = np.asarray(prefix_lens, dtype=np.int64).reshape(-1)
             if pre.shape[0] != B or np.any(pre < 0):

@@ -136,3 +136,23 @@ def test_prompt_chunks_size_no_split_workspace(lib, dtype):
     rows = 4 * 8 * 15 * 4                    # partial rows of the batch's ranges at least
     assert need(lib.cx_paged_workspace_bytes, 15) > rows * 130 * 4
     assert need(lib.cx_paged_attend_workspace_bytes, 15) > rows * 130 * 4
+
+
+def test_kept_prefixes_are_for_the_same_sequences(lib):
+    def batch():
+        return PagedBatch(_cache(), [[0, 1], [2], []], [20, 5, 0], n_q_heads=4,
+                          prefix_lens=[3, 9, 0])
+    for tables, ctx in (([[0, 1, 4], [2, 5], []], [40, 17, 0]),     # grown
+                        ([[0], [2], []], [16, 4, 0]), ([[0, 1], [2], []], [21, 6, 0])):
+        b = batch()
+        b.set(tables, ctx)
+        assert b.prefix_lens.tolist() == [3, 9, 0]
+    for tables, ctx in (([[2], [0, 1], []], [5, 20, 0]), ([[0, 3], [2], []], [20, 5, 0]),
+                        ([[0, 1], [6], []], [20, 5, 0]), ([[0, 1], [2], [3]], [20, 5, 1]),
+                        ([[0, 1], [], []], [20, 0, 0])):
+        b = batch()
+        with pytest.raises(ValueError):
+            b.set(tables, ctx)
+        assert b.ctx_host.tolist() == [20, 5, 0]
+        b.set(tables, ctx, prefix_lens=[1, 1, 1])
+        assert b.prefix_lens.tolist() == [1, 1, 1]
