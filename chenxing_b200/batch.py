@@ -158,6 +158,14 @@ class PagedBatch:
                           count=int(lens.sum()))
         if ids.size and (ids.min() < 0 or ids.max() >= self.cache.n_blocks):
             raise IndexError(f"block id outside [0, {self.cache.n_blocks})")
+        if self.verify:
+            ql = np.asarray(q_lens, dtype=np.int64).reshape(-1)
+            if ql.shape[0] != B or np.any(ql < 0) or np.any(ql > ctx):
+                raise ValueError("q_lens must be per sequence and <= ctx_lens")
+            qs = np.zeros(B + 1, dtype=np.int64)
+            np.cumsum(ql, out=qs[1:])
+        # nothing is refused from here on: a batch is reloaded whole or stays as it was
+        self.needs_plan = True
         tab = np.zeros((B, stride), dtype=np.int32)
         tab[np.arange(stride) < lens[:, None]] = ids   # row-major mask order = concatenation
         self.batch = B
@@ -167,11 +175,6 @@ class PagedBatch:
         self.block_tables = upload(tab, self.device)
         self.ctx_lens = upload(ctx.astype(np.int32), self.device)
         if self.verify:
-            ql = np.asarray(q_lens, dtype=np.int64).reshape(-1)
-            if ql.shape[0] != B or np.any(ql < 0) or np.any(ql > ctx):
-                raise ValueError("q_lens must be per sequence and <= ctx_lens")
-            qs = np.zeros(B + 1, dtype=np.int64)
-            np.cumsum(ql, out=qs[1:])
             self.q_lens_host = ql
             self.q_start = upload(qs.astype(np.int32), self.device)
             self.max_q = int(ql.max(initial=1))
@@ -193,7 +196,6 @@ class PagedBatch:
         if need > self._ws_bytes:
             self._ws = torch.zeros(need, dtype=torch.uint8, device=self.device)
             self._ws_bytes = need
-        self.needs_plan = True
 
     def advance(self, n: int = 1) -> None:
         """Every context grows by ``n`` tokens (one decode step); re-plans."""

@@ -156,3 +156,23 @@ def test_kept_prefixes_are_for_the_same_sequences(lib):
         assert b.ctx_host.tolist() == [20, 5, 0]
         b.set(tables, ctx, prefix_lens=[1, 1, 1])
         assert b.prefix_lens.tolist() == [1, 1, 1]
+
+
+@pytest.mark.parametrize("kw", [
+    dict(q_lens=[9, 1]), dict(q_lens=[1]), dict(q_lens=[-1, 2]), dict(q_lens=None),
+    dict(q_lens=[1, 1], prefix_lens=[1]), dict(q_lens=[1, 1], ctx=[99, 1])])
+def test_a_refused_reload_leaves_the_batch_as_it_was(lib, kw):
+    """Its struct's pointers are those of the tensors it holds."""
+    b = PagedBatch(_cache(), [[0, 1], [2]], [20, 5], n_q_heads=4, q_lens=[3, 2],
+                   prefix_lens=[2, 0])
+
+    def state():
+        c = b.c_struct()
+        return (b.batch, b.max_q, b.total_q, b.ctx_host.tolist(), b.q_lens_host.tolist(),
+                b.block_tables.tolist(), b.ctx_lens.tolist(), b.q_start.tolist(),
+                b.prefix_lens.tolist(), c.batch, c.max_q_len, c.block_tables, c.ctx_lens,
+                c.q_start, b.block_tables.data_ptr(), b.ctx_lens.data_ptr(), b.q_start.data_ptr())
+    was = state()
+    with pytest.raises((ValueError, TypeError)):
+        b.set([[0, 3], [2]], kw.pop("ctx", [8, 8]), **{"prefix_lens": [1, 1], **kw})
+    assert state() == was
