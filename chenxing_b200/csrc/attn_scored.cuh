@@ -220,6 +220,7 @@ static int attend_tc(const cx_pool* pool, int64_t layer, const cx_attn_batch& b,
     p.z_scale = m.softcap > 0.f ? fabsf(scale) / m.softcap : 0.f;
     p.cap_log2 = m.softcap * 1.4426950408889634f;
     p.neg = scale < 0.f;
+    p.wait_ns = wait_limit_ns();
     if (m.softcap > 0.f && p.z_scale > 0.f) {
         // In double: z_scale^9 may be small, but its product with the score is not.
         // Where a coefficient falls below fp32's normal range (caps beyond some

@@ -76,6 +76,7 @@ struct ScoredTcParams {
     float c4[4], c5[5];          // the polynomials in the raw score (ScPoly), base 2
     float s4_max, s5_max;        // |score| up to which each holds
     int32_t neg;                 // scale < 0: Q is negated (tanh is odd)
+    uint64_t wait_ns;            // limit of every pipeline wait (cx_set_wait_limit_ns)
 };
 
 template <int D_>
@@ -409,7 +410,7 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
             for (int i = 0; i < g.n_tiles; ++i) {
                 if (ok)
                     ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[w], i & 1, s_abort,
-                                                                   kWaitLimitNs));
+                                                                   p.wait_ns));
                 const int tile = g.first - i;
                 const int b0 = tile < g.n_pre ? tile * BPT : g.kb0 + (tile - g.n_pre) * BPT;
                 const int kb = b0 * kBlockTok + c * 64;      // this half's first key
@@ -618,7 +619,7 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
                         const int q = sc_pos_v(i, g.n_tiles);
                         ok = __all_sync(0xffffffffu,
                                         mbar_wait_bounded(&full[q % SLOTS], (q / SLOTS) & 1,
-                                                          s_abort, kWaitLimitNs));
+                                                          s_abort, p.wait_ns));
                         if (!ok) continue;
                         if (dead(kbase + r)) {
                             // half c of the row's 16-byte chunks
@@ -647,7 +648,7 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
             const int n_tiles = g.n_tiles;
             if (n_tiles > 0 && ok) {
                 ok = __all_sync(0xffffffffu, mbar_wait_bounded(&o_done[w], (n_tiles - 1) & 1,
-                                                                s_abort, kWaitLimitNs));
+                                                                s_abort, p.wait_ns));
                 if (ok) tc_fence_after();
             }
             l = both(l, true);
@@ -747,7 +748,7 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
                 const int s = q % SLOTS, use = q / SLOTS;
                 bool go = true;
                 if (lane == 0 && use > 0 &&
-                    !mbar_wait_bounded(&empty[s], (use - 1) & 1, s_abort, kWaitLimitNs))
+                    !mbar_wait_bounded(&empty[s], (use - 1) & 1, s_abort, p.wait_ns))
                     go = false;
                 go = __shfl_sync(0xffffffffu, go, 0) && !*s_abort;
                 // all three warps issue an item or none does: s_issued stays exact
@@ -789,7 +790,7 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
                 const uint64_t v_desc = tc_sdesc(smem_addr(ring), C::KV_HALF, 1024);
                 bool ok = true;
                 auto wait = [&](uint64_t* bar, int parity) {
-                    const bool r = mbar_wait_bounded(bar, parity & 1, s_abort, kWaitLimitNs);
+                    const bool r = mbar_wait_bounded(bar, parity & 1, s_abort, p.wait_ns);
                     if (r) tc_fence_after();
                     return r;
                 };

@@ -188,7 +188,10 @@ __device__ __forceinline__ uint64_t global_ns() {
 
 // Bounded wait on an mbarrier phase.  Gives up after `limit_ns` nanoseconds
 // or as soon as *abort is set (abort may be NULL), and reports whether the
-// phase completed.
+// phase completed.  Both are looked at after every EVERY-th try.  A try suspends
+// the thread, and where few threads arrive 64 of them outlast long waits (some
+// 70 us on the stages of the staged append): such waits look after each.
+template <uint32_t EVERY = 64>
 __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity,
                                                   volatile int* abort, uint64_t limit_ns) {
     if (mbar_try_wait(bar, parity)) return true;
@@ -196,7 +199,7 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
     uint32_t spins = 0;
     while (true) {
         if (mbar_try_wait(bar, parity)) return true;
-        if ((++spins & 63u) == 0) {
+        if ((++spins & (EVERY - 1)) == 0) {
             if (abort && *abort) return false;
             if (global_ns() - t0 > limit_ns) return false;
         }

@@ -23,6 +23,7 @@ struct NormRopeParams {
     void* vp;
     void* q_out;
     int32_t pool_dtype, q_out_dtype;
+    uint64_t wait_ns;          // limit of the staged form's waits (cx_set_wait_limit_ns)
 };
 
 template <typename S>
@@ -394,6 +395,7 @@ __device__ __forceinline__ void pairs_chunk(const f2 (&x)[V / 2], Chunk<T, V>& c
 constexpr int kTokStages = 3;
 constexpr int kTokRows = 3;        // rows a group takes, about
 constexpr int kTokThreads = 288;   // at most: 8 warps and the producer
+constexpr uint64_t kDrainLimitNs = 2000000000ull;   // of the producer's last wait
 
 struct TokStage {          // beside the rows of a stage
     int64_t kv_dst;        // pool element of the token's row of head 0
@@ -427,7 +429,6 @@ __global__ void __launch_bounds__(kTokThreads, 3)
     }
     __syncthreads();
     volatile int* abort = &s_abort;
-    constexpr uint64_t kWait = 2000000000ull;         // ns, every wait
 
     if (tid >= n_warps * 32) {
         // ---- producer: lane 0; the position and slot of the next token are loaded
@@ -443,7 +444,7 @@ __global__ void __launch_bounds__(kTokThreads, 3)
                 pos = p.positions[t + step];
                 slot = p.slots[t + step];
             }
-            if (!mbar_wait_bounded(&empty[s], phase, abort, kWait)) {
+            if (!mbar_wait_bounded<1>(&empty[s], phase, abort, p.wait_ns)) {
                 *abort = 1;
                 raise_flag(CX_DEV_WAIT_TIMEOUT);
                 break;
@@ -474,7 +475,8 @@ __global__ void __launch_bounds__(kTokThreads, 3)
         }
         // the CTA's shared memory stays until its copies have landed
         for (int i = issued > kTokStages ? issued - kTokStages : 0; i < issued; ++i)
-            mbar_wait_bounded(&full[i % kTokStages], (i / kTokStages) & 1, nullptr, kWait);
+            mbar_wait_bounded<1>(&full[i % kTokStages], (i / kTokStages) & 1, nullptr,
+                              kDrainLimitNs);
         return;
     }
 
@@ -492,7 +494,7 @@ __global__ void __launch_bounds__(kTokThreads, 3)
     const int64_t head_step = p.g.block_size * D;
     int s = 0, phase = 0;
     for (int64_t t = blockIdx.x; t < T; t += step) {
-        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[s], phase, abort, kWait))) {
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded<1>(&full[s], phase, abort, p.wait_ns))) {
             if (lane == 0 && !*abort) {
                 *abort = 1;
                 raise_flag(CX_DEV_WAIT_TIMEOUT);
@@ -742,7 +744,8 @@ extern "C" int cx_kv_append_norm_rope(const cx_pool* pool, int64_t layer, const 
     if (rows->n_q_heads > 0 && elem_bytes(q_out_dtype) == 0)
         return fail(CX_ERR_DTYPE, "cx_kv_append_norm_rope: unknown q_out type");
     const NormRopeParams p{geom_of(pool), layer,    *rows,    *how,  slot_mapping, positions,
-                           pool->k,       pool->v, q_out, pool->dtype, q_out_dtype};
+                           pool->k,       pool->v, q_out, pool->dtype, q_out_dtype,
+                           wait_limit_ns()};
     cudaStream_t st = as_stream(stream);
     switch (rows->dtype) {
         case CX_F32: return launch_norm_rope<float>(p, st);

@@ -246,8 +246,10 @@ int cx_paged_verify(const cx_pool* pool, int64_t layer, const cx_attn_batch* bat
 int cx_paged_decode_static(const cx_pool* pool, int64_t layer, const cx_attn_batch* batch,
                            const void* q, int32_t q_dtype, float* out, void* stream);
 
-/* Limit, in nanoseconds, of every pipeline wait inside the decode / verify
- * kernels of later calls in this process (0 restores the default, 2 s).  A
+/* Limit, in nanoseconds, of every pipeline wait inside the split-K kernels of
+ * later decode / verify calls, all kernels of cx_paged_attend and the staged
+ * form of cx_kv_append_norm_rope in this process (0 restores the default, 2 s;
+ * the tcgen05 kernels of cx_paged_verify keep that).  A
  * wait that runs out makes its CTA stop, wait (with the default limit) for its
  * own copies in flight, raise CX_DEV_WAIT_TIMEOUT and return; that call's
  * output is then undefined and the device stays usable.  Meant for tests of

@@ -177,3 +177,56 @@ def test_steepest_slopes(hq, hk, d, dtype, q_lens, ctx):
     out = c.run(out_dtype=dtype).cpu()
     own = c.v[0][-len(out):].to(dtype).repeat_interleave(hq // hk, 1)
     assert torch.equal(out, own)
+
+
+def timed_out(call):
+    """Flags of ``call`` under a wait limit of a few ns."""
+    from chenxing_b200 import _lib
+    try:
+        _lib.lib().cx_set_wait_limit_ns(5)
+        call()
+        return _lib.device_flags(clear=True)
+    finally:
+        _lib.lib().cx_set_wait_limit_ns(0)
+
+
+@pytest.mark.parametrize("hq,hk,q_lens,ctx", [
+    (32, 8, [300, 200, 300, 129], [9000, 3000, 300, 6000]),       # a CTA a pair of query tiles
+    (4, 1, [33], [20000])])                                       # keys split over many CTAs
+@pytest.mark.parametrize("mods", [dict(softcap=30.0), dict(slopes=True)])
+def test_tcgen05_waits_that_run_out_return_and_flag(hq, hk, q_lens, ctx, mods):
+    """The call returns with the flag raised; the next one has the bits of the
+    one before."""
+    if mods.get("slopes"):
+        mods = dict(slopes=alibi(hq))
+    c = ScoredCase(hq=hq, hk=hk, d=128, ctx=ctx, q_lens=q_lens, **mods)
+    batch = c.batch()
+    assert batch.kernel_kind() == "tcgen05"
+    ref = c.run(batch, out_dtype=BF)
+    assert timed_out(lambda: c.run(batch, out_dtype=BF)) == 8
+    assert torch.equal(c.run(batch, out_dtype=BF), ref)
+
+
+def test_staged_append_waits_that_run_out_return_and_flag():
+    """Q stored to pinned host memory, which takes a token's rows much longer to
+    leave the stage than a copy takes to fill it."""
+    from chenxing_b200 import _lib
+    r = Rows(3000, 32, 8, 128, 128)
+    slots, pos, rope = r.slots.cuda(), r.pos.cuda(), r.rope
+    w = [x.cuda() for x in (r.qw, r.kw)]
+    st = [n for x in r.dev for n in (x.stride(0), x.stride(1))]
+    rows = _lib.CxQkv(*(x.data_ptr() for x in r.dev), *st, r.T, r.hq, _lib.CX_BF16, 0)
+    how = _lib.CxNormRope(w[0].data_ptr(), w[1].data_ptr(), _lib.CX_BF16, _lib.CX_BF16, r.eps, 0,
+                          rope.cos.data_ptr(), rope.sin.data_ptr(), rope.rows, rope.head_dim)
+    host = torch.zeros(r.T, r.hq, r.d, dtype=BF).pin_memory()
+
+    def call():
+        _lib.check(_lib.lib().cx_kv_append_norm_rope(
+            r.cache.cx_pool(), 0, rows, slots.data_ptr(), pos.data_ptr(), how, host.data_ptr(),
+            _lib.CX_BF16, _lib.stream_ptr()), "cx_kv_append_norm_rope")
+        torch.cuda.synchronize()
+    assert timed_out(call) == 8
+    for pool, fill in ((r.cache.k_pool, 3.0), (r.cache.v_pool, 5.0)):
+        pool.fill_(fill)
+    call()
+    r.check(host.cuda())
