@@ -49,8 +49,16 @@ int cx_device_error(void* stream, int clear, uint32_t* flags) {
     if (!flags) return cx::fail(CX_ERR_SHAPE, "cx_device_error: flags is NULL");
     cudaStream_t s = cx::as_stream(stream);
     unsigned int v = 0, w = 0;
-    int rc = cx::read_dev_flags(s, clear, &v);
-    if (rc == CX_OK) rc = cx::read_dev_flags_scored(s, clear, &w);
+    int rc = cx::copy_dev_flags(s, &v);
+    const int rc2 = cx::copy_dev_flags_scored(s, &w);
+    // (both copies are waited for before v and w go out of scope)
+    CX_CUDA_CHECK(cudaStreamSynchronize(s));
+    if (rc == CX_OK) rc = rc2;
+    if (rc == CX_OK && clear) {
+        rc = cx::clear_dev_flags(s);
+        if (rc == CX_OK) rc = cx::clear_dev_flags_scored(s);
+        CX_CUDA_CHECK(cudaStreamSynchronize(s));
+    }
     if (rc != CX_OK) return rc;
     *flags = v | w;
     return CX_OK;

@@ -63,21 +63,22 @@ static inline int check_pool(const cx_pool* p) {
 // device code); cx_device_error reads and clears both.
 static __device__ unsigned int g_dev_flags = 0;
 
-// Reads this translation unit's word on `s` and clears it when asked.
-static int read_dev_flags(cudaStream_t s, int clear, unsigned int* v) {
+// Starts the copy of this translation unit's word to `v` on `s`, or its clearing;
+// the caller synchronises.
+static int copy_dev_flags(cudaStream_t s, unsigned int* v) {
     CX_CUDA_CHECK(cudaMemcpyFromSymbolAsync(v, g_dev_flags, sizeof(*v), 0,
                                             cudaMemcpyDeviceToHost, s));
-    CX_CUDA_CHECK(cudaStreamSynchronize(s));
-    if (clear) {
-        unsigned int z = 0;
-        CX_CUDA_CHECK(cudaMemcpyToSymbolAsync(g_dev_flags, &z, sizeof(z), 0,
-                                              cudaMemcpyHostToDevice, s));
-        CX_CUDA_CHECK(cudaStreamSynchronize(s));
-    }
+    return CX_OK;
+}
+static int clear_dev_flags(cudaStream_t s) {
+    static const unsigned int zero = 0;
+    CX_CUDA_CHECK(cudaMemcpyToSymbolAsync(g_dev_flags, &zero, sizeof(zero), 0,
+                                          cudaMemcpyHostToDevice, s));
     return CX_OK;
 }
 
-int read_dev_flags_scored(cudaStream_t s, int clear, unsigned int* v);  // cxkv_scored.cu
+int copy_dev_flags_scored(cudaStream_t s, unsigned int* v);   // of cxkv_scored.cu
+int clear_dev_flags_scored(cudaStream_t s);
 
 __device__ __forceinline__ void raise_flag(unsigned int bit) {
     atomicOr(&g_dev_flags, bit);

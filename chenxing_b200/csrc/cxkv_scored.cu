@@ -8,8 +8,7 @@
 
 namespace cx {
 
-int read_dev_flags_scored(cudaStream_t s, int clear, unsigned int* v) {
-    return read_dev_flags(s, clear, v);
-}
+int copy_dev_flags_scored(cudaStream_t s, unsigned int* v) { return copy_dev_flags(s, v); }
+int clear_dev_flags_scored(cudaStream_t s) { return clear_dev_flags(s); }
 
 }  // namespace cx

@@ -230,3 +230,27 @@ def test_staged_append_waits_that_run_out_return_and_flag():
         pool.fill_(fill)
     call()
     r.check(host.cuda())
+
+
+@pytest.mark.parametrize("clear,most", [(False, 1), (True, 2)])
+def test_reading_the_flags_waits_once(clear, most):
+    """Two flag words, one wait for both (and one for clearing them)."""
+    from torch.profiler import ProfilerActivity, profile
+
+    from chenxing_b200 import _lib
+    with profile(activities=[ProfilerActivity.CPU, ProfilerActivity.CUDA]) as prof:
+        assert _lib.device_flags(clear=clear) == 0
+    waits = sum(e.count for e in prof.key_averages() if e.key == "cudaStreamSynchronize")
+    assert 1 <= waits <= most
+
+
+@pytest.mark.parametrize("scored", [False, True])
+def test_flags_of_both_units_are_read_and_cleared(scored):
+    from chenxing_b200 import _lib
+    c = ScoredCase(hq=8, hk=2, d=64, ctx=[100], softcap=30.0 if scored else None, poison=False)
+    batch = c.batch()
+    batch.block_tables[0, 2] = c.cache.n_blocks + 5
+    c.run(batch)
+    assert _lib.device_flags(clear=False) == 2
+    assert _lib.device_flags(clear=True) == 2
+    assert _lib.device_flags(clear=True) == 0
