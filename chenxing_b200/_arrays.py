@@ -75,8 +75,7 @@ def rows_on_device(x, device: torch.device) -> torch.Tensor:
     """``x`` (tokens, heads, dim) on ``device`` with its innermost dimension
     contiguous; a tensor that is so already keeps its strides (a slice of a
     fused projection is read in place), float64 is narrowed to float32."""
-    if isinstance(x, torch.Tensor) and x.dtype != torch.float64 and (
-            x.device == device or (x.is_cuda and device.index is None)):
+    if isinstance(x, torch.Tensor) and x.dtype != torch.float64 and x.device == device:
         return x if x.dim() != 3 or x.shape[2] <= 1 or x.stride(2) == 1 else x.contiguous()
     return to_device(x, device)
 

@@ -156,7 +156,8 @@ def require_cuda(device=None) -> torch.device:
         else torch.device(device)
     if dev.type != "cuda":
         raise CxError(f"chenxing_b200 runs on CUDA devices only, got {dev}")
-    return dev
+    # "cuda" is the device that is current now, also when another one is later
+    return dev if dev.index is not None else torch.device("cuda", torch.cuda.current_device())
 
 
 def same_device(a: torch.device, b: torch.device) -> bool:

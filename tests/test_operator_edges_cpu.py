@@ -176,3 +176,14 @@ def test_a_refused_reload_leaves_the_batch_as_it_was(lib, kw):
     with pytest.raises((ValueError, TypeError)):
         b.set([[0, 3], [2]], kw.pop("ctx", [8, 8]), **{"prefix_lens": [1, 1], **kw})
     assert state() == was
+
+
+def test_a_device_without_an_index_is_the_current_one(monkeypatch):
+    """A cache made on "cuda" stays on that device when another becomes current."""
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    for dev in (None, "cuda", torch.device("cuda")):
+        assert _lib.require_cuda(dev) == torch.device("cuda", 3)
+    assert _lib.require_cuda("cuda:1") == torch.device("cuda", 1)
+    with pytest.raises(_lib.CxError):
+        _lib.require_cuda("cpu")
