@@ -106,3 +106,12 @@ def to_numpy(t: torch.Tensor) -> np.ndarray:
             raise TypeError("ml_dtypes is needed to return bfloat16 NumPy arrays")
         return t.detach().view(torch.int16).cpu().numpy().view(NP_BF16)
     return t.detach().cpu().numpy()
+
+
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors meet (strides >= 0)."""
+    def ends(t):
+        n = sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+        return t.data_ptr(), t.data_ptr() + n * t.element_size()
+    (a0, a1), (b0, b1) = ends(a), ends(b)
+    return max(a0, b0) < min(a1, b1)

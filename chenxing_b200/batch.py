@@ -21,7 +21,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._arrays import rows_on_device, to_device, upload
+from ._arrays import overlap, rows_on_device, to_device, upload
 
 __all__ = ["PagedBatch", "slot_mapping", "decode_batch", "verify_batch"]
 
@@ -295,6 +295,10 @@ def _attend_scored(cache, layer: int, q, batch: PagedBatch, out, replan, out_dty
             or not _lib.same_device(out.device, dev):
         raise ValueError(f"out must be a contiguous {out_dtype} tensor of shape {expect} "
                          f"on {dev}")
+    elif overlap(out, qt) and not (out.data_ptr() == qt.data_ptr() and out.dtype == qt.dtype
+                                   and qt.is_contiguous()):
+        # (every kernel has read a row's queries when it stores that row)
+        raise ValueError("out may be q itself, but not share part of its memory")
     if batch.total_q == 0:               # no query row at all
         return out
     mods = _lib.CxAttnMods(batch.softcap or 0.0, _lib.cx_dtype(out_dtype),
@@ -315,7 +319,8 @@ def _attend_scored(cache, layer: int, q, batch: PagedBatch, out, replan, out_dty
 def decode_batch(cache, layer: int, q, batch: PagedBatch, out=None, replan=None,
                  out_dtype=None):
     """One query token per sequence: q (B, hq, D) -> (B, hq, D), float32 unless
-    ``out`` or ``out_dtype`` says bfloat16 or float16."""
+    ``out`` or ``out_dtype`` says bfloat16 or float16.  With modifiers or a
+    16-bit output, ``out`` may be ``q`` itself."""
     if batch.verify:
         raise ValueError("decode_batch needs a PagedBatch built without q_lens")
     return _attend(cache, layer, q, batch, out, replan, out_dtype, "cx_paged_decode")

@@ -300,7 +300,7 @@ typedef struct cx_attn_mods {
  *     seen = j < prefix  or  (j <= pos and (window <= 0 or j > pos - window))
  * over keys j < ctx_lens[b].  out is [rows][n_q_heads][head_dim] of
  * out_dtype, rounded once from the fp32 accumulators; a row that sees no key is
- * zero.  What the pool holds at positions that no query row of a sequence sees
+ * zero; out may be q itself (one type, contiguous) but not overlap it otherwise.  What the pool holds at positions that no query row of a sequence sees
  * (past the context in its last block, left of every row's window) does not
  * reach the result, NaN and infinity included; at a position that only some
  * rows see, V must be finite.  Sums are fp32 and their terms at most 2^8 |V|:

@@ -238,7 +238,8 @@ def test_reading_the_flags_waits_once(clear, most):
     from torch.profiler import ProfilerActivity, profile
 
     from chenxing_b200 import _lib
-    with profile(activities=[ProfilerActivity.CPU, ProfilerActivity.CUDA]) as prof:
+    with profile(activities=[ProfilerActivity.CPU, ProfilerActivity.CUDA],
+                 acc_events=True) as prof:
         assert _lib.device_flags(clear=clear) == 0
     waits = sum(e.count for e in prof.key_averages() if e.key == "cudaStreamSynchronize")
     assert 1 <= waits <= most
@@ -254,3 +255,36 @@ def test_flags_of_both_units_are_read_and_cleared(scored):
     assert _lib.device_flags(clear=False) == 2
     assert _lib.device_flags(clear=True) == 2
     assert _lib.device_flags(clear=True) == 0
+
+
+@pytest.mark.parametrize("hq,hk,d,dtype,q_lens,ctx", [
+    (8, 2, 128, BF, None, [900, 20000, 33]), (8, 2, 64, F16, [6, 3], [9000, 70]),
+    (4, 2, 128, F32, [3], [7000]), (8, 2, 128, BF, [300, 64], [700, 129]),
+    (4, 1, 64, F16, [40], [9000]), (6, 3, 96, BF, [5, 50], [300, 77])])
+def test_output_in_place_of_the_queries(hq, hk, d, dtype, q_lens, ctx):
+    c = ScoredCase(hq=hq, hk=hk, d=d, ctx=ctx, q_lens=q_lens, dtype=dtype, softcap=20.0)
+    batch = c.batch()
+    apart = c.run(batch, out_dtype=dtype)
+    c.check(apart)
+    own = c.q_dev.clone()
+    for _ in range(2):
+        c.q_dev = own.clone()
+        assert c.run(batch, out=c.q_dev).data_ptr() == c.q_dev.data_ptr()
+        assert torch.equal(c.q_dev, apart)
+
+
+def test_output_over_part_of_the_queries_is_refused():
+    c = ScoredCase(hq=8, hk=2, d=64, ctx=[70, 300], q_lens=[3, 2], softcap=20.0)
+    buf = torch.zeros(6, 8, 64, dtype=BF, device="cuda")
+    buf[:5] = c.q_dev
+    c.q_dev = buf[:5]
+    with pytest.raises(ValueError):
+        c.run(out=buf[1:])
+    with pytest.raises(ValueError):        # the same memory as another type
+        c.run(out=buf[:5].view(F16))
+    wide = torch.zeros(5, 12, 64, dtype=BF, device="cuda")
+    wide[:, :8] = c.q_dev
+    c.q_dev = wide[:, :8]
+    with pytest.raises(ValueError):
+        c.run(out=wide.flatten()[:5 * 8 * 64].view(5, 8, 64))
+    c.check(c.run(out=torch.empty(5, 8, 64, dtype=BF, device="cuda")))

@@ -187,3 +187,12 @@ def test_a_device_without_an_index_is_the_current_one(monkeypatch):
     assert _lib.require_cuda("cuda:1") == torch.device("cuda", 1)
     with pytest.raises(_lib.CxError):
         _lib.require_cuda("cpu")
+
+
+def test_overlap():
+    from chenxing_b200._arrays import overlap
+    x = torch.zeros(4, 6, 8)
+    assert overlap(x, x) and overlap(x[1:], x[:2]) and overlap(x[:, :2], x[:, 3:])
+    assert not overlap(x[:2], x[2:]) and not overlap(x[0, :3], x[0, 3:])
+    assert not overlap(x[:0], x) and not overlap(x, torch.zeros(4))
+    assert overlap(x[:1].expand(4, 6, 8), x[0]) and not overlap(x[:1].expand(4, 6, 8), x[1])
