@@ -672,6 +672,7 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
 #pragma unroll 1
                 for (int k = 0; k < D / 64; ++k) {
                     float ov[32];
+                    __syncwarp();          // padding rows have skipped the stores
                     if (n_tiles > 0) {
                         tc_ld32(tm_o + k * 32, ov);
                         tc_wait_ld();
