@@ -73,7 +73,7 @@ constexpr float kTanhC0 = 0.9999951345111643f, kTanhC1 = -0.3331742660309651f,
 // MmaParams.  tanh(z) of a warp's scores is the polynomial above while all of
 // them are in its range, else 1 - 2 / (1 + 2^(2 z log2 e)): two special-function
 // instructions, absolute error about 2^-22 (the score's error is that times the
-// cap).  The latter alone took 502 instead of 491 us for 128 chains of up to 5
+// cap).  The latter alone takes 448 instead of 445 us for 128 chains of up to 5
 // rows (window 4096).  The fp32 kernel calls tanhf.
 struct ScoreMod {
     float scale;             // scale / cap

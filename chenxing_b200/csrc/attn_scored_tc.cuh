@@ -21,8 +21,8 @@
 //                [64 c, 64 c + 64) of row r (TMEM lane r), 32 at a time, so that
 //                four warps an SM sub-partition fit.  Half c's P goes over its own
 //                S columns, [64 c, 64 c + 32).  Both halves of a row use one
-//                reference maximum, which follows only when a half's maximum grows
-//                by as much as P's type holds (exact after the final division), so
+//                reference maximum, which follows only when a half's maximum is far
+//                above the last one (Half16; exact after the final division), so that
 //                nearly all tiles need one pass and a vote of the two warps that
 //                share the rows.
 //
@@ -34,11 +34,15 @@
 // take a path with per-key tests.
 //
 // Measured, 4 sequences x 1024 rows behind 4k to 8k keys, 32 / 8 heads of 128,
-// bf16: 509 us uncapped (843 TFLOP/s), 611 us capped (702), 541 us with the
-// distance bias, 1015 us when nearly all scores are beyond the polynomials; 405 us
-// with the softmax left out, the MMAs at cuBLAS's rate 263 us.  What bounds it is
-// the chain S -> softmax -> P -> PV of each tile, which TMEM (512 columns: two S,
-// two O) leaves no room to run ahead of.
+// bf16: 530 us uncapped (805 TFLOP/s), 649 us capped (660), 567 us with the
+// distance bias, 682 us with both, 1016 us when nearly all scores are beyond the
+// polynomials; the MMAs at cuBLAS's rate would take 263 us.  The tensor pipe is
+// active 35 % of the time and the issue slots are 56 % taken: each tile is a chain
+// S -> softmax -> P -> PV -> next S, and for heads of 128 two S and two O fill the
+// 512 TMEM columns, so that no whole third S runs ahead (two half-width S a tile
+// were not tried; heads of 64 leave 128 columns).  6 ragged prompts of up to 700
+// rows, 16 heads of 64, fp16, prefix and bias: 90 us for 6.3 us of MMAs; 288 CTAs,
+// one an SM, are two waves, with the tensor pipe active 10 % of the time.
 //
 // V rows that no row of the CTA sees (past the context, past the last row's
 // position, left of the first row's window, all past the prefix) are zeroed in
@@ -481,9 +485,9 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
                 };
                 // ---- p = 2^(x - m) as 16-bit pairs, and this half's row maximum, in one
                 // pass against the reference maximum so far; again, against a new one,
-                // when the maximum grew by more than kRescale, or key by key when a score
+                // when the maximum is kRescale above it, or key by key when a score
                 // was beyond the polynomial.  Both are rare past the first tile, and the
-                // exponentials need not wait for a maximum.  (A limit of 2^8, as the
+                // exponentials need not wait for a maximum.  (A growth of 2^8 alone, as the
                 // kernels beside this one have, took 712 instead of 548 us here: some of
                 // 32 rows grows by that in every few tiles.) ----
                 // one packed expression scores a pair: all keys seen, none ahead of its

@@ -382,8 +382,10 @@ __device__ __forceinline__ void pairs_chunk(const f2 (&x)[V / 2], Chunk<T, V>& c
 // registers and the arithmetic on packed pairs; chunks of four elements, so that
 // fp32 loads from shared memory are contiguous across lanes.
 // 8192 tokens of 48 rows of 128 bf16 (210 MB, 32 us at the HBM copy rate) take
-// 46 us, bound by instruction issue (68 % of the slots); the same arithmetic on
-// scalars takes 48.  What was tried before: the register form, 68 us (a thread
+// 45 us.  Issue slots are 69 % taken, DRAM 42 % busy; warps wait in about equal
+// parts for fixed latencies, shared memory and their turn to issue.  The same
+// arithmetic on scalars took 48 where this took 46; what was tried before, at the
+// same time: the register form, 68 us (a thread
 // waits for the position, then for cos / sin, with 32 bytes of its row in
 // flight) and 121 us with four rows a thread (one block an SM); per-thread
 // copies and one CTA barrier a token, 76 us; chunks of eight, where cos / sin and

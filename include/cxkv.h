@@ -300,16 +300,21 @@ typedef struct cx_attn_mods {
  *     seen = j < prefix  or  (j <= pos and (window <= 0 or j > pos - window))
  * over keys j < ctx_lens[b].  out is [rows][n_q_heads][head_dim] of
  * out_dtype, rounded once from the fp32 accumulators; a row that sees no key is
- * zero; out may be q itself (one type, contiguous) but not overlap it otherwise.  What the pool holds at positions that no query row of a sequence sees
- * (past the context in its last block, left of every row's window) does not
- * reach the result, NaN and infinity included; at a position that only some
- * rows see, V must be finite.  Sums are fp32 and their terms at most 2^8 |V|:
- * |V| below 2^96 overflows in no context of up to 2^23 keys (bf16 pools keep
- * their bits down to |V| of 2^-74).  Workspace: cx_paged_attend_workspace_bytes,
- * zero-filled once; a plan made by cx_paged_decode / cx_paged_verify does not
- * serve this call, nor the other way round, nor one for another window or made
- * without the prefix (replan = 0 then raises CX_DEV_BAD_QLEN and leaves out as
- * it was). */
+ * zero.  out may be q itself (one type, contiguous), but not overlap it
+ * otherwise.
+ * What the pool holds at positions that no query row of a sequence sees (past
+ * the context in its last block, left of every row's window) does not reach the
+ * result, NaN and infinity included; at a position that only some rows see, V
+ * must be finite.
+ * Over 16-bit pools the tensor-core kernels round fp32 queries, and the softmax
+ * probabilities, to the pool's type; the denominator sums the rounded ones.
+ * Over bf16 and fp32 pools the terms of the fp32 sums are at most 2^8 |V|: |V|
+ * below 2^96 overflows in no context of up to 2^23 keys (bf16 pools keep their
+ * bits down to |V| of 2^-74).
+ * Workspace: cx_paged_attend_workspace_bytes, zero-filled once; a plan made by
+ * cx_paged_decode / cx_paged_verify does not serve this call, nor the other way
+ * round, nor one for another window or made without the prefix (replan = 0 then
+ * raises CX_DEV_BAD_QLEN and leaves out as it was). */
 int cx_paged_attend(const cx_pool* pool, int64_t layer, const cx_attn_batch* batch,
                     const cx_attn_mods* mods, const void* q, int32_t q_dtype, void* out,
                     void* workspace, size_t workspace_bytes, int32_t replan, void* stream);
