@@ -83,7 +83,8 @@ class PagedBatch:
       keeps); what lies past the context is cut off.
 
     A batch holds one workspace: its calls run in order on one stream, the one
-    it was made on.
+    it was made on.  A captured graph reads the device arrays of its capture:
+    after ``set`` or ``advance`` it is captured again.
     """
 
     def __init__(self, cache, block_tables, ctx_lens, *, n_q_heads: int, q_lens=None,
