@@ -289,7 +289,7 @@ def _prepare_accept(case, seed):
         from chenxing_b200 import LatentBatch, LatentPagedKVCache, PagedBatch, RadixPagedKVCache
         q_lens = [case["nodes"]] * case["B"]
         if case["latent"]:
-            cache = LatentPagedKVCache(nb, BLOCK, case["layers"], case["d"] - 32, 32, dtype=dt,
+            cache = LatentPagedKVCache(nb, BLOCK, case["layers"], case["d"] - 64, 64, dtype=dt,
                                        host_io=False)
             cache.kv_pool.copy_(s["pools"][0][..., 0, :])
             s["batch"] = LatentBatch(cache, tables, ctx, n_q_heads=1, q_lens=q_lens, scale=1.0)
