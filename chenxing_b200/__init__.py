@@ -9,6 +9,7 @@ library is loaded on first use and there is no CPU fallback.
 from .attention import flash_attention, gqa_expand, naive_attention
 from .batch import PagedBatch, decode_batch, slot_mapping, verify_batch
 from .engine import BatchedKVEngine
+from .latent import LatentBatch, LatentPagedKVCache
 from .radix_kv import OutOfKVCacheError, PrefixHit, RadixIndex, RadixPagedKVCache
 from .rope import RopeTables, build_rope_cache
 from .tensor import CausalMask
@@ -16,4 +17,4 @@ from .tensor import CausalMask
 __all__ = ["RadixPagedKVCache", "RadixIndex", "PrefixHit", "OutOfKVCacheError",
            "flash_attention", "naive_attention", "gqa_expand", "CausalMask",
            "PagedBatch", "decode_batch", "verify_batch", "slot_mapping", "BatchedKVEngine",
-           "RopeTables", "build_rope_cache"]
+           "LatentPagedKVCache", "LatentBatch", "RopeTables", "build_rope_cache"]

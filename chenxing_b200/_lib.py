@@ -23,13 +23,16 @@ CX_F32, CX_BF16, CX_F16 = 0, 1, 2
 # device flag bits
 DEV_FLAG_NAMES = {1: "bad slot", 2: "bad block id", 4: "context longer than its block table",
                   8: "pipeline wait timeout", 16: "bad query length",
-                  32: "RoPE position outside the table"}
+                  32: "RoPE position outside the table", 64: "bad path of accepted nodes"}
 
 EXPORTS = ("cx_version", "cx_last_error", "cx_device_error", "cx_kv_append", "cx_kv_gather",
            "cx_block_copy", "cx_paged_workspace_bytes", "cx_paged_decode", "cx_paged_verify",
            "cx_attention_dense", "cx_paged_decode_static", "cx_paged_kernel_kind",
            "cx_kv_append_rope", "cx_set_wait_limit_ns", "cx_kv_append_norm_rope",
-           "cx_paged_attend", "cx_paged_attend_workspace_bytes", "cx_paged_attend_kind")
+           "cx_paged_attend", "cx_paged_attend_workspace_bytes", "cx_paged_attend_kind",
+           "cx_paged_attend_tree", "cx_kv_accept", "cx_latent_append", "cx_latent_gather",
+           "cx_latent_block_copy", "cx_latent_accept", "cx_latent_attend",
+           "cx_latent_attend_workspace_bytes", "cx_latent_attend_kind")
 KERNEL_KINDS = {0: "generic", 1: "mma", 2: "tcgen05", 3: "fma"}
 
 
@@ -72,6 +75,33 @@ class CxAttnMods(ctypes.Structure):
                 ("q_stride", ctypes.c_int64)]
 
 
+class CxTree(ctypes.Structure):
+    _fields_ = [("masks", ctypes.c_void_p), ("words", ctypes.c_int64),
+                ("depths", ctypes.c_void_p)]
+
+
+class CxLatentPool(ctypes.Structure):
+    _fields_ = [("kv", ctypes.c_void_p), ("n_layers", ctypes.c_int64),
+                ("n_blocks", ctypes.c_int64), ("block_size", ctypes.c_int64),
+                ("latent_dim", ctypes.c_int64), ("rope_dim", ctypes.c_int64),
+                ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class CxLatentRows(ctypes.Structure):
+    _fields_ = [("latent", ctypes.c_void_p), ("rope", ctypes.c_void_p), ("q", ctypes.c_void_p),
+                ("latent_token_stride", ctypes.c_int64), ("rope_token_stride", ctypes.c_int64),
+                ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+                ("n_tokens", ctypes.c_int64), ("n_q_heads", ctypes.c_int64),
+                ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class CxLatentQ(ctypes.Structure):
+    _fields_ = [("latent", ctypes.c_void_p), ("rope", ctypes.c_void_p),
+                ("latent_token_stride", ctypes.c_int64), ("latent_head_stride", ctypes.c_int64),
+                ("rope_token_stride", ctypes.c_int64), ("rope_head_stride", ctypes.c_int64),
+                ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
 class CxError(RuntimeError):
     """A libcxkv call returned a non-OK status."""
 
@@ -112,6 +142,26 @@ _SIGS = {
                                         ctypes.c_size_t),
     "cx_paged_attend_kind": ([ctypes.POINTER(CxPool), ctypes.POINTER(CxAttnBatch), _I32],
                              ctypes.c_int),
+    "cx_paged_attend_tree": ([ctypes.POINTER(CxPool), _I64, ctypes.POINTER(CxAttnBatch),
+                              ctypes.POINTER(CxAttnMods), ctypes.POINTER(CxTree), _VP, _I32, _VP,
+                              _VP, ctypes.c_size_t, _I32, _VP], ctypes.c_int),
+    "cx_kv_accept": ([ctypes.POINTER(CxPool), ctypes.POINTER(CxAttnBatch), _VP, _I64, _I64, _VP],
+                     ctypes.c_int),
+    "cx_latent_append": ([ctypes.POINTER(CxLatentPool), _I64, ctypes.POINTER(CxLatentRows), _VP,
+                          _VP, ctypes.POINTER(CxNormRope), _VP, _I32, _VP], ctypes.c_int),
+    "cx_latent_gather": ([ctypes.POINTER(CxLatentPool), _I64, _VP, _I64, _VP, _VP, _VP],
+                         ctypes.c_int),
+    "cx_latent_block_copy": ([ctypes.POINTER(CxLatentPool), _I64, _VP, _VP, _VP, _I64, _I64, _VP],
+                             ctypes.c_int),
+    "cx_latent_accept": ([ctypes.POINTER(CxLatentPool), ctypes.POINTER(CxAttnBatch), _VP, _I64,
+                          _I64, _VP], ctypes.c_int),
+    "cx_latent_attend": ([ctypes.POINTER(CxLatentPool), _I64, ctypes.POINTER(CxAttnBatch),
+                          ctypes.POINTER(CxTree), ctypes.POINTER(CxLatentQ), _VP, _I32, _VP,
+                          ctypes.c_size_t, _VP], ctypes.c_int),
+    "cx_latent_attend_workspace_bytes": ([ctypes.POINTER(CxLatentPool),
+                                          ctypes.POINTER(CxAttnBatch)], ctypes.c_size_t),
+    "cx_latent_attend_kind": ([ctypes.POINTER(CxLatentPool), ctypes.POINTER(CxAttnBatch), _I32],
+                              ctypes.c_int),
 }
 
 

@@ -11,6 +11,8 @@ and ``n_tokens`` values; nothing here changes them.
 
 A batch may also change the scores (``softcap``, ``alibi_slopes``,
 ``prefix_lens``) or ask for a 16-bit output; ``cx_paged_attend`` serves those.
+Its query rows may be the nodes of a drafted tree per sequence
+(``tree_parents``), which ``cx_paged_attend_tree`` serves.
 """
 from __future__ import annotations
 
@@ -63,6 +65,43 @@ def _same_start(a, b) -> bool:
     return list(a[:n]) == list(b[:n]) and (n > 0 or len(a) == len(b))
 
 
+def tree_arrays(parents, q_lens, window: int = 0):
+    """(masks, depths) of a drafted tree per sequence, rows concatenated: masks
+    (rows, words) uint32, bit u set where the row sees node u (itself and its
+    ancestors, with ``window`` > 0 the nearest ``window`` of them); depths (rows,)
+    int32, a node's ancestors.  ``parents[b][i]``: node i's parent, below i, or -1
+    behind the committed context."""
+    q_lens = np.asarray(q_lens, dtype=np.int64).reshape(-1)
+    if len(parents) != q_lens.shape[0] or any(len(p) != n for p, n in zip(parents, q_lens)):
+        raise ValueError("tree_parents must be one list per sequence with one parent per query "
+                         "token")
+    total, words = int(q_lens.sum()), max(1, -(-int(q_lens.max(initial=1)) // 32))
+    own = np.concatenate([np.arange(n) for n in q_lens] or [np.zeros(0, np.int64)]).astype(np.int64)
+    up = np.concatenate([np.asarray(p, dtype=np.int64).reshape(-1) for p in parents]
+                        or [np.zeros(0, np.int64)])
+    if np.any(up < -1) or np.any(up >= own):
+        raise ValueError("tree_parents: a node's parent comes before it, or is -1")
+    first = np.repeat(np.cumsum(q_lens) - q_lens, q_lens)
+    up = np.where(up < 0, -1, up + first)                   # rows
+    masks = np.zeros((total, words), dtype=np.uint32)
+    masks[np.arange(total), own >> 5] = np.uint32(1) << (own & 31).astype(np.uint32)
+    depths = np.where(up < 0, 0, -1).astype(np.int32)
+    level = np.flatnonzero(up >= 0)
+    while level.size:                                       # children of what is done
+        ready = depths[up[level]] >= 0
+        rows = level[ready]
+        depths[rows] = depths[up[rows]] + 1
+        masks[rows] |= masks[up[rows]]
+        level = level[~ready]
+    if window > 0 and depths.max(initial=0) >= window:
+        far = np.flatnonzero(depths >= window)              # rows with an ancestor out of sight
+        at = far
+        for _ in range(window):
+            at = up[at]
+        masks[far] &= ~masks[at].copy()
+    return masks, depths
+
+
 class PagedBatch:
     """Device metadata + workspace for batched decode / verify on one cache.
 
@@ -82,6 +121,14 @@ class PagedBatch:
       first tokens see one another) and the window (tokens that a long stream
       keeps); what lies past the context is cut off.
 
+    ``tree_parents`` (with ``q_lens``): the query rows of a sequence are the nodes of
+    a drafted tree, parents before children; ``tree_parents[b][i]`` is node i's parent
+    or -1 behind the committed context.  Node i's K/V are at position
+    ``ctx_lens[b] - q_lens[b] + i``; it sees the committed context and its own
+    ancestors, and stands ``depths_host`` steps behind the last committed token (for
+    the window, the bias and its rotation, ``row_positions``).  A prefix ends where the
+    tree begins.  ``cache.accept_paths`` then keeps a path of the tree.
+
     A batch holds one workspace: its calls run in order on one stream, the one
     it was made on.  A captured graph reads the device arrays of its capture:
     after ``set`` or ``advance`` it is captured again.
@@ -90,7 +137,7 @@ class PagedBatch:
     def __init__(self, cache, block_tables, ctx_lens, *, n_q_heads: int, q_lens=None,
                  window: int | None = None, scale: float | None = None,
                  table_stride: int | None = None, softcap: float | None = None,
-                 alibi_slopes=None, prefix_lens=None) -> None:
+                 alibi_slopes=None, prefix_lens=None, tree_parents=None) -> None:
         self.cache = cache
         self.device = cache.device
         self.n_q_heads = int(n_q_heads)
@@ -101,6 +148,10 @@ class PagedBatch:
             raise ValueError("window must be positive (or None)")
         self.scale = (1.0 / math.sqrt(cache.head_dim)) if scale is None else float(scale)
         self.verify = q_lens is not None
+        self.is_tree = tree_parents is not None
+        if self.is_tree and not self.verify:
+            raise ValueError("tree_parents needs q_lens")
+        self.tree_parents = self.depths_host = self._tree = self._tree_dev = None
         self.table_stride = table_stride
         self.softcap = None if softcap is None else float(softcap)
         if softcap is not None and not (1e-30 <= self.softcap <= 1e30):
@@ -120,13 +171,15 @@ class PagedBatch:
         self._planned_by = None          # entry point that made the workspace's plan
         self._ws = None
         self._ws_bytes = 0
-        self.set(block_tables, ctx_lens, q_lens, prefix_lens)
+        self.set(block_tables, ctx_lens, q_lens, prefix_lens, tree_parents)
 
     # ------------------------------------------------------------------ #
-    def set(self, block_tables, ctx_lens, q_lens=None, prefix_lens=None) -> None:
+    def set(self, block_tables, ctx_lens, q_lens=None, prefix_lens=None,
+            tree_parents=None) -> None:
         """(Re)load tables and lengths; the next attention call re-plans.  Without
         ``prefix_lens`` a batch that has some keeps them, for the same sequences:
-        as many, and each table the one before, grown or cut."""
+        as many, and each table the one before, grown or cut.  A batch made with
+        ``tree_parents`` takes new ones every time."""
         bs = self.cache.block_size
         B = len(block_tables)
         ctx = np.asarray(ctx_lens, dtype=np.int64).reshape(-1)
@@ -165,6 +218,12 @@ class PagedBatch:
                 raise ValueError("q_lens must be per sequence and <= ctx_lens")
             qs = np.zeros(B + 1, dtype=np.int64)
             np.cumsum(ql, out=qs[1:])
+        if (tree_parents is not None) != self.is_tree:
+            raise ValueError("tree_parents must be given again for a batch made with them, and "
+                             "for no other")
+        if self.is_tree:
+            tree_parents = [list(p) for p in tree_parents]
+            masks, depths = tree_arrays(tree_parents, ql, self.window)
         # nothing is refused from here on: a batch is reloaded whole or stays as it was
         self.needs_plan = True
         tab = np.zeros((B, stride), dtype=np.int32)
@@ -189,19 +248,38 @@ class PagedBatch:
                                    self.ctx_lens.data_ptr(),
                                    _lib.ptr(self.q_start), B, self.max_q, self.n_q_heads,
                                    self.scale, 0, self.window)
+        if self.is_tree:
+            self.tree_parents, self.depths_host = tree_parents, depths
+            self._tree_dev = (upload(masks.view(np.int32), self.device),
+                              upload(depths, self.device))
+            self._tree = _lib.CxTree(self._tree_dev[0].data_ptr(), masks.shape[1],
+                                     self._tree_dev[1].data_ptr())
         if pre is not None:
             self.prefix_host = np.minimum(pre, np.iinfo(np.int32).max)
             self.prefix_lens = upload(self.prefix_host.astype(np.int32), self.device)
-        need = max(int(_lib.lib().cx_paged_workspace_bytes(self.cache.cx_pool(), self._c)),
-                   int(_lib.lib().cx_paged_attend_workspace_bytes(self.cache.cx_pool(), self._c)))
+        need = self._workspace_need()
         if need > self._ws_bytes:
             self._ws = torch.zeros(need, dtype=torch.uint8, device=self.device)
             self._ws_bytes = need
 
+    def _workspace_need(self) -> int:
+        pool = self.cache.cx_pool()
+        return max(int(_lib.lib().cx_paged_workspace_bytes(pool, self._c)),
+                   int(_lib.lib().cx_paged_attend_workspace_bytes(pool, self._c)))
+
     def advance(self, n: int = 1) -> None:
         """Every context grows by ``n`` tokens (one decode step); re-plans."""
         self.set(self.tables_host, self.ctx_host + n,
-                 self.q_lens_host if self.verify else None)
+                 self.q_lens_host if self.verify else None, tree_parents=self.tree_parents)
+
+    def row_positions(self) -> np.ndarray:
+        """The position of every query row (int64, rows concatenated): where its
+        rotation turns it to.  A node of a tree stands by its depth."""
+        base = np.repeat(self.ctx_host - self.q_lens_host, self.q_lens_host)
+        if self.is_tree:
+            return base + self.depths_host
+        return base + np.concatenate([np.arange(n) for n in self.q_lens_host]
+                                     or [np.zeros(0, np.int64)]).astype(np.int64)
 
     @property
     def kv_tokens(self) -> int:
@@ -227,7 +305,7 @@ class PagedBatch:
     def scored(self) -> bool:
         """Whether the batch changes the scores or the visible keys."""
         return self.softcap is not None or self.alibi_slopes is not None \
-            or self.prefix_lens is not None
+            or self.prefix_lens is not None or self.is_tree
 
     def takes_attend(self, out_dtype) -> bool:
         """Whether calls with this output type are ``cx_paged_attend``'s."""
@@ -281,7 +359,8 @@ def _plans(batch: PagedBatch, replan, by: str) -> bool:
 
 
 def _attend_scored(cache, layer: int, q, batch: PagedBatch, out, replan, out_dtype):
-    """``cx_paged_attend``: score modifiers, 16-bit outputs, strided query rows."""
+    """``cx_paged_attend`` and ``cx_paged_attend_tree``: score modifiers, 16-bit
+    outputs, strided query rows."""
     dev = cache.device
     qt = rows_on_device(q, dev)
     hq, d = batch.n_q_heads, cache.head_dim
@@ -306,11 +385,16 @@ def _attend_scored(cache, layer: int, q, batch: PagedBatch, out, replan, out_dty
                            _lib.ptr(batch.alibi_slopes), _lib.ptr(batch.prefix_lens),
                            0 if qt.is_contiguous() else qt.stride(0))
     do_plan = _plans(batch, replan, "scored")
+    rest = (qt.data_ptr(), _lib.cx_dtype(qt.dtype), out.data_ptr(), batch.workspace.data_ptr(),
+            batch.workspace.numel(), int(do_plan), _lib.raw_stream(dev))
     with _lib.on_device(dev):
-        _lib.check(_lib.lib().cx_paged_attend(
-            cache.cx_pool(), int(layer), batch.c_struct(), mods, qt.data_ptr(),
-            _lib.cx_dtype(qt.dtype), out.data_ptr(), batch.workspace.data_ptr(),
-            batch.workspace.numel(), int(do_plan), _lib.raw_stream(dev)), "cx_paged_attend")
+        if batch.is_tree:
+            _lib.check(_lib.lib().cx_paged_attend_tree(
+                cache.cx_pool(), int(layer), batch.c_struct(), mods, batch._tree, *rest),
+                "cx_paged_attend_tree")
+        else:
+            _lib.check(_lib.lib().cx_paged_attend(
+                cache.cx_pool(), int(layer), batch.c_struct(), mods, *rest), "cx_paged_attend")
     if do_plan:
         batch.needs_plan = False
         batch._planned_by = "scored"
@@ -329,8 +413,8 @@ def decode_batch(cache, layer: int, q, batch: PagedBatch, out=None, replan=None,
 
 def verify_batch(cache, layer: int, q, batch: PagedBatch, out=None, replan=None,
                  out_dtype=None):
-    """q_lens[b] query tokens per sequence (speculative verify / prefill chunk):
-    q (sum q_lens, hq, D) -> (sum q_lens, hq, D), float32 unless ``out`` or
+    """q_lens[b] query tokens per sequence (speculative verify, chains or trees /
+    prefill chunk): q (sum q_lens, hq, D) -> (sum q_lens, hq, D), float32 unless ``out`` or
     ``out_dtype`` says bfloat16 or float16."""
     if not batch.verify:
         raise ValueError("verify_batch needs a PagedBatch built with q_lens")

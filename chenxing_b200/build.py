@@ -2,8 +2,8 @@
 
     python -m chenxing_b200.build
 
-The library is two translation units (csrc/cxkv.cu and csrc/cxkv_scored.cu
-include the parts; compiled side by side), linked against the static CUDA
+The library is four translation units (the csrc/*.cu include the parts;
+compiled side by side), linked against the static CUDA
 runtime, so it only needs the NVIDIA driver at run time.  Rebuilds unless the
 stamp file beside the library records the SHA-256 of exactly the current
 sources, headers, nvcc flags and nvcc version (file times are not trusted: a
@@ -25,7 +25,7 @@ ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libcxkv.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O2", "-Xptxas", "-v"]
-UNITS = ("cxkv.cu", "cxkv_scored.cu")
+UNITS = ("cxkv.cu", "cxkv_scored.cu", "cxkv_tree.cu", "cxkv_latent.cu")
 
 
 def sources():

@@ -48,6 +48,7 @@ struct GenericParams {
     const int32_t* q_start;  // NULL: one query per sequence
     cx_attn_mods mod;        // read by the MOD instantiations only
     void* mod_out;           // their output, of mod.out_dtype
+    TreeMask tree;           // read by the TREE instantiations only
 };
 
 constexpr int kGenRows = 8;     // packed rows per CTA
@@ -81,8 +82,8 @@ struct GenSmem {
 };
 
 // MOD (paged only): tanh cap, distance bias, visible prefix, strided queries and
-// output type of cx_paged_attend.
-template <typename QT, typename KT, bool PAGED, bool MOD = false>
+// output type of cx_paged_attend.  TREE: the rows are nodes of drafted trees.
+template <typename QT, typename KT, bool PAGED, bool MOD = false, bool TREE = false>
 __global__ void __launch_bounds__(kGenWarps * 32) attn_generic_kernel(GenericParams p) {
     extern __shared__ float gsm[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -133,6 +134,7 @@ __global__ void __launch_bounds__(kGenWarps * 32) attn_generic_kernel(GenericPar
     int64_t pre = 0;                                   // keys every row sees
     if constexpr (MOD) {
         if (p.mod.prefix_lens) pre = min(max((int64_t)p.mod.prefix_lens[b], (int64_t)0), sk);
+        if constexpr (TREE) pre = min(pre, max(sk - sq, (int64_t)0));
     }
     // key range over all rows of the CTA: [lo_all, hi_all]
     int64_t lo_all = sk, hi_all = -1;
@@ -141,7 +143,8 @@ __global__ void __launch_bounds__(kGenWarps * 32) attn_generic_kernel(GenericPar
         int64_t lo = 0, hi = sk - 1;
         if (p.mask_kind == 1) {
             hi = pos < hi ? pos : hi;
-            if (p.window > 0) lo = pos - p.window + 1 > 0 ? pos - p.window + 1 : 0;
+            const int64_t at = TREE ? sk - sq : pos;     // (a node stands at sk - sq or behind)
+            if (p.window > 0) lo = at - p.window + 1 > 0 ? at - p.window + 1 : 0;
         }
         if (hi >= lo) {
             lo_all = lo < lo_all ? lo : lo_all;
@@ -292,7 +295,19 @@ __global__ void __launch_bounds__(kGenWarps * 32) attn_generic_kernel(GenericPar
             bool ok = r < nr && ((valid >> j) & 1u);
             if (ok) {
                 const int64_t iq = (r0 + r) / G, pos = sk - sq + iq;
-                if constexpr (MOD) {
+                if constexpr (TREE) {
+                    const int64_t base = sk - sq, at = base + p.tree.depths[q0 + iq];
+                    ok = key < base ? key < pre || p.window <= 0 || key > at - p.window
+                                    : tree_bits(p.tree, q0 + iq, (int)iq, (int)(key - base)) & 1u;
+                    if (p.mod.softcap > 0.f) sc = p.mod.softcap * tanhf(sc / p.mod.softcap);
+                    if (p.mod.alibi_slopes) {
+                        const int64_t to = key < base ? key
+                                                      : tree_key_pos(p.tree, q0, (int)sq, (int)base,
+                                                                     (int)(key - base));
+                        const int64_t dist = at > to ? at - to : to - at;
+                        sc -= p.mod.alibi_slopes[kh * G + (r0 + r) % G] * (float)dist;
+                    }
+                } else if constexpr (MOD) {
                     ok = key < pre || (key <= pos && (p.window <= 0 || key > pos - p.window));
                     if (p.mod.softcap > 0.f)
                         sc = p.mod.softcap * tanhf(sc / p.mod.softcap);
@@ -413,24 +428,24 @@ __global__ void __launch_bounds__(kGenWarps * 32) attn_generic_kernel(GenericPar
     }
 }
 
-template <bool PAGED, typename QT, bool MOD>
+template <bool PAGED, typename QT, bool MOD, bool TREE>
 static int launch_generic_kv(int32_t kvdt, const GenericParams& p, dim3 grid, size_t smem,
                              cudaStream_t st) {
     switch (kvdt) {
         case CX_F32: {
-            auto k = attn_generic_kernel<QT, float, PAGED, MOD>;
+            auto k = attn_generic_kernel<QT, float, PAGED, MOD, TREE>;
             CX_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
             k<<<grid, kGenWarps * 32, smem, st>>>(p);
             break;
         }
         case CX_BF16: {
-            auto k = attn_generic_kernel<QT, __nv_bfloat16, PAGED, MOD>;
+            auto k = attn_generic_kernel<QT, __nv_bfloat16, PAGED, MOD, TREE>;
             CX_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
             k<<<grid, kGenWarps * 32, smem, st>>>(p);
             break;
         }
         case CX_F16: {
-            auto k = attn_generic_kernel<QT, __half, PAGED, MOD>;
+            auto k = attn_generic_kernel<QT, __half, PAGED, MOD, TREE>;
             CX_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
             k<<<grid, kGenWarps * 32, smem, st>>>(p);
             break;
@@ -440,7 +455,7 @@ static int launch_generic_kv(int32_t kvdt, const GenericParams& p, dim3 grid, si
     return check_launch("attn_generic_kernel");
 }
 
-template <bool PAGED, bool MOD = false>
+template <bool PAGED, bool MOD = false, bool TREE = false>
 static int launch_generic(int32_t qdt, int32_t kvdt, const GenericParams& p, cudaStream_t st) {
     const int64_t G = p.hq / p.hk;
     const int64_t rows = G * p.max_q;
@@ -451,9 +466,9 @@ static int launch_generic(int32_t qdt, int32_t kvdt, const GenericParams& p, cud
     const size_t smem = GenSmem::of(p.d, p.dv).bytes(p.dv);
     dim3 grid((unsigned)(p.batch * p.hk), (unsigned)gy);
     switch (qdt) {
-        case CX_F32: return launch_generic_kv<PAGED, float, MOD>(kvdt, p, grid, smem, st);
-        case CX_BF16: return launch_generic_kv<PAGED, __nv_bfloat16, MOD>(kvdt, p, grid, smem, st);
-        case CX_F16: return launch_generic_kv<PAGED, __half, MOD>(kvdt, p, grid, smem, st);
+        case CX_F32: return launch_generic_kv<PAGED, float, MOD, TREE>(kvdt, p, grid, smem, st);
+        case CX_BF16: return launch_generic_kv<PAGED, __nv_bfloat16, MOD, TREE>(kvdt, p, grid, smem, st);
+        case CX_F16: return launch_generic_kv<PAGED, __half, MOD, TREE>(kvdt, p, grid, smem, st);
         default: return fail(CX_ERR_DTYPE, "attention: unknown query dtype");
     }
 }

@@ -72,7 +72,7 @@ struct F32Cfg {
     }
 };
 
-template <int D, int HG, int RT, bool MOD = false>
+template <int D, int HG, int RT, bool MOD = false, bool TREE = false>
 __global__ void __launch_bounds__(MOD ? F32Cfg<D, HG, RT>::MAX_THREADS_MOD
                                       : F32Cfg<D, HG, RT>::MAX_THREADS, 1)
     paged_attn_f32_kernel(const __grid_constant__ CUtensorMap tmk,
@@ -160,7 +160,8 @@ __global__ void __launch_bounds__(MOD ? F32Cfg<D, HG, RT>::MAX_THREADS_MOD
         const int64_t qs = p.q_start ? p.q_start[b] : b;
         const int rows_b = G * sq;
         const int pos0 = ctx - sq;  // position of query row 0
-        const int pre = MOD ? prefix_of(p, b, ctx) : 0;
+        const int pre = MOD ? prefix_of(p, b, TREE ? max(pos0, 0) : ctx) : 0;
+        const int all_pos = TREE ? pos0 - 1 : pos0;   // the last key that every row sees
         const DeadTok dead{ctx, MOD && p.window > 0 ? pos0 - p.window + 1 : 0, pre};
 
         // stage the group's query rows (fp32, zero padding rows): tile
@@ -207,6 +208,15 @@ __global__ void __launch_bounds__(MOD ? F32Cfg<D, HG, RT>::MAX_THREADS_MOD
         for (int i = 0; i < RPL; ++i) {
             const int R = mt * RT + rh + 2 * i;
             rpos[i] = R < rows_b ? pos0 + R / G : -1;
+        }
+        int dpos[RPL];      // where the rows stand
+#pragma unroll
+        for (int i = 0; i < RPL; ++i) {
+            dpos[i] = rpos[i];
+            if constexpr (TREE) {
+                const int R = mt * RT + rh + 2 * i;
+                if (R < rows_b) dpos[i] = pos0 + p.mod.tree.depths[qs + R / G];
+            }
         }
         float slope[RPL];   // MOD: this lane's rows' slopes (base 2)
         if constexpr (MOD) {
@@ -266,7 +276,7 @@ __global__ void __launch_bounds__(MOD ? F32Cfg<D, HG, RT>::MAX_THREADS_MOD
                 }
                 const int t0 = seg_block<MOD>(seg, k) * kBlockTok;
                 bool edge =
-                    (t0 + kBlockTok - 1 > pos0) || (p.window > 0 && t0 <= ctx - 1 - p.window);
+                    (t0 + kBlockTok - 1 > all_pos) || (p.window > 0 && t0 <= ctx - 1 - p.window);
                 if constexpr (MOD) edge = edge && t0 + kBlockTok > pre;
                 float x[RPL], mx[RPL];
 #pragma unroll
@@ -276,13 +286,28 @@ __global__ void __launch_bounds__(MOD ? F32Cfg<D, HG, RT>::MAX_THREADS_MOD
                         if (p.mod.cap_log2 != 0.f)
                             x[i] = p.mod.cap_log2 * tanhf((sa[i] + sb[i]) * p.mod.scale);
                         if (p.mod.slopes)
-                            x[i] = fmaf(-slope[i], (float)abs(rpos[i] - (t0 + t)), x[i]);
+                        {
+                            int tok = t0 + t;
+                            if (TREE && tok >= pos0)
+                                tok = tree_key_pos(p.mod.tree, qs, sq, pos0, tok - pos0);
+                            x[i] = fmaf(-slope[i], (float)abs(dpos[i] - tok), x[i]);
+                        }
                     }
                     if (edge) {
                         const int tok = t0 + t;
-                        if (!((MOD && tok < pre) ||
-                              (tok <= rpos[i] && (p.window <= 0 || tok > rpos[i] - p.window))))
-                            x[i] = -INFINITY;
+                        bool sees;
+                        if constexpr (TREE) {
+                            const int R = mt * RT + rh + 2 * i;
+                            if (tok < pos0)
+                                sees = tok < pre || p.window <= 0 || tok > dpos[i] - p.window;
+                            else
+                                sees = R < rows_b && (tree_bits(p.mod.tree, qs + R / G, R / G,
+                                                                tok - pos0) & 1u);
+                        } else {
+                            sees = (MOD && tok < pre) ||
+                                   (tok <= rpos[i] && (p.window <= 0 || tok > rpos[i] - p.window));
+                        }
+                        if (!sees) x[i] = -INFINITY;
                     }
                     float v = x[i];
                     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));

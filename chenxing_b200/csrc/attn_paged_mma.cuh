@@ -34,20 +34,16 @@
 //
 // The MOD instantiations (cx_paged_attend) run the same units with the scores
 // capped and biased, a prefix of keys that every row sees, the pool's element
-// type E (bf16 or fp16), strided queries and an output of any type.
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
+// type E (bf16 or fp16), strided queries and an output of any type.  TREE
+// (cx_paged_attend_tree): the query rows are the nodes of a drafted tree; units
+// that hold drafted keys are masked by 32 bits of each row's word.
 #include <atomic>
-#include <mutex>
 #include <type_traits>
 
 #include "cx_common.cuh"  // unity build: included from cxkv.cu
+#include "tma_map.cuh"
 
 namespace cx {
-
-constexpr int kBlockTok = 16;
-constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s per wait
 
 #ifdef CX_API_TU
 // Limit of the decode / verify pipeline waits (default kWaitLimitNs).  A test
@@ -86,6 +82,7 @@ struct ScoreMod {
     int32_t out_dtype, q_dtype;
     int32_t join_min;        // ranges cut into more partials are joined by paged_join_kernel;
                              // 0: none
+    TreeMask tree;           // TREE instantiations
 };
 
 struct MmaParams {
@@ -654,7 +651,7 @@ __device__ __forceinline__ bool plan_ok_zero_empty(const MmaParams& p) {
 // rows to take one after the other): 473 of the 505 us of one chain of 6 rows over
 // 15,000 bf16 keys, 16 query heads over 4, which takes 34 us with this kernel, and a
 // single token over 60,000 keys 39 instead of 110.
-template <int D>
+template <int D, bool TREE = false>      // (TREE: the one of its translation unit)
 __global__ void __launch_bounds__(256) paged_join_kernel(const MmaParams p) {
     __shared__ float s_o[8][D], s_m[8], s_l[8];
     // (launched while the split kernel's last CTAs still run: 2 us less a call)
@@ -850,7 +847,8 @@ struct MmaCfg {
     }
 };
 
-template <int D, int MT, int HG, typename QT, typename E = __nv_bfloat16, bool MOD = false>
+template <int D, int MT, int HG, typename QT, typename E = __nv_bfloat16, bool MOD = false,
+          bool TREE = false>
 __global__ void __launch_bounds__(MOD ? MmaCfg<D, MT, HG>::THREADS_MOD
                                       : MmaCfg<D, MT, HG>::THREADS, 1)
     paged_attn_mma_kernel(const __grid_constant__ CUtensorMap tmk,
@@ -974,8 +972,15 @@ __global__ void __launch_bounds__(MOD ? MmaCfg<D, MT, HG>::THREADS_MOD
         const int pos0 = ctx - sq;  // position of query row 0
         const int rpos0 = R0 < rows_b ? pos0 + R0 / G : -1;
         const int rpos1 = R1 < rows_b ? pos0 + R1 / G : -1;
+        // where the rows stand, and the last key that every row of a chain sees
+        int dpos0 = rpos0, dpos1 = rpos1;
+        const int all_pos = TREE ? pos0 - 1 : pos0;
+        if constexpr (TREE) {
+            if (R0 < rows_b) dpos0 = pos0 + p.mod.tree.depths[qs + R0 / G];
+            if (R1 < rows_b) dpos1 = pos0 + p.mod.tree.depths[qs + R1 / G];
+        }
         // MOD: the prefix, the tokens no row sees, this lane's rows' slopes (base 2)
-        const int pre = MOD ? prefix_of(p, b, ctx) : 0;
+        const int pre = MOD ? prefix_of(p, b, TREE ? max(pos0, 0) : ctx) : 0;
         const DeadTok dead{ctx, MOD && p.window > 0 ? pos0 - p.window + 1 : 0, pre};
         float slope0 = 0.f, slope1 = 0.f;
         if constexpr (MOD) {
@@ -1114,7 +1119,7 @@ __global__ void __launch_bounds__(MOD ? MmaCfg<D, MT, HG>::THREADS_MOD
                         for (int e = 0; e < 4; ++e)
                             x[u][n][e] = (sa[n][e] + sb[n][e]) * p.scale_log2;
                     const int t0 = seg_block<MOD>(seg, k + u * KS) * kBlockTok;
-                    bool edge = !FAST && ((t0 + kBlockTok - 1 > pos0) ||
+                    bool edge = !FAST && ((t0 + kBlockTok - 1 > all_pos) ||
                                           (p.window > 0 && t0 <= ctx - 1 - p.window));
                     if constexpr (MOD) {
                         edge = edge && t0 + kBlockTok > pre;
@@ -1153,23 +1158,42 @@ __global__ void __launch_bounds__(MOD ? MmaCfg<D, MT, HG>::THREADS_MOD
                                 for (int e = 0; e < 4; ++e) {
                                     // the distance is exact in fp32, so near keys, whose
                                     // weights count, lose nothing in long contexts
-                                    const int tok = t0 + n * 8 + qc + (e & 1);
-                                    const int dist = abs((e < 2 ? rpos0 : rpos1) - tok);
+                                    int tok = t0 + n * 8 + qc + (e & 1);
+                                    if (TREE && !FAST && tok >= pos0)
+                                        tok = tree_key_pos(p.mod.tree, qs, sq, pos0, tok - pos0);
+                                    const int dist = abs((e < 2 ? dpos0 : dpos1) - tok);
                                     x[u][n][e] = fmaf(-(e < 2 ? slope0 : slope1), (float)dist,
                                                       x[u][n][e]);
                                 }
                         }
                     }
                     if (edge) {
+                        uint32_t kin0 = 0, kin1 = 0;     // TREE: nodes from t0 - pos0 on
+                        if constexpr (TREE) {
+                            if (t0 + kBlockTok > pos0) {
+                                if (R0 < rows_b)
+                                    kin0 = tree_bits(p.mod.tree, qs + R0 / G, R0 / G, t0 - pos0);
+                                if (R1 < rows_b)
+                                    kin1 = tree_bits(p.mod.tree, qs + R1 / G, R1 / G, t0 - pos0);
+                            }
+                        }
 #pragma unroll
                         for (int n = 0; n < 2; ++n)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 const int tok = t0 + n * 8 + qc + (e & 1);
                                 const int rp = (e < 2) ? rpos0 : rpos1;
-                                const bool ok_t =
-                                    (MOD && tok < pre) ||
-                                    (tok <= rp && (p.window <= 0 || tok > rp - p.window));
+                                bool ok_t;
+                                if constexpr (TREE) {
+                                    const uint32_t kin = (e < 2) ? kin0 : kin1;
+                                    const int dp = (e < 2) ? dpos0 : dpos1;
+                                    ok_t = tok < pos0 ? tok < pre || p.window <= 0 ||
+                                                            tok > dp - p.window
+                                                      : (kin >> (tok - t0)) & 1u;
+                                } else {
+                                    ok_t = (MOD && tok < pre) ||
+                                           (tok <= rp && (p.window <= 0 || tok > rp - p.window));
+                                }
                                 if (!ok_t) x[u][n][e] = -INFINITY;
                             }
                     }
@@ -1276,7 +1300,7 @@ __global__ void __launch_bounds__(MOD ? MmaCfg<D, MT, HG>::THREADS_MOD
                         const int t0 = seg_block<MOD>(seg, k + u * KS) * kBlockTok;
                         fast = fast && !bad[u] &&
                                (t0 + kBlockTok <= pre ||
-                                (t0 + kBlockTok - 1 <= pos0 &&
+                                (t0 + kBlockTok - 1 <= all_pos &&
                                  (p.window <= 0 || t0 > ctx - 1 - p.window)));
                     }
                     if (fast && (U == 1 || two))
@@ -1384,20 +1408,6 @@ namespace cx {
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-static PFN_cuTensorMapEncodeTiled_v12000 tmap_encoder() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* f = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) ==
-                cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
-    });
-    return fn;
-}
-
 // 3-D view of a bf16, fp16 or fp32 pool: (head_dim, 16 slots, layers*blocks*heads
 // tiles), box of one 128-byte column (64 bf16 or 32 fp32 values) x 16 x hg
 // (hg consecutive heads of one block) with 128-byte swizzle.
@@ -1488,11 +1498,11 @@ static WsLayout ws_layout(int64_t batch, const MmaShape& sh, int64_t rows, int64
     return w;
 }
 
-template <int D, int MT, int HG, typename QT, typename E, bool MOD>
+template <int D, int MT, int HG, typename QT, typename E, bool MOD, bool TREE>
 static int launch_mma_cfg(const CUtensorMap& tk, const CUtensorMap& tv, MmaParams p,
                           cudaStream_t st, int grid) {
     using C = MmaCfg<D, MT, HG>;
-    auto kern = paged_attn_mma_kernel<D, MT, HG, QT, E, MOD>;
+    auto kern = paged_attn_mma_kernel<D, MT, HG, QT, E, MOD, TREE>;
     p.stages = C::stages_for(p.rows);
     if constexpr (MOD) {                   // (both are powers of two)
         constexpr int m = C::KS > C::PRODUCERS_MOD ? C::KS : C::PRODUCERS_MOD;
@@ -1507,12 +1517,12 @@ static int launch_mma_cfg(const CUtensorMap& tk, const CUtensorMap& tv, MmaParam
     return check_launch("paged_attn_mma_kernel");
 }
 
-template <int D, typename QT, typename E = __nv_bfloat16, bool MOD = false>
+template <int D, typename QT, typename E = __nv_bfloat16, bool MOD = false, bool TREE = false>
 static int launch_mma_d(const MmaShape& sh, const CUtensorMap& tk, const CUtensorMap& tv,
                         const MmaParams& p, cudaStream_t st, int grid) {
 #define CX_CASE(MT_, HG_) \
     if (sh.mt == MT_ && sh.hg == HG_)        \
-        return launch_mma_cfg<D, MT_, HG_, QT, E, MOD>(tk, tv, p, st, grid);
+        return launch_mma_cfg<D, MT_, HG_, QT, E, MOD, TREE>(tk, tv, p, st, grid);
     if constexpr (!MOD) {
         CX_CASE(1, 8)
     }
@@ -1524,11 +1534,11 @@ static int launch_mma_d(const MmaShape& sh, const CUtensorMap& tk, const CUtenso
     return fail(CX_ERR_UNSUPPORTED, "paged attention: no kernel for this row/head shape");
 }
 
-template <int D, int HG, int RT, bool MOD>
+template <int D, int HG, int RT, bool MOD, bool TREE>
 static int launch_f32_cfg(const CUtensorMap& tk, const CUtensorMap& tv, MmaParams p,
                           cudaStream_t st, int grid) {
     using C = F32Cfg<D, HG, RT>;
-    auto kern = paged_attn_f32_kernel<D, HG, RT, MOD>;
+    auto kern = paged_attn_f32_kernel<D, HG, RT, MOD, TREE>;
     // key slices: the ring length must be a multiple of them (each stage is
     // always consumed by the same slice).  Take the most consumer warps whose
     // ring still holds at least 4 stages and 3/4 of the longest ring: one warp
@@ -1563,12 +1573,12 @@ static int launch_f32_cfg(const CUtensorMap& tk, const CUtensorMap& tv, MmaParam
     return check_launch("paged_attn_f32_kernel");
 }
 
-template <int D, bool MOD = false>
+template <int D, bool MOD = false, bool TREE = false>
 static int launch_f32_d(const MmaShape& sh, const CUtensorMap& tk, const CUtensorMap& tv,
                         const MmaParams& p, cudaStream_t st, int grid) {
     const int rt = f32_rt(p.rows);
 #define CX_CASE(HG_, RT_) \
-    if (sh.hg == HG_ && rt == RT_) return launch_f32_cfg<D, HG_, RT_, MOD>(tk, tv, p, st, grid);
+    if (sh.hg == HG_ && rt == RT_) return launch_f32_cfg<D, HG_, RT_, MOD, TREE>(tk, tv, p, st, grid);
     CX_CASE(1, 4) CX_CASE(1, 8) CX_CASE(1, 16)
     CX_CASE(2, 4) CX_CASE(2, 8) CX_CASE(2, 16)
     if constexpr (D == 64) {

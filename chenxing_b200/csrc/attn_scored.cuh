@@ -77,9 +77,10 @@ static size_t attend_workspace(const cx_pool* pool, const cx_attn_batch* b) {
 }
 
 // The split-K kernels (attn_paged_mma.cuh, attn_paged_f32.cuh) with MOD.
+template <bool TREE>
 static int attend_split(const cx_pool* pool, int64_t layer, const cx_attn_batch& b,
-                        const cx_attn_mods& m, float scale, const void* q, int32_t q_dtype,
-                        void* out, void* ws, size_t ws_bytes, int32_t replan, bool plan_only,
+                        const cx_attn_mods& m, const TreeMask& tree, float scale, const void* q,
+                        int32_t q_dtype, void* out, void* ws, size_t ws_bytes, int32_t replan, bool plan_only,
                         cudaStream_t st) {
     const int64_t G = b.n_q_heads / pool->n_kv_heads, rows = G * b.max_q_len;
     const MmaShape sh = unit_shape(pool, rows);
@@ -122,6 +123,7 @@ static int attend_split(const cx_pool* pool, int64_t layer, const cx_attn_batch&
     p.mod.out = out;
     p.mod.out_dtype = m.out_dtype;
     p.mod.q_dtype = q_dtype;
+    p.mod.tree = tree;
     if (m.softcap > 0.f) {
         p.mod.cap_log2 = m.softcap * 1.4426950408889634f;
         p.mod.scale = scale / m.softcap;
@@ -153,19 +155,19 @@ static int attend_split(const cx_pool* pool, int64_t layer, const cx_attn_batch&
         p.mod.join_min = 16;
     switch (pool->dtype) {
         case CX_F32:
-            rc = d128 ? launch_f32_d<128, true>(sh, tk, tv, p, st, grid)
-                      : launch_f32_d<64, true>(sh, tk, tv, p, st, grid);
+            rc = d128 ? launch_f32_d<128, true, TREE>(sh, tk, tv, p, st, grid)
+                      : launch_f32_d<64, true, TREE>(sh, tk, tv, p, st, grid);
             break;
         case CX_BF16: {
             using E = __nv_bfloat16;
-            rc = d128 ? launch_mma_d<128, E, E, true>(sh, tk, tv, p, st, grid)
-                      : launch_mma_d<64, E, E, true>(sh, tk, tv, p, st, grid);
+            rc = d128 ? launch_mma_d<128, E, E, true, TREE>(sh, tk, tv, p, st, grid)
+                      : launch_mma_d<64, E, E, true, TREE>(sh, tk, tv, p, st, grid);
             break;
         }
         default: {
             using E = __half;
-            rc = d128 ? launch_mma_d<128, E, E, true>(sh, tk, tv, p, st, grid)
-                      : launch_mma_d<64, E, E, true>(sh, tk, tv, p, st, grid);
+            rc = d128 ? launch_mma_d<128, E, E, true, TREE>(sh, tk, tv, p, st, grid)
+                      : launch_mma_d<64, E, E, true, TREE>(sh, tk, tv, p, st, grid);
         }
     }
     if (rc || !p.mod.join_min) return rc;
@@ -179,15 +181,16 @@ static int attend_split(const cx_pool* pool, int64_t layer, const cx_attn_batch&
     cfg.stream = st;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    CX_CUDA_CHECK(cudaLaunchKernelEx(&cfg, d128 ? paged_join_kernel<128> : paged_join_kernel<64>,
-                                     p));
+    CX_CUDA_CHECK(cudaLaunchKernelEx(
+        &cfg, d128 ? paged_join_kernel<128, TREE> : paged_join_kernel<64, TREE>, p));
     return check_launch("paged_join_kernel");
 }
 
 // The tcgen05 kernel (attn_scored_tc.cuh).
+template <bool TREE>
 static int attend_tc(const cx_pool* pool, int64_t layer, const cx_attn_batch& b,
-                     const cx_attn_mods& m, float scale, const void* q, int32_t q_dtype, void* out,
-                     void* ws, size_t ws_bytes, cudaStream_t st) {
+                     const cx_attn_mods& m, const TreeMask& tree, float scale, const void* q,
+                     int32_t q_dtype, void* out, void* ws, size_t ws_bytes, cudaStream_t st) {
     ScoredTcParams p{};
     int64_t n_ctiles = 0;
     tc_grid(pool, &b, &p.tpt, &n_ctiles, &p.n_split);
@@ -202,6 +205,7 @@ static int attend_tc(const cx_pool* pool, int64_t layer, const cx_attn_batch& b,
     p.q_start = b.q_start;
     p.slopes = m.alibi_slopes;
     p.prefix = m.prefix_lens;
+    p.tree = tree;
     p.q = q;
     p.out = out;
     p.part = static_cast<float*>(ws);
@@ -249,15 +253,17 @@ static int attend_tc(const cx_pool* pool, int64_t layer, const cx_attn_batch& b,
     rc = make_pool_tmap(&tv, pool->v, pool, 1);
     if (rc) return rc;
     if (pool->dtype == CX_BF16)
-        return pool->head_dim == 128 ? launch_scored_tc<128, __nv_bfloat16>(tk, tv, p, st)
-                                     : launch_scored_tc<64, __nv_bfloat16>(tk, tv, p, st);
-    return pool->head_dim == 128 ? launch_scored_tc<128, __half>(tk, tv, p, st)
-                                 : launch_scored_tc<64, __half>(tk, tv, p, st);
+        return pool->head_dim == 128 ? launch_scored_tc<128, __nv_bfloat16, TREE>(tk, tv, p, st)
+                                     : launch_scored_tc<64, __nv_bfloat16, TREE>(tk, tv, p, st);
+    return pool->head_dim == 128 ? launch_scored_tc<128, __half, TREE>(tk, tv, p, st)
+                                 : launch_scored_tc<64, __half, TREE>(tk, tv, p, st);
 }
 
+template <bool TREE>
 static int attend_scored(const cx_pool* pool, int64_t layer, const cx_attn_batch* bt,
-                         const cx_attn_mods* mods, const void* q, int32_t q_dtype, void* out,
-                         void* ws, size_t ws_bytes, int32_t replan, void* stream) {
+                         const cx_attn_mods* mods, const TreeMask& tree, const void* q,
+                         int32_t q_dtype, void* out, void* ws, size_t ws_bytes, int32_t replan,
+                         void* stream) {
     int rc = check_pool(pool);
     if (rc) return rc;
     if (!bt || !mods) return fail(CX_ERR_SHAPE, "cx_paged_attend: NULL batch or mods");
@@ -295,14 +301,14 @@ static int attend_scored(const cx_pool* pool, int64_t layer, const cx_attn_batch
     cudaStream_t st = as_stream(stream);
     const int kind = attend_kind(pool, &b, q_dtype, (al & 15) == 0);
     if (kind == CX_KERNEL_MMA || kind == CX_KERNEL_FMA)
-        return attend_split(pool, layer, b, m, scale, q, q_dtype, out, ws, ws_bytes, replan,
+        return attend_split<TREE>(pool, layer, b, m, tree, scale, q, q_dtype, out, ws, ws_bytes, replan,
                             false, st);
     if (kind == CX_KERNEL_TCGEN05)
-        return attend_tc(pool, layer, b, m, scale, q, q_dtype, out, ws, ws_bytes, st);
+        return attend_tc<TREE>(pool, layer, b, m, tree, scale, q, q_dtype, out, ws, ws_bytes, st);
     // a later layer of the step may have queries that the split-K kernels take:
     // the plan it then reads is made now
     if (replan && split_shape(pool, &b) && ws) {
-        rc = attend_split(pool, layer, b, m, scale, q, q_dtype, out, ws, ws_bytes, 1, true, st);
+        rc = attend_split<TREE>(pool, layer, b, m, tree, scale, q, q_dtype, out, ws, ws_bytes, 1, true, st);
         if (rc) return rc;
     }
 
@@ -328,33 +334,8 @@ static int attend_scored(const cx_pool* pool, int64_t layer, const cx_attn_batch
     g.table_stride = b.table_stride;
     g.ctx_lens = b.ctx_lens;
     g.q_start = b.q_start;
-    return launch_generic<true, true>(q_dtype, pool->dtype, g, st);
+    g.tree = tree;
+    return launch_generic<true, true, TREE>(q_dtype, pool->dtype, g, st);
 }
 
 }  // namespace cx
-
-extern "C" {
-
-int cx_paged_attend(const cx_pool* pool, int64_t layer, const cx_attn_batch* batch,
-                    const cx_attn_mods* mods, const void* q, int32_t q_dtype, void* out,
-                    void* workspace, size_t workspace_bytes, int32_t replan, void* stream) {
-    return cx::attend_scored(pool, layer, batch, mods, q, q_dtype, out, workspace,
-                             workspace_bytes, replan, stream);
-}
-
-size_t cx_paged_attend_workspace_bytes(const cx_pool* pool, const cx_attn_batch* batch) {
-    if (!pool || !batch || pool->n_kv_heads <= 0 || batch->n_q_heads <= 0 || batch->batch < 0)
-        return 0;
-    cx_attn_batch b = *batch;
-    if (!b.q_start || b.max_q_len < 1) b.max_q_len = 1;
-    return cx::attend_workspace(pool, &b);
-}
-
-int cx_paged_attend_kind(const cx_pool* pool, const cx_attn_batch* batch, int32_t q_dtype) {
-    if (!pool || !batch || pool->n_kv_heads <= 0) return CX_KERNEL_GENERIC;
-    cx_attn_batch b = *batch;
-    if (!b.q_start || b.max_q_len < 1) b.max_q_len = 1;
-    return cx::attend_kind(pool, &b, q_dtype, true);
-}
-
-}  // extern "C"

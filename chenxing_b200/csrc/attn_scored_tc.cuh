@@ -68,6 +68,7 @@ struct ScoredTcParams {
     const int32_t* q_start;      // NULL: one query row per sequence
     const float* slopes;
     const int32_t* prefix;
+    TreeMask tree;               // TREE instantiations
     const void* q;
     void* out;
     float* part;                 // n_split > 1: [CTA][split][256][D + 2]
@@ -135,38 +136,6 @@ __device__ __forceinline__ float cap_any(float z, float cap_log2) {
     return fmaf(-2.f * cap_log2, rcp_approx(1.f + ex2_sfu(z * 2.8853900817779268f)), cap_log2);
 }
 
-// 16 consecutive 32-bit columns of this thread's TMEM lane.
-__device__ __forceinline__ void sc_st16(uint32_t taddr, const uint32_t (&v)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
-        "r"(v[15])
-        : "memory");
-}
-
-__device__ __forceinline__ void sc_ld16(uint32_t taddr, float (&v)[16]) {
-    uint32_t r[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-          "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
-
-template <typename E>
-__host__ __device__ constexpr uint32_t sc_idesc(int m, int n, int b_mn) {
-    // operand types: 1 bf16, 0 fp16
-    const uint32_t ty = std::is_same<E, __nv_bfloat16>::value ? 1u : 0u;
-    return (1u << 4) | (ty << 7) | (ty << 10) | ((uint32_t)b_mn << 16) |
-           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
-}
-
 // tcgen05.mma with A (M x 16, 16-bit pairs per 32-bit column, row i in lane i)
 // read from TMEM.
 __device__ __forceinline__ void sc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b,
@@ -198,6 +167,9 @@ struct ScTiles {
     }
 };
 
+// The `n` lowest bits, 0 <= n <= 32.
+__device__ __forceinline__ uint32_t sc_below(int n) { return n >= 32 ? ~0u : (1u << n) - 1; }
+
 // What the softmax warps need of a CTA's geometry, in shared memory and read
 // there where it is used: their registers are all taken (two more values kept
 // through the key loop, and the spills inside it, took 650 instead of 509 us for
@@ -228,7 +200,9 @@ __device__ __forceinline__ void sc_place(const ScoredTcParams& p, int cta, int l
     b = __ffs((int)at) - 1;
 }
 
-template <int DH, typename E, bool CAP, bool ALIBI>
+// TREE: the query rows are the nodes of a drafted tree; tiles that hold drafted keys
+// are masked by 32 bits of a row's word at a time.
+template <int DH, typename E, bool CAP, bool ALIBI, bool TREE = false>
 __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
     scored_tc_kernel(const __grid_constant__ CUtensorMap tmk,
                      const __grid_constant__ CUtensorMap tmv, const ScoredTcParams p) {
@@ -268,9 +242,9 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
     const int t_end = min(T, t0 + nq * tpt);
     const int pos0 = ctx - T;                                // position of token 0
     const int win = p.window;
-    const int pre = p.prefix ? min(max(p.prefix[b], 0), ctx) : 0;
+    const int pre = p.prefix ? min(max(p.prefix[b], 0), TREE ? max(pos0, 0) : ctx) : 0;
     const int run_hi = min(pos0 + t_end - 1, ctx - 1);       // last key past the prefix
-    const int run_lo = win > 0 ? max(0, pos0 + t0 - win + 1) : 0;
+    const int run_lo = win > 0 ? max(0, pos0 + (TREE ? 0 : t0) - win + 1) : 0;
     ScTiles tiles;
     {
         const int hi = max(run_hi, pre - 1);
@@ -361,7 +335,7 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
             const uint32_t tm_s = tmem + w * kScKeys + c * 64 + lane_off;
             const uint32_t tm_o = tmem + 2 * kScKeys + w * D + c * (D / 2) + lane_off;
             volatile const ScGeom& g = *reinterpret_cast<const ScGeom*>(sm + C::OFF_GEOM);
-            const int pos = pos0 + t;
+            int pos = pos0 + t;
             const float slope = ALIBI ? p.slopes[head] * 1.4426950408889634f : 0.f;
             const float cl = p.cap_log2;
             const f2 sl2 = f2_of(p.scale_log2, p.scale_log2);
@@ -387,9 +361,13 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
                 any_bad |= id < 0 || id >= p.n_blocks;
             }
             any_bad = __any_sync(0xffffffffu, any_bad);
-            // positions of this warp's first and last row
-            const int w_lo = __shfl_sync(0xffffffffu, pos, 0);
+            // positions of this warp's first and last row (TREE: of the last key that
+            // every node sees, and behind every node)
+            const int w_lo = TREE ? pos0 - 1 : __shfl_sync(0xffffffffu, pos, 0);
             const int w_hi = __shfl_sync(0xffffffffu, pos, 31);
+            if constexpr (TREE) {
+                if (t < t_end) pos = pos0 + p.tree.depths[qs + t];
+            }
             // the reference of a row (base 2): kLead above the maximum it is set to, and
             // following a maximum that is kRescale above it (Half16)
             constexpr float kRescale = Half16<E>::kGrowLog2, kLead = Half16<E>::kLeadLog2;
@@ -458,7 +436,15 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
                         // slope * -|pos - key|: the distance is exact, so near keys, whose
                         // weights count, lose nothing in long contexts
                         const float d0 = (float)(k0j - pos);
-                        if (ahead) {
+                        if (TREE && ahead) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                int key = k0j + j;
+                                if (key >= pos0)
+                                    key = tree_key_pos(p.tree, qs, T, pos0, key - pos0);
+                                v[j] = fmaf(-slope, fabsf((float)(key - pos)), v[j]);
+                            }
+                        } else if (ahead) {
 #pragma unroll
                             for (int j = 0; j < 32; ++j)
                                 v[j] = fmaf(-slope, fabsf(d0 + (float)j), v[j]);
@@ -471,10 +457,22 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
                     if (edge) {
                         const int jp = g.pre - k0j, hi = pos - k0j, win = g.win;
                         const int lo = win > 0 ? hi - win : INT32_MIN;
+                        if constexpr (TREE) {
+                            // bits of the committed keys that the row sees, then of its kin
+                            const int jb = min(max(pos0 - k0j, 0), 32);
+                            const int first = min(max(lo + 1, 0), 32);
+                            uint32_t keep = sc_below(jb) & (~sc_below(first) | sc_below(min(max(jp, 0), 32)));
+                            if (jb < 32 && t < t_end)
+                                keep |= tree_bits(p.tree, qs + t, t, k0j - pos0);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const bool keep = j < jp || (j <= hi && j > lo);
-                            v[j] = keep ? v[j] : -INFINITY;
+                            for (int j = 0; j < 32; ++j)
+                                v[j] = (keep >> j) & 1u ? v[j] : -INFINITY;
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                const bool keep = j < jp || (j <= hi && j > lo);
+                                v[j] = keep ? v[j] : -INFINITY;
+                            }
                         }
                         if (bad4 != 0) {
 #pragma unroll
@@ -872,7 +870,7 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
 
 // Joins the parts of split rows: one warp per (CTA, row); part rows hold the
 // unnormalised O, its reference maximum (base 2) and the denominator.
-template <int D>
+template <int D, bool TREE = false>      // (TREE: the one of its translation unit)
 __global__ void __launch_bounds__(256) scored_tc_join_kernel(const ScoredTcParams p) {
     const int lane = threadIdx.x & 31;
     const int64_t job = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -905,7 +903,7 @@ __global__ void __launch_bounds__(256) scored_tc_join_kernel(const ScoredTcParam
     for (int e = 0; e < D / 32; ++e) store_as(p.out, p.out_dtype, row + e * 32 + lane, o[e] * inv);
 }
 
-template <int DH, typename E>
+template <int DH, typename E, bool TREE>
 static int launch_scored_tc(const CUtensorMap& tk, const CUtensorMap& tv, const ScoredTcParams& p,
                             cudaStream_t st) {
     using C = ScCfg<DH>;
@@ -919,12 +917,12 @@ static int launch_scored_tc(const CUtensorMap& tk, const CUtensorMap& tv, const 
         kern<<<dim3((unsigned)grid, (unsigned)p.n_split), C::THREADS, C::SMEM, st>>>(tk, tv, p);
         return check_launch("scored_tc_kernel");
     };
-    int rc = p.cap_log2 > 0.f ? (p.slopes ? go(scored_tc_kernel<DH, E, true, true>)
-                                          : go(scored_tc_kernel<DH, E, true, false>))
-                              : (p.slopes ? go(scored_tc_kernel<DH, E, false, true>)
-                                          : go(scored_tc_kernel<DH, E, false, false>));
+    int rc = p.cap_log2 > 0.f ? (p.slopes ? go(scored_tc_kernel<DH, E, true, true, TREE>)
+                                          : go(scored_tc_kernel<DH, E, true, false, TREE>))
+                              : (p.slopes ? go(scored_tc_kernel<DH, E, false, true, TREE>)
+                                          : go(scored_tc_kernel<DH, E, false, false, TREE>));
     if (rc != CX_OK || p.n_split == 1) return rc;
-    scored_tc_join_kernel<DH><<<(unsigned)(grid * 32), 256, 0, st>>>(p);
+    scored_tc_join_kernel<DH, TREE><<<(unsigned)(grid * 32), 256, 0, st>>>(p);
     return check_launch("scored_tc_join_kernel");
 }
 

@@ -48,19 +48,23 @@ const char* cx_last_error(void) { return cx::t_last_error.c_str(); }
 int cx_device_error(void* stream, int clear, uint32_t* flags) {
     if (!flags) return cx::fail(CX_ERR_SHAPE, "cx_device_error: flags is NULL");
     cudaStream_t s = cx::as_stream(stream);
-    unsigned int v = 0, w = 0;
-    int rc = cx::copy_dev_flags(s, &v);
-    const int rc2 = cx::copy_dev_flags_scored(s, &w);
-    // (both copies are waited for before v and w go out of scope)
+    unsigned int v[4] = {};
+    const int rcs[4] = {cx::copy_dev_flags(s, v), cx::copy_dev_flags_scored(s, v + 1),
+                        cx::copy_dev_flags_tree(s, v + 2), cx::copy_dev_flags_latent(s, v + 3)};
+    // (all copies are waited for before v goes out of scope)
     CX_CUDA_CHECK(cudaStreamSynchronize(s));
-    if (rc == CX_OK) rc = rc2;
+    int rc = CX_OK;
+    for (int r : rcs)
+        if (rc == CX_OK) rc = r;
     if (rc == CX_OK && clear) {
         rc = cx::clear_dev_flags(s);
         if (rc == CX_OK) rc = cx::clear_dev_flags_scored(s);
+        if (rc == CX_OK) rc = cx::clear_dev_flags_tree(s);
+        if (rc == CX_OK) rc = cx::clear_dev_flags_latent(s);
         CX_CUDA_CHECK(cudaStreamSynchronize(s));
     }
     if (rc != CX_OK) return rc;
-    *flags = v | w;
+    *flags = v[0] | v[1] | v[2] | v[3];
     return CX_OK;
 }
 

@@ -42,6 +42,9 @@ inline int elem_bytes(int32_t dt) {
     }
 }
 
+constexpr int kBlockTok = 16;                               // tokens per block of the TMA kernels
+constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s per wait
+
 int num_sms();  // SM count of the current device (cached per device)
 
 // Limit of the decode / verify pipeline waits of later launches, ns
@@ -59,8 +62,8 @@ static inline int check_pool(const cx_pool* p) {
 }
 
 // ---- device-side error flags ---------------------------------------------
-// One word per translation unit (cxkv.cu, cxkv_scored.cu: no relocatable
-// device code); cx_device_error reads and clears both.
+// One word per translation unit (no relocatable device code); cx_device_error
+// reads and clears them all.
 static __device__ unsigned int g_dev_flags = 0;
 
 // Starts the copy of this translation unit's word to `v` on `s`, or its clearing;
@@ -79,6 +82,10 @@ static int clear_dev_flags(cudaStream_t s) {
 
 int copy_dev_flags_scored(cudaStream_t s, unsigned int* v);   // of cxkv_scored.cu
 int clear_dev_flags_scored(cudaStream_t s);
+int copy_dev_flags_tree(cudaStream_t s, unsigned int* v);     // of cxkv_tree.cu
+int clear_dev_flags_tree(cudaStream_t s);
+int copy_dev_flags_latent(cudaStream_t s, unsigned int* v);   // of cxkv_latent.cu
+int clear_dev_flags_latent(cudaStream_t s);
 
 __device__ __forceinline__ void raise_flag(unsigned int bit) {
     atomicOr(&g_dev_flags, bit);
@@ -118,6 +125,34 @@ __device__ __forceinline__ void store2_as(void* p, int32_t dtype, int64_t i, flo
             __floats2bfloat162_rn(x, y);
     else
         *reinterpret_cast<__half2*>(static_cast<__half*>(p) + i) = __floats2half2_rn(x, y);
+}
+
+// ---- drafted trees (cx_tree) ------------------------------------------------
+struct TreeMask {
+    const uint32_t* masks;   // [rows][words]; NULL: chains
+    const int32_t* depths;   // [rows]
+    int64_t words;
+};
+
+// Bits [u0, u0 + 32) of a row of `words` mask words; bits outside it are 0.
+__device__ __forceinline__ uint32_t mask_bits32(const uint32_t* row, int words, int u0) {
+    const int w = u0 >> 5, sh = u0 & 31;      // (floor, also below 0)
+    const uint32_t lo = w >= 0 && w < words ? __ldg(row + w) : 0u;
+    const uint32_t hi = sh && w + 1 >= 0 && w + 1 < words ? __ldg(row + w + 1) : 0u;
+    return __funnelshift_r(lo, hi, sh);
+}
+
+// Nodes [u0, u0 + 32) that query row `row` (node u_row of its sequence) sees: those
+// of its mask up to itself.
+__device__ __forceinline__ uint32_t tree_bits(const TreeMask& t, int64_t row, int u_row, int u0) {
+    const uint32_t m = mask_bits32(t.masks + row * t.words, (int)t.words, u0);
+    const int n = u_row + 1 - u0;
+    return n >= 32 ? m : n <= 0 ? 0u : m & ((1u << n) - 1);
+}
+
+// Where drafted key u of the sequence with query rows [q0, q0 + n) stands: base + its depth.
+__device__ __forceinline__ int tree_key_pos(const TreeMask& t, int64_t q0, int n, int base, int u) {
+    return u >= 0 && u < n ? base + __ldg(t.depths + q0 + u) : base + u;
 }
 
 // ---- packed fp32 pairs ------------------------------------------------------

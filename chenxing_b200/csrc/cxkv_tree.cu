@@ -1,0 +1,31 @@
+// Translation unit of libcxkv.so with the attention of drafted trees
+// (cx_paged_attend_tree): the TREE instantiations of the kernels with score
+// modifiers.  It keeps a device flag word of its own, like the others.
+#include "cx_common.cuh"
+#include "attn_generic.cuh"
+#include "attn_paged_mma.cuh"
+#include "attn_scored.cuh"
+
+namespace cx {
+
+int copy_dev_flags_tree(cudaStream_t s, unsigned int* v) { return copy_dev_flags(s, v); }
+int clear_dev_flags_tree(cudaStream_t s) { return clear_dev_flags(s); }
+
+}  // namespace cx
+
+extern "C" {
+
+int cx_paged_attend_tree(const cx_pool* pool, int64_t layer, const cx_attn_batch* batch,
+                         const cx_attn_mods* mods, const cx_tree* tree, const void* q,
+                         int32_t q_dtype, void* out, void* workspace, size_t workspace_bytes,
+                         int32_t replan, void* stream) {
+    using namespace cx;
+    if (!batch || !tree || !batch->q_start || !tree->masks || !tree->depths || tree->words < 1 ||
+        tree->words > (1 << 20) || tree->words * 32 < batch->max_q_len)
+        return fail(CX_ERR_SHAPE,
+                    "cx_paged_attend_tree: a tree needs q_start, masks of max_q_len bits and depths");
+    return attend_scored<true>(pool, layer, batch, mods, {tree->masks, tree->depths, tree->words},
+                               q, q_dtype, out, workspace, workspace_bytes, replan, stream);
+}
+
+}  // extern "C"

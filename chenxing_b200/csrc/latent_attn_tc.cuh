@@ -1,0 +1,921 @@
+// Attention over a latent cache on tcgen05, absorbed form: one row a token,
+// [latent (dc) | rotated shared key part (dr)], is the key of every query head and
+// its latent part is their value.
+//
+//     s[t, h, j] = scale * (q_latent[t, h] . c[j] + q_rope[t, h] . r[j])
+//     o[t, h]    = sum_j softmax_j(s[t, h, :])[j] c[j]
+//
+// Packed rows (row = query token x head) are cut into tiles of N = 16, 32 or 64.
+// Both products run transposed, so that the tile of keys is the M operand, any
+// number of rows is the N operand, and one copy of the keys in shared memory
+// serves both:
+//
+//     S^T (64 keys x N)  = C (64 x dim, K-major)   . Q^T   (N x dim, K-major)
+//     O^T (dc   x N)    += C^T (dc x 64, MN-major) . P^T   (N x 64, MN-major)
+//
+// O^T takes 4 N TMEM columns (dc <= 512: four tiles of 128 lanes), S^T two buffers
+// of N.  With the rows as M, 512 value columns would fill the TMEM and leave S no
+// room, and 16 rows (16 heads, one token) would run MMAs of 128.
+//
+// A CTA has a contiguous run of the batch's 64-key tiles, which are dealt out evenly
+// over the CTAs (every CTA works its share out from the lengths); a (sequence, row
+// tile) that is cut is joined by latent_join_kernel.  Roles:
+//
+//   warps 0-3: softmax of a tile's 64 keys (warp w: keys [16 w, 16 w + 16), two keys
+//              and N / 4 rows a thread), Q tiles in, output out.
+//   warp 4   : one thread issues the MMAs: S^T of a tile as its parts arrive, up to
+//              two tiles ahead of O^T, whichever can run.
+//   warp 5   : producer.  A tile arrives as pairs of 64-column chunks (16 KB, what one
+//              128-lane MMA of O^T reads) and a rest chunk with what lies past the
+//              last pair, each in a ring of its own (TMA, 128-byte swizzle).  Blocks
+//              past the sequence and ids outside the pool are read outside the tensor
+//              map, which fills zeros.
+//
+// The reference of a row's exponentials follows its maximum as in the kernels beside
+// this one (Half16), so that a tile nearly always needs one pass and one vote.
+// Tiles that some row sees only in part are masked by one 64-bit word a row, which
+// also holds the nodes that a row of a drafted tree sees; keys that no row of
+// the CTA sees are zeroed in shared memory first (0 * NaN is NaN).
+// Every wait is bounded.
+#pragma once
+
+#include "attn_prefill_tc.cuh"
+#include "tma_map.cuh"
+
+namespace cx {
+
+constexpr int kLatKeys = 64;          // keys per tile
+constexpr int kLatMaxDim = 576;       // latent + rotary part
+constexpr int kLatMaxLatent = 512;
+constexpr int kLatPair = 2 * kLatKeys * 128;   // a pair of chunks
+constexpr int kLatChunk = kLatKeys * 128;
+constexpr int kLatThreads = 192;
+constexpr int kLatMaxPairs = 16, kLatMaxRest = 4;
+constexpr int kLatMinTiles = 4;       // tiles per CTA before another CTA starts
+
+struct LatParams {
+    const int32_t* tables;
+    int64_t table_stride;
+    const int32_t* ctx_lens;
+    const int32_t* q_start;     // NULL: one query token per sequence
+    TreeMask tree;
+    const void* q_lat;
+    const void* q_rope;
+    int64_t ql_tok, ql_head, qr_tok, qr_head;
+    void* out;                  // [rows][heads][dc]
+    float* part_o;              // [CTA][2][N][dc]
+    float* part_ml;             // [CTA][2][N][2]
+    int32_t* desc;              // [CTA][8] the range that a CTA's last partial opens
+    int32_t batch, heads, max_q, rtiles, sub, n_units;
+    int32_t n_blocks, block_size, layer, window, dc, dim;
+    int32_t q_dtype, out_dtype, q_vec;
+    int32_t pairs, rests;       // ring lengths
+    float scale_log2;
+    uint64_t wait_ns;
+};
+
+// One (sequence, row tile) and its key tiles.
+struct LatUnit {
+    int b, T, qs, ctx, base;    // base: committed tokens (ctx - T)
+    int r0, n_rows;             // packed rows [r0, r0 + n_rows) of the sequence
+    int tile0, n_tiles;         // of the `sub` row tiles that run side by side
+};
+
+__device__ __forceinline__ LatUnit lat_unit(const LatParams& p, int u, int sub_id, int N) {
+    const int per_seq = (p.rtiles + p.sub - 1) / p.sub;
+    LatUnit x;
+    x.b = u / per_seq;
+    const int s = u - x.b * per_seq;
+    x.qs = p.q_start ? p.q_start[x.b] : x.b;
+    x.T = p.q_start ? min(max(p.q_start[x.b + 1] - x.qs, 0), p.max_q) : 1;
+    x.ctx = (int)min((int64_t)max(p.ctx_lens[x.b], 0), p.table_stride * p.block_size);
+    x.base = x.ctx - x.T;
+    const int rows = x.T * p.heads, first = s * p.sub * N, end = min(rows, first + p.sub * N);
+    x.r0 = first + sub_id * N;
+    x.n_rows = min(max(rows - x.r0, 0), N);
+    x.tile0 = x.n_tiles = 0;
+    if (end <= first || x.ctx == 0) return x;
+    const int hi = min(x.ctx - 1, x.base + (end - 1) / p.heads);
+    int lo = 0;
+    if (p.window > 0) lo = max(0, x.base + (p.tree.masks ? 0 : first / p.heads) - p.window + 1);
+    if (hi >= lo) x.tile0 = lo / kLatKeys;
+    x.n_tiles = hi >= lo ? hi / kLatKeys - x.tile0 + 1 : 1;
+    return x;
+}
+
+// A run of tiles of one unit.
+struct LatSeg {
+    LatUnit x;
+    int from, to;
+    __device__ __forceinline__ bool whole() const { return from == 0 && to == x.n_tiles; }
+};
+
+struct LatCursor {
+    int u, off, left;
+    __device__ __forceinline__ bool next(const LatParams& p, int sub_id, int N, LatSeg& s) {
+        while (left > 0 && u < p.n_units) {
+            s.x = lat_unit(p, u, sub_id, N);
+            const int have = s.x.n_tiles - off;
+            if (have <= 0) {
+                ++u;
+                off = 0;
+                continue;
+            }
+            s.from = off;
+            s.to = off + min(left, have);
+            left -= s.to - s.from;
+            ++u;
+            off = 0;
+            if (s.x.n_rows > 0) return true;      // (a side-by-side tile past the rows: none)
+        }
+        return false;
+    }
+};
+
+template <int N>
+struct LatCfg {
+    static constexpr int Q_CHUNK = N * 128;
+    static constexpr int MISC = 2048;
+    static constexpr int TMEM_COLS = 512;
+    static constexpr int S_COL = 4 * N;
+    // ring lengths of `dim` (rows beside pairs of 128 latent columns)
+    __host__ static void rings(int dc, int dim, int& pairs, int& rests, int& smem) {
+        const int nch = (dim + 63) / 64, nm = (dc + 127) / 128;
+        const int fixed = 1024 + nch * Q_CHUNK + kLatChunk + MISC;
+        rests = nch > 2 * nm ? 2 : 0;
+        pairs = (232448 - fixed - rests * kLatChunk) / kLatPair;
+        if (pairs > kLatMaxPairs) pairs = kLatMaxPairs;
+        smem = fixed + rests * kLatChunk + pairs * kLatPair;
+        // above half of the SM's shared memory: one CTA an SM, which owns the TMEM
+        if (smem < 117 * 1024) smem = 117 * 1024;
+    }
+};
+
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+
+// OR of `pred` over the `nthreads` threads that meet at named barrier `id`.
+__device__ __forceinline__ bool bar_red_or(int id, int nthreads, bool pred) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 q, %3, 0;\n\t"
+        "bar.red.or.pred p, %1, %2, q;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r)
+        : "r"(id), "r"(nthreads), "r"((uint32_t)pred)
+        : "memory");
+    return r != 0;
+}
+
+// N columns of 16 TMEM lanes: v[4 j + e] is lane `lane / 4 + 8 (e / 2)`, column
+// 8 j + 2 (lane % 4) + e % 2.
+template <int N>
+__device__ __forceinline__ void lat_ld_s(uint32_t taddr, float (&v)[N / 2]) {
+    uint32_t r[N / 2];
+    if constexpr (N == 16) {
+        asm volatile(
+            "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+              "=r"(r[6]), "=r"(r[7])
+            : "r"(taddr));
+    } else if constexpr (N == 32) {
+        asm volatile(
+            "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+            "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+              "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+              "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+            : "r"(taddr));
+    } else {
+        asm volatile(
+            "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+            "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+            "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, "
+            "[%32];"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+              "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+              "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+              "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+              "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+              "=r"(r[30]), "=r"(r[31])
+            : "r"(taddr));
+    }
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// 64-bit word with bits [a, b) set, 0 <= a, b <= 64 (none when b <= a).
+__device__ __forceinline__ uint64_t bit_run(int a, int b) {
+    if (b <= a) return 0;
+    const uint64_t upto = b >= 64 ? ~0ull : (1ull << b) - 1;
+    return a >= 64 ? 0 : upto & ~((1ull << a) - 1);
+}
+
+// Which of the keys [k0, k0 + 64) packed row r of the unit sees.
+__device__ __forceinline__ uint64_t lat_visible(const LatParams& p, const LatUnit& x, int r,
+                                                int k0) {
+    const int t = r / p.heads, last = x.base + t;
+    int pos = last, up = last;                 // `up`: the last key of the plain run
+    if (p.tree.masks) {
+        pos = x.base + p.tree.depths[x.qs + t];
+        up = x.base - 1;
+    }
+    const int lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+    uint64_t v = bit_run(min(max(lo - k0, 0), 64), min(max(up + 1 - k0, 0), 64));
+    if (p.tree.masks && last >= k0 && x.base < k0 + kLatKeys) {
+        const int u0 = k0 - x.base;
+        v |= tree_bits(p.tree, x.qs + t, t, u0) |
+             (uint64_t)tree_bits(p.tree, x.qs + t, t, u0 + 32) << 32;
+    }
+    return v;
+}
+
+// 8 consecutive elements of a query row (latent part, then rotary part) as 16-bit
+// type E; zeros past the row.
+template <typename E>
+__device__ __forceinline__ uint4 lat_q8(const LatParams& p, int64_t lat, int64_t rope, int d) {
+    if (p.q_vec) {            // both parts, rows and widths: multiples of 8 elements
+        if (d >= p.dim) return make_uint4(0, 0, 0, 0);
+        const bool in_lat = d < p.dc;
+        const int64_t at = in_lat ? lat + d : rope + (d - p.dc);
+        const void* base = in_lat ? p.q_lat : p.q_rope;
+        if (p.q_dtype != CX_F32)
+            return __ldg(reinterpret_cast<const uint4*>(static_cast<const E*>(base) + at));
+        const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
+        const float4 a = __ldg(s), b = __ldg(s + 1);
+        return make_uint4(Half16<E>::pack(a.x, a.y), Half16<E>::pack(a.z, a.w),
+                          Half16<E>::pack(b.x, b.y), Half16<E>::pack(b.z, b.w));
+    }
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int i = d + e;
+        x[e] = 0.f;
+        if (i < p.dim) {
+            const bool in_lat = i < p.dc;
+            const int64_t at = in_lat ? lat + i : rope + (i - p.dc);
+            const void* base = in_lat ? p.q_lat : p.q_rope;
+            x[e] = p.q_dtype == CX_F32 ? static_cast<const float*>(base)[at]
+                                       : Conv<E>::to_f(static_cast<const E*>(base)[at]);
+        }
+    }
+    return make_uint4(Half16<E>::pack(x[0], x[1]), Half16<E>::pack(x[2], x[3]),
+                      Half16<E>::pack(x[4], x[5]), Half16<E>::pack(x[6], x[7]));
+}
+
+template <typename E>
+__host__ __device__ constexpr uint32_t lat_idesc(int m, int n, int a_mn, int b_mn) {
+    return sc_idesc<E>(m, n, b_mn) | ((uint32_t)a_mn << 15);
+}
+
+template <int N, typename E>
+__global__ void __launch_bounds__(kLatThreads, 1)
+    latent_tc_kernel(const __grid_constant__ CUtensorMap tm, const LatParams p) {
+    using C = LatCfg<N>;
+    constexpr int NJ = N / 8;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* sm = reinterpret_cast<unsigned char*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int sub_id = (int)blockIdx.x % p.sub, g = (int)blockIdx.x / p.sub;
+    const int G = (int)gridDim.x / p.sub;
+    const int NM = (p.dc + 127) / 128, NCH = (p.dim + 63) / 64, KSTEPS = (p.dim + 15) / 16;
+    const int PS = p.pairs, RS = p.rests;
+    const bool has_rest = RS > 0;
+
+    unsigned char* s_q = sm;
+    unsigned char* s_p = s_q + NCH * C::Q_CHUNK;
+    unsigned char* s_pairs = s_p + kLatChunk;
+    unsigned char* s_rest = s_pairs + PS * kLatPair;
+    unsigned char* misc = s_rest + RS * kLatChunk;
+    uint64_t* full_p = reinterpret_cast<uint64_t*>(misc);
+    uint64_t* empty_p = full_p + kLatMaxPairs;
+    uint64_t* full_r = empty_p + kLatMaxPairs;
+    uint64_t* empty_r = full_r + kLatMaxRest;
+    uint64_t* s_full = empty_r + kLatMaxRest;     // [2] S^T of a tile is there
+    uint64_t* p_full = s_full + 2;                // P^T written, O^T rescaled
+    uint64_t* o_done = p_full + 1;                // O^T of a tile is done
+    uint64_t* q_full = o_done + 1;                // Q of a range is there
+    uint64_t* drain = q_full + 1;                 // last commit of the MMA thread
+    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drain + 1);
+    volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
+    volatile int* s_issued = s_abort + 1;         // [2] ring items whose loads were issued
+    int* s_start = const_cast<int*>(s_issued) + 2;    // [4] unit, offset, tiles, all tiles
+    int* s_warp = s_start + 4;                    // [6]
+    uint64_t* s_vis = reinterpret_cast<uint64_t*>(misc + 512);        // [64]
+    float* s_alpha = reinterpret_cast<float*>(misc + 512);            // [64], after s_vis
+    float* s_red = reinterpret_cast<float*>(misc + 1024);             // [4][64]
+
+    asm volatile("griddepcontrol.launch_dependents;");
+    if (tid == 0) p.desc[(int64_t)blockIdx.x * 8] = 0;
+
+    // ---- rows of sequences without a key: zeros ----
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+        const int raw = p.ctx_lens[b];
+        const int qs = p.q_start ? p.q_start[b] : b;
+        const int n = p.q_start ? p.q_start[b + 1] - qs : 1;
+        const int64_t cap = p.table_stride * p.block_size;
+        if (tid == 0) {
+            if (raw > cap) raise_flag(CX_DEV_TABLE_OVERRUN);
+            if (n < 0 || n > p.max_q || (raw > 0 && n > min((int64_t)raw, cap)))
+                raise_flag(CX_DEV_BAD_QLEN);
+        }
+        if (raw > 0) continue;
+        const int64_t o0 = (int64_t)qs * p.heads * p.dc;
+        const int64_t cnt = (int64_t)min(max(n, 0), p.max_q) * p.heads * p.dc;
+        for (int64_t i = tid; i < cnt; i += kLatThreads) store_as(p.out, p.out_dtype, o0 + i, 0.f);
+    }
+
+    // ---- this CTA's share of the tiles ----
+    {
+        const int per = (p.n_units + kLatThreads - 1) / kLatThreads;
+        const int u0 = min(p.n_units, tid * per), u1 = min(p.n_units, u0 + per);
+        int sum = 0;
+        for (int u = u0; u < u1; ++u) sum += lat_unit(p, u, 0, N).n_tiles;
+        int incl = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += o;
+        }
+        if (lane == 31) s_warp[warp] = incl;
+        __syncthreads();
+        int before = incl - sum, W = 0;
+#pragma unroll
+        for (int w = 0; w < kLatThreads / 32; ++w) {
+            if (w < warp) before += s_warp[w];
+            W += s_warp[w];
+        }
+        const int P = min(G, max(1, (W + kLatMinTiles - 1) / kLatMinTiles));
+        const int w0 = g < P ? (int)((int64_t)g * W / P) : W;
+        const int w1 = g < P ? (int)((int64_t)(g + 1) * W / P) : W;
+        if (w1 <= w0) return;
+        if (before <= w0 && w0 < before + sum) {
+            int u = u0, at = before;
+            for (; u < u1; ++u) {
+                const int n = lat_unit(p, u, 0, N).n_tiles;
+                if (w0 < at + n) break;
+                at += n;
+            }
+            s_start[0] = u;
+            s_start[1] = w0 - at;
+            s_start[2] = w1 - w0;
+            s_start[3] = W;
+        }
+    }
+    if (tid == 0) {
+        for (int s = 0; s < PS; ++s) {
+            mbar_init(&full_p[s], 1);
+            mbar_init(&empty_p[s], 1);
+        }
+        for (int s = 0; s < RS; ++s) {
+            mbar_init(&full_r[s], 1);
+            mbar_init(&empty_r[s], 1);
+        }
+        mbar_init(&s_full[0], 1);
+        mbar_init(&s_full[1], 1);
+        mbar_init(p_full, 128);
+        mbar_init(o_done, 1);
+        mbar_init(q_full, 128);
+        mbar_init(drain, 1);
+        *s_abort = 0;
+        s_issued[0] = s_issued[1] = 0;
+        fence_mbar_init();
+    }
+    if (warp == 4) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_addr(s_tmem)),
+                     "r"(C::TMEM_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *s_tmem;
+    LatCursor cur{s_start[0], s_start[1], s_start[2]};
+    LatSeg seg;
+    int tile = 0;               // tiles of this CTA before the range
+    const int bs = p.block_size, per_tile = kLatKeys / bs;    // blocks a tile (bs 16, 32, 64)
+
+    if (warp < 4) {
+        // ---------------- Q in, softmax, output ----------------
+        const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+        const int tq = lane >> 2, c = lane & 3;
+        const int tok0 = warp * 16 + tq, tok1 = tok0 + 8;
+        constexpr float kGrow = Half16<E>::kGrowLog2, kLead = Half16<E>::kLeadLog2;
+        bool ok = true;
+        int slot = 0;
+        while (ok && cur.next(p, sub_id, N, seg)) {
+            const LatUnit& x = seg.x;
+            const int n = seg.to - seg.from;
+            // ---- Q: every MMA that read the last range's is done ----
+#pragma unroll 4
+            for (int i = tid; i < N * NCH * 8; i += 128) {
+                const int r = i / (NCH * 8), ch = i - r * (NCH * 8);
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (r < x.n_rows) {
+                    const int t = (x.r0 + r) / p.heads, h = (x.r0 + r) - t * p.heads;
+                    v = lat_q8<E>(p, (x.qs + t) * p.ql_tok + h * p.ql_head,
+                                  (x.qs + t) * p.qr_tok + h * p.qr_head, ch * 8);
+                }
+                *reinterpret_cast<uint4*>(s_q + (ch >> 3) * C::Q_CHUNK + r * 128 +
+                                          (((ch & 7) ^ (r & 7)) << 4)) = v;
+            }
+            fence_async_smem();
+            mbar_arrive(q_full);
+            const int32_t* tab = p.tables + (int64_t)x.b * p.table_stride;
+            const int nblk = (x.ctx + bs - 1) / bs;
+            const int first_k = (x.tile0 + seg.from) * kLatKeys;
+            bool bad = false;
+            for (int k = first_k / bs + tid; k < min(nblk, (first_k + n * kLatKeys) / bs); k += 128) {
+                const int id = tab[k];
+                bad |= id < 0 || id >= p.n_blocks;
+            }
+            const bool any_bad = bar_red_or(1, 128, bad);
+            // keys up to `all_hi` and from `all_lo` on are seen by every row
+            const int t_first = x.r0 / p.heads, t_last = (x.r0 + x.n_rows - 1) / p.heads;
+            const int all_hi = p.tree.masks ? x.base - 1 : x.base + t_first;
+            const int all_lo = p.window > 0 ? x.base + t_last - p.window + 1 : 0;
+
+            float m[NJ][2], l[NJ][2];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                m[j][0] = m[j][1] = -INFINITY;
+                l[j][0] = l[j][1] = 0.f;
+            }
+            for (int i = 0; i < n; ++i, ++tile) {
+                const int k0 = first_k + i * kLatKeys;
+                ok = mbar_wait_bounded(&s_full[tile & 1], (tile >> 1) & 1, s_abort, p.wait_ns);
+                if (!(ok = bar_red_and(1, 128, ok))) break;
+                tc_fence_after();
+                float v[N / 2];
+                lat_ld_s<N>(tmem + C::S_COL + (tile & 1) * N + lane_base, v);
+                tc_wait_ld();
+#pragma unroll
+                for (int e = 0; e < N / 2; ++e) v[e] *= p.scale_log2;
+                const bool edge = any_bad || k0 + kLatKeys - 1 > all_hi || k0 < all_lo;
+                uint64_t dead = 0;
+                if (edge) {
+                    uint64_t vis = 0;
+                    if (tid < x.n_rows) {
+                        vis = lat_visible(p, x, x.r0 + tid, k0);
+                        for (int k = 0; any_bad && k < per_tile; ++k) {
+                            const int blk = k0 / bs + k, id = blk < nblk ? tab[blk] : 0;
+                            if (id < 0 || id >= p.n_blocks) vis &= ~bit_run(k * bs, k * bs + bs);
+                        }
+                    }
+                    if (tid < 64) s_vis[tid] = vis;
+                    named_bar_sync(1, 128);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const uint64_t w = s_vis[8 * j + 2 * c + e];
+                            if (!((w >> tok0) & 1)) v[4 * j + e] = -INFINITY;
+                            if (!((w >> tok1) & 1)) v[4 * j + 2 + e] = -INFINITY;
+                        }
+                    }
+                    // keys that no row sees
+                    uint64_t any = s_vis[lane] | s_vis[lane + 32];
+                    const uint32_t a0 = __reduce_or_sync(0xffffffffu, (uint32_t)any);
+                    const uint32_t a1 = __reduce_or_sync(0xffffffffu, (uint32_t)(any >> 32));
+                    dead = ~((uint64_t)a1 << 32 | a0);
+                }
+                // ---- the references; again with a maximum that outgrew one ----
+                bool grow = false;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        grow |= fmaxf(v[4 * j + e], v[4 * j + 2 + e]) > m[j][e] + kGrow;
+                if (bar_red_or(1, 128, grow)) {
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float y = fmaxf(v[4 * j + e], v[4 * j + 2 + e]);
+                            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
+                            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
+                            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
+                            if (lane < 4) s_red[warp * 64 + 8 * j + 2 * c + e] = y;
+                        }
+                    named_bar_sync(1, 128);
+                    bool moved = false;
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float* q = s_red + 8 * j + 2 * c + e;
+                            const float y = fmaxf(fmaxf(q[0], q[64]), fmaxf(q[128], q[192]));
+                            float alpha = 1.f;
+                            if (y > m[j][e] + kGrow) {      // (m -inf: any score that is not)
+                                const float mn = y + kLead;
+                                alpha = exp2f(m[j][e] - mn);
+                                m[j][e] = mn;
+                                moved = true;
+                            }
+                            l[j][e] *= alpha;
+                            if (warp == 0 && lane < 4) s_alpha[8 * j + 2 * c + e] = alpha;
+                        }
+                    // (every thread of a column c has the same alphas)
+                    moved = bar_red_or(1, 128, moved);
+                    if (moved && i > 0) {
+                        // O^T holds the tiles before this one
+                        ok = mbar_wait_bounded(o_done, (tile - 1) & 1, s_abort, p.wait_ns);
+                        if (!(ok = bar_red_and(1, 128, ok))) break;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int k = 0; k < NM * (N / 16); ++k) {
+                            const int col = (k / (N / 16)) * N + (k % (N / 16)) * 16;
+                            const uint32_t at = tmem + col + lane_base;
+                            float o[16];
+                            sc_ld16(at, o);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] *= s_alpha[(k % (N / 16)) * 16 + e];
+                            sc_st16(at, reinterpret_cast<const uint32_t(&)[16]>(o));
+                        }
+                        tc_wait_st();
+                    }
+                    named_bar_sync(1, 128);     // s_alpha and s_red are read
+                }
+                uint32_t pk[N / 4];
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    const float b0 = m[j][0] == -INFINITY ? 0.f : m[j][0];
+                    const float b1 = m[j][1] == -INFINITY ? 0.f : m[j][1];
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const uint32_t u = Half16<E>::pack(ex2_sfu(v[4 * j + 2 * t] - b0),
+                                                           ex2_sfu(v[4 * j + 2 * t + 1] - b1));
+                        // (the sum of what the second product gets: numerator and denominator
+                        // round alike)
+                        float e0, e1;
+                        f2_get(Half16<E>::unpack(u), e0, e1);
+                        l[j][0] += e0;
+                        l[j][1] += e1;
+                        pk[2 * j + t] = u;
+                    }
+                }
+                // ---- P^T over the last tile's, when O^T has read that ----
+                if (tile > 0)
+                    ok = mbar_wait_bounded(o_done, (tile - 1) & 1, s_abort, p.wait_ns);
+                if (!ok) {
+                    *s_abort = 1;               // the next vote ends the loop for all
+                    continue;
+                }
+                if (dead != 0) {
+                    const int tok = tid & 63;
+                    if ((dead >> tok) & 1) {
+                        for (int mm = 0; mm < NM; ++mm) {
+                            const int q = tile * NM + mm;
+                            uint4* z = reinterpret_cast<uint4*>(
+                                s_pairs + (q % PS) * kLatPair + (tid >> 6) * kLatChunk + tok * 128);
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) z[k] = make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    *reinterpret_cast<uint32_t*>(s_p + tok0 * 128 + ((j ^ (tok0 & 7)) << 4) +
+                                                 c * 4) = pk[2 * j];
+                    *reinterpret_cast<uint32_t*>(s_p + tok1 * 128 + ((j ^ (tok1 & 7)) << 4) +
+                                                 c * 4) = pk[2 * j + 1];
+                }
+                fence_async_smem();
+                tc_fence_before();
+                mbar_arrive(p_full);
+            }
+            // (a wait before the last P^T may have given up in some threads only)
+            if (!(ok = bar_red_and(1, 128, ok))) break;
+            // ---- denominators, then O^T to the output or to this CTA's part ----
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float y = l[j][e];
+                    y += __shfl_xor_sync(0xffffffffu, y, 4);
+                    y += __shfl_xor_sync(0xffffffffu, y, 8);
+                    y += __shfl_xor_sync(0xffffffffu, y, 16);
+                    if (lane < 4) s_red[warp * 64 + 8 * j + 2 * c + e] = y;
+                }
+            ok = mbar_wait_bounded(o_done, (tile - 1) & 1, s_abort, p.wait_ns);
+            if (!(ok = bar_red_and(1, 128, ok))) break;
+            tc_fence_after();
+            const bool whole = seg.whole();
+            const int64_t part = ((int64_t)blockIdx.x * 2 + slot) * N;
+            if (tid < N) {
+                const float L = (s_red[tid] + s_red[64 + tid]) + (s_red[128 + tid] + s_red[192 + tid]);
+                s_alpha[tid] = whole ? (L > 0.f ? 1.f / L : 0.f) : 1.f;
+                if (!whole) p.part_ml[(part + tid) * 2 + 1] = L;
+            }
+            if (!whole && warp == 0 && lane < 4) {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        p.part_ml[(part + 8 * j + 2 * c + e) * 2] = m[j][e];
+            }
+            named_bar_sync(1, 128);
+            const int64_t row0 = (int64_t)x.qs * p.heads + x.r0;
+#pragma unroll 1
+            for (int k = 0; k < NM * (N / 16); ++k) {
+                const int mm = k / (N / 16), n0 = (k % (N / 16)) * 16;
+                const int d = mm * 128 + warp * 32 + lane;
+                float o[16];
+                __syncwarp();
+                sc_ld16(tmem + mm * N + n0 + lane_base, o);
+                tc_wait_ld();
+                if (d >= p.dc) continue;
+                if (whole) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (n0 + e < x.n_rows)
+                            store_as(p.out, p.out_dtype, (row0 + n0 + e) * p.dc + d,
+                                     o[e] * s_alpha[n0 + e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (n0 + e < x.n_rows) p.part_o[(part + n0 + e) * p.dc + d] = o[e];
+                }
+            }
+            tc_fence_before();
+            if (!whole && seg.from == 0 && tid == 0) {
+                // the unit starts here and goes on: who has the rest of it
+                const int W = s_start[3];
+                const int P = min(G, max(1, (W + kLatMinTiles - 1) / kLatMinTiles));
+                const int end = (int)((int64_t)(g + 1) * W / P) + x.n_tiles - seg.to;
+                int last = g + 1;
+                while (last + 1 < P && (int)((int64_t)(last + 1) * W / P) < end) ++last;
+                int32_t* d = p.desc + (int64_t)blockIdx.x * 8;
+                d[1] = slot;
+                d[2] = x.n_rows;
+                d[3] = (int32_t)(row0 & 0xffffffff);
+                d[4] = (int32_t)(row0 >> 32);
+                d[0] = last - g + 1;
+            }
+            slot = 1;
+            named_bar_sync(1, 128);             // s_alpha and s_red are read
+        }
+        if (!ok) {
+            *s_abort = 1;
+            if (tid == 0) raise_flag(CX_DEV_WAIT_TIMEOUT);
+        }
+    } else if (warp == 5) {
+        // ---------------- producer ----------------
+        const uint32_t box = (uint32_t)bs * 128;      // a block's rows of a 64-column chunk
+        bool go = true;
+        while (go && cur.next(p, sub_id, N, seg)) {
+            const LatUnit& x = seg.x;
+            const int32_t* tab = p.tables + (int64_t)x.b * p.table_stride;
+            const int nblk = (x.ctx + bs - 1) / bs, n = seg.to - seg.from;
+            const int blk0 = (x.tile0 + seg.from) * per_tile;
+            auto block_of = [&](int i) {              // this lane's block of tile i
+                const int blk = blk0 + i * per_tile + lane;
+                int id = -1;
+                if (lane < per_tile && i < n && blk < nblk) {
+                    id = tab[blk];
+                    if (id < 0 || id >= p.n_blocks) {
+                        raise_flag(CX_DEV_BAD_BLOCK);
+                        id = -1;
+                    }
+                }
+                return id;
+            };
+            int ids = block_of(0);
+            for (int i = 0; go && i < n; ++i, ++tile) {
+                const int next = block_of(i + 1);
+                for (int q = 0; go && q < NM + (has_rest ? 1 : 0); ++q) {
+                    const bool rest = q == NM;
+                    const int item = rest ? tile : tile * NM + q;
+                    const int ring = rest ? RS : PS, s = item % ring, use = item / ring;
+                    uint64_t* full = (rest ? full_r : full_p) + s;
+                    uint64_t* empty = (rest ? empty_r : empty_p) + s;
+                    unsigned char* dst = rest ? s_rest + s * kLatChunk : s_pairs + s * kLatPair;
+                    if (lane == 0) {
+                        go = use == 0 ||
+                             mbar_wait_bounded(empty, (use - 1) & 1, s_abort, p.wait_ns);
+                        go = go && !*s_abort;
+                        if (go) mbar_arrive_expect_tx(full, rest ? kLatChunk : kLatPair);
+                    }
+                    go = __shfl_sync(0xffffffffu, (int)go, 0) != 0;
+                    if (!go) break;
+                    const int half = lane / per_tile, k = lane - half * per_tile;
+                    const int id = __shfl_sync(0xffffffffu, ids, k);
+                    if (half < (rest ? 1 : 2)) {
+                        // outside the map: the copy fills zeros
+                        const int z = id >= 0 ? p.layer * p.n_blocks + id : -1;
+                        tma_load_3d(dst + half * kLatChunk + k * box, &tm, full,
+                                    (q * 2 + half) * 64, 0, z);
+                    }
+                    __syncwarp();
+                    if (lane == 0) s_issued[rest ? 1 : 0] = item + 1;
+                }
+                ids = next;
+            }
+        }
+        if (!go && lane == 0) {
+            *s_abort = 1;
+            raise_flag(CX_DEV_WAIT_TIMEOUT);
+        }
+    } else if (lane == 0) {
+        // ---------------- MMA issuer ----------------
+        constexpr uint32_t idesc_s = lat_idesc<E>(kLatKeys, N, 0, 0);
+        constexpr uint32_t idesc_o = lat_idesc<E>(128, N, 1, 1);
+        const uint64_t q_desc = tc_sdesc(smem_addr(s_q), 16, 1024);
+        const uint64_t kp_desc = tc_sdesc(smem_addr(s_pairs), 16, 1024);
+        const uint64_t kr_desc = tc_sdesc(smem_addr(s_rest), 16, 1024);
+        const uint64_t v_desc = tc_sdesc(smem_addr(s_pairs), kLatChunk, 1024);
+        const uint64_t p_desc = tc_sdesc(smem_addr(s_p), kLatChunk, 1024);
+        bool ok = true;
+        int ranges = 0;
+        const int pieces = NM + (has_rest ? 1 : 0);
+        while (ok && cur.next(p, sub_id, N, seg)) {
+            const int n = seg.to - seg.from;
+            ok = mbar_wait_bounded(q_full, ranges & 1, s_abort, p.wait_ns);
+            ++ranges;
+            if (!ok) break;
+            tc_fence_after();
+            int si = 0, oi = 0, piece = 0;
+            uint32_t idle = 0;
+            uint64_t since = 0;
+            while (oi < n) {
+                bool did = false;
+                if (oi < si && mbar_test(p_full, (tile + oi) & 1)) {
+                    tc_fence_after();
+                    for (int mm = 0; mm < NM; ++mm) {
+                        const int s = ((tile + oi) * NM + mm) % PS;
+                        const uint64_t vd = v_desc + (uint32_t)(s * (kLatPair >> 4));
+#pragma unroll
+                        for (int kk = 0; kk < kLatKeys / 16; ++kk)
+                            tc_mma(tmem + mm * N, vd + kk * (2048 >> 4), p_desc + kk * (2048 >> 4),
+                                   idesc_o, (oi > 0 || kk > 0) ? 1u : 0u);
+                        tc_commit(&empty_p[s]);
+                    }
+                    tc_commit(o_done);
+                    ++oi;
+                    did = true;
+                } else if (si < n && si < oi + 2) {
+                    const bool rest = piece == NM;
+                    const int item = rest ? tile + si : (tile + si) * NM + piece;
+                    const int ring = rest ? RS : PS, s = item % ring;
+                    if (mbar_test((rest ? full_r : full_p) + s, (item / ring) & 1)) {
+                        tc_fence_after();
+                        const uint32_t d = tmem + C::S_COL + ((tile + si) & 1) * N;
+                        const uint64_t kd = rest ? kr_desc + (uint32_t)(s * (kLatChunk >> 4))
+                                                 : kp_desc + (uint32_t)(s * (kLatPair >> 4));
+                        const int k_end = min(KSTEPS - piece * 8, rest ? 4 : 8);
+#pragma unroll
+                        for (int kk = 0; kk < 8; ++kk) {
+                            if (kk >= k_end) break;
+                            const uint32_t ko = ((kk >> 2) * kLatChunk + (kk & 3) * 32) >> 4;
+                            const uint32_t qo =
+                                ((piece * 2 + (kk >> 2)) * C::Q_CHUNK + (kk & 3) * 32) >> 4;
+                            tc_mma(d, kd + ko, q_desc + qo, idesc_s, (piece > 0 || kk > 0) ? 1u : 0u);
+                        }
+                        if (++piece == pieces) {
+                            if (rest) tc_commit(&empty_r[s]);
+                            tc_commit(&s_full[(tile + si) & 1]);
+                            piece = 0;
+                            ++si;
+                        }
+                        did = true;
+                    }
+                }
+                if (did) {
+                    idle = 0;
+                } else if ((++idle & 63) == 0) {
+                    const uint64_t now = global_ns();
+                    if (idle == 64) since = now;
+                    if (*s_abort || now - since > p.wait_ns) {
+                        ok = false;
+                        break;
+                    }
+                }
+            }
+            tile += n;
+        }
+        if (!ok) {
+            *s_abort = 1;
+            raise_flag(CX_DEV_WAIT_TIMEOUT);
+        }
+        tc_commit(drain);       // completes once every MMA issued above has
+    }
+
+    // ---- teardown: drain this CTA's own copies and MMAs, then free TMEM ----
+    tc_fence_before();
+    __syncthreads();
+    if (*s_abort && tid == 0) {
+        for (int r = 0; r < 2; ++r) {
+            const int issued = s_issued[r], ring = r ? RS : PS;
+            for (int s = 0; s < ring; ++s) {
+                const int uses = issued > s ? (issued - 1 - s) / ring + 1 : 0;
+                if (uses > 0)
+                    mbar_wait_bounded((r ? full_r : full_p) + s, (uses - 1) & 1, nullptr,
+                                      kWaitLimitNs);
+            }
+        }
+    }
+    if (tid == 4 * 32) mbar_wait_bounded(drain, 0, nullptr, kWaitLimitNs);
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 4)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                     "r"(C::TMEM_COLS)
+                     : "memory");
+}
+
+// Joins the parts of cut ranges: block (x, y) has rows [4 y, 4 y + 4) of the range
+// that CTA x's last partial opens, 64 threads a row.
+template <int N>
+__global__ void __launch_bounds__(256) latent_join_kernel(const LatParams p) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int32_t* d = p.desc + (int64_t)blockIdx.x * 8;
+    const int parts = d[0], slot = d[1], n_rows = d[2];
+    const int r = blockIdx.y * 4 + (threadIdx.x >> 6), i0 = threadIdx.x & 63;
+    if (parts < 2 || r >= n_rows) return;
+    const int64_t row = ((int64_t)(uint32_t)d[3] | (int64_t)d[4] << 32) + r;
+    auto at = [&](int k) {
+        return (((int64_t)blockIdx.x + (int64_t)k * p.sub) * 2 + (k == 0 ? slot : 0)) * N + r;
+    };
+    float M = -INFINITY, L = 0.f;
+    for (int k = 0; k < parts; ++k) M = fmaxf(M, p.part_ml[at(k) * 2]);
+    float o[kLatMaxLatent / 64];
+#pragma unroll
+    for (int e = 0; e < kLatMaxLatent / 64; ++e) o[e] = 0.f;
+    for (int k = 0; k < parts; ++k) {
+        const int64_t a = at(k);
+        const float m = p.part_ml[a * 2];
+        if (m == -INFINITY) continue;             // a part that saw no key
+        const float f = exp2f(m - M);
+        L = fmaf(p.part_ml[a * 2 + 1], f, L);
+#pragma unroll
+        for (int e = 0; e < kLatMaxLatent / 64; ++e)
+            if (i0 + 64 * e < p.dc) o[e] = fmaf(p.part_o[a * p.dc + i0 + 64 * e], f, o[e]);
+    }
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+#pragma unroll
+    for (int e = 0; e < kLatMaxLatent / 64; ++e)
+        if (i0 + 64 * e < p.dc)
+            store_as(p.out, p.out_dtype, row * p.dc + i0 + 64 * e, o[e] * inv);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+
+// 3-D view of a 16-bit latent pool: (row, slot, layer * block), box of 64 columns x
+// a block's slots.
+static int make_latent_tmap(CUtensorMap* m, const cx_latent_pool* p) {
+    auto enc = tmap_encoder();
+    if (!enc) return fail(CX_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    const cuuint64_t dim = (cuuint64_t)(p->latent_dim + p->rope_dim);
+    const cuuint64_t dims[3] = {dim, (cuuint64_t)p->block_size,
+                                (cuuint64_t)(p->n_layers * p->n_blocks)};
+    const cuuint64_t strides[2] = {dim * 2, dim * 2 * (cuuint64_t)p->block_size};
+    const cuuint32_t box[3] = {64, (cuuint32_t)p->block_size, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = enc(m, p->dtype == CX_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                           3, p->kv, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(CX_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+    return CX_OK;
+}
+
+template <int N, typename E>
+static int launch_latent_tc(const CUtensorMap& tm, LatParams p, int grid, cudaStream_t st) {
+    int smem = 0;
+    LatCfg<N>::rings(p.dc, p.dim, p.pairs, p.rests, smem);
+    auto kern = latent_tc_kernel<N, E>;
+    CX_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    kern<<<grid, kLatThreads, smem, st>>>(tm, p);
+    int rc = check_launch("latent_tc_kernel");
+    if (rc) return rc;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid, N / 4);
+    cfg.blockDim = 256;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    CX_CUDA_CHECK(cudaLaunchKernelEx(&cfg, latent_join_kernel<N>, p));
+    return check_launch("latent_join_kernel");
+}
+
+}  // namespace cx

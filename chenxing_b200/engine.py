@@ -24,7 +24,11 @@ What the reference does not have and this adds, each opt-in:
   fused into the append launch);
 * ``free_private_blocks=True`` returns a finished sequence's private blocks
   to the free list (the reference leaks them, engine.py:98-104);
-* ``compact()`` packs in-use blocks into the lowest ids after eviction.
+* ``compact()`` packs in-use blocks into the lowest ids after eviction;
+* ``plan(..., tree_parents=)`` verifies a drafted tree per sequence, and
+  ``accept(plan, paths)`` keeps one path of each;
+* a ``LatentPagedKVCache`` in the cache's place: K and V are then the latent
+  rows and the shared key part, Q is (latent, rotary) queries.
 Model projections, sampling and the scheduler's admission policy stay with
 the caller.
 """
@@ -38,6 +42,7 @@ import torch
 
 from ._arrays import upload
 from .batch import PagedBatch, slot_mapping
+from .latent import LatentBatch, LatentPagedKVCache
 from .radix_kv import RadixPagedKVCache
 
 __all__ = ["KVSequence", "StepPlan", "BatchedKVEngine"]
@@ -68,6 +73,7 @@ class StepPlan:
     appended: set = field(default_factory=set)
     positions: torch.Tensor | None = None   # (sum q_lens,) absolute positions, built lazily
     cow_done: bool = False
+    tree: bool = False                 # the rows are nodes of drafted trees
 
     @property
     def n_rows(self) -> int:
@@ -75,14 +81,20 @@ class StepPlan:
 
 
 class BatchedKVEngine:
-    """Owns the live sequences' block tables over one ``RadixPagedKVCache``."""
+    """Owns the live sequences' block tables over one ``RadixPagedKVCache`` or
+    ``LatentPagedKVCache`` (which needs ``scale`` and takes no score modifiers)."""
 
-    def __init__(self, cache: RadixPagedKVCache, *, n_q_heads: int, window: int | None = None,
+    _latent = False
+
+    def __init__(self, cache: RadixPagedKVCache | LatentPagedKVCache, *, n_q_heads: int, window: int | None = None,
                  scale: float | None = None, free_private_blocks: bool = False,
                  publish_mode: str = "reference", softcap: float | None = None,
                  alibi_slopes=None) -> None:
         if publish_mode not in ("reference", "suffix"):
             raise ValueError("publish_mode must be 'reference' or 'suffix'")
+        self._latent = isinstance(cache, LatentPagedKVCache)
+        if self._latent and (scale is None or softcap is not None or alibi_slopes is not None):
+            raise ValueError("a latent cache needs scale, and takes no softcap or alibi_slopes")
         self.cache = cache
         self.publish_mode = publish_mode
         self.n_q_heads = int(n_q_heads)
@@ -211,7 +223,7 @@ class BatchedKVEngine:
     # one step
     # ------------------------------------------------------------------ #
     def plan(self, seq_ids, q_lens=None, *, verify: bool | None = None,
-             attend: bool = True, prefix_lens=None) -> StepPlan:
+             attend: bool = True, prefix_lens=None, tree_parents=None) -> StepPlan:
         """Host metadata for one step: ``q_lens[i]`` new positions for
         sequence ``seq_ids[i]`` starting at its ``n_tokens``.  Grows tables like
         ``LLMEngine._ensure_capacity`` (engine.py:74-85, LRU eviction through
@@ -221,7 +233,12 @@ class BatchedKVEngine:
         lengths) onto the device.  ``attend=False`` is for steps that only
         write K/V (a prompt whose attention the caller does elsewhere).
         ``prefix_lens``: per sequence, the leading tokens that every query row
-        sees (``PagedBatch``)."""
+        sees (``PagedBatch``).  ``tree_parents``: the new positions are the nodes of a
+        drafted tree (``PagedBatch``); ``accept`` ends such a step."""
+        if tree_parents is not None and not attend:
+            raise ValueError("tree_parents needs attend=True")
+        if self._latent and prefix_lens is not None:
+            raise ValueError("a latent cache takes no prefix_lens")
         p = self.plan_host(seq_ids, q_lens)
         c = self.cache
         dev = c.device
@@ -230,11 +247,18 @@ class BatchedKVEngine:
                          dev)
         if attend:
             is_verify = bool(np.any(p.q_lens != 1)) if verify is None else verify
-            p.batch = PagedBatch(c, [s.block_table for s in p.seqs], p.n_past + p.q_lens,
-                                 n_q_heads=self.n_q_heads,
-                                 q_lens=p.q_lens if is_verify else None,
-                                 window=self.window, scale=self.scale, softcap=self.softcap,
-                                 alibi_slopes=self.alibi_slopes, prefix_lens=prefix_lens)
+            kw = dict(n_q_heads=self.n_q_heads, window=self.window, scale=self.scale,
+                      q_lens=p.q_lens if is_verify or tree_parents is not None else None,
+                      tree_parents=tree_parents)
+            tables, ctx = [s.block_table for s in p.seqs], p.n_past + p.q_lens
+            if self._latent:
+                p.batch = LatentBatch(c, tables, ctx, **kw)
+            else:
+                p.batch = PagedBatch(c, tables, ctx, softcap=self.softcap, prefix_lens=prefix_lens,
+                                     alibi_slopes=self.alibi_slopes, **kw)
+            if tree_parents is not None:
+                p.tree = True
+                p.positions = upload(p.batch.row_positions(), dev)
         if p.cow_host:
             arr = np.asarray(p.cow_host, dtype=np.int32).T.copy()
             p.cow = tuple(upload(a, dev) for a in arr)
@@ -298,7 +322,9 @@ class BatchedKVEngine:
         ``cache.append_norm_rope``; without weights, tables of part of the head
         are refused unless ``rot_dim`` says that they are meant.  Q is returned as bfloat16 from the plain
         rotation and, from the other, in the pool's type, which the attention
-        over it takes as it is; ``q_out_dtype`` says otherwise."""
+        over it takes as it is; ``q_out_dtype`` says otherwise.  Over a latent
+        cache k and v are the latent and the shared key part, ``k_weight`` the
+        latent's norm and q the queries' rotary part."""
         if rot_dim is not None and rot_dim != rope.head_dim:
             raise ValueError(f"rot_dim {rot_dim} with RoPE tables of {rope.head_dim} dims")
         if plan.cow_host and not plan.cow_done:
@@ -311,6 +337,14 @@ class BatchedKVEngine:
                                   for n0, n in zip(plan.n_past, plan.q_lens)]) \
                 if len(plan.q_lens) else np.zeros(0, dtype=np.int64)
             plan.positions = upload(pos, self.cache.device)
+        if self._latent:
+            if q_weight is not None:
+                raise ValueError("a latent cache norms the latent only: no q_weight")
+            qo = self.cache.append_norm_rope(layer, k, v, plan.slots, plan.positions, rope, q,
+                                             weight=k_weight, eps=eps,
+                                             q_out_dtype=q_out_dtype or self.cache.torch_dtype)
+            plan.appended.add(int(layer))
+            return qo
         if q_weight is not None or k_weight is not None or rot_dim is not None:
             qo = self.cache.append_norm_rope(layer, k, v, plan.slots, plan.positions, rope, q,
                                              q_weight=q_weight, k_weight=k_weight, eps=eps,
@@ -334,8 +368,25 @@ class BatchedKVEngine:
             return self.cache.verify_batch(layer, q, plan.batch, out, out_dtype=out_dtype)
         return self.cache.decode_batch(layer, q, plan.batch, out, out_dtype=out_dtype)
 
+    def accept(self, plan: StepPlan, paths) -> None:
+        """End a verified step with one path of each sequence's tree (or of its
+        chain): lists of query rows of ``plan``, ascending.  Their K/V move behind the
+        committed context in every layer, and as many positions are committed
+        (``commit`` is for steps that keep every row).  The tokens are the
+        caller's to record (``extend_tokens``)."""
+        if plan.batch is None:
+            raise RuntimeError("plan(..., attend=False) has no attention batch")
+        paths = [list(map(int, p)) for p in paths]
+        if any(s.n_tokens != n for s, n in zip(plan.seqs, plan.n_past)):
+            raise RuntimeError("accept() after the plan's sequences moved on")
+        self.cache.accept_paths(plan.batch, paths)
+        for s, p in zip(plan.seqs, paths):
+            s.n_tokens += len(p)
+
     def commit(self, plan: StepPlan) -> None:
         """``forward_ids``'s ``seq.n_tokens += len(new_ids)`` (engine.py:127)."""
+        if plan.tree:
+            raise RuntimeError("a step with tree_parents ends with accept()")
         for s, n in zip(plan.seqs, plan.q_lens):
             s.n_tokens += int(n)
 
@@ -347,7 +398,7 @@ class BatchedKVEngine:
         recorded around the copy launch (when there is one)."""
         live = [s.block_table for s in self.seqs.values()]
         src, dst = self.cache.plan_compaction(live, max_moves)
-        if src and isinstance(self.cache, RadixPagedKVCache):
+        if src and isinstance(self.cache, (RadixPagedKVCache, LatentPagedKVCache)):
             self.cache.copy_blocks(src, dst, events=events)   # bare RadixIndex: metadata only
         n = len(src)
         for a, b in zip(src, dst):

@@ -15,6 +15,8 @@ libcxkv kernel:
 * ``read_layer``   -> ``cx_kv_gather``  (radix_kv.py:130-144)
 * ``copy_blocks`` / ``cow_tail`` / ``compact`` -> ``cx_block_copy`` (no reference
   counterpart)
+* ``accept_paths`` -> ``cx_kv_accept`` (a drafted tree's accepted path, no
+  reference counterpart)
 * ``append_batch`` / ``decode_batch`` / ``verify_batch`` — batched forms over
   many sequences (see ``chenxing_b200.batch``).
 
@@ -398,7 +400,107 @@ def _check_cow_slots(slots, cow, block_size: int) -> None:
                              f"{int(n)} copied rows")
 
 
-class RadixPagedKVCache(RadixIndex):
+class _BlockPool(RadixIndex):
+    """What the caches over a pool of blocks share: moves of whole blocks and of
+    accepted nodes.  A subclass launches them (``_copy_launch``, ``_accept_launch``)."""
+
+    def _check_ids(self, ids) -> None:
+        for b in ids:
+            if not 0 <= int(b) < self.n_blocks:
+                raise IndexError(f"block id {b} outside [0, {self.n_blocks})")
+
+    def copy_blocks(self, src: list, dst: list, n_slots: int | None = None,
+                    events=None) -> None:
+        """Copy slots [0, n_slots) of block src[i] into block dst[i], every layer,
+        (eviction compaction / prefix forking).  ``events``: an optional
+        pair of CUDA events recorded right before and after the copy launch."""
+        if len(src) != len(dst):
+            raise ValueError("src and dst must have the same length")
+        if not src:
+            return
+        self._check_ids(src)
+        self._check_ids(dst)
+        if len(set(dst)) != len(dst) or set(src) & set(dst):
+            raise ValueError("copy_blocks needs distinct destinations disjoint from sources")
+        n_slots = self.block_size if n_slots is None else int(n_slots)
+        s = upload(np.asarray(src, dtype=np.int32), self.device)
+        t = upload(np.asarray(dst, dtype=np.int32), self.device)
+        if events is not None:
+            events[0].record()
+        self._copy_launch(s, t, len(src), n_slots)
+        if events is not None:
+            events[1].record()
+
+    def compact(self, tables=(), max_moves: int | None = None) -> int:
+        """Pack in-use blocks into the lowest ids (``plan_compaction``) and move
+        their K/V, every layer, with one ``cx_block_copy``; returns the number
+        of blocks moved.  Runs on the cache's current stream, so later kernels
+        on that stream see the moved data."""
+        src, dst = self.plan_compaction(tables, max_moves)
+        if src:
+            self.copy_blocks(src, dst)
+        return len(src)
+
+    def cow_tail(self, block_table: list, n_tokens: int, is_shared) -> tuple | None:
+        """Copy-on-write of a shared, partially filled tail block.
+
+        If position ``n_tokens`` (the next write) falls inside block
+        ``block_table[j]`` with ``r = n_tokens % block_size > 0`` valid slots
+        and ``is_shared(block_id)`` is true, allocate a private block, copy the
+        r valid slots of every layer, and swap it into the table in place.
+        Returns (src, dst, r) or None.  The reference has no CoW: it shares
+        whole blocks only (radix_kv.py:16-21).
+        """
+        j, r = divmod(int(n_tokens), self.block_size)
+        if r == 0 or j >= len(block_table) or not is_shared(block_table[j]):
+            return None
+        src = block_table[j]
+        dst = self.alloc_block()
+        self.copy_blocks([src], [dst], r)
+        block_table[j] = dst
+        return src, dst, r
+
+    # ------------------------------------------------------------------ #
+    # speculative trees
+    # ------------------------------------------------------------------ #
+    def accept_paths(self, batch, paths) -> None:
+        """Keep one path of each sequence's drafted tree: row ``paths[b][k]`` (a query
+        row of ``batch``, which was verified) moves to the position ``k`` behind the
+        committed context, in every layer and in place.  The caller then commits as
+        many tokens as the path has.
+
+        paths: lists of node numbers, or an integer tensor (B, n) in which a negative
+        entry ends a path (a device tensor is read in stream order, so that a
+        captured graph takes each replay's paths).  A path ascends strictly; lists are
+        checked here, a tensor by the kernel ("bad path of accepted nodes")."""
+        if batch.cache is not self:
+            raise ValueError("the batch belongs to a different cache")
+        if isinstance(paths, torch.Tensor):
+            if paths.dim() != 2 or paths.shape[0] != batch.batch:
+                raise ValueError(f"paths must be ({batch.batch}, n), got {tuple(paths.shape)}")
+            if paths.dtype.is_floating_point or paths.dtype == torch.bool or paths.is_complex():
+                raise TypeError("paths must be integers")
+            t = paths.to(self.device, torch.int32, non_blocking=True)
+            if t.shape[1] > 1 and t.stride(1) != 1 or t.stride(0) < t.shape[1]:
+                t = t.contiguous()
+        else:
+            rows = [list(map(int, p)) for p in paths]
+            if len(rows) != batch.batch:
+                raise ValueError("paths must be one list per sequence")
+            for p, n in zip(rows, batch.q_lens_host):
+                if any(not 0 <= x < n for x in p) or any(a >= b for a, b in zip(p, p[1:])):
+                    raise ValueError("a path must ascend over the sequence's query rows")
+            a = np.full((len(rows), max(map(len, rows), default=0)), -1, dtype=np.int32)
+            for b, p in enumerate(rows):
+                a[b, :len(p)] = p
+            t = upload(a, self.device)
+        if t.numel() == 0:
+            return
+        with _lib.on_device(self.device):
+            self._accept_launch(batch.c_struct(), t, max(t.stride(0), t.shape[1]), t.shape[1])
+
+
+class RadixPagedKVCache(_BlockPool):
     """Physical block pool (all layers, in HBM) + logical radix prefix tree."""
 
     def __init__(self, n_blocks: int, block_size: int, n_layers: int, n_kv_heads: int,
@@ -447,11 +549,6 @@ class RadixPagedKVCache(RadixIndex):
     # ------------------------------------------------------------------ #
     # physical layer (radix_kv.py:113-144)
     # ------------------------------------------------------------------ #
-    def _check_ids(self, ids) -> None:
-        for b in ids:
-            if not 0 <= int(b) < self.n_blocks:
-                raise IndexError(f"block id {b} outside [0, {self.n_blocks})")
-
     def write_layer(self, block_table: list, slot_start: int, layer: int, k, v) -> None:
         """Store K/V rows for positions [slot_start, slot_start + T) of one layer.
 
@@ -520,58 +617,13 @@ class RadixPagedKVCache(RadixIndex):
             return to_numpy(ko), to_numpy(vo)
         return ko, vo
 
-    def copy_blocks(self, src: list, dst: list, n_slots: int | None = None,
-                    events=None) -> None:
-        """Copy slots [0, n_slots) of block src[i] into block dst[i], every layer,
-        K and V (eviction compaction / prefix forking).  ``events``: an optional
-        pair of CUDA events recorded right before and after the copy launch."""
-        if len(src) != len(dst):
-            raise ValueError("src and dst must have the same length")
-        if not src:
-            return
-        self._check_ids(src)
-        self._check_ids(dst)
-        if len(set(dst)) != len(dst) or set(src) & set(dst):
-            raise ValueError("copy_blocks needs distinct destinations disjoint from sources")
-        n_slots = self.block_size if n_slots is None else int(n_slots)
-        s = upload(np.asarray(src, dtype=np.int32), self.device)
-        t = upload(np.asarray(dst, dtype=np.int32), self.device)
-        if events is not None:
-            events[0].record()
-        _lib.check(_lib.lib().cx_block_copy(self._pool, s.data_ptr(), t.data_ptr(), len(src),
-                                            n_slots, _lib.stream_ptr(self.device)),
-                   "cx_block_copy")
-        if events is not None:
-            events[1].record()
+    def _copy_launch(self, src: torch.Tensor, dst: torch.Tensor, n: int, n_slots: int) -> None:
+        _lib.check(_lib.lib().cx_block_copy(self._pool, src.data_ptr(), dst.data_ptr(), n, n_slots,
+                                            _lib.stream_ptr(self.device)), "cx_block_copy")
 
-    def compact(self, tables=(), max_moves: int | None = None) -> int:
-        """Pack in-use blocks into the lowest ids (``plan_compaction``) and move
-        their K/V, every layer, with one ``cx_block_copy``; returns the number
-        of blocks moved.  Runs on the cache's current stream, so later kernels
-        on that stream see the moved data."""
-        src, dst = self.plan_compaction(tables, max_moves)
-        if src:
-            self.copy_blocks(src, dst)
-        return len(src)
-
-    def cow_tail(self, block_table: list, n_tokens: int, is_shared) -> tuple | None:
-        """Copy-on-write of a shared, partially filled tail block.
-
-        If position ``n_tokens`` (the next write) falls inside block
-        ``block_table[j]`` with ``r = n_tokens % block_size > 0`` valid slots
-        and ``is_shared(block_id)`` is true, allocate a private block, copy the
-        r valid slots of every layer, and swap it into the table in place.
-        Returns (src, dst, r) or None.  The reference has no CoW: it shares
-        whole blocks only (radix_kv.py:16-21).
-        """
-        j, r = divmod(int(n_tokens), self.block_size)
-        if r == 0 or j >= len(block_table) or not is_shared(block_table[j]):
-            return None
-        src = block_table[j]
-        dst = self.alloc_block()
-        self.copy_blocks([src], [dst], r)
-        block_table[j] = dst
-        return src, dst, r
+    def _accept_launch(self, batch, paths: torch.Tensor, stride: int, length: int) -> None:
+        _lib.check(_lib.lib().cx_kv_accept(self._pool, batch, paths.data_ptr(), stride, length,
+                                           _lib.raw_stream(self.device)), "cx_kv_accept")
 
     # ------------------------------------------------------------------ #
     # batched forms (many sequences per launch)
@@ -703,6 +755,7 @@ class RadixPagedKVCache(RadixIndex):
         return decode_batch(self, layer, q, batch, out, replan, out_dtype)
 
     def verify_batch(self, layer: int, q, batch, out=None, replan=None, out_dtype=None):
-        """Paged multi-query attention (speculative verify / prefill chunk)."""
+        """Paged multi-query attention (speculative verify / prefill chunk, drafted
+        trees)."""
         from .batch import verify_batch
         return verify_batch(self, layer, q, batch, out, replan, out_dtype)

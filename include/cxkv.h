@@ -50,7 +50,8 @@ enum {
     CX_DEV_TABLE_OVERRUN = 1u << 2,/* context longer than its block table     */
     CX_DEV_WAIT_TIMEOUT = 1u << 3, /* a bounded pipeline wait gave up         */
     CX_DEV_BAD_QLEN = 1u << 4,     /* query length > context or > max_q_len   */
-    CX_DEV_BAD_POSITION = 1u << 5  /* RoPE position outside the cos/sin table */
+    CX_DEV_BAD_POSITION = 1u << 5, /* RoPE position outside the cos/sin table */
+    CX_DEV_BAD_PATH = 1u << 6      /* accepted nodes not ascending, or not drafted */
 };
 
 /* A block pool: K and V device buffers plus their shape. */
@@ -321,6 +322,132 @@ int cx_paged_attend(const cx_pool* pool, int64_t layer, const cx_attn_batch* bat
 size_t cx_paged_attend_workspace_bytes(const cx_pool* pool, const cx_attn_batch* batch);
 /* Which kernel cx_paged_attend runs (CX_KERNEL_*), as cx_paged_kernel_kind. */
 int cx_paged_attend_kind(const cx_pool* pool, const cx_attn_batch* batch, int32_t q_dtype);
+
+/* A drafted tree per sequence, behind its committed context (no counterpart in
+ * the reference, which verifies chains).  The q_len query rows of a sequence are
+ * the tree's nodes, parents before children; node u's K and V sit at position
+ * base + u, base = ctx_lens[b] - q_len, whatever its depth.  A node counts as
+ * standing `depth` steps behind the last committed token: windows and distance
+ * biases use base + depth for rows and drafted keys alike (and so should the
+ * rotation).  Arrays are on the device; rows are those of q. */
+typedef struct cx_tree {
+    const uint32_t* masks;   /* [rows][words]: bit u % 32 of word u / 32 is set when  */
+                             /* the row sees node u; bits past the row's own node    */
+                             /* count as 0.  The window does not apply among nodes:  */
+                             /* leave out the bits of ancestors that it hides        */
+    int64_t words;           /* >= max_q_len / 32, rounded up                        */
+    const int32_t* depths;   /* [rows] ancestors of the node                         */
+} cx_tree;
+
+/* cx_paged_attend for drafted trees (batch->q_start given): committed keys are
+ * seen as there (a prefix ends at base), drafted keys by the masks.  Everything
+ * else, workspace and plan included, is cx_paged_attend's. */
+int cx_paged_attend_tree(const cx_pool* pool, int64_t layer, const cx_attn_batch* batch,
+                         const cx_attn_mods* mods, const cx_tree* tree, const void* q,
+                         int32_t q_dtype, void* out, void* workspace, size_t workspace_bytes,
+                         int32_t replan, void* stream);
+
+/* After verification: the K and V of the accepted nodes, in every layer, move to
+ * the positions behind the committed context: of sequence b, node
+ * paths[b * path_stride + k] to position base + k (base as in cx_tree), for k up
+ * to the first negative entry or path_len.  A path ascends strictly; an entry that
+ * does not, or is no node of the call's q_len, raises CX_DEV_BAD_PATH and ends its
+ * path there.  The copies read what was there before the call, and a node that is
+ * in its place already is left alone.  No counterpart in the reference
+ * (speculative.py:86-92 only shrinks a chain's length). */
+int cx_kv_accept(const cx_pool* pool, const cx_attn_batch* batch, const int32_t* paths,
+                 int64_t path_stride, int64_t path_len, void* stream);
+
+/* A latent block pool (no counterpart in the reference): one row a token, which is
+ * the key of every query head and in its first latent_dim elements their value.
+ * Layout [n_layers][n_blocks][block_size][latent_dim + rope_dim].  latent_dim is
+ * at most 512, latent_dim + rope_dim at most 576, rope_dim even. */
+typedef struct cx_latent_pool {
+    void* kv;
+    int64_t n_layers;
+    int64_t n_blocks;
+    int64_t block_size;
+    int64_t latent_dim;
+    int64_t rope_dim;
+    int32_t dtype;           /* CX_F32 / CX_BF16 / CX_F16 */
+    int32_t reserved;
+} cx_latent_pool;
+
+/* New rows of one step: latent [n_tokens][latent_dim], rope [n_tokens][rope_dim] and
+ * q [n_tokens][n_q_heads][rope_dim] (the queries' rotary parts; NULL with n_q_heads
+ * 0), all of `dtype`, innermost dimension contiguous, strides in elements. */
+typedef struct cx_latent_rows {
+    const void* latent;
+    const void* rope;
+    const void* q;
+    int64_t latent_token_stride;
+    int64_t rope_token_stride;
+    int64_t q_token_stride, q_head_stride;
+    int64_t n_tokens;
+    int64_t n_q_heads;
+    int32_t dtype;
+    int32_t reserved;
+} cx_latent_rows;
+
+/* Append to the latent cache: the latent x becomes x * rsqrt(mean(x^2) + eps) *
+ * how->k_weight (NULL: as it is), the shared key part is rotated at positions[t]
+ * (NULL: as it is; else how->rot_dim is rope_dim), both in fp32, rounded once and
+ * stored at slot_mapping[t] (negative: nowhere; the slots of one call must differ).
+ * The queries' rotary parts are rotated into q_out [n_tokens][n_q_heads][rope_dim]
+ * whatever their slot; they need positions.  how->q_weight is not read.  A position
+ * outside the table raises CX_DEV_BAD_POSITION and skips the token. */
+int cx_latent_append(const cx_latent_pool* pool, int64_t layer, const cx_latent_rows* rows,
+                     const int64_t* slot_mapping, const int64_t* positions,
+                     const cx_norm_rope* how, void* q_out, int32_t q_out_dtype, void* stream);
+
+/* The first n_tokens rows of a sequence as latent_out [n_tokens][latent_dim] and
+ * rope_out [n_tokens][rope_dim] (pool dtype). */
+int cx_latent_gather(const cx_latent_pool* pool, int64_t layer, const int32_t* block_table,
+                     int64_t n_tokens, void* latent_out, void* rope_out, void* stream);
+
+/* cx_block_copy for a latent pool: slots [0, n_valid[i]) (NULL: n_slots) of block
+ * dst[i] := block src[i], in one layer or, with layer < 0, in every one. */
+int cx_latent_block_copy(const cx_latent_pool* pool, int64_t layer, const int32_t* src,
+                         const int32_t* dst, const int32_t* n_valid, int64_t n, int64_t n_slots,
+                         void* stream);
+
+/* cx_kv_accept for a latent pool. */
+int cx_latent_accept(const cx_latent_pool* pool, const cx_attn_batch* batch, const int32_t* paths,
+                     int64_t path_stride, int64_t path_len, void* stream);
+
+/* Queries in the latent space: latent [rows][heads][latent_dim] (each head's query
+ * multiplied into the latent space by its key projection), rope [rows][heads]
+ * [rope_dim], of one type, any token and head strides (elements). */
+typedef struct cx_latent_q {
+    const void* latent;
+    const void* rope;
+    int64_t latent_token_stride, latent_head_stride;
+    int64_t rope_token_stride, rope_head_stride;
+    int32_t dtype;
+    int32_t reserved;
+} cx_latent_q;
+
+/* Attention over the latent cache, absorbed form: of query row (t, h)
+ *     s[j] = scale * (q.latent . row_j[:latent_dim] + q.rope . row_j[latent_dim:])
+ *     out  = sum_j softmax(s)[j] row_j[:latent_dim]
+ * over the keys that cx_paged_decode (q_start NULL) or cx_paged_verify would show it,
+ * or with `tree` those of cx_paged_attend_tree.  out is [rows][n_q_heads][latent_dim]
+ * of out_dtype, rounded once from fp32; a row that sees no key is zero.  scale NaN
+ * selects 1/sqrt(latent_dim + rope_dim); a model's scale is that of its heads before
+ * they were absorbed.  What the pool holds where no query row sees it does not
+ * reach the result; at a position that only some rows see, it must be finite.
+ * 16-bit pools with block_size 16, 32 or 64 and (latent_dim + rope_dim) a multiple of
+ * 8, at least 64, take a tcgen05 kernel, which rounds fp32 queries and the
+ * probabilities to the pool's type (the denominator sums the rounded ones); all
+ * else, and queries of the other 16-bit type, an fp32 kernel.  The plan is made in the call: a workspace
+ * holds nothing between calls, but calls that overlap need one each. */
+int cx_latent_attend(const cx_latent_pool* pool, int64_t layer, const cx_attn_batch* batch,
+                     const cx_tree* tree, const cx_latent_q* q, void* out, int32_t out_dtype,
+                     void* workspace, size_t workspace_bytes, void* stream);
+size_t cx_latent_attend_workspace_bytes(const cx_latent_pool* pool, const cx_attn_batch* batch);
+/* Which kernel cx_latent_attend runs: CX_KERNEL_TCGEN05 or CX_KERNEL_GENERIC. */
+int cx_latent_attend_kind(const cx_latent_pool* pool, const cx_attn_batch* batch,
+                          int32_t q_dtype);
 
 /* Dense attention — replaces flash_attention / naive_attention on contiguous
  * arrays (chenxing/core/attention.py:43-148): q [b][hq][sq][d],
