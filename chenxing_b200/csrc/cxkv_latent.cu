@@ -15,7 +15,7 @@ static bool latent_tc(const cx_latent_pool* pool, int32_t q_dtype) {
     const int64_t dim = pool->latent_dim + pool->rope_dim;
     return pool->dtype != CX_F32 && (q_dtype == CX_F32 || q_dtype == pool->dtype) &&
            dim % 8 == 0 && dim >= 64 && (reinterpret_cast<uintptr_t>(pool->kv) & 15) == 0 &&
-           (pool->block_size == 16 || pool->block_size == 32 || pool->block_size == 64);
+           pool->block_size % 8 == 0;
 }
 
 // Rows of a tile, row tiles of the longest sequence, how many of them run side by
@@ -163,14 +163,15 @@ static int latent_attend(const cx_latent_pool* pool, int64_t layer, const cx_att
     p.desc = reinterpret_cast<int32_t*>(w);
     p.part_ml = reinterpret_cast<float*>(w + (size_t)x.grid * 32);
     p.part_o = p.part_ml + (size_t)x.grid * 2 * x.n * 2;
-    CUtensorMap tm;
-    rc = make_latent_tmap(&tm, pool);
+    CUtensorMap tm, tail;
+    rc = make_latent_tmap(&tm, pool, false);
+    if (rc == CX_OK) rc = make_latent_tmap(&tail, pool, true);
     if (rc) return rc;
     auto go = [&](auto e16) {
         using E = decltype(e16);
-        return x.n == 16   ? launch_latent_tc<16, E>(tm, p, x.grid, st)
-               : x.n == 32 ? launch_latent_tc<32, E>(tm, p, x.grid, st)
-                           : launch_latent_tc<64, E>(tm, p, x.grid, st);
+        return x.n == 16   ? launch_latent_tc<16, E>(tm, tail, p, x.grid, st)
+               : x.n == 32 ? launch_latent_tc<32, E>(tm, tail, p, x.grid, st)
+                           : launch_latent_tc<64, E>(tm, tail, p, x.grid, st);
     };
     return pool->dtype == CX_BF16 ? go(__nv_bfloat16{}) : go(__half{});
 }

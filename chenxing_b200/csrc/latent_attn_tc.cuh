@@ -23,13 +23,16 @@
 //
 //   warps 0-3: softmax of a tile's 64 keys (warp w: keys [16 w, 16 w + 16), two keys
 //              and N / 4 rows a thread), Q tiles in, output out.
-//   warp 4   : one thread issues the MMAs: S^T of a tile as its parts arrive, up to
-//              two tiles ahead of O^T, whichever can run.
-//   warp 5   : producer.  A tile arrives as pairs of 64-column chunks (16 KB, what one
-//              128-lane MMA of O^T reads) and a rest chunk with what lies past the
-//              last pair, each in a ring of its own (TMA, 128-byte swizzle).  Blocks
-//              past the sequence and ids outside the pool are read outside the tensor
-//              map, which fills zeros.
+//   warp 4   : issues the MMAs: S^T of a tile up to two tiles ahead of O^T, whichever can
+//              run.
+//   warp 5   : producer.  A tile is 8 groups of 8 rows; a group is one TMA box of all its
+//              64-column chunks (8 rows x 64 columns x chunks, 128-byte swizzle): one run
+//              of global memory, and [chunk][8 rows][128 bytes] in shared memory, so that
+//              both operands are lines of 128 bytes with one stride between groups and
+//              one between chunks.  (A box of 16 rows of one chunk, 2 KB, costs the SM's
+//              TMA unit as much as one of 9 KB: 64 x 8k tokens, 16 heads, 99 us so.)
+//              O^T frees a tile 16 keys at a time.  Groups past the sequence and
+//              ids outside the pool are read outside the tensor map, which fills zeros.
 //
 // The reference of a row's exponentials follows its maximum as in the kernels beside
 // this one (Half16), so that a tile nearly always needs one pass and one vote.
@@ -47,10 +50,11 @@ namespace cx {
 constexpr int kLatKeys = 64;          // keys per tile
 constexpr int kLatMaxDim = 576;       // latent + rotary part
 constexpr int kLatMaxLatent = 512;
-constexpr int kLatPair = 2 * kLatKeys * 128;   // a pair of chunks
-constexpr int kLatChunk = kLatKeys * 128;
-constexpr int kLatThreads = 192;
-constexpr int kLatMaxPairs = 16, kLatMaxRest = 4;
+constexpr int kLatGroups = kLatKeys / 8;       // TMA boxes a tile
+constexpr int kLatP = kLatKeys * 128;          // P^T: a line of up to 64 rows per key
+constexpr int kLatProd = 2;                   // producer warps
+constexpr int kLatThreads = (5 + kLatProd) * 32;
+constexpr int kLatMaxStages = 8;
 constexpr int kLatMinTiles = 4;       // tiles per CTA before another CTA starts
 
 struct LatParams {
@@ -69,7 +73,7 @@ struct LatParams {
     int32_t batch, heads, max_q, rtiles, sub, n_units;
     int32_t n_blocks, block_size, layer, window, dc, dim;
     int32_t q_dtype, out_dtype, q_vec;
-    int32_t pairs, rests;       // ring lengths
+    int32_t stages;             // tiles in shared memory
     float scale_log2;
     uint64_t wait_ns;
 };
@@ -138,14 +142,13 @@ struct LatCfg {
     static constexpr int MISC = 2048;
     static constexpr int TMEM_COLS = 512;
     static constexpr int S_COL = 4 * N;
-    // ring lengths of `dim` (rows beside pairs of 128 latent columns)
-    __host__ static void rings(int dc, int dim, int& pairs, int& rests, int& smem) {
-        const int nch = (dim + 63) / 64, nm = (dc + 127) / 128;
-        const int fixed = 1024 + nch * Q_CHUNK + kLatChunk + MISC;
-        rests = nch > 2 * nm ? 2 : 0;
-        pairs = (232448 - fixed - rests * kLatChunk) / kLatPair;
-        if (pairs > kLatMaxPairs) pairs = kLatMaxPairs;
-        smem = fixed + rests * kLatChunk + pairs * kLatPair;
+    __host__ static void ring(int dim, int& stages, int& smem) {
+        const int nch = (dim + 63) / 64, stage = kLatGroups * nch * 1024;
+        // (behind the last stage comes MISC: O^T's MMAs may read a chunk past a row's last)
+        const int fixed = 1024 + nch * Q_CHUNK + kLatP + MISC;
+        stages = (232448 - fixed) / stage;
+        if (stages > kLatMaxStages) stages = kLatMaxStages;
+        smem = fixed + stages * stage;
         // above half of the SM's shared memory: one CTA an SM, which owns the TMEM
         if (smem < 117 * 1024) smem = 117 * 1024;
     }
@@ -273,45 +276,123 @@ __device__ __forceinline__ uint4 lat_q8(const LatParams& p, int64_t lat, int64_t
                       Half16<E>::pack(x[4], x[5]), Half16<E>::pack(x[6], x[7]));
 }
 
+// Upper word of a descriptor of 128-byte swizzled lines in groups of 8, `stride` bytes
+// apart (tc_sdesc); the lower one holds the address and the leading offset.
+__host__ __device__ constexpr uint32_t lat_desc_hi(uint32_t stride) {
+    return (stride >> 4) | 1u << 14 | 2u << 29;
+}
+
+__device__ __forceinline__ uint32_t lat_desc_lo(const void* p, uint32_t lbo) {
+    return ((smem_addr(p) >> 4) & 0x3FFFu) | (lbo >> 4) << 16;
+}
+
+// tcgen05.mma, tcgen05.commit and a TMA load by one elected thread of a warp that comes
+// here as a whole, with the same operands in every lane: only then do they stay in
+// uniform registers.  An MMA issued by a thread in a branch of its own took 180
+// cycles here whatever its shape (a tile of 52 of them 8,600), one whose thread is
+// chosen by a comparison 50, by elect.sync 25 to 49, which is what the tensor pipe
+// takes for it (64 keys: 25 / 26 / 33 cycles at 16 / 32 / 64 rows; 128 columns: 40 / 41
+// / 49).
+__device__ __forceinline__ void lat_mma(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi,
+                                        uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "mov.b64 a, {%1, %6};\n\t"
+        "mov.b64 b, {%2, %5};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(lat_desc_hi(1024)), "r"(a_hi)
+        : "memory");
+}
+__device__ __forceinline__ void lat_commit(uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+            smem_addr(bar))
+        : "memory");
+}
+__device__ __forceinline__ void lat_tma4(uint32_t dst, const void* tmap, uint32_t bar, int y,
+                                         int z) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %2, %4}], [%5];\n\t}" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(0), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void lat_tma3(uint32_t dst, const void* tmap, uint32_t bar, int x, int y,
+                                         int z) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];\n\t}" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t warp_uniform(uint32_t x) {
+    return __shfl_sync(0xffffffffu, x, 0);
+}
+
+// Asynchronous 16-byte copy to shared memory; zeros when `there` is not set.
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src),
+                 "r"(there ? 16 : 0)
+                 : "memory");
+}
+
 template <typename E>
 __host__ __device__ constexpr uint32_t lat_idesc(int m, int n, int a_mn, int b_mn) {
     return sc_idesc<E>(m, n, b_mn) | ((uint32_t)a_mn << 15);
 }
 
+// A call of f(std::integral_constant<int, n>), 1 <= n <= MAX.
+template <int MAX, typename F>
+__device__ __forceinline__ void with_constant(int n, const F& f) {
+    if constexpr (MAX > 1) {
+        if (n < MAX) {
+            with_constant<MAX - 1>(n, f);
+            return;
+        }
+    }
+    f(std::integral_constant<int, MAX>{});
+}
+
 template <int N, typename E>
 __global__ void __launch_bounds__(kLatThreads, 1)
-    latent_tc_kernel(const __grid_constant__ CUtensorMap tm, const LatParams p) {
+    latent_tc_kernel(const __grid_constant__ CUtensorMap tm,
+                     const __grid_constant__ CUtensorMap tm_tail, const LatParams p) {
     using C = LatCfg<N>;
     constexpr int NJ = N / 8;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = (int)warp_uniform(tid >> 5);
     const int sub_id = (int)blockIdx.x % p.sub, g = (int)blockIdx.x / p.sub;
     const int G = (int)gridDim.x / p.sub;
-    const int NM = (p.dc + 127) / 128, NCH = (p.dim + 63) / 64, KSTEPS = (p.dim + 15) / 16;
-    const int PS = p.pairs, RS = p.rests;
-    const bool has_rest = RS > 0;
+    const int NM = (p.dc + 127) / 128, NCH = (p.dim + 63) / 64;
+    const int ST = p.stages, GS = NCH * 1024, STAGE = kLatGroups * GS;
 
     unsigned char* s_q = sm;
     unsigned char* s_p = s_q + NCH * C::Q_CHUNK;
-    unsigned char* s_pairs = s_p + kLatChunk;
-    unsigned char* s_rest = s_pairs + PS * kLatPair;
-    unsigned char* misc = s_rest + RS * kLatChunk;
-    uint64_t* full_p = reinterpret_cast<uint64_t*>(misc);
-    uint64_t* empty_p = full_p + kLatMaxPairs;
-    uint64_t* full_r = empty_p + kLatMaxPairs;
-    uint64_t* empty_r = full_r + kLatMaxRest;
-    uint64_t* s_full = empty_r + kLatMaxRest;     // [2] S^T of a tile is there
+    unsigned char* s_c = s_p + kLatP;
+    unsigned char* misc = s_c + ST * STAGE;
+    uint64_t* full = reinterpret_cast<uint64_t*>(misc);
+    uint64_t* empty = full + kLatMaxStages;       // [stage][4] 16 keys of a tile are free
+    uint64_t* s_full = empty + 4 * kLatMaxStages; // [2] S^T of a tile is there
     uint64_t* p_full = s_full + 2;                // P^T written, O^T rescaled
     uint64_t* o_done = p_full + 1;                // O^T of a tile is done
     uint64_t* q_full = o_done + 1;                // Q of a range is there
     uint64_t* drain = q_full + 1;                 // last commit of the MMA thread
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
-    volatile int* s_issued = s_abort + 1;         // [2] ring items whose loads were issued
-    int* s_start = const_cast<int*>(s_issued) + 2;    // [4] unit, offset, tiles, all tiles
-    int* s_warp = s_start + 4;                    // [6]
+    volatile int* s_issued = s_abort + 1;         // [kLatProd] tiles whose loads were begun
+    int* s_start = const_cast<int*>(s_issued) + kLatProd;     // [4] unit, offset, tiles, all tiles
+    volatile int* s_n = s_start + 4;              // tiles of the range whose Q is there; 0: no more
+    int* s_warp = s_start + 5;                    // [kLatThreads / 32]
     uint64_t* s_vis = reinterpret_cast<uint64_t*>(misc + 512);        // [64]
     float* s_alpha = reinterpret_cast<float*>(misc + 512);            // [64], after s_vis
     float* s_red = reinterpret_cast<float*>(misc + 1024);             // [4][64]
@@ -374,13 +455,9 @@ __global__ void __launch_bounds__(kLatThreads, 1)
         }
     }
     if (tid == 0) {
-        for (int s = 0; s < PS; ++s) {
-            mbar_init(&full_p[s], 1);
-            mbar_init(&empty_p[s], 1);
-        }
-        for (int s = 0; s < RS; ++s) {
-            mbar_init(&full_r[s], 1);
-            mbar_init(&empty_r[s], 1);
+        for (int s = 0; s < ST; ++s) {
+            mbar_init(&full[s], kLatProd);
+            for (int k = 0; k < 4; ++k) mbar_init(&empty[4 * s + k], 1);
         }
         mbar_init(&s_full[0], 1);
         mbar_init(&s_full[1], 1);
@@ -389,7 +466,7 @@ __global__ void __launch_bounds__(kLatThreads, 1)
         mbar_init(q_full, 128);
         mbar_init(drain, 1);
         *s_abort = 0;
-        s_issued[0] = s_issued[1] = 0;
+        for (int k = 0; k < kLatProd; ++k) s_issued[k] = 0;
         fence_mbar_init();
     }
     if (warp == 4) {
@@ -406,7 +483,7 @@ __global__ void __launch_bounds__(kLatThreads, 1)
     LatCursor cur{s_start[0], s_start[1], s_start[2]};
     LatSeg seg;
     int tile = 0;               // tiles of this CTA before the range
-    const int bs = p.block_size, per_tile = kLatKeys / bs;    // blocks a tile (bs 16, 32, 64)
+    const int bs = p.block_size;                  // (a multiple of 8)
 
     if (warp < 4) {
         // ---------------- Q in, softmax, output ----------------
@@ -416,11 +493,30 @@ __global__ void __launch_bounds__(kLatThreads, 1)
         constexpr float kGrow = Half16<E>::kGrowLog2, kLead = Half16<E>::kLeadLog2;
         bool ok = true;
         int slot = 0;
-        while (ok && cur.next(p, sub_id, N, seg)) {
-            const LatUnit& x = seg.x;
-            const int n = seg.to - seg.from;
-            // ---- Q: every MMA that read the last range's is done ----
-#pragma unroll 4
+        // A range's queries, 16-bit, K-major, swizzled, zero padding rows.  Of the pool's
+        // type and on 16-byte rows they are copied asynchronously.
+        const bool q_async = p.q_vec && p.q_dtype != CX_F32;
+        auto load_q = [&](const LatUnit& x) {
+            if (q_async) {
+                // a warp per row
+                for (int r = warp; r < N; r += 4) {
+                    const bool row_ok = r < x.n_rows;
+                    const int R = x.r0 + r, t = R / p.heads, h = R - t * p.heads;
+                    const E* lat = static_cast<const E*>(p.q_lat) + (x.qs + t) * p.ql_tok +
+                                   h * p.ql_head;
+                    const E* rope = static_cast<const E*>(p.q_rope) + (x.qs + t) * p.qr_tok +
+                                    h * p.qr_head - p.dc;
+                    unsigned char* dst = s_q + r * 128;
+                    for (int ch = lane; ch < NCH * 8; ch += 32) {
+                        const int d = ch * 8;
+                        const bool there = row_ok && d < p.dim;
+                        const E* src = (d < p.dc ? lat : rope) + d;
+                        cp_async16(dst + (ch >> 3) * C::Q_CHUNK + (((ch & 7) ^ (r & 7)) << 4),
+                                   there ? src : static_cast<const E*>(p.q_lat), there);
+                    }
+                }
+                return;
+            }
             for (int i = tid; i < N * NCH * 8; i += 128) {
                 const int r = i / (NCH * 8), ch = i - r * (NCH * 8);
                 uint4 v = make_uint4(0, 0, 0, 0);
@@ -432,13 +528,25 @@ __global__ void __launch_bounds__(kLatThreads, 1)
                 *reinterpret_cast<uint4*>(s_q + (ch >> 3) * C::Q_CHUNK + r * 128 +
                                           (((ch & 7) ^ (r & 7)) << 4)) = v;
             }
+        };
+        auto q_ready = [&](int n) {                  // n tiles; 0: no further range
+            if (tid == 0) *s_n = n;
+            if (q_async) asm volatile("cp.async.wait_all;" ::: "memory");
             fence_async_smem();
             mbar_arrive(q_full);
+        };
+        bool more = cur.next(p, sub_id, N, seg);
+        if (more) load_q(seg.x);
+        q_ready(more ? seg.to - seg.from : 0);
+        while (more) {
+            const LatUnit x = seg.x;
+            const int n = seg.to - seg.from, from = seg.from;
+            const bool whole = seg.whole();
             const int32_t* tab = p.tables + (int64_t)x.b * p.table_stride;
             const int nblk = (x.ctx + bs - 1) / bs;
-            const int first_k = (x.tile0 + seg.from) * kLatKeys;
+            const int first_k = (x.tile0 + from) * kLatKeys;
             bool bad = false;
-            for (int k = first_k / bs + tid; k < min(nblk, (first_k + n * kLatKeys) / bs); k += 128) {
+            for (int k = first_k / bs + tid; k < nblk && k * bs < first_k + n * kLatKeys; k += 128) {
                 const int id = tab[k];
                 bad |= id < 0 || id >= p.n_blocks;
             }
@@ -459,6 +567,11 @@ __global__ void __launch_bounds__(kLatThreads, 1)
                 ok = mbar_wait_bounded(&s_full[tile & 1], (tile >> 1) & 1, s_abort, p.wait_ns);
                 if (!(ok = bar_red_and(1, 128, ok))) break;
                 tc_fence_after();
+                if (i == n - 1) {
+                    // every MMA that reads this range's queries is done: the next range's
+                    more = cur.next(p, sub_id, N, seg);
+                    if (more) load_q(seg.x);
+                }
                 float v[N / 2];
                 lat_ld_s<N>(tmem + C::S_COL + (tile & 1) * N + lane_base, v);
                 tc_wait_ld();
@@ -470,9 +583,9 @@ __global__ void __launch_bounds__(kLatThreads, 1)
                     uint64_t vis = 0;
                     if (tid < x.n_rows) {
                         vis = lat_visible(p, x, x.r0 + tid, k0);
-                        for (int k = 0; any_bad && k < per_tile; ++k) {
-                            const int blk = k0 / bs + k, id = blk < nblk ? tab[blk] : 0;
-                            if (id < 0 || id >= p.n_blocks) vis &= ~bit_run(k * bs, k * bs + bs);
+                        for (int k = 0; any_bad && k < kLatGroups; ++k) {
+                            const int blk = (k0 + 8 * k) / bs, id = blk < nblk ? tab[blk] : 0;
+                            if (id < 0 || id >= p.n_blocks) vis &= ~(0xffull << 8 * k);
                         }
                     }
                     if (tid < 64) s_vis[tid] = vis;
@@ -521,7 +634,7 @@ __global__ void __launch_bounds__(kLatThreads, 1)
                             float alpha = 1.f;
                             if (y > m[j][e] + kGrow) {      // (m -inf: any score that is not)
                                 const float mn = y + kLead;
-                                alpha = exp2f(m[j][e] - mn);
+                                alpha = ex2_sfu(m[j][e] - mn);
                                 m[j][e] = mn;
                                 moved = true;
                             }
@@ -578,10 +691,10 @@ __global__ void __launch_bounds__(kLatThreads, 1)
                 if (dead != 0) {
                     const int tok = tid & 63;
                     if ((dead >> tok) & 1) {
-                        for (int mm = 0; mm < NM; ++mm) {
-                            const int q = tile * NM + mm;
-                            uint4* z = reinterpret_cast<uint4*>(
-                                s_pairs + (q % PS) * kLatPair + (tid >> 6) * kLatChunk + tok * 128);
+                        unsigned char* line = s_c + (tile % ST) * STAGE + (tok >> 3) * GS +
+                                              (tok & 7) * 128;
+                        for (int ch = tid >> 6; ch < min(2 * NM, NCH); ch += 2) {
+                            uint4* z = reinterpret_cast<uint4*>(line + ch * 1024);
 #pragma unroll
                             for (int k = 0; k < 8; ++k) z[k] = make_uint4(0, 0, 0, 0);
                         }
@@ -600,6 +713,7 @@ __global__ void __launch_bounds__(kLatThreads, 1)
             }
             // (a wait before the last P^T may have given up in some threads only)
             if (!(ok = bar_red_and(1, 128, ok))) break;
+            q_ready(more ? seg.to - seg.from : 0);      // S^T of the next range runs beside what follows
             // ---- denominators, then O^T to the output or to this CTA's part ----
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
@@ -614,7 +728,6 @@ __global__ void __launch_bounds__(kLatThreads, 1)
             ok = mbar_wait_bounded(o_done, (tile - 1) & 1, s_abort, p.wait_ns);
             if (!(ok = bar_red_and(1, 128, ok))) break;
             tc_fence_after();
-            const bool whole = seg.whole();
             const int64_t part = ((int64_t)blockIdx.x * 2 + slot) * N;
             if (tid < N) {
                 const float L = (s_red[tid] + s_red[64 + tid]) + (s_red[128 + tid] + s_red[192 + tid]);
@@ -633,30 +746,55 @@ __global__ void __launch_bounds__(kLatThreads, 1)
 #pragma unroll 1
             for (int k = 0; k < NM * (N / 16); ++k) {
                 const int mm = k / (N / 16), n0 = (k % (N / 16)) * 16;
-                const int d = mm * 128 + warp * 32 + lane;
+                const int d = mm * 128 + warp * 32 + lane, rows = x.n_rows - n0;
+                if (rows <= 0) continue;                     // (the same for the warp)
                 float o[16];
-                __syncwarp();
                 sc_ld16(tmem + mm * N + n0 + lane_base, o);
                 tc_wait_ld();
-                if (d >= p.dc) continue;
-                if (whole) {
+                if (!whole) {
+                    float* dst = p.part_o + (part + n0) * p.dc + d;
+                    if (d < p.dc) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (n0 + e < x.n_rows)
-                            store_as(p.out, p.out_dtype, (row0 + n0 + e) * p.dc + d,
-                                     o[e] * s_alpha[n0 + e]);
+                        for (int e = 0; e < 16; ++e)
+                            if (e < rows) dst[(int64_t)e * p.dc] = o[e];
+                    }
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (n0 + e < x.n_rows) p.part_o[(part + n0 + e) * p.dc + d] = o[e];
+                    for (int e = 0; e < 16; ++e) o[e] *= s_alpha[n0 + e];
+                    if (p.out_dtype == CX_F32 || (p.dc & 1) ||
+                        (reinterpret_cast<uintptr_t>(p.out) & 3)) {
+                        if (d < p.dc) {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                if (e < rows)
+                                    store_as(p.out, p.out_dtype, (row0 + n0 + e) * p.dc + d, o[e]);
+                        }
+                    } else {
+                        // pairs of columns: an even lane writes the even rows of both, its
+                        // neighbour the odd ones
+                        uint32_t* dst = static_cast<uint32_t*>(p.out) +
+                                        ((row0 + n0 + (lane & 1)) * p.dc + (d & ~1)) / 2;
+                        const bool bf = p.out_dtype == CX_BF16, in = (d & ~1) < p.dc;
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) {
+                            const float give = lane & 1 ? o[e] : o[e + 1];
+                            const float keep = lane & 1 ? o[e + 1] : o[e];
+                            const float got = __shfl_xor_sync(0xffffffffu, give, 1);
+                            const float a = lane & 1 ? got : keep, b = lane & 1 ? keep : got;
+                            const uint32_t u = bf ? Half16<__nv_bfloat16>::pack(a, b)
+                                                  : Half16<__half>::pack(a, b);
+                            if (in && e + (lane & 1) < rows) dst[(int64_t)e * p.dc / 2] = u;
+                        }
+                    }
                 }
+                __syncwarp();
             }
             tc_fence_before();
-            if (!whole && seg.from == 0 && tid == 0) {
+            if (!whole && from == 0 && tid == 0) {
                 // the unit starts here and goes on: who has the rest of it
                 const int W = s_start[3];
                 const int P = min(G, max(1, (W + kLatMinTiles - 1) / kLatMinTiles));
-                const int end = (int)((int64_t)(g + 1) * W / P) + x.n_tiles - seg.to;
+                const int end = (int)((int64_t)(g + 1) * W / P) + x.n_tiles - (from + n);
                 int last = g + 1;
                 while (last + 1 < P && (int)((int64_t)(last + 1) * W / P) < end) ++last;
                 int32_t* d = p.desc + (int64_t)blockIdx.x * 8;
@@ -673,159 +811,157 @@ __global__ void __launch_bounds__(kLatThreads, 1)
             *s_abort = 1;
             if (tid == 0) raise_flag(CX_DEV_WAIT_TIMEOUT);
         }
-    } else if (warp == 5) {
+    } else if (warp > 4) {
         // ---------------- producer ----------------
-        const uint32_t box = (uint32_t)bs * 128;      // a block's rows of a 64-column chunk
+        const int NF = p.dim / 64;                    // whole chunks; a partial one is apart
+        const bool tail = NF < NCH;
         bool go = true;
         while (go && cur.next(p, sub_id, N, seg)) {
             const LatUnit& x = seg.x;
             const int32_t* tab = p.tables + (int64_t)x.b * p.table_stride;
-            const int nblk = (x.ctx + bs - 1) / bs, n = seg.to - seg.from;
-            const int blk0 = (x.tile0 + seg.from) * per_tile;
-            auto block_of = [&](int i) {              // this lane's block of tile i
-                const int blk = blk0 + i * per_tile + lane;
+            const int n = seg.to - seg.from;
+            const int key0 = (x.tile0 + seg.from) * kLatKeys;
+            // lane l < 8: block and row of group l of tile i
+            auto place = [&](int i, int& z, int& row) {
+                const int key = key0 + i * kLatKeys + 8 * lane, blk = key / bs;
+                row = key - blk * bs;
                 int id = -1;
-                if (lane < per_tile && i < n && blk < nblk) {
+                if (lane < kLatGroups && i < n && key < x.ctx) {
                     id = tab[blk];
                     if (id < 0 || id >= p.n_blocks) {
                         raise_flag(CX_DEV_BAD_BLOCK);
                         id = -1;
                     }
                 }
-                return id;
+                // outside the map: the copy fills zeros
+                z = id >= 0 ? p.layer * p.n_blocks + id : -1;
             };
-            int ids = block_of(0);
+            int z, row;
+            place(0, z, row);
             for (int i = 0; go && i < n; ++i, ++tile) {
-                const int next = block_of(i + 1);
-                for (int q = 0; go && q < NM + (has_rest ? 1 : 0); ++q) {
-                    const bool rest = q == NM;
-                    const int item = rest ? tile : tile * NM + q;
-                    const int ring = rest ? RS : PS, s = item % ring, use = item / ring;
-                    uint64_t* full = (rest ? full_r : full_p) + s;
-                    uint64_t* empty = (rest ? empty_r : empty_p) + s;
-                    unsigned char* dst = rest ? s_rest + s * kLatChunk : s_pairs + s * kLatPair;
-                    if (lane == 0) {
-                        go = use == 0 ||
-                             mbar_wait_bounded(empty, (use - 1) & 1, s_abort, p.wait_ns);
-                        go = go && !*s_abort;
-                        if (go) mbar_arrive_expect_tx(full, rest ? kLatChunk : kLatPair);
-                    }
-                    go = __shfl_sync(0xffffffffu, (int)go, 0) != 0;
+                int z_next, row_next;
+                place(i + 1, z_next, row_next);
+                const int s = tile % ST, use = tile / ST;
+                const uint32_t bar = warp_uniform(smem_addr(full + s));
+                const uint32_t dst = warp_uniform(smem_addr(s_c + s * STAGE));
+                for (int k = warp - 5; k < kLatGroups; k += kLatProd) {
+                    go = use == 0 || mbar_wait_bounded(&empty[4 * s + (k >> 1)], (use - 1) & 1,
+                                                       s_abort, p.wait_ns);
+                    go = __all_sync(0xffffffffu, go && !*s_abort);
                     if (!go) break;
-                    const int half = lane / per_tile, k = lane - half * per_tile;
-                    const int id = __shfl_sync(0xffffffffu, ids, k);
-                    if (half < (rest ? 1 : 2)) {
-                        // outside the map: the copy fills zeros
-                        const int z = id >= 0 ? p.layer * p.n_blocks + id : -1;
-                        tma_load_3d(dst + half * kLatChunk + k * box, &tm, full,
-                                    (q * 2 + half) * 64, 0, z);
+                    if (k == warp - 5 && lane == 0) {
+                        mbar_arrive_expect_tx(full + s, STAGE / kLatProd);
+                        s_issued[k] = tile + 1;
                     }
                     __syncwarp();
-                    if (lane == 0) s_issued[rest ? 1 : 0] = item + 1;
+                    const int zk = __shfl_sync(0xffffffffu, z, k);
+                    const int rk = __shfl_sync(0xffffffffu, row, k);
+                    lat_tma4(dst + k * GS, &tm, bar, rk, zk);
+                    if (tail) lat_tma3(dst + k * GS + NF * 1024, &tm_tail, bar, NF * 64, rk, zk);
                 }
-                ids = next;
+                z = z_next;
+                row = row_next;
             }
         }
         if (!go && lane == 0) {
             *s_abort = 1;
             raise_flag(CX_DEV_WAIT_TIMEOUT);
         }
-    } else if (lane == 0) {
-        // ---------------- MMA issuer ----------------
+    } else {
+        // ---------------- MMA issuer: the whole warp, one thread's instructions ----------------
         constexpr uint32_t idesc_s = lat_idesc<E>(kLatKeys, N, 0, 0);
         constexpr uint32_t idesc_o = lat_idesc<E>(128, N, 1, 1);
-        const uint64_t q_desc = tc_sdesc(smem_addr(s_q), 16, 1024);
-        const uint64_t kp_desc = tc_sdesc(smem_addr(s_pairs), 16, 1024);
-        const uint64_t kr_desc = tc_sdesc(smem_addr(s_rest), 16, 1024);
-        const uint64_t v_desc = tc_sdesc(smem_addr(s_pairs), kLatChunk, 1024);
-        const uint64_t p_desc = tc_sdesc(smem_addr(s_p), kLatChunk, 1024);
+        const uint32_t tm = warp_uniform(tmem);
+        const uint32_t q_lo = warp_uniform(lat_desc_lo(s_q, 16));
+        const uint32_t c_lo = warp_uniform(lat_desc_lo(s_c, 1024));
+        const uint32_t c_hi = warp_uniform(lat_desc_hi(GS));
+        const uint32_t p_lo = warp_uniform(lat_desc_lo(s_p, 16));
         bool ok = true;
         int ranges = 0;
-        const int pieces = NM + (has_rest ? 1 : 0);
-        while (ok && cur.next(p, sub_id, N, seg)) {
-            const int n = seg.to - seg.from;
-            ok = mbar_wait_bounded(q_full, ranges & 1, s_abort, p.wait_ns);
+        int o_st = 0, s_st = 0;                   // stages of the next tiles of O^T and S^T
+        uint32_t s_use = 0;                       // parity of s_st's fill
+        for (;;) {
+            ok = warp_uniform(mbar_wait_bounded(q_full, ranges & 1, s_abort, p.wait_ns)) != 0;
             ++ranges;
-            if (!ok) break;
+            const int n = (int)warp_uniform(*s_n);
+            if (!ok || n == 0) break;
             tc_fence_after();
-            int si = 0, oi = 0, piece = 0;
+            int si = 0, oi = 0;
             uint32_t idle = 0;
             uint64_t since = 0;
             while (oi < n) {
                 bool did = false;
-                if (oi < si && mbar_test(p_full, (tile + oi) & 1)) {
+                if (oi < si && warp_uniform(mbar_test(p_full, (tile + oi) & 1))) {
                     tc_fence_after();
-                    for (int mm = 0; mm < NM; ++mm) {
-                        const int s = ((tile + oi) * NM + mm) % PS;
-                        const uint64_t vd = v_desc + (uint32_t)(s * (kLatPair >> 4));
+                    const uint32_t acc = warp_uniform(oi > 0);
+                    uint32_t cd = warp_uniform(c_lo + (uint32_t)(o_st * (STAGE >> 4)));
+                    // (a condition at every MMA doubles what it takes, and triples S^T's)
+                    with_constant<kLatMaxLatent / 128>(NM, [&](auto nm) {
 #pragma unroll
-                        for (int kk = 0; kk < kLatKeys / 16; ++kk)
-                            tc_mma(tmem + mm * N, vd + kk * (2048 >> 4), p_desc + kk * (2048 >> 4),
-                                   idesc_o, (oi > 0 || kk > 0) ? 1u : 0u);
-                        tc_commit(&empty_p[s]);
-                    }
-                    tc_commit(o_done);
+                        for (int kk = 0; kk < kLatKeys / 16; ++kk) {
+#pragma unroll
+                            for (int mm = 0; mm < decltype(nm)::value; ++mm)
+                                lat_mma(tm + mm * N, cd + mm * (2048 >> 4), c_hi,
+                                        p_lo + kk * (2048 >> 4), idesc_o, kk > 0 ? 1u : acc);
+                            lat_commit(&empty[4 * o_st + kk]);
+                            cd += 2 * GS >> 4;
+                        }
+                    });
+                    lat_commit(o_done);
+                    if (++o_st == ST) o_st = 0;
                     ++oi;
                     did = true;
-                } else if (si < n && si < oi + 2) {
-                    const bool rest = piece == NM;
-                    const int item = rest ? tile + si : (tile + si) * NM + piece;
-                    const int ring = rest ? RS : PS, s = item % ring;
-                    if (mbar_test((rest ? full_r : full_p) + s, (item / ring) & 1)) {
-                        tc_fence_after();
-                        const uint32_t d = tmem + C::S_COL + ((tile + si) & 1) * N;
-                        const uint64_t kd = rest ? kr_desc + (uint32_t)(s * (kLatChunk >> 4))
-                                                 : kp_desc + (uint32_t)(s * (kLatPair >> 4));
-                        const int k_end = min(KSTEPS - piece * 8, rest ? 4 : 8);
+                } else if (si < n && si < oi + 2 &&
+                           warp_uniform(mbar_test(full + s_st, s_use))) {
+                    tc_fence_after();
+                    const int b = (tile + si) & 1;
+                    const uint32_t d = warp_uniform(tm + C::S_COL + b * N);
+                    const uint32_t cd = warp_uniform(c_lo + (uint32_t)(s_st * (STAGE >> 4)));
+                    with_constant<(kLatMaxDim + 63) / 64>(NCH, [&](auto nch) {
 #pragma unroll
-                        for (int kk = 0; kk < 8; ++kk) {
-                            if (kk >= k_end) break;
-                            const uint32_t ko = ((kk >> 2) * kLatChunk + (kk & 3) * 32) >> 4;
-                            const uint32_t qo =
-                                ((piece * 2 + (kk >> 2)) * C::Q_CHUNK + (kk & 3) * 32) >> 4;
-                            tc_mma(d, kd + ko, q_desc + qo, idesc_s, (piece > 0 || kk > 0) ? 1u : 0u);
-                        }
-                        if (++piece == pieces) {
-                            if (rest) tc_commit(&empty_r[s]);
-                            tc_commit(&s_full[(tile + si) & 1]);
-                            piece = 0;
-                            ++si;
-                        }
-                        did = true;
+                        for (int k = 0; k < 4 * decltype(nch)::value; ++k)
+                            lat_mma(d, cd + (((k >> 2) * 1024 + (k & 3) * 32) >> 4), c_hi,
+                                    q_lo + (((k >> 2) * C::Q_CHUNK + (k & 3) * 32) >> 4), idesc_s,
+                                    k > 0 ? 1u : 0u);
+                    });
+                    lat_commit(&s_full[b]);
+                    if (++s_st == ST) {
+                        s_st = 0;
+                        s_use ^= 1;
                     }
+                    ++si;
+                    did = true;
                 }
                 if (did) {
                     idle = 0;
-                } else if ((++idle & 63) == 0) {
+                } else if ((idle++ & 15) == 0) {
                     const uint64_t now = global_ns();
-                    if (idle == 64) since = now;
-                    if (*s_abort || now - since > p.wait_ns) {
-                        ok = false;
-                        break;
-                    }
+                    if (idle == 1) since = now;
+                    ok = warp_uniform(!(*s_abort || now - since > p.wait_ns)) != 0;
+                    if (!ok) break;
                 }
             }
+            if (!ok) break;
             tile += n;
         }
-        if (!ok) {
+        if (!ok && lane == 0) {
             *s_abort = 1;
             raise_flag(CX_DEV_WAIT_TIMEOUT);
         }
-        tc_commit(drain);       // completes once every MMA issued above has
+        lat_commit(drain);       // completes once every MMA issued above has
     }
 
     // ---- teardown: drain this CTA's own copies and MMAs, then free TMEM ----
     tc_fence_before();
     __syncthreads();
     if (*s_abort && tid == 0) {
-        for (int r = 0; r < 2; ++r) {
-            const int issued = s_issued[r], ring = r ? RS : PS;
-            for (int s = 0; s < ring; ++s) {
-                const int uses = issued > s ? (issued - 1 - s) / ring + 1 : 0;
-                if (uses > 0)
-                    mbar_wait_bounded((r ? full_r : full_p) + s, (uses - 1) & 1, nullptr,
-                                      kWaitLimitNs);
-            }
+        // (a tile that was given up in the middle never completes: what of it was issued
+        // ends well within the wait)
+        int issued = 0;
+        for (int k = 0; k < kLatProd; ++k) issued = max(issued, s_issued[k]);
+        for (int s = 0; s < ST; ++s) {
+            const int uses = issued > s ? (issued - 1 - s) / ST + 1 : 0;
+            if (uses > 0) mbar_wait_bounded(&full[s], (uses - 1) & 1, nullptr, 20000000ull);
         }
     }
     if (tid == 4 * 32) mbar_wait_bounded(drain, 0, nullptr, kWaitLimitNs);
@@ -876,20 +1012,22 @@ __global__ void __launch_bounds__(256) latent_join_kernel(const LatParams p) {
 // host side
 // ---------------------------------------------------------------------------
 
-// 3-D view of a 16-bit latent pool: (row, slot, layer * block), box of 64 columns x
-// a block's slots.
-static int make_latent_tmap(CUtensorMap* m, const cx_latent_pool* p) {
+// Views of a 16-bit latent pool.  `tail` false: (64 columns, slot, chunk, layer * block),
+// box of 8 slots of every whole chunk; true: (row, slot, layer * block), box of 64
+// columns x 8 slots, for the columns behind the whole chunks.
+static int make_latent_tmap(CUtensorMap* m, const cx_latent_pool* p, bool tail) {
     auto enc = tmap_encoder();
     if (!enc) return fail(CX_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
-    const cuuint64_t dim = (cuuint64_t)(p->latent_dim + p->rope_dim);
-    const cuuint64_t dims[3] = {dim, (cuuint64_t)p->block_size,
-                                (cuuint64_t)(p->n_layers * p->n_blocks)};
-    const cuuint64_t strides[2] = {dim * 2, dim * 2 * (cuuint64_t)p->block_size};
-    const cuuint32_t box[3] = {64, (cuuint32_t)p->block_size, 1};
-    const cuuint32_t estr[3] = {1, 1, 1};
+    const cuuint64_t dim = (cuuint64_t)(p->latent_dim + p->rope_dim), chunks = dim / 64;
+    const cuuint64_t bs = (cuuint64_t)p->block_size, n = (cuuint64_t)(p->n_layers * p->n_blocks);
+    const cuuint64_t dims4[4] = {64, bs, chunks, n}, dims3[3] = {dim, bs, n};
+    const cuuint64_t str4[3] = {dim * 2, 128, dim * 2 * bs}, str3[2] = {dim * 2, dim * 2 * bs};
+    const cuuint32_t box4[4] = {64, 8, (cuuint32_t)chunks, 1}, box3[3] = {64, 8, 1};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
     const CUresult r = enc(m, p->dtype == CX_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                  : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                           3, p->kv, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           tail ? 3 : 4, p->kv, tail ? dims3 : dims4, tail ? str3 : str4,
+                           tail ? box3 : box4, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(CX_ERR_CUDA, "cuTensorMapEncodeTiled failed");
@@ -897,12 +1035,13 @@ static int make_latent_tmap(CUtensorMap* m, const cx_latent_pool* p) {
 }
 
 template <int N, typename E>
-static int launch_latent_tc(const CUtensorMap& tm, LatParams p, int grid, cudaStream_t st) {
+static int launch_latent_tc(const CUtensorMap& tm, const CUtensorMap& tail, LatParams p, int grid,
+                            cudaStream_t st) {
     int smem = 0;
-    LatCfg<N>::rings(p.dc, p.dim, p.pairs, p.rests, smem);
+    LatCfg<N>::ring(p.dim, p.stages, smem);
     auto kern = latent_tc_kernel<N, E>;
     CX_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    kern<<<grid, kLatThreads, smem, st>>>(tm, p);
+    kern<<<grid, kLatThreads, smem, st>>>(tm, tail, p);
     int rc = check_launch("latent_tc_kernel");
     if (rc) return rc;
     cudaLaunchAttribute attr{};
