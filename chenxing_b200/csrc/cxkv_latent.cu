@@ -36,7 +36,7 @@ static LatPlan latent_plan(const cx_latent_pool* pool, const cx_attn_batch* b) {
     const int sms = std::max(num_sms(), x.sub);
     int64_t keys = b->table_stride * pool->block_size;
     if (b->window > 0) keys = std::min(keys, b->window + b->max_q_len + 2 * kLatKeys);
-    const int64_t tiles = x.units * ((keys + kLatKeys - 1) / kLatKeys);
+    const int64_t tiles = x.units * ((keys + kLatKeys - 1) / kLatKeys + kLatRangeCost);
     const int64_t want = std::max<int64_t>(1, (tiles + kLatMinTiles - 1) / kLatMinTiles);
     x.grid = (int)std::min<int64_t>(sms / x.sub, want) * x.sub;
     return x;
@@ -117,6 +117,7 @@ static int latent_attend(const cx_latent_pool* pool, int64_t layer, const cx_att
     p.qr_tok = q->rope_token_stride;
     p.qr_head = q->rope_head_stride;
     p.out = out;
+    p.pool = pool->kv;
     p.batch = (int)b.batch;
     p.heads = (int)b.n_q_heads;
     p.max_q = (int)b.max_q_len;
@@ -129,7 +130,8 @@ static int latent_attend(const cx_latent_pool* pool, int64_t layer, const cx_att
     p.q_dtype = q->dtype;
     p.out_dtype = out_dtype;
     p.scale_log2 = scale * 1.4426950408889634f;
-    p.wait_ns = wait_limit_ns();
+    // (a try suspends for half a microsecond at most)
+    p.tries = (uint32_t)std::min<unsigned long long>(1ull << 30, wait_limit_ns() / 500 + 1);
     if (!tc) {
         LatGenParams g{};
         g.a = p;
@@ -149,7 +151,7 @@ static int latent_attend(const cx_latent_pool* pool, int64_t layer, const cx_att
         }
     }
     const LatPlan x = latent_plan(pool, &b);
-    if (x.units * (cap / kLatKeys + 1) > INT32_MAX)
+    if (x.units * (cap / kLatKeys + 1 + kLatRangeCost) > INT32_MAX)
         return bad(CX_ERR_UNSUPPORTED, "batch x context too large");
     p.rtiles = x.rtiles;
     p.sub = x.sub;
@@ -162,16 +164,16 @@ static int latent_attend(const cx_latent_pool* pool, int64_t layer, const cx_att
     char* w = static_cast<char*>(ws);
     p.desc = reinterpret_cast<int32_t*>(w);
     p.part_ml = reinterpret_cast<float*>(w + (size_t)x.grid * 32);
-    p.part_o = p.part_ml + (size_t)x.grid * 2 * x.n * 2;
-    CUtensorMap tm, tail;
-    rc = make_latent_tmap(&tm, pool, false);
-    if (rc == CX_OK) rc = make_latent_tmap(&tail, pool, true);
+    p.part_o = p.part_ml + (size_t)x.grid * 2 * x.n * 2;   // (16-byte aligned)
+    p.box_rows = latent_box_rows(pool->block_size);
+    CUtensorMap tm;
+    rc = make_latent_tmap(&tm, pool);
     if (rc) return rc;
     auto go = [&](auto e16) {
         using E = decltype(e16);
-        return x.n == 16   ? launch_latent_tc<16, E>(tm, tail, p, x.grid, st)
-               : x.n == 32 ? launch_latent_tc<32, E>(tm, tail, p, x.grid, st)
-                           : launch_latent_tc<64, E>(tm, tail, p, x.grid, st);
+        return x.n == 16   ? launch_latent_tc<16, E>(tm, p, x.grid, st)
+               : x.n == 32 ? launch_latent_tc<32, E>(tm, p, x.grid, st)
+                           : launch_latent_tc<64, E>(tm, p, x.grid, st);
     };
     return pool->dtype == CX_BF16 ? go(__nv_bfloat16{}) : go(__half{});
 }

@@ -21,18 +21,18 @@
 // over the CTAs (every CTA works its share out from the lengths); a (sequence, row
 // tile) that is cut is joined by latent_join_kernel.  Roles:
 //
-//   warps 0-3: softmax of a tile's 64 keys (warp w: keys [16 w, 16 w + 16), two keys
-//              and N / 4 rows a thread), Q tiles in, output out.
-//   warp 4   : issues the MMAs: S^T of a tile up to two tiles ahead of O^T, whichever can
-//              run.
-//   warp 5   : producer.  A tile is 8 groups of 8 rows; a group is one TMA box of all its
-//              64-column chunks (8 rows x 64 columns x chunks, 128-byte swizzle): one run
-//              of global memory, and [chunk][8 rows][128 bytes] in shared memory, so that
-//              both operands are lines of 128 bytes with one stride between groups and
-//              one between chunks.  (A box of 16 rows of one chunk, 2 KB, costs the SM's
-//              TMA unit as much as one of 9 KB: 64 x 8k tokens, 16 heads, 99 us so.)
-//              O^T frees a tile 16 keys at a time.  Groups past the sequence and
-//              ids outside the pool are read outside the tensor map, which fills zeros.
+//   4 or 8 warps: softmax of a tile's 64 keys (16 keys and all or half of the rows a
+//              warp), Q tiles in, output out.
+//   2 warps  : issue the MMAs: one S^T of a tile piece by piece as it arrives, up to two
+//              tiles ahead, the other O^T.  (One warp that polled for whichever could run
+//              took 150 to 350 cycles to see either.)
+//   2 warps  : producers, one for either chunk of a piece.  A tile is [64-column chunk]
+//              [64 keys][128 bytes] (128-byte swizzle) and arrives in pieces of two
+//              chunks, which O^T's MMAs free one after the other; a TMA box is a block's
+//              rows of a chunk.  (Boxes of 16 rows of a chunk take the SM's TMA unit 25
+//              cycles; 8 rows of two chunks in one box, 2 KB as well, 72, and of nine
+//              113.)  Blocks past the sequence and ids outside the pool are read outside
+//              the tensor map, which fills zeros.
 //
 // The reference of a row's exponentials follows its maximum as in the kernels beside
 // this one (Half16), so that a tile nearly always needs one pass and one vote.
@@ -50,18 +50,24 @@ namespace cx {
 constexpr int kLatKeys = 64;          // keys per tile
 constexpr int kLatMaxDim = 576;       // latent + rotary part
 constexpr int kLatMaxLatent = 512;
-constexpr int kLatGroups = kLatKeys / 8;       // TMA boxes a tile
+constexpr int kLatChunk = kLatKeys * 128;      // 64 columns of a tile
 constexpr int kLatP = kLatKeys * 128;          // P^T: a line of up to 64 rows per key
 constexpr int kLatProd = 2;                   // producer warps
-constexpr int kLatThreads = (5 + kLatProd) * 32;
-constexpr int kLatMaxStages = 8;
+constexpr int kLatMaxStages = 4;
+constexpr int kLatMaxPieces = (kLatMaxDim + 127) / 128;
+constexpr int kLatAhead = 3;                  // tiles from the one in work to the one asked for
 constexpr int kLatMinTiles = 4;       // tiles per CTA before another CTA starts
+// What a range costs its CTA beside its tiles (output, first tile), in tiles: with shares
+// of equal tiles the CTAs that two ranges meet in took 72 instead of 66 us (64 x 8k
+// tokens, 16 heads).
+constexpr int kLatRangeCost = 3;
 
 struct LatParams {
     const int32_t* tables;
     int64_t table_stride;
     const int32_t* ctx_lens;
     const int32_t* q_start;     // NULL: one query token per sequence
+    const void* pool;
     TreeMask tree;
     const void* q_lat;
     const void* q_rope;
@@ -74,8 +80,9 @@ struct LatParams {
     int32_t n_blocks, block_size, layer, window, dc, dim;
     int32_t q_dtype, out_dtype, q_vec;
     int32_t stages;             // tiles in shared memory
+    int32_t box_rows;
     float scale_log2;
-    uint64_t wait_ns;
+    uint32_t tries;             // of a wait
 };
 
 // One (sequence, row tile) and its key tiles.
@@ -83,6 +90,9 @@ struct LatUnit {
     int b, T, qs, ctx, base;    // base: committed tokens (ctx - T)
     int r0, n_rows;             // packed rows [r0, r0 + n_rows) of the sequence
     int tile0, n_tiles;         // of the `sub` row tiles that run side by side
+    __device__ __forceinline__ int cost() const {
+        return n_tiles > 0 ? n_tiles + kLatRangeCost : 0;
+    }
 };
 
 __device__ __forceinline__ LatUnit lat_unit(const LatParams& p, int u, int sub_id, int N) {
@@ -107,7 +117,8 @@ __device__ __forceinline__ LatUnit lat_unit(const LatParams& p, int u, int sub_i
     return x;
 }
 
-// A run of tiles of one unit.
+// A run of tiles of one unit.  Shares are counted in cost: a unit's first kLatRangeCost
+// are no tiles.
 struct LatSeg {
     LatUnit x;
     int from, to;
@@ -119,32 +130,41 @@ struct LatCursor {
     __device__ __forceinline__ bool next(const LatParams& p, int sub_id, int N, LatSeg& s) {
         while (left > 0 && u < p.n_units) {
             s.x = lat_unit(p, u, sub_id, N);
-            const int have = s.x.n_tiles - off;
-            if (have <= 0) {
-                ++u;
-                off = 0;
-                continue;
-            }
-            s.from = off;
-            s.to = off + min(left, have);
-            left -= s.to - s.from;
+            const int take = min(left, s.x.cost() - off);
+            s.from = max(off - kLatRangeCost, 0);
+            s.to = off + take - kLatRangeCost;
+            left -= max(take, 0);
             ++u;
             off = 0;
-            if (s.x.n_rows > 0) return true;      // (a side-by-side tile past the rows: none)
+            // (a side-by-side tile past the rows: none)
+            if (s.to > s.from && s.x.n_rows > 0) return true;
         }
         return false;
     }
 };
 
+// Bytes of a tile in shared memory: its chunks, and as many as O^T's MMAs of 128
+// columns read.
+__host__ __device__ inline int lat_stage(int dc, int dim) {
+    const int nch = (dim + 63) / 64, read = (dc + 127) / 128 * 2;
+    return (nch > read ? nch : read) * kLatChunk;
+}
+
 template <int N>
 struct LatCfg {
+    // softmax warps: rows of 64 in two halves, so that a tile takes half as long (the way
+    // from S^T to P^T is part of what a tile in shared memory waits for: 163 us for 32 x
+    // 16k tokens of 128 heads with four warps)
+    static constexpr int SW = N == 64 ? 8 : 4;
+    static constexpr int ST = SW * 32;
+    static constexpr int NW = N / (SW / 4);       // rows of a warp
+    static constexpr int THREADS = (SW + 2 + kLatProd) * 32;
     static constexpr int Q_CHUNK = N * 128;
     static constexpr int MISC = 2048;
     static constexpr int TMEM_COLS = 512;
     static constexpr int S_COL = 4 * N;
-    __host__ static void ring(int dim, int& stages, int& smem) {
-        const int nch = (dim + 63) / 64, stage = kLatGroups * nch * 1024;
-        // (behind the last stage comes MISC: O^T's MMAs may read a chunk past a row's last)
+    __host__ static void ring(int dc, int dim, int& stages, int& smem) {
+        const int nch = (dim + 63) / 64, stage = lat_stage(dc, dim);
         const int fixed = 1024 + nch * Q_CHUNK + kLatP + MISC;
         stages = (232448 - fixed) / stage;
         if (stages > kLatMaxStages) stages = kLatMaxStages;
@@ -153,18 +173,6 @@ struct LatCfg {
         if (smem < 117 * 1024) smem = 117 * 1024;
     }
 };
-
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_addr(bar)), "r"(parity)
-        : "memory");
-    return done != 0;
-}
 
 // OR of `pred` over the `nthreads` threads that meet at named barrier `id`.
 __device__ __forceinline__ bool bar_red_or(int id, int nthreads, bool pred) {
@@ -276,11 +284,9 @@ __device__ __forceinline__ uint4 lat_q8(const LatParams& p, int64_t lat, int64_t
                       Half16<E>::pack(x[4], x[5]), Half16<E>::pack(x[6], x[7]));
 }
 
-// Upper word of a descriptor of 128-byte swizzled lines in groups of 8, `stride` bytes
+// Upper word of a descriptor of 128-byte swizzled lines in groups of 8, 1024 bytes
 // apart (tc_sdesc); the lower one holds the address and the leading offset.
-__host__ __device__ constexpr uint32_t lat_desc_hi(uint32_t stride) {
-    return (stride >> 4) | 1u << 14 | 2u << 29;
-}
+constexpr uint32_t kLatDescHi = (1024u >> 4) | 1u << 14 | 2u << 29;
 
 __device__ __forceinline__ uint32_t lat_desc_lo(const void* p, uint32_t lbo) {
     return ((smem_addr(p) >> 4) & 0x3FFFu) | (lbo >> 4) << 16;
@@ -293,16 +299,16 @@ __device__ __forceinline__ uint32_t lat_desc_lo(const void* p, uint32_t lbo) {
 // chosen by a comparison 50, by elect.sync 25 to 49, which is what the tensor pipe
 // takes for it (64 keys: 25 / 26 / 33 cycles at 16 / 32 / 64 rows; 128 columns: 40 / 41
 // / 49).
-__device__ __forceinline__ void lat_mma(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi,
-                                        uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void lat_mma(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo,
+                                        uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
         "elect.sync _|q, 0xffffffff;\n\t"
-        "mov.b64 a, {%1, %6};\n\t"
+        "mov.b64 a, {%1, %5};\n\t"
         "mov.b64 b, {%2, %5};\n\t"
         "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(lat_desc_hi(1024)), "r"(a_hi)
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(kLatDescHi)
         : "memory");
 }
 __device__ __forceinline__ void lat_commit(uint64_t* bar) {
@@ -313,17 +319,16 @@ __device__ __forceinline__ void lat_commit(uint64_t* bar) {
             smem_addr(bar))
         : "memory");
 }
-__device__ __forceinline__ void lat_tma4(uint32_t dst, const void* tmap, uint32_t bar, int y,
-                                         int z) {
+// Arrival of one elected thread that adds `bytes` to what the phase waits for.
+__device__ __forceinline__ void lat_expect(uint32_t bar, uint32_t bytes) {
     asm volatile(
         "{\n\t.reg .pred q;\n\t"
         "elect.sync _|q, 0xffffffff;\n\t"
-        "@q cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %2, %4}], [%5];\n\t}" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(0), "r"(y), "r"(z), "r"(bar)
+        "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
+        "r"(bytes)
         : "memory");
 }
-__device__ __forceinline__ void lat_tma3(uint32_t dst, const void* tmap, uint32_t bar, int x, int y,
+__device__ __forceinline__ void lat_tma(uint32_t dst, const void* tmap, uint32_t bar, int x, int y,
                                          int z) {
     asm volatile(
         "{\n\t.reg .pred q;\n\t"
@@ -332,6 +337,10 @@ __device__ __forceinline__ void lat_tma3(uint32_t dst, const void* tmap, uint32_
         " [%0], [%1, {%2, %3, %4}], [%5];\n\t}" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
+}
+// The 256 bytes at `src` into L2 (a load whose value nobody waits for).
+__device__ __forceinline__ void lat_prefetch(const void* src) {
+    asm volatile("{\n\t.reg .b32 x;\n\tld.global.L1::no_allocate.L2::256B.b32 x, [%0];\n\t}" ::"l"(src));
 }
 __device__ __forceinline__ uint32_t warp_uniform(uint32_t x) {
     return __shfl_sync(0xffffffffu, x, 0);
@@ -342,6 +351,35 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool ther
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src),
                  "r"(there ? 16 : 0)
                  : "memory");
+}
+
+// A bounded wait of a whole warp on an mbarrier phase, and whether it completed.  A
+// try suspends for up to half a microsecond; `tries` of them, or *abort, end it.  (One
+// loop in one piece, which the warp leaves together: behind a loop that its threads
+// leave one by one, an MMA takes up to 370 cycles.)
+__device__ __forceinline__ bool lat_wait(uint64_t* bar, uint32_t parity, volatile int* abort,
+                                         uint32_t tries) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b32 n, a;\n\t"
+        "mov.b32 n, %4;\n\t"
+        "mov.b32 %0, 1;\n\t"
+        "TRY:\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 500;\n\t"
+        "@p bra DONE;\n\t"
+        "ld.volatile.shared.b32 a, [%3];\n\t"
+        "setp.ne.b32 p, a, 0;\n\t"
+        "@p bra FAIL;\n\t"
+        "sub.u32 n, n, 1;\n\t"
+        "setp.ne.b32 p, n, 0;\n\t"
+        "@p bra TRY;\n\t"
+        "FAIL:\n\t"
+        "mov.b32 %0, 0;\n\t"
+        "DONE:\n\t}"
+        : "=&r"(ok)
+        : "r"(smem_addr(bar)), "r"(parity), "r"(smem_addr(const_cast<int*>(abort))), "r"(tries)
+        : "memory");
+    return __all_sync(0xffffffffu, ok != 0);
 }
 
 template <typename E>
@@ -362,11 +400,10 @@ __device__ __forceinline__ void with_constant(int n, const F& f) {
 }
 
 template <int N, typename E>
-__global__ void __launch_bounds__(kLatThreads, 1)
-    latent_tc_kernel(const __grid_constant__ CUtensorMap tm,
-                     const __grid_constant__ CUtensorMap tm_tail, const LatParams p) {
+__global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
+    latent_tc_kernel(const __grid_constant__ CUtensorMap tm, const LatParams p) {
     using C = LatCfg<N>;
-    constexpr int NJ = N / 8;
+    constexpr int SW = C::SW, SMT = C::ST, NW = C::NW, NJ = NW / 8;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -374,25 +411,26 @@ __global__ void __launch_bounds__(kLatThreads, 1)
     const int sub_id = (int)blockIdx.x % p.sub, g = (int)blockIdx.x / p.sub;
     const int G = (int)gridDim.x / p.sub;
     const int NM = (p.dc + 127) / 128, NCH = (p.dim + 63) / 64;
-    const int ST = p.stages, GS = NCH * 1024, STAGE = kLatGroups * GS;
+    const int ST = p.stages, STAGE = lat_stage(p.dc, p.dim), NP = (NCH + 1) / 2;
 
     unsigned char* s_q = sm;
     unsigned char* s_p = s_q + NCH * C::Q_CHUNK;
     unsigned char* s_c = s_p + kLatP;
     unsigned char* misc = s_c + ST * STAGE;
     uint64_t* full = reinterpret_cast<uint64_t*>(misc);
-    uint64_t* empty = full + kLatMaxStages;       // [stage][4] 16 keys of a tile are free
-    uint64_t* s_full = empty + 4 * kLatMaxStages; // [2] S^T of a tile is there
-    uint64_t* p_full = s_full + 2;                // P^T written, O^T rescaled
-    uint64_t* o_done = p_full + 1;                // O^T of a tile is done
+    // [stage][piece] two chunks of a tile
+    uint64_t* empty = full + kLatMaxStages * kLatMaxPieces;
+    uint64_t* s_full = empty + kLatMaxStages * kLatMaxPieces;     // [2] S^T of a tile is there
+    uint64_t* p_full = s_full + 2;                // [2] P^T written, O^T rescaled
+    uint64_t* o_done = p_full + 2;                // O^T of a tile is done
     uint64_t* q_full = o_done + 1;                // Q of a range is there
-    uint64_t* drain = q_full + 1;                 // last commit of the MMA thread
-    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drain + 1);
+    uint64_t* drain = q_full + 1;                 // [2] last commits of the MMA warps
+    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drain + 2);
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
     volatile int* s_issued = s_abort + 1;         // [kLatProd] tiles whose loads were begun
-    int* s_start = const_cast<int*>(s_issued) + kLatProd;     // [4] unit, offset, tiles, all tiles
-    volatile int* s_n = s_start + 4;              // tiles of the range whose Q is there; 0: no more
-    int* s_warp = s_start + 5;                    // [kLatThreads / 32]
+    int* s_start = const_cast<int*>(s_issued) + kLatProd;     // [4] unit, offset, share, all shares
+    volatile int* s_n = s_start + 4;              // [2] tiles of a range (by its parity); 0: no more
+    int* s_warp = s_start + 6;                    // [C::THREADS / 32]
     uint64_t* s_vis = reinterpret_cast<uint64_t*>(misc + 512);        // [64]
     float* s_alpha = reinterpret_cast<float*>(misc + 512);            // [64], after s_vis
     float* s_red = reinterpret_cast<float*>(misc + 1024);             // [4][64]
@@ -400,29 +438,31 @@ __global__ void __launch_bounds__(kLatThreads, 1)
     asm volatile("griddepcontrol.launch_dependents;");
     if (tid == 0) p.desc[(int64_t)blockIdx.x * 8] = 0;
 
-    // ---- rows of sequences without a key: zeros ----
-    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-        const int raw = p.ctx_lens[b];
-        const int qs = p.q_start ? p.q_start[b] : b;
-        const int n = p.q_start ? p.q_start[b + 1] - qs : 1;
-        const int64_t cap = p.table_stride * p.block_size;
-        if (tid == 0) {
-            if (raw > cap) raise_flag(CX_DEV_TABLE_OVERRUN);
-            if (n < 0 || n > p.max_q || (raw > 0 && n > min((int64_t)raw, cap)))
-                raise_flag(CX_DEV_BAD_QLEN);
+    // rows of sequences without a key: zeros (threads t0, t0 + n_t, ..)
+    auto zero_rows = [&](int t0, int n_t) {
+        for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+            const int raw = p.ctx_lens[b];
+            const int qs = p.q_start ? p.q_start[b] : b;
+            const int n = p.q_start ? p.q_start[b + 1] - qs : 1;
+            const int64_t cap = p.table_stride * p.block_size;
+            if (t0 == 0) {
+                if (raw > cap) raise_flag(CX_DEV_TABLE_OVERRUN);
+                if (n < 0 || n > p.max_q || (raw > 0 && n > min((int64_t)raw, cap)))
+                    raise_flag(CX_DEV_BAD_QLEN);
+            }
+            if (raw > 0) continue;
+            const int64_t o0 = (int64_t)qs * p.heads * p.dc;
+            const int64_t cnt = (int64_t)min(max(n, 0), p.max_q) * p.heads * p.dc;
+            for (int64_t i = t0; i < cnt; i += n_t) store_as(p.out, p.out_dtype, o0 + i, 0.f);
         }
-        if (raw > 0) continue;
-        const int64_t o0 = (int64_t)qs * p.heads * p.dc;
-        const int64_t cnt = (int64_t)min(max(n, 0), p.max_q) * p.heads * p.dc;
-        for (int64_t i = tid; i < cnt; i += kLatThreads) store_as(p.out, p.out_dtype, o0 + i, 0.f);
-    }
+    };
 
     // ---- this CTA's share of the tiles ----
     {
-        const int per = (p.n_units + kLatThreads - 1) / kLatThreads;
+        const int per = (p.n_units + C::THREADS - 1) / C::THREADS;
         const int u0 = min(p.n_units, tid * per), u1 = min(p.n_units, u0 + per);
         int sum = 0;
-        for (int u = u0; u < u1; ++u) sum += lat_unit(p, u, 0, N).n_tiles;
+        for (int u = u0; u < u1; ++u) sum += lat_unit(p, u, 0, N).cost();
         int incl = sum;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -433,18 +473,22 @@ __global__ void __launch_bounds__(kLatThreads, 1)
         __syncthreads();
         int before = incl - sum, W = 0;
 #pragma unroll
-        for (int w = 0; w < kLatThreads / 32; ++w) {
+        for (int w = 0; w < C::THREADS / 32; ++w) {
             if (w < warp) before += s_warp[w];
             W += s_warp[w];
         }
+        W = (int)warp_uniform(W);     // (the branch below is then one for the whole warp)
         const int P = min(G, max(1, (W + kLatMinTiles - 1) / kLatMinTiles));
         const int w0 = g < P ? (int)((int64_t)g * W / P) : W;
         const int w1 = g < P ? (int)((int64_t)(g + 1) * W / P) : W;
-        if (w1 <= w0) return;
+        if (w1 <= w0) {
+            zero_rows(tid, C::THREADS);
+            return;
+        }
         if (before <= w0 && w0 < before + sum) {
             int u = u0, at = before;
             for (; u < u1; ++u) {
-                const int n = lat_unit(p, u, 0, N).n_tiles;
+                const int n = lat_unit(p, u, 0, N).cost();
                 if (w0 < at + n) break;
                 at += n;
             }
@@ -455,21 +499,23 @@ __global__ void __launch_bounds__(kLatThreads, 1)
         }
     }
     if (tid == 0) {
-        for (int s = 0; s < ST; ++s) {
+        for (int s = 0; s < ST * kLatMaxPieces; ++s) {
             mbar_init(&full[s], kLatProd);
-            for (int k = 0; k < 4; ++k) mbar_init(&empty[4 * s + k], 1);
+            mbar_init(&empty[s], 1);
         }
         mbar_init(&s_full[0], 1);
         mbar_init(&s_full[1], 1);
-        mbar_init(p_full, 128);
+        mbar_init(&p_full[0], SW);
+        mbar_init(&p_full[1], SW);
         mbar_init(o_done, 1);
-        mbar_init(q_full, 128);
-        mbar_init(drain, 1);
+        mbar_init(q_full, SW);
+        mbar_init(&drain[0], 1);
+        mbar_init(&drain[1], 1);
         *s_abort = 0;
         for (int k = 0; k < kLatProd; ++k) s_issued[k] = 0;
         fence_mbar_init();
     }
-    if (warp == 4) {
+    if (warp == SW) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                          smem_addr(s_tmem)),
                      "r"(C::TMEM_COLS)
@@ -485,11 +531,13 @@ __global__ void __launch_bounds__(kLatThreads, 1)
     int tile = 0;               // tiles of this CTA before the range
     const int bs = p.block_size;                  // (a multiple of 8)
 
-    if (warp < 4) {
+    if (warp < SW) {
         // ---------------- Q in, softmax, output ----------------
-        const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+        const int quad = warp & 3, wg = warp >> 2;    // keys [16 quad, ..), rows [NW wg, ..)
+        const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
         const int tq = lane >> 2, c = lane & 3;
-        const int tok0 = warp * 16 + tq, tok1 = tok0 + 8;
+        const int tok0 = quad * 16 + tq, tok1 = tok0 + 8;
+        const int col0 = wg * NW + 2 * c;             // this thread's first row
         constexpr float kGrow = Half16<E>::kGrowLog2, kLead = Half16<E>::kLeadLog2;
         bool ok = true;
         int slot = 0;
@@ -498,26 +546,34 @@ __global__ void __launch_bounds__(kLatThreads, 1)
         const bool q_async = p.q_vec && p.q_dtype != CX_F32;
         auto load_q = [&](const LatUnit& x) {
             if (q_async) {
-                // a warp per row
-                for (int r = warp; r < N; r += 4) {
-                    const bool row_ok = r < x.n_rows;
-                    const int R = x.r0 + r, t = R / p.heads, h = R - t * p.heads;
-                    const E* lat = static_cast<const E*>(p.q_lat) + (x.qs + t) * p.ql_tok +
-                                   h * p.ql_head;
-                    const E* rope = static_cast<const E*>(p.q_rope) + (x.qs + t) * p.qr_tok +
-                                    h * p.qr_head - p.dc;
+                // a warp per row; lane k first finds the warp's k-th row
+                const E *lat = static_cast<const E*>(p.q_lat), *rope = lat;
+                const int r_k = warp + SW * lane;
+                if (r_k < x.n_rows) {
+                    const int R = x.r0 + r_k, t = R / p.heads, h = R - t * p.heads;
+                    lat += (x.qs + t) * p.ql_tok + h * p.ql_head;
+                    rope = static_cast<const E*>(p.q_rope) + (x.qs + t) * p.qr_tok +
+                           h * p.qr_head - p.dc;
+                }
+#pragma unroll 2
+                for (int k = 0; k < N / SW; ++k) {
+                    const int r = warp + SW * k;
+                    const E* l_k = reinterpret_cast<const E*>(
+                        __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(lat), k));
+                    const E* r_k = reinterpret_cast<const E*>(
+                        __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(rope), k));
                     unsigned char* dst = s_q + r * 128;
                     for (int ch = lane; ch < NCH * 8; ch += 32) {
                         const int d = ch * 8;
-                        const bool there = row_ok && d < p.dim;
-                        const E* src = (d < p.dc ? lat : rope) + d;
+                        const bool there = r < x.n_rows && d < p.dim;
+                        const E* src = (d < p.dc ? l_k : r_k) + d;
                         cp_async16(dst + (ch >> 3) * C::Q_CHUNK + (((ch & 7) ^ (r & 7)) << 4),
                                    there ? src : static_cast<const E*>(p.q_lat), there);
                     }
                 }
                 return;
             }
-            for (int i = tid; i < N * NCH * 8; i += 128) {
+            for (int i = tid; i < N * NCH * 8; i += SMT) {
                 const int r = i / (NCH * 8), ch = i - r * (NCH * 8);
                 uint4 v = make_uint4(0, 0, 0, 0);
                 if (r < x.n_rows) {
@@ -529,11 +585,14 @@ __global__ void __launch_bounds__(kLatThreads, 1)
                                           (((ch & 7) ^ (r & 7)) << 4)) = v;
             }
         };
+        int ranges = 0;
         auto q_ready = [&](int n) {                  // n tiles; 0: no further range
-            if (tid == 0) *s_n = n;
+            if (tid == 0) s_n[ranges & 1] = n;
+            ++ranges;
             if (q_async) asm volatile("cp.async.wait_all;" ::: "memory");
             fence_async_smem();
-            mbar_arrive(q_full);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
         };
         bool more = cur.next(p, sub_id, N, seg);
         if (more) load_q(seg.x);
@@ -546,11 +605,11 @@ __global__ void __launch_bounds__(kLatThreads, 1)
             const int nblk = (x.ctx + bs - 1) / bs;
             const int first_k = (x.tile0 + from) * kLatKeys;
             bool bad = false;
-            for (int k = first_k / bs + tid; k < nblk && k * bs < first_k + n * kLatKeys; k += 128) {
+            for (int k = first_k / bs + tid; k < nblk && k * bs < first_k + n * kLatKeys; k += SMT) {
                 const int id = tab[k];
                 bad |= id < 0 || id >= p.n_blocks;
             }
-            const bool any_bad = bar_red_or(1, 128, bad);
+            const bool any_bad = bar_red_or(1, SMT, bad);
             // keys up to `all_hi` and from `all_lo` on are seen by every row
             const int t_first = x.r0 / p.heads, t_last = (x.r0 + x.n_rows - 1) / p.heads;
             const int all_hi = p.tree.masks ? x.base - 1 : x.base + t_first;
@@ -562,39 +621,53 @@ __global__ void __launch_bounds__(kLatThreads, 1)
                 m[j][0] = m[j][1] = -INFINITY;
                 l[j][0] = l[j][1] = 0.f;
             }
+            // Rows of the tiles behind those in shared memory are asked into L2, two or four
+            // threads a row: what follows an O^T is then a load from L2.
+            constexpr int kPer = SMT / kLatKeys;
+            const int pf_row = tid / kPer, row_bytes = p.dim * 2;
+            auto pf_block = [&](int i) {
+                const int key = first_k + i * kLatKeys + pf_row;
+                return i < n && key < x.ctx ? tab[key / bs] : -1;
+            };
+            int pf_id = pf_block(kLatAhead);
             for (int i = 0; i < n; ++i, ++tile) {
                 const int k0 = first_k + i * kLatKeys;
-                ok = mbar_wait_bounded(&s_full[tile & 1], (tile >> 1) & 1, s_abort, p.wait_ns);
-                if (!(ok = bar_red_and(1, 128, ok))) break;
-                tc_fence_after();
-                if (i == n - 1) {
-                    // every MMA that reads this range's queries is done: the next range's
-                    more = cur.next(p, sub_id, N, seg);
-                    if (more) load_q(seg.x);
+                {
+                    const int id = pf_id, key = k0 + kLatAhead * kLatKeys + pf_row;
+                    pf_id = pf_block(i + 1 + kLatAhead);
+                    if (id >= 0 && id < p.n_blocks) {
+                        const char* row = static_cast<const char*>(p.pool) +
+                                          (((int64_t)p.layer * p.n_blocks + id) * bs + key % bs) *
+                                              row_bytes;
+                        for (int o = tid % kPer * 256; o < row_bytes; o += kPer * 256)
+                            lat_prefetch(row + o);
+                    }
                 }
-                float v[N / 2];
-                lat_ld_s<N>(tmem + C::S_COL + (tile & 1) * N + lane_base, v);
+                ok = lat_wait(&s_full[tile & 1], (tile >> 1) & 1, s_abort, p.tries);
+                tc_fence_after();
+                float v[NW / 2];
+                lat_ld_s<NW>(tmem + C::S_COL + (tile & 1) * N + wg * NW + lane_base, v);
                 tc_wait_ld();
 #pragma unroll
-                for (int e = 0; e < N / 2; ++e) v[e] *= p.scale_log2;
+                for (int e = 0; e < NW / 2; ++e) v[e] *= p.scale_log2;
                 const bool edge = any_bad || k0 + kLatKeys - 1 > all_hi || k0 < all_lo;
                 uint64_t dead = 0;
                 if (edge) {
                     uint64_t vis = 0;
                     if (tid < x.n_rows) {
                         vis = lat_visible(p, x, x.r0 + tid, k0);
-                        for (int k = 0; any_bad && k < kLatGroups; ++k) {
+                        for (int k = 0; any_bad && k < kLatKeys / 8; ++k) {
                             const int blk = (k0 + 8 * k) / bs, id = blk < nblk ? tab[blk] : 0;
                             if (id < 0 || id >= p.n_blocks) vis &= ~(0xffull << 8 * k);
                         }
                     }
                     if (tid < 64) s_vis[tid] = vis;
-                    named_bar_sync(1, 128);
+                    named_bar_sync(1, SMT);
 #pragma unroll
                     for (int j = 0; j < NJ; ++j) {
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            const uint64_t w = s_vis[8 * j + 2 * c + e];
+                            const uint64_t w = s_vis[col0 + 8 * j + e];
                             if (!((w >> tok0) & 1)) v[4 * j + e] = -INFINITY;
                             if (!((w >> tok1) & 1)) v[4 * j + 2 + e] = -INFINITY;
                         }
@@ -612,7 +685,8 @@ __global__ void __launch_bounds__(kLatThreads, 1)
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
                         grow |= fmaxf(v[4 * j + e], v[4 * j + 2 + e]) > m[j][e] + kGrow;
-                if (bar_red_or(1, 128, grow)) {
+                if (bar_red_or(1, SMT, grow || !ok)) {
+                    if (!(ok = bar_red_and(1, SMT, ok))) break;
 #pragma unroll
                     for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -621,15 +695,15 @@ __global__ void __launch_bounds__(kLatThreads, 1)
                             y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
                             y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
                             y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
-                            if (lane < 4) s_red[warp * 64 + 8 * j + 2 * c + e] = y;
+                            if (lane < 4) s_red[quad * 64 + col0 + 8 * j + e] = y;
                         }
-                    named_bar_sync(1, 128);
+                    named_bar_sync(1, SMT);
                     bool moved = false;
 #pragma unroll
                     for (int j = 0; j < NJ; ++j)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            const float* q = s_red + 8 * j + 2 * c + e;
+                            const float* q = s_red + col0 + 8 * j + e;
                             const float y = fmaxf(fmaxf(q[0], q[64]), fmaxf(q[128], q[192]));
                             float alpha = 1.f;
                             if (y > m[j][e] + kGrow) {      // (m -inf: any score that is not)
@@ -639,17 +713,17 @@ __global__ void __launch_bounds__(kLatThreads, 1)
                                 moved = true;
                             }
                             l[j][e] *= alpha;
-                            if (warp == 0 && lane < 4) s_alpha[8 * j + 2 * c + e] = alpha;
+                            if (quad == 0 && lane < 4) s_alpha[col0 + 8 * j + e] = alpha;
                         }
                     // (every thread of a column c has the same alphas)
-                    moved = bar_red_or(1, 128, moved);
+                    moved = bar_red_or(1, SMT, moved);
                     if (moved && i > 0) {
                         // O^T holds the tiles before this one
-                        ok = mbar_wait_bounded(o_done, (tile - 1) & 1, s_abort, p.wait_ns);
-                        if (!(ok = bar_red_and(1, 128, ok))) break;
+                        ok = lat_wait(o_done, (tile - 1) & 1, s_abort, p.tries);
+                        if (!(ok = bar_red_and(1, SMT, ok))) break;
                         tc_fence_after();
 #pragma unroll 1
-                        for (int k = 0; k < NM * (N / 16); ++k) {
+                        for (int k = wg; k < NM * (N / 16); k += SW / 4) {
                             const int col = (k / (N / 16)) * N + (k % (N / 16)) * 16;
                             const uint32_t at = tmem + col + lane_base;
                             float o[16];
@@ -661,29 +735,21 @@ __global__ void __launch_bounds__(kLatThreads, 1)
                         }
                         tc_wait_st();
                     }
-                    named_bar_sync(1, 128);     // s_alpha and s_red are read
+                    named_bar_sync(1, SMT);     // s_alpha and s_red are read
                 }
-                uint32_t pk[N / 4];
+                uint32_t pk[NW / 4];
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
                     const float b0 = m[j][0] == -INFINITY ? 0.f : m[j][0];
                     const float b1 = m[j][1] == -INFINITY ? 0.f : m[j][1];
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const uint32_t u = Half16<E>::pack(ex2_sfu(v[4 * j + 2 * t] - b0),
-                                                           ex2_sfu(v[4 * j + 2 * t + 1] - b1));
-                        // (the sum of what the second product gets: numerator and denominator
-                        // round alike)
-                        float e0, e1;
-                        f2_get(Half16<E>::unpack(u), e0, e1);
-                        l[j][0] += e0;
-                        l[j][1] += e1;
-                        pk[2 * j + t] = u;
-                    }
+                    for (int t = 0; t < 2; ++t)
+                        pk[2 * j + t] = Half16<E>::pack(ex2_sfu(v[4 * j + 2 * t] - b0),
+                                                        ex2_sfu(v[4 * j + 2 * t + 1] - b1));
                 }
                 // ---- P^T over the last tile's, when O^T has read that ----
                 if (tile > 0)
-                    ok = mbar_wait_bounded(o_done, (tile - 1) & 1, s_abort, p.wait_ns);
+                    ok = lat_wait(o_done, (tile - 1) & 1, s_abort, p.tries);
                 if (!ok) {
                     *s_abort = 1;               // the next vote ends the loop for all
                     continue;
@@ -691,10 +757,9 @@ __global__ void __launch_bounds__(kLatThreads, 1)
                 if (dead != 0) {
                     const int tok = tid & 63;
                     if ((dead >> tok) & 1) {
-                        unsigned char* line = s_c + (tile % ST) * STAGE + (tok >> 3) * GS +
-                                              (tok & 7) * 128;
-                        for (int ch = tid >> 6; ch < min(2 * NM, NCH); ch += 2) {
-                            uint4* z = reinterpret_cast<uint4*>(line + ch * 1024);
+                        unsigned char* line = s_c + (tile % ST) * STAGE + tok * 128;
+                        for (int ch = tid >> 6; ch < min(2 * NM, NCH); ch += SMT / 64) {
+                            uint4* z = reinterpret_cast<uint4*>(line + ch * kLatChunk);
 #pragma unroll
                             for (int k = 0; k < 8; ++k) z[k] = make_uint4(0, 0, 0, 0);
                         }
@@ -702,17 +767,34 @@ __global__ void __launch_bounds__(kLatThreads, 1)
                 }
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
-                    *reinterpret_cast<uint32_t*>(s_p + tok0 * 128 + ((j ^ (tok0 & 7)) << 4) +
+                    const int ch = wg * NJ + j;
+                    *reinterpret_cast<uint32_t*>(s_p + tok0 * 128 + ((ch ^ (tok0 & 7)) << 4) +
                                                  c * 4) = pk[2 * j];
-                    *reinterpret_cast<uint32_t*>(s_p + tok1 * 128 + ((j ^ (tok1 & 7)) << 4) +
+                    *reinterpret_cast<uint32_t*>(s_p + tok1 * 128 + ((ch ^ (tok1 & 7)) << 4) +
                                                  c * 4) = pk[2 * j + 1];
                 }
                 fence_async_smem();
                 tc_fence_before();
-                mbar_arrive(p_full);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[tile & 1]);
+                // (the sums of what the second product gets: numerator and denominator round
+                // alike)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    float e0, e1, f0, f1;
+                    f2_get(Half16<E>::unpack(pk[2 * j]), e0, e1);
+                    f2_get(Half16<E>::unpack(pk[2 * j + 1]), f0, f1);
+                    l[j][0] += e0 + f0;
+                    l[j][1] += e1 + f1;
+                }
+                if (i == n - 1) {
+                    // every MMA that reads this range's queries is done: the next range's
+                    more = cur.next(p, sub_id, N, seg);
+                    if (more) load_q(seg.x);
+                }
             }
             // (a wait before the last P^T may have given up in some threads only)
-            if (!(ok = bar_red_and(1, 128, ok))) break;
+            if (!(ok = bar_red_and(1, SMT, ok))) break;
             q_ready(more ? seg.to - seg.from : 0);      // S^T of the next range runs beside what follows
             // ---- denominators, then O^T to the output or to this CTA's part ----
 #pragma unroll
@@ -723,10 +805,10 @@ __global__ void __launch_bounds__(kLatThreads, 1)
                     y += __shfl_xor_sync(0xffffffffu, y, 4);
                     y += __shfl_xor_sync(0xffffffffu, y, 8);
                     y += __shfl_xor_sync(0xffffffffu, y, 16);
-                    if (lane < 4) s_red[warp * 64 + 8 * j + 2 * c + e] = y;
+                    if (lane < 4) s_red[quad * 64 + col0 + 8 * j + e] = y;
                 }
-            ok = mbar_wait_bounded(o_done, (tile - 1) & 1, s_abort, p.wait_ns);
-            if (!(ok = bar_red_and(1, 128, ok))) break;
+            ok = lat_wait(o_done, (tile - 1) & 1, s_abort, p.tries);
+            if (!(ok = bar_red_and(1, SMT, ok))) break;
             tc_fence_after();
             const int64_t part = ((int64_t)blockIdx.x * 2 + slot) * N;
             if (tid < N) {
@@ -734,19 +816,19 @@ __global__ void __launch_bounds__(kLatThreads, 1)
                 s_alpha[tid] = whole ? (L > 0.f ? 1.f / L : 0.f) : 1.f;
                 if (!whole) p.part_ml[(part + tid) * 2 + 1] = L;
             }
-            if (!whole && warp == 0 && lane < 4) {
+            if (!whole && quad == 0 && lane < 4) {
 #pragma unroll
                 for (int j = 0; j < NJ; ++j)
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
-                        p.part_ml[(part + 8 * j + 2 * c + e) * 2] = m[j][e];
+                        p.part_ml[(part + col0 + 8 * j + e) * 2] = m[j][e];
             }
-            named_bar_sync(1, 128);
+            named_bar_sync(1, SMT);
             const int64_t row0 = (int64_t)x.qs * p.heads + x.r0;
 #pragma unroll 1
-            for (int k = 0; k < NM * (N / 16); ++k) {
+            for (int k = wg; k < NM * (N / 16); k += SW / 4) {
                 const int mm = k / (N / 16), n0 = (k % (N / 16)) * 16;
-                const int d = mm * 128 + warp * 32 + lane, rows = x.n_rows - n0;
+                const int d = mm * 128 + quad * 32 + lane, rows = x.n_rows - n0;
                 if (rows <= 0) continue;                     // (the same for the warp)
                 float o[16];
                 sc_ld16(tmem + mm * N + n0 + lane_base, o);
@@ -805,62 +887,74 @@ __global__ void __launch_bounds__(kLatThreads, 1)
                 d[0] = last - g + 1;
             }
             slot = 1;
-            named_bar_sync(1, 128);             // s_alpha and s_red are read
+            named_bar_sync(1, SMT);             // s_alpha and s_red are read
         }
         if (!ok) {
             *s_abort = 1;
             if (tid == 0) raise_flag(CX_DEV_WAIT_TIMEOUT);
         }
-    } else if (warp > 4) {
-        // ---------------- producer ----------------
-        const int NF = p.dim / 64;                    // whole chunks; a partial one is apart
-        const bool tail = NF < NCH;
+        zero_rows(tid, SMT);
+    } else if (warp >= SW + 2) {
+        // ---------------- producers: one for either chunk of a piece ----------------
+        const int br = p.box_rows, nb = kLatKeys / br, w0 = warp - SW - 2;
         bool go = true;
-        while (go && cur.next(p, sub_id, N, seg)) {
+        while (go && warp_uniform(cur.next(p, sub_id, N, seg))) {
             const LatUnit& x = seg.x;
             const int32_t* tab = p.tables + (int64_t)x.b * p.table_stride;
-            const int n = seg.to - seg.from;
+            const int n = (int)warp_uniform(seg.to - seg.from);
             const int key0 = (x.tile0 + seg.from) * kLatKeys;
-            // lane l < 8: block and row of group l of tile i
-            auto place = [&](int i, int& z, int& row) {
-                const int key = key0 + i * kLatKeys + 8 * lane, blk = key / bs;
+            // lane l < nb: block (INT32_MIN: none) and row of box l of tile i
+            auto place = [&](int i, int& id, int& row) {
+                const int key = key0 + i * kLatKeys + br * lane, blk = key / bs;
                 row = key - blk * bs;
-                int id = -1;
-                if (lane < kLatGroups && i < n && key < x.ctx) {
-                    id = tab[blk];
-                    if (id < 0 || id >= p.n_blocks) {
-                        raise_flag(CX_DEV_BAD_BLOCK);
-                        id = -1;
-                    }
-                }
-                // outside the map: the copy fills zeros
-                z = id >= 0 ? p.layer * p.n_blocks + id : -1;
+                id = lane < nb && i < n && key < x.ctx ? tab[blk] : INT32_MIN;
             };
-            int z, row;
-            place(0, z, row);
+            int id, row, id_next, row_next;
+            place(0, id, row);
+            place(1, id_next, row_next);
             for (int i = 0; go && i < n; ++i, ++tile) {
-                int z_next, row_next;
-                place(i + 1, z_next, row_next);
+                int z = -1;           // outside the map: the copy fills zeros
+                if (id >= 0 && id < p.n_blocks)
+                    z = p.layer * p.n_blocks + id;
+                else if (id != INT32_MIN)
+                    raise_flag(CX_DEV_BAD_BLOCK);
                 const int s = tile % ST, use = tile / ST;
-                const uint32_t bar = warp_uniform(smem_addr(full + s));
-                const uint32_t dst = warp_uniform(smem_addr(s_c + s * STAGE));
-                for (int k = warp - 5; k < kLatGroups; k += kLatProd) {
-                    go = use == 0 || mbar_wait_bounded(&empty[4 * s + (k >> 1)], (use - 1) & 1,
-                                                       s_abort, p.wait_ns);
-                    go = __all_sync(0xffffffffu, go && !*s_abort);
-                    if (!go) break;
-                    if (k == warp - 5 && lane == 0) {
-                        mbar_arrive_expect_tx(full + s, STAGE / kLatProd);
-                        s_issued[k] = tile + 1;
-                    }
-                    __syncwarp();
-                    const int zk = __shfl_sync(0xffffffffu, z, k);
-                    const int rk = __shfl_sync(0xffffffffu, row, k);
-                    lat_tma4(dst + k * GS, &tm, bar, rk, zk);
-                    if (tail) lat_tma3(dst + k * GS + NF * 1024, &tm_tail, bar, NF * 64, rk, zk);
+                const uint32_t dst0 = warp_uniform(smem_addr(s_c + s * STAGE));
+                const uint32_t bar0 = warp_uniform(smem_addr(full + s * kLatMaxPieces));
+                if (lane == 0) s_issued[w0] = tile + 1;
+                // (what the boxes of every piece share; for other block sizes see below)
+                int z4[4], row4[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    z4[k] = __shfl_sync(0xffffffffu, z, k);
+                    row4[k] = __shfl_sync(0xffffffffu, row, k);
                 }
-                z = z_next;
+                for (int j = 0; j < NP; ++j) {
+                    // the pieces that O^T does not read are free first
+                    const int q = j + NM < NP ? j + NM : j + NM - NP, ch = 2 * q + w0;
+                    if (use > 0) {
+                        go = lat_wait(&empty[s * kLatMaxPieces + q], (use - 1) & 1, s_abort,
+                                      p.tries);
+                        if (!go) break;
+                    }
+                    const uint32_t bar = bar0 + q * 8, dst = dst0 + ch * kLatChunk;
+                    lat_expect(bar, ch < NCH ? kLatChunk : 0);
+                    if (ch >= NCH) continue;
+                    // (a condition at every box would triple what they take)
+                    if (nb == 4) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            lat_tma(dst + k * 2048, &tm, bar, ch * 64, row4[k], z4[k]);
+                    } else {
+                        for (int k = 0; k < nb; ++k)
+                            lat_tma(dst + k * br * 128, &tm, bar, ch * 64,
+                                    __shfl_sync(0xffffffffu, row, k),
+                                    __shfl_sync(0xffffffffu, z, k));
+                    }
+                }
+                id = id_next;
                 row = row_next;
+                place(i + 2, id_next, row_next);
             }
         }
         if (!go && lane == 0) {
@@ -868,87 +962,82 @@ __global__ void __launch_bounds__(kLatThreads, 1)
             raise_flag(CX_DEV_WAIT_TIMEOUT);
         }
     } else {
-        // ---------------- MMA issuer: the whole warp, one thread's instructions ----------------
-        constexpr uint32_t idesc_s = lat_idesc<E>(kLatKeys, N, 0, 0);
-        constexpr uint32_t idesc_o = lat_idesc<E>(128, N, 1, 1);
+        // ---------------- MMA issuers: whole warps, one thread's instructions ----------------
+        const bool is_s = warp == SW;
         const uint32_t tm = warp_uniform(tmem);
-        const uint32_t q_lo = warp_uniform(lat_desc_lo(s_q, 16));
-        const uint32_t c_lo = warp_uniform(lat_desc_lo(s_c, 1024));
-        const uint32_t c_hi = warp_uniform(lat_desc_hi(GS));
-        const uint32_t p_lo = warp_uniform(lat_desc_lo(s_p, 16));
+        const uint32_t c_lo = warp_uniform(lat_desc_lo(s_c, kLatChunk));
+        const uint32_t b_lo = warp_uniform(lat_desc_lo(is_s ? s_q : s_p, 16));
         bool ok = true;
-        int ranges = 0;
-        int o_st = 0, s_st = 0;                   // stages of the next tiles of O^T and S^T
-        uint32_t s_use = 0;                       // parity of s_st's fill
-        for (;;) {
-            ok = warp_uniform(mbar_wait_bounded(q_full, ranges & 1, s_abort, p.wait_ns)) != 0;
-            ++ranges;
-            const int n = (int)warp_uniform(*s_n);
+        int st = 0;                               // stage of the next tile
+        uint32_t use = 0;                         // parity of its fill
+        for (int range = 0;; ++range) {
+            ok = lat_wait(q_full, range & 1, s_abort, p.tries);
+            const int n = (int)warp_uniform(s_n[range & 1]);
             if (!ok || n == 0) break;
-            tc_fence_after();
-            int si = 0, oi = 0;
-            uint32_t idle = 0;
-            uint64_t since = 0;
-            while (oi < n) {
-                bool did = false;
-                if (oi < si && warp_uniform(mbar_test(p_full, (tile + oi) & 1))) {
+            for (int i = 0; ok && i < n; ++i, ++tile) {
+                const uint32_t cd = warp_uniform(c_lo + (uint32_t)(st * STAGE >> 4));
+                if (is_s) {
+                    constexpr uint32_t idesc = lat_idesc<E>(kLatKeys, N, 0, 0);
+                    const int b = tile & 1;
+                    const uint32_t d = warp_uniform(tm + C::S_COL + b * N);
+                    // S^T of two tiles before was read
+                    if (tile >= 2)
+                        ok = lat_wait(&p_full[b], ((tile >> 1) - 1) & 1, s_abort, p.tries);
+                    for (int j = 0; ok && j < NP; ++j) {
+                        const int q = j + NM < NP ? j + NM : j + NM - NP;
+                        ok = lat_wait(&full[st * kLatMaxPieces + q], use, s_abort,
+                                                   p.tries);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t ad = warp_uniform(cd + (uint32_t)(q * 2 * kLatChunk >> 4));
+                        const uint32_t qd = warp_uniform(b_lo + (uint32_t)(q * 2 * C::Q_CHUNK >> 4));
+                        const uint32_t acc = warp_uniform(j > 0);
+                        // (a condition at every MMA triples what they take)
+                        auto steps = [&](auto k_end) {
+#pragma unroll
+                            for (int k = 0; k < decltype(k_end)::value; ++k)
+                                lat_mma(d, ad + (((k >> 2) * kLatChunk + (k & 3) * 32) >> 4),
+                                        qd + (((k >> 2) * C::Q_CHUNK + (k & 3) * 32) >> 4), idesc,
+                                        k > 0 ? 1u : acc);
+                        };
+                        if (2 * q + 1 < NCH)
+                            steps(std::integral_constant<int, 8>{});
+                        else
+                            steps(std::integral_constant<int, 4>{});
+                        if (q >= NM) lat_commit(&empty[st * kLatMaxPieces + q]);
+                    }
+                    if (ok) lat_commit(&s_full[b]);
+                } else {
+                    constexpr uint32_t idesc = lat_idesc<E>(128, N, 1, 1);
+                    ok = lat_wait(&p_full[tile & 1], (tile >> 1) & 1, s_abort,
+                                               p.tries);
+                    if (!ok) break;
                     tc_fence_after();
-                    const uint32_t acc = warp_uniform(oi > 0);
-                    uint32_t cd = warp_uniform(c_lo + (uint32_t)(o_st * (STAGE >> 4)));
-                    // (a condition at every MMA doubles what it takes, and triples S^T's)
+                    const uint32_t acc = warp_uniform(i > 0);
                     with_constant<kLatMaxLatent / 128>(NM, [&](auto nm) {
 #pragma unroll
-                        for (int kk = 0; kk < kLatKeys / 16; ++kk) {
+                        for (int mm = 0; mm < decltype(nm)::value; ++mm) {
 #pragma unroll
-                            for (int mm = 0; mm < decltype(nm)::value; ++mm)
-                                lat_mma(tm + mm * N, cd + mm * (2048 >> 4), c_hi,
-                                        p_lo + kk * (2048 >> 4), idesc_o, kk > 0 ? 1u : acc);
-                            lat_commit(&empty[4 * o_st + kk]);
-                            cd += 2 * GS >> 4;
+                            for (int kk = 0; kk < kLatKeys / 16; ++kk)
+                                lat_mma(tm + mm * N, cd + ((mm * 2 * kLatChunk + kk * 2048) >> 4),
+                                        b_lo + kk * (2048 >> 4), idesc, kk > 0 ? 1u : acc);
+                            lat_commit(&empty[st * kLatMaxPieces + mm]);
                         }
                     });
                     lat_commit(o_done);
-                    if (++o_st == ST) o_st = 0;
-                    ++oi;
-                    did = true;
-                } else if (si < n && si < oi + 2 &&
-                           warp_uniform(mbar_test(full + s_st, s_use))) {
-                    tc_fence_after();
-                    const int b = (tile + si) & 1;
-                    const uint32_t d = warp_uniform(tm + C::S_COL + b * N);
-                    const uint32_t cd = warp_uniform(c_lo + (uint32_t)(s_st * (STAGE >> 4)));
-                    with_constant<(kLatMaxDim + 63) / 64>(NCH, [&](auto nch) {
-#pragma unroll
-                        for (int k = 0; k < 4 * decltype(nch)::value; ++k)
-                            lat_mma(d, cd + (((k >> 2) * 1024 + (k & 3) * 32) >> 4), c_hi,
-                                    q_lo + (((k >> 2) * C::Q_CHUNK + (k & 3) * 32) >> 4), idesc_s,
-                                    k > 0 ? 1u : 0u);
-                    });
-                    lat_commit(&s_full[b]);
-                    if (++s_st == ST) {
-                        s_st = 0;
-                        s_use ^= 1;
-                    }
-                    ++si;
-                    did = true;
                 }
-                if (did) {
-                    idle = 0;
-                } else if ((idle++ & 15) == 0) {
-                    const uint64_t now = global_ns();
-                    if (idle == 1) since = now;
-                    ok = warp_uniform(!(*s_abort || now - since > p.wait_ns)) != 0;
-                    if (!ok) break;
+                if (++st == ST) {
+                    st = 0;
+                    use ^= 1;
                 }
             }
             if (!ok) break;
-            tile += n;
         }
         if (!ok && lane == 0) {
             *s_abort = 1;
             raise_flag(CX_DEV_WAIT_TIMEOUT);
         }
-        lat_commit(drain);       // completes once every MMA issued above has
+        lat_commit(&drain[is_s ? 0 : 1]);         // completes once this warp's MMAs have
     }
 
     // ---- teardown: drain this CTA's own copies and MMAs, then free TMEM ----
@@ -961,73 +1050,101 @@ __global__ void __launch_bounds__(kLatThreads, 1)
         for (int k = 0; k < kLatProd; ++k) issued = max(issued, s_issued[k]);
         for (int s = 0; s < ST; ++s) {
             const int uses = issued > s ? (issued - 1 - s) / ST + 1 : 0;
-            if (uses > 0) mbar_wait_bounded(&full[s], (uses - 1) & 1, nullptr, 20000000ull);
+            for (int q = 0; uses > 0 && q < NP; ++q)
+                mbar_wait_bounded(&full[s * kLatMaxPieces + q], (uses - 1) & 1, nullptr,
+                                  20000000ull);
         }
     }
-    if (tid == 4 * 32) mbar_wait_bounded(drain, 0, nullptr, kWaitLimitNs);
+    if (tid == SW * 32 || tid == SW * 32 + 32)
+        mbar_wait_bounded(&drain[tid == SW * 32 ? 0 : 1], 0, nullptr, kWaitLimitNs);
     __syncthreads();
     tc_fence_after();
-    if (warp == 4)
+    if (warp == SW)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                      "r"(C::TMEM_COLS)
                      : "memory");
 }
 
-// Joins the parts of cut ranges: block (x, y) has rows [4 y, 4 y + 4) of the range
-// that CTA x's last partial opens, 64 threads a row.
+// Joins the parts of cut ranges: block (x, y) has rows 2 y and 2 y + 1 of the range that
+// CTA x's last partial opens, 128 threads a row.  Lanes fetch the parts' references
+// side by side, then every thread adds up four columns of all parts.
 template <int N>
 __global__ void __launch_bounds__(256) latent_join_kernel(const LatParams p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int32_t* d = p.desc + (int64_t)blockIdx.x * 8;
-    const int parts = d[0], slot = d[1], n_rows = d[2];
-    const int r = blockIdx.y * 4 + (threadIdx.x >> 6), i0 = threadIdx.x & 63;
+    const int4 d = *reinterpret_cast<const int4*>(p.desc + (int64_t)blockIdx.x * 8);
+    const int parts = d.x, slot = d.y, n_rows = d.z;
+    const int r = blockIdx.y * 2 + (threadIdx.x >> 7), lane = threadIdx.x & 31;
     if (parts < 2 || r >= n_rows) return;
-    const int64_t row = ((int64_t)(uint32_t)d[3] | (int64_t)d[4] << 32) + r;
+    const int64_t row = ((int64_t)(uint32_t)d.w |
+                         (int64_t)p.desc[(int64_t)blockIdx.x * 8 + 4] << 32) + r;
     auto at = [&](int k) {
         return (((int64_t)blockIdx.x + (int64_t)k * p.sub) * 2 + (k == 0 ? slot : 0)) * N + r;
     };
-    float M = -INFINITY, L = 0.f;
-    for (int k = 0; k < parts; ++k) M = fmaxf(M, p.part_ml[at(k) * 2]);
-    float o[kLatMaxLatent / 64];
+    const int col = (threadIdx.x & 127) * 4;
+    float M = -INFINITY, L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int k0 = 0; k0 < parts; k0 += 32) {
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (k0 + lane < parts) ml = *reinterpret_cast<const float2*>(p.part_ml + at(k0 + lane) * 2);
+        float top = fmaxf(ml.x, M);
 #pragma unroll
-    for (int e = 0; e < kLatMaxLatent / 64; ++e) o[e] = 0.f;
-    for (int k = 0; k < parts; ++k) {
-        const int64_t a = at(k);
-        const float m = p.part_ml[a * 2];
-        if (m == -INFINITY) continue;             // a part that saw no key
-        const float f = exp2f(m - M);
-        L = fmaf(p.part_ml[a * 2 + 1], f, L);
+        for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+        if (top == -INFINITY) continue;           // parts that saw no key
+        const float old = exp2f(M - top), f = exp2f(ml.x - top);
+        M = top;
+        float sum = ml.y * f;
 #pragma unroll
-        for (int e = 0; e < kLatMaxLatent / 64; ++e)
-            if (i0 + 64 * e < p.dc) o[e] = fmaf(p.part_o[a * p.dc + i0 + 64 * e], f, o[e]);
+        for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        L = fmaf(L, old, sum);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] *= old;
+        const int n = min(32, parts - k0);
+#pragma unroll 4
+        for (int k = 0; k < n; ++k) {
+            const float fk = __shfl_sync(0xffffffffu, f, k);
+            const float* src = p.part_o + at(k0 + k) * p.dc + col;
+            if (fk == 0.f) continue;              // (also what a part without a key left)
+            if (p.dc % 4 == 0) {
+                const float4 v = col < p.dc ? *reinterpret_cast<const float4*>(src)
+                                            : make_float4(0.f, 0.f, 0.f, 0.f);
+                o[0] = fmaf(v.x, fk, o[0]);
+                o[1] = fmaf(v.y, fk, o[1]);
+                o[2] = fmaf(v.z, fk, o[2]);
+                o[3] = fmaf(v.w, fk, o[3]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (col + e < p.dc) o[e] = fmaf(src[e], fk, o[e]);
+            }
+        }
     }
     const float inv = L > 0.f ? 1.f / L : 0.f;
 #pragma unroll
-    for (int e = 0; e < kLatMaxLatent / 64; ++e)
-        if (i0 + 64 * e < p.dc)
-            store_as(p.out, p.out_dtype, row * p.dc + i0 + 64 * e, o[e] * inv);
+    for (int e = 0; e < 4; ++e)
+        if (col + e < p.dc) store_as(p.out, p.out_dtype, row * p.dc + col + e, o[e] * inv);
 }
 
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 
-// Views of a 16-bit latent pool.  `tail` false: (64 columns, slot, chunk, layer * block),
-// box of 8 slots of every whole chunk; true: (row, slot, layer * block), box of 64
-// columns x 8 slots, for the columns behind the whole chunks.
-static int make_latent_tmap(CUtensorMap* m, const cx_latent_pool* p, bool tail) {
+// Rows of a TMA box: of one block, and of a tile.
+static int latent_box_rows(int64_t block_size) {
+    return block_size % 64 == 0 ? 64 : block_size % 32 == 0 ? 32 : block_size % 16 == 0 ? 16 : 8;
+}
+
+// View of a 16-bit latent pool: (row, slot, layer * block), box of 64 columns x some slots.
+static int make_latent_tmap(CUtensorMap* m, const cx_latent_pool* p) {
     auto enc = tmap_encoder();
     if (!enc) return fail(CX_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
-    const cuuint64_t dim = (cuuint64_t)(p->latent_dim + p->rope_dim), chunks = dim / 64;
-    const cuuint64_t bs = (cuuint64_t)p->block_size, n = (cuuint64_t)(p->n_layers * p->n_blocks);
-    const cuuint64_t dims4[4] = {64, bs, chunks, n}, dims3[3] = {dim, bs, n};
-    const cuuint64_t str4[3] = {dim * 2, 128, dim * 2 * bs}, str3[2] = {dim * 2, dim * 2 * bs};
-    const cuuint32_t box4[4] = {64, 8, (cuuint32_t)chunks, 1}, box3[3] = {64, 8, 1};
-    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    const cuuint64_t dim = (cuuint64_t)(p->latent_dim + p->rope_dim);
+    const cuuint64_t dims[3] = {dim, (cuuint64_t)p->block_size,
+                                (cuuint64_t)(p->n_layers * p->n_blocks)};
+    const cuuint64_t strides[2] = {dim * 2, dim * 2 * (cuuint64_t)p->block_size};
+    const cuuint32_t box[3] = {64, (cuuint32_t)latent_box_rows(p->block_size), 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
     const CUresult r = enc(m, p->dtype == CX_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                  : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                           tail ? 3 : 4, p->kv, tail ? dims3 : dims4, tail ? str3 : str4,
-                           tail ? box3 : box4, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           3, p->kv, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(CX_ERR_CUDA, "cuTensorMapEncodeTiled failed");
@@ -1035,20 +1152,19 @@ static int make_latent_tmap(CUtensorMap* m, const cx_latent_pool* p, bool tail) 
 }
 
 template <int N, typename E>
-static int launch_latent_tc(const CUtensorMap& tm, const CUtensorMap& tail, LatParams p, int grid,
-                            cudaStream_t st) {
+static int launch_latent_tc(const CUtensorMap& tm, LatParams p, int grid, cudaStream_t st) {
     int smem = 0;
-    LatCfg<N>::ring(p.dim, p.stages, smem);
+    LatCfg<N>::ring(p.dc, p.dim, p.stages, smem);
     auto kern = latent_tc_kernel<N, E>;
     CX_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    kern<<<grid, kLatThreads, smem, st>>>(tm, tail, p);
+    kern<<<grid, LatCfg<N>::THREADS, smem, st>>>(tm, p);
     int rc = check_launch("latent_tc_kernel");
     if (rc) return rc;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid, N / 4);
+    cfg.gridDim = dim3(grid, N / 2);
     cfg.blockDim = 256;
     cfg.stream = st;
     cfg.attrs = &attr;
