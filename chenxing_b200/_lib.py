@@ -30,7 +30,8 @@ EXPORTS = ("cx_version", "cx_last_error", "cx_device_error", "cx_kv_append", "cx
            "cx_attention_dense", "cx_paged_decode_static", "cx_paged_kernel_kind",
            "cx_kv_append_rope", "cx_set_wait_limit_ns", "cx_kv_append_norm_rope",
            "cx_paged_attend", "cx_paged_attend_workspace_bytes", "cx_paged_attend_kind",
-           "cx_paged_attend_tree", "cx_kv_accept", "cx_latent_append", "cx_latent_gather",
+           "cx_paged_attend_tree", "cx_paged_attend_tree_workspace_bytes",
+           "cx_paged_attend_tree_kind", "cx_kv_accept", "cx_latent_append", "cx_latent_gather",
            "cx_latent_block_copy", "cx_latent_accept", "cx_latent_attend",
            "cx_latent_attend_workspace_bytes", "cx_latent_attend_kind")
 KERNEL_KINDS = {0: "generic", 1: "mma", 2: "tcgen05", 3: "fma"}
@@ -145,6 +146,10 @@ _SIGS = {
     "cx_paged_attend_tree": ([ctypes.POINTER(CxPool), _I64, ctypes.POINTER(CxAttnBatch),
                               ctypes.POINTER(CxAttnMods), ctypes.POINTER(CxTree), _VP, _I32, _VP,
                               _VP, ctypes.c_size_t, _I32, _VP], ctypes.c_int),
+    "cx_paged_attend_tree_workspace_bytes": ([ctypes.POINTER(CxPool),
+                                              ctypes.POINTER(CxAttnBatch)], ctypes.c_size_t),
+    "cx_paged_attend_tree_kind": ([ctypes.POINTER(CxPool), ctypes.POINTER(CxAttnBatch), _I32],
+                                  ctypes.c_int),
     "cx_kv_accept": ([ctypes.POINTER(CxPool), ctypes.POINTER(CxAttnBatch), _VP, _I64, _I64, _VP],
                      ctypes.c_int),
     "cx_latent_append": ([ctypes.POINTER(CxLatentPool), _I64, ctypes.POINTER(CxLatentRows), _VP,

@@ -264,6 +264,8 @@ class PagedBatch:
 
     def _workspace_need(self) -> int:
         pool = self.cache.cx_pool()
+        if self.is_tree:
+            return int(_lib.lib().cx_paged_attend_tree_workspace_bytes(pool, self._c))
         return max(int(_lib.lib().cx_paged_workspace_bytes(pool, self._c)),
                    int(_lib.lib().cx_paged_attend_workspace_bytes(pool, self._c)))
 
@@ -294,8 +296,9 @@ class PagedBatch:
         """Which libcxkv kernel attends this batch for queries and outputs of these
         types: "generic", "mma", "tcgen05" or "fma"."""
         if self.takes_attend(out_dtype):
-            k = _lib.lib().cx_paged_attend_kind(self.cache.cx_pool(), self._c,
-                                                _lib.cx_dtype(q_dtype))
+            kind = _lib.lib().cx_paged_attend_tree_kind if self.is_tree \
+                else _lib.lib().cx_paged_attend_kind
+            k = kind(self.cache.cx_pool(), self._c, _lib.cx_dtype(q_dtype))
         else:
             k = _lib.lib().cx_paged_kernel_kind(self.cache.cx_pool(), self._c,
                                                 _lib.cx_dtype(q_dtype), int(self.verify))

@@ -185,6 +185,107 @@ __device__ __forceinline__ uint32_t tc_swz(int row, int col, int rows) {
                       ((((col & 63) >> 3) ^ (row & 7)) << 4) + (col & 7) * 2);
 }
 
+// ---- one elected thread of a whole warp ------------------------------------
+// Upper word of a descriptor of 128-byte swizzled lines in groups of 8, 1024 bytes
+// apart (tc_sdesc); the lower one holds the address and the leading offset.
+constexpr uint32_t kElDescHi = (1024u >> 4) | 1u << 14 | 2u << 29;
+
+__device__ __forceinline__ uint32_t el_desc_lo(const void* p, uint32_t lbo) {
+    return ((smem_addr(p) >> 4) & 0x3FFFu) | (lbo >> 4) << 16;
+}
+
+// tcgen05.mma, tcgen05.commit and a TMA load by one elected thread of a warp that comes
+// here as a whole, with the same operands in every lane: only then do they stay in
+// uniform registers.  An MMA issued by a thread in a branch of its own took 180
+// cycles here whatever its shape (a tile of 52 of them 8,600), one whose thread is
+// chosen by a comparison 50, by elect.sync 25 to 49, which is what the tensor pipe
+// takes for it (64 keys: 25 / 26 / 33 cycles at 16 / 32 / 64 rows; 128 columns: 40 / 41
+// / 49).
+__device__ __forceinline__ void el_mma(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo,
+                                        uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "mov.b64 a, {%1, %5};\n\t"
+        "mov.b64 b, {%2, %5};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(kElDescHi)
+        : "memory");
+}
+__device__ __forceinline__ void el_commit(uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+            smem_addr(bar))
+        : "memory");
+}
+// Arrival of one elected thread that adds `bytes` to what the phase waits for.
+__device__ __forceinline__ void el_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
+        "r"(bytes)
+        : "memory");
+}
+__device__ __forceinline__ void el_tma(uint32_t dst, const void* tmap, uint32_t bar, int x, int y,
+                                         int z) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];\n\t}" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t warp_uniform(uint32_t x) {
+    return __shfl_sync(0xffffffffu, x, 0);
+}
+
+// A bounded wait of a whole warp on an mbarrier phase, and whether it completed.  A
+// try suspends for up to half a microsecond; `tries` of them, or *abort, end it.  (One
+// loop in one piece, which the warp leaves together: behind a loop that its threads
+// leave one by one, an MMA takes up to 370 cycles.)
+__device__ __forceinline__ bool el_wait(uint64_t* bar, uint32_t parity, volatile int* abort,
+                                         uint32_t tries) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b32 n, a;\n\t"
+        "mov.b32 n, %4;\n\t"
+        "mov.b32 %0, 1;\n\t"
+        "TRY:\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 500;\n\t"
+        "@p bra DONE;\n\t"
+        "ld.volatile.shared.b32 a, [%3];\n\t"
+        "setp.ne.b32 p, a, 0;\n\t"
+        "@p bra FAIL;\n\t"
+        "sub.u32 n, n, 1;\n\t"
+        "setp.ne.b32 p, n, 0;\n\t"
+        "@p bra TRY;\n\t"
+        "FAIL:\n\t"
+        "mov.b32 %0, 0;\n\t"
+        "DONE:\n\t}"
+        : "=&r"(ok)
+        : "r"(smem_addr(bar)), "r"(parity), "r"(smem_addr(const_cast<int*>(abort))), "r"(tries)
+        : "memory");
+    return __all_sync(0xffffffffu, ok != 0);
+}
+
+// el_mma with A (16-bit pairs per 32-bit column, row i in lane i) read from TMEM.
+__device__ __forceinline__ void el_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo,
+                                          uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "mov.b64 b, {%2, %5};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(kElDescHi)
+        : "memory");
+}
+
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------

@@ -21,28 +21,31 @@ static bool tma_shape(const cx_pool* pool, const cx_attn_batch* b) {
 
 // The tcgen05 kernel: 16-bit pools from 64 packed rows (query tokens x GQA
 // group) of more than one token, and groups that the split-K kernels' 64 rows
-// do not hold.
-static bool tc_shape(const cx_pool* pool, const cx_attn_batch* b) {
+// do not hold.  Trees, whose rows it takes as one query tile in two places, from
+// kTreeTcRows on.
+constexpr int64_t kTreeTcRows = 33;
+static bool tc_shape(const cx_pool* pool, const cx_attn_batch* b, bool tree) {
     const int64_t G = b->n_q_heads / pool->n_kv_heads, rows = G * b->max_q_len;
     return pool->dtype != CX_F32 && tma_shape(pool, b) && G <= kTcRows &&
-           (rows > 64 || (rows == 64 && b->max_q_len > 1));
+           (rows > 64 || ((tree ? rows >= kTreeTcRows : rows == 64) && b->max_q_len > 1));
 }
 
 // The split-K kernels: up to 64 packed rows.
-static bool split_shape(const cx_pool* pool, const cx_attn_batch* b) {
+static bool split_shape(const cx_pool* pool, const cx_attn_batch* b, bool tree) {
     const int64_t rows = b->n_q_heads / pool->n_kv_heads * b->max_q_len;
-    return tma_shape(pool, b) && rows >= 1 && rows <= 64 && !tc_shape(pool, b);
+    return tma_shape(pool, b) && rows >= 1 && rows <= 64 && !tc_shape(pool, b, tree);
 }
 
 // The kernel of a call.  `vec`: q, its token stride and out are 16-byte aligned.
 // 16-bit pools take queries of their own type or fp32, fp32 pools any type.
-static int attend_kind(const cx_pool* pool, const cx_attn_batch* b, int32_t q_dtype, bool vec) {
+static int attend_kind(const cx_pool* pool, const cx_attn_batch* b, int32_t q_dtype, bool vec,
+                       bool tree) {
     if (!vec) return CX_KERNEL_GENERIC;
-    if (pool->dtype == CX_F32) return split_shape(pool, b) ? CX_KERNEL_FMA : CX_KERNEL_GENERIC;
+    if (pool->dtype == CX_F32) return split_shape(pool, b, tree) ? CX_KERNEL_FMA : CX_KERNEL_GENERIC;
     if (q_dtype != CX_F32 && q_dtype != pool->dtype) return CX_KERNEL_GENERIC;
-    return tc_shape(pool, b)      ? CX_KERNEL_TCGEN05
-           : split_shape(pool, b) ? CX_KERNEL_MMA
-                                  : CX_KERNEL_GENERIC;
+    return tc_shape(pool, b, tree)      ? CX_KERNEL_TCGEN05
+           : split_shape(pool, b, tree) ? CX_KERNEL_MMA
+                                        : CX_KERNEL_GENERIC;
 }
 
 // CTAs of the tcgen05 kernel, and over how many the key tiles of each are split
@@ -62,9 +65,9 @@ static void tc_grid(const cx_pool* pool, const cx_attn_batch* b, int* tpt, int64
     *n_split = (int)std::max<int64_t>(1, s);
 }
 
-static size_t attend_workspace(const cx_pool* pool, const cx_attn_batch* b) {
+static size_t attend_workspace(const cx_pool* pool, const cx_attn_batch* b, bool tree) {
     const int64_t rows = b->n_q_heads / pool->n_kv_heads * b->max_q_len;
-    if (tc_shape(pool, b)) {
+    if (tc_shape(pool, b, tree)) {
         int tpt, n_split;
         int64_t n_ctiles;
         tc_grid(pool, b, &tpt, &n_ctiles, &n_split);
@@ -72,7 +75,7 @@ static size_t attend_workspace(const cx_pool* pool, const cx_attn_batch* b) {
                             : (size_t)(n_ctiles * b->batch * pool->n_kv_heads) * n_split * 256 *
                                   (pool->head_dim + 2) * 4;
     }
-    if (!split_shape(pool, b)) return 256;
+    if (!split_shape(pool, b, tree)) return 256;
     return ws_layout(b->batch, unit_shape(pool, rows), rows, pool->head_dim, grid_size()).total;
 }
 
@@ -195,7 +198,7 @@ static int attend_tc(const cx_pool* pool, int64_t layer, const cx_attn_batch& b,
     int64_t n_ctiles = 0;
     tc_grid(pool, &b, &p.tpt, &n_ctiles, &p.n_split);
     if (n_ctiles > (1 << 24)) return fail(CX_ERR_UNSUPPORTED, "cx_paged_attend: grid too large");
-    if (p.n_split > 1 && (!ws || ws_bytes < attend_workspace(pool, &b) ||
+    if (p.n_split > 1 && (!ws || ws_bytes < attend_workspace(pool, &b, TREE) ||
                           (reinterpret_cast<uintptr_t>(ws) & 255) != 0))
         return fail(CX_ERR_WORKSPACE,
                     "cx_paged_attend: workspace missing, too small or not 256-byte aligned");
@@ -299,7 +302,7 @@ static int attend_scored(const cx_pool* pool, int64_t layer, const cx_attn_batch
     const uintptr_t al = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) |
                          static_cast<uintptr_t>(m.q_stride * elem_bytes(q_dtype));
     cudaStream_t st = as_stream(stream);
-    const int kind = attend_kind(pool, &b, q_dtype, (al & 15) == 0);
+    const int kind = attend_kind(pool, &b, q_dtype, (al & 15) == 0, TREE);
     if (kind == CX_KERNEL_MMA || kind == CX_KERNEL_FMA)
         return attend_split<TREE>(pool, layer, b, m, tree, scale, q, q_dtype, out, ws, ws_bytes, replan,
                             false, st);
@@ -307,7 +310,7 @@ static int attend_scored(const cx_pool* pool, int64_t layer, const cx_attn_batch
         return attend_tc<TREE>(pool, layer, b, m, tree, scale, q, q_dtype, out, ws, ws_bytes, st);
     // a later layer of the step may have queries that the split-K kernels take:
     // the plan it then reads is made now
-    if (replan && split_shape(pool, &b) && ws) {
+    if (replan && split_shape(pool, &b, TREE) && ws) {
         rc = attend_split<TREE>(pool, layer, b, m, tree, scale, q, q_dtype, out, ws, ws_bytes, 1, true, st);
         if (rc) return rc;
     }

@@ -157,6 +157,16 @@ __device__ __forceinline__ void sc_item(int q, int n, bool& is_v, int& i) {
 __device__ __forceinline__ int sc_pos_k(int i) { return i == 0 ? 0 : 2 * i - 1; }
 __device__ __forceinline__ int sc_pos_v(int i, int n) { return i == n - 1 ? 2 * n - 1 : 2 * i + 2; }
 
+// The same where the two query tiles' places work on one tile's keys in turn (TREE):
+// K(0), K(1), then K(i + 2), V(i), and the last two V.
+__device__ __forceinline__ void sc_item2(int q, int n, bool& is_v, int& i) {
+    const bool tail = q >= 2 * n - 2;
+    is_v = q >= min(2, n) && (tail || (q & 1));
+    i = q < min(2, n) ? q : tail ? q - n : is_v ? (q - 3) / 2 : q / 2 + 1;
+}
+__device__ __forceinline__ int sc_pos_k2(int i) { return i < 2 ? i : 2 * i - 2; }
+__device__ __forceinline__ int sc_pos_v2(int i, int n) { return i >= n - 2 ? i + n : 2 * i + 3; }
+
 // The key tiles of a CTA: n_pre tiles from block 0 (the prefix left of the
 // window), then tiles from block kb0 on.
 struct ScTiles {
@@ -181,7 +191,9 @@ struct ScGeom {
 // Which sequence, KV head and pair of query tiles CTA `cta` has: the longest
 // contexts first (batches of up to 32; beyond, in order), within a sequence the
 // latest tiles first, so that the last CTAs to start are short (without it the
-// SMs idled 15 % of 512 CTAs' time).  Every lane of a warp calls it.
+// SMs idled 15 % of 512 CTAs' time).  Every lane of a warp calls it.  (WIDE: batches of
+// up to 128, the same way.)
+template <bool WIDE>
 __device__ __forceinline__ void sc_place(const ScoredTcParams& p, int cta, int lane, int& b,
                                          int& h, int& ctile) {
     const int per_seq = p.hk * p.n_ctiles;
@@ -189,6 +201,31 @@ __device__ __forceinline__ void sc_place(const ScoredTcParams& p, int cta, int l
     h = rem % p.hk;
     ctile = p.n_ctiles - 1 - rem / p.hk;
     b = place;
+    if constexpr (WIDE) {
+        if (p.batch > 128 || p.batch == 1) return;
+        int ctx[4], before[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            ctx[k] = lane + 32 * k < p.batch ? p.ctx_lens[lane + 32 * k] : INT32_MIN;
+            before[k] = 0;
+        }
+#pragma unroll
+        for (int k0 = 0; k0 < 4; ++k0) {
+            for (int j = 32 * k0; j < min(p.batch, 32 * k0 + 32); ++j) {
+                const int o = __shfl_sync(0xffffffffu, ctx[k0], j & 31);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    before[k] += o > ctx[k] || (o == ctx[k] && j < lane + 32 * k);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const unsigned at = __ballot_sync(
+                0xffffffffu, lane + 32 * k < p.batch && before[k] == place);
+            if (at) b = 32 * k + __ffs((int)at) - 1;
+        }
+        return;
+    }
     if (p.batch > 32 || p.batch == 1) return;
     const int ctx = lane < p.batch ? p.ctx_lens[lane] : INT32_MIN;
     int before = 0;
@@ -201,7 +238,11 @@ __device__ __forceinline__ void sc_place(const ScoredTcParams& p, int cta, int l
 }
 
 // TREE: the query rows are the nodes of a drafted tree; tiles that hold drafted keys
-// are masked by 32 bits of a row's word at a time.
+// are masked by 32 bits of a row's word at a time.  A tree whose rows fill one query
+// tile would run as one chain S -> softmax -> P -> PV -> next S, with half of the
+// softmax warps idle: both query tiles then hold its rows and take the key tiles in
+// turn (`turns`), each with its own maxima, sums and O, which are joined at the end.  64
+// trees of 26 nodes (104 rows) behind 1k to 8k keys, 8 KV heads of 128: 391 -> TURNS us.
 template <int DH, typename E, bool CAP, bool ALIBI, bool TREE = false>
 __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
     scored_tc_kernel(const __grid_constant__ CUtensorMap tmk,
@@ -220,12 +261,13 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
     uint64_t* mma_drain = o_done + 2;      // last commit of the MMA thread
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(mma_drain + 1);
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
-    volatile int* s_issued = s_abort + 1;  // ring items whose loads were issued
+    volatile int* s_issued = s_abort + 1;  // ring items whose loads were issued (TREE: by warp)
 
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = TREE ? (int)warp_uniform(tid >> 5) : tid >> 5;
     const int cta = (int)blockIdx.x;
     int b, h, ctile;
-    sc_place(p, cta, lane, b, h, ctile);
+    sc_place<TREE>(p, cta, lane, b, h, ctile);
     const int G = p.group, tpt = p.tpt;
     const int qs = p.q_start ? p.q_start[b] : b;
     const int T = p.q_start ? p.q_start[b + 1] - qs : 1;
@@ -239,6 +281,7 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
     const int t0 = ctile * 2 * tpt;                          // first token of tile 0
     if (t0 >= T) return;
     const int nq = t0 + tpt < T ? 2 : 1;
+    const bool turns = TREE && nq == 1;
     const int t_end = min(T, t0 + nq * tpt);
     const int pos0 = ctx - T;                                // position of token 0
     const int win = p.window;
@@ -274,6 +317,7 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
         mbar_init(mma_drain, 1);
         *s_abort = 0;
         *s_issued = 0;
+        if (TREE) s_issued[1] = s_issued[2] = 0;
         *reinterpret_cast<ScGeom*>(sm + C::OFF_GEOM) =
             ScGeom{tiles.n_pre, tiles.kb0, first, n_tiles, pre,  win,  ctx,
                    run_hi,      run_lo,    nblk_seq, pos0, t0, t_end};
@@ -295,13 +339,14 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REG_SOFTMAX));
         const int w = warp >> 3, c = (warp >> 2) & 1, r = tid & 127;
         const int pair_bar = 4 + w * 4 + (warp & 3);         // the two warps of these 32 rows
-        const int t = t0 + w * tpt + r / G;                  // this row's token
+        const int tw = turns ? 0 : w;                        // the query tile of its rows
+        const int t = t0 + tw * tpt + r / G;                 // this row's token
         const int head = h * G + r % G;
         // ---- half a row of Q_w -> shared memory: 16-bit, K-major, swizzled, zero
         // padding rows.  Only the MMA warp waits for it (named barrier 3).
         {
             unsigned char* qdst = sm + w * C::Q_BYTES;
-            const bool row_ok = t < min(t_end, t0 + (w + 1) * tpt) && r < tpt * G;
+            const bool row_ok = t < min(t_end, t0 + (tw + 1) * tpt) && r < tpt * G;
             const int64_t row = (int64_t)(qs + t) * p.q_stride + (int64_t)head * D;
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
@@ -330,7 +375,7 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
             fence_async_smem();
             named_bar_arrive(3, C::SOFTMAX + 32);
         }
-        if (w < nq) {
+        if (w < nq || turns) {
             const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t tm_s = tmem + w * kScKeys + c * 64 + lane_off;
             const uint32_t tm_o = tmem + 2 * kScKeys + w * D + c * (D / 2) + lane_off;
@@ -389,11 +434,11 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
                 named_bar_sync(pair_bar, 64);
                 return c == 0 ? x : *red;    // (c == 1 alone reads it now: it writes it next)
             };
-            for (int i = 0; i < g.n_tiles; ++i) {
+            for (int i = 0; i < (turns ? (g.n_tiles + 1 - w) >> 1 : g.n_tiles); ++i) {
                 if (ok)
                     ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[w], i & 1, s_abort,
                                                                    p.wait_ns));
-                const int tile = g.first - i;
+                const int tile = g.first - (turns ? 2 * i + w : i);
                 const int b0 = tile < g.n_pre ? tile * BPT : g.kb0 + (tile - g.n_pre) * BPT;
                 const int kb = b0 * kBlockTok + c * 64;      // this half's first key
                 unsigned bad4 = 0;                           // its bad blocks
@@ -608,7 +653,7 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
                 }
                 if (!ok) continue;
                 // zero the V rows that no row of the CTA sees
-                if (w == 0) {
+                if (w == 0 || turns) {
                     const int pre = g.pre, ctx = g.ctx, run_hi = g.run_hi, run_lo = g.run_lo;
                     const int kbase = kb - c * 64;
                     auto dead = [&](int key) {
@@ -618,7 +663,8 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
                                           (kbase + kScKeys > pre &&
                                            (kbase + kScKeys - 1 > run_hi || kbase < run_lo));
                     if (any_dead) {
-                        const int q = sc_pos_v(i, g.n_tiles);
+                        const int q = turns ? sc_pos_v2(2 * i + w, g.n_tiles)
+                                            : sc_pos_v(i, g.n_tiles);
                         ok = __all_sync(0xffffffffu,
                                         mbar_wait_bounded(&full[q % SLOTS], (q / SLOTS) & 1,
                                                           s_abort, p.wait_ns));
@@ -647,7 +693,7 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
             }
             // ---- epilogue: the row's denominator over both halves, then this half's
             // columns to the output, or to this split's part ----
-            const int n_tiles = g.n_tiles;
+            const int n_tiles = turns ? (g.n_tiles + 1 - w) >> 1 : g.n_tiles;
             if (n_tiles > 0 && ok) {
                 ok = __all_sync(0xffffffffu, mbar_wait_bounded(&o_done[w], (n_tiles - 1) & 1,
                                                                 s_abort, p.wait_ns));
@@ -660,6 +706,62 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
             const int r_e = tid_e & 127, t_e = g.t0 + w * tpt + r_e / G, head_e = h * G + r_e % G;
             const bool row_ok = t_e < min((int)g.t_end, (int)g.t0 + (w + 1) * tpt) && r_e < tpt * G;
             float* part = nullptr;
+            if (TREE && turns) {
+                // both places' rows: references and sums through the ring, which nothing
+                // reads any more behind the barrier
+                float* x = reinterpret_cast<float*>(ring);
+                named_bar_sync(2, C::SOFTMAX);
+                if (c == 0) {
+                    x[w * 128 + r] = m;
+                    x[256 + w * 128 + r] = l;
+                }
+                if (!ok) *s_abort = 1;
+                named_bar_sync(2, C::SOFTMAX);
+                ok = __all_sync(0xffffffffu, !*s_abort);
+                const float m0 = x[r], m1 = x[128 + r], M = fmaxf(m0, m1);
+                const float f0 = M == -INFINITY ? 0.f : exp2f(m0 - M);
+                const float f1 = M == -INFINITY ? 0.f : exp2f(m1 - M);
+                const float L = x[256 + r] * f0 + x[384 + r] * f1;
+                const bool two = g.n_tiles > 1;              // (the second has an O)
+                const int64_t o_row = ((int64_t)(qs + (g.t0 + r / G)) * p.hq + h * G + r % G) * D;
+                const bool in = (g.t0 + r / G) < min((int)g.t_end, (int)g.t0 + tpt) && r < tpt * G;
+                float* to = nullptr;
+                if (p.n_split > 1) {
+                    to = p.part + (((int64_t)cta * p.n_split + blockIdx.y) * 256 + r) * (D + 2);
+                    if (c == 0 && w == 0) {
+                        to[D] = ok ? M : -INFINITY;
+                        to[D + 1] = L;
+                    }
+                }
+                const float inv = to ? 1.f : L > 0.f ? 1.f / L : 0.f;
+                // a quarter of the columns a thread: 16 at a time
+                const uint32_t tm_c = tmem + 2 * kScKeys + lane_off;
+#pragma unroll 1
+                for (int k = 0; ok && k < D / 64; ++k) {
+                    const int col = c * (D / 2) + w * (D / 4) + k * 16;
+                    float a[16], b[16];
+                    __syncwarp();
+                    if (g.n_tiles > 0) {
+                        sc_ld16(tm_c + col, a);
+                        if (two) sc_ld16(tm_c + D + col, b);
+                        tc_wait_ld();
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float y = g.n_tiles > 0 ? a[e] * f0 : 0.f;
+                        a[e] = (two ? fmaf(b[e], f1, y) : y) * inv;
+                    }
+                    if (!in) continue;
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        if (to)
+                            *reinterpret_cast<float2*>(to + col + e) = make_float2(a[e], a[e + 1]);
+                        else
+                            store2_as(p.out, p.out_dtype, o_row + col + e, a[e], a[e + 1]);
+                    }
+                }
+                if (!ok) raise_flag(CX_DEV_WAIT_TIMEOUT);
+            } else {
             if (p.n_split > 1) {
                 part = p.part + (((int64_t)cta * p.n_split + blockIdx.y) * 256 + w * 128 + r_e) *
                                     (D + 2);
@@ -715,10 +817,145 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
                 *s_abort = 1;
                 raise_flag(CX_DEV_WAIT_TIMEOUT);
             }
+            }
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REG_OTHER));
-        if (warp < C::MMA_WARP) {
+        if constexpr (TREE) {
+            // Whole warps that elect a thread for every MMA and box (as latent_tc_kernel's).
+            const uint32_t tries =
+                (uint32_t)min((unsigned long long)p.wait_ns / 500 + 1, 1ull << 30);
+            const int n = (int)warp_uniform(n_tiles);
+            const bool tn = warp_uniform(turns) != 0;
+            bool ok = true;
+            if (warp < C::MMA_WARP) {
+                const int pw = warp - C::PROD_WARP;
+                const int32_t* tab = p.tables + (int64_t)b * p.table_stride;
+                auto id_of = [&](int q) {             // this lane's block of item q; INT32_MIN: none
+                    bool is_v;
+                    int i;
+                    if (tn)
+                        sc_item2(q, n, is_v, i);
+                    else
+                        sc_item(q, n, is_v, i);
+                    const int blk = tiles.block(first - i) + lane;
+                    return q < 2 * n && lane < BPT && blk < nblk_seq ? tab[blk] : INT32_MIN;
+                };
+                int id = id_of(0), id_next = id_of(1), s = 0;
+                uint32_t use = 0;                     // parity of the fill before, of slot s
+                for (int q = 0; q < 2 * n; ++q) {
+                    bool is_v;
+                    int i;
+                    if (tn)
+                        sc_item2(q, n, is_v, i);
+                    else
+                        sc_item(q, n, is_v, i);
+                    int z = -1;                       // outside the map: the copy fills zeros
+                    if (id >= 0 && id < p.n_blocks)
+                        z = (p.layer * p.n_blocks + id) * p.hk + h;
+                    else if (id != INT32_MIN)
+                        raise_flag(CX_DEV_BAD_BLOCK);
+                    int z3[3];
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) z3[k] = __shfl_sync(0xffffffffu, z, pw + 3 * k);
+                    id = id_next;
+                    id_next = id_of(q + 2);
+                    if (q >= SLOTS && !(ok = el_wait(&empty[s], use ^ 1, s_abort, tries))) break;
+                    const uint32_t bar = warp_uniform(smem_addr(&full[s]));
+                    const uint32_t dst = warp_uniform(smem_addr(ring + s * C::SLOT + pw * 2048));
+                    const bool v = warp_uniform(is_v) != 0;
+                    el_expect(bar, (pw < 2 ? 3 : 2) * (C::SLOT / BPT));
+                    auto boxes = [&](const CUtensorMap* m, auto count) {
+#pragma unroll
+                        for (int k = 0; k < decltype(count)::value; ++k)
+#pragma unroll
+                            for (int hf = 0; hf < C::HALVES; ++hf)
+                                el_tma(dst + hf * C::KV_HALF + k * 3 * 2048, m, bar, hf * 64, 0,
+                                       z3[k]);
+                    };
+                    if (pw < 2) {
+                        if (v)
+                            boxes(&tmv, std::integral_constant<int, 3>{});
+                        else
+                            boxes(&tmk, std::integral_constant<int, 3>{});
+                    } else {
+                        if (v)
+                            boxes(&tmv, std::integral_constant<int, 2>{});
+                        else
+                            boxes(&tmk, std::integral_constant<int, 2>{});
+                    }
+                    if (lane == 0) s_issued[pw] = q + 1;
+                    if (++s == SLOTS) {
+                        s = 0;
+                        use ^= 1;
+                    }
+                }
+            } else {
+                constexpr uint32_t idesc_s = sc_idesc<E>(kTcRows, kScKeys, 0);
+                constexpr uint32_t idesc_o = sc_idesc<E>(kTcRows, D, 1);
+                named_bar_sync(3, C::SOFTMAX + 32);    // Q_0, Q_1 are in shared memory
+                const uint32_t tm = warp_uniform(tmem);
+                const uint32_t q_lo = warp_uniform(el_desc_lo(sm, 16));
+                const uint32_t k_lo = warp_uniform(el_desc_lo(ring, 16));
+                const uint32_t v_lo = warp_uniform(el_desc_lo(ring, C::KV_HALF));
+                auto wait = [&](uint64_t* bar, int parity) {
+                    const bool r = el_wait(bar, parity & 1, s_abort, tries);
+                    if (r) tc_fence_after();
+                    return r;
+                };
+                auto issue_s = [&](int w, int slot) {
+                    const uint32_t kd = warp_uniform(k_lo + (uint32_t)(slot * (C::SLOT >> 4)));
+                    const uint32_t qd = warp_uniform(q_lo + (uint32_t)(w * (C::Q_BYTES >> 4)));
+                    const uint32_t d = warp_uniform(tm + w * kScKeys);
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk)
+                        el_mma(d, qd + (((kk >> 2) * C::Q_HALF + (kk & 3) * 32) >> 4),
+                               kd + (((kk >> 2) * C::KV_HALF + (kk & 3) * 32) >> 4), idesc_s,
+                               kk > 0 ? 1u : 0u);
+                    el_commit(&s_full[w]);
+                };
+                auto issue_pv = [&](int w, int slot, bool acc) {
+                    const uint32_t vd = warp_uniform(v_lo + (uint32_t)(slot * (C::SLOT >> 4)));
+                    const uint32_t o_t = warp_uniform(tm + 2 * kScKeys + w * D);
+                    const uint32_t p_t = warp_uniform(tm + w * kScKeys), a0 = warp_uniform(acc);
+#pragma unroll
+                    for (int kk = 0; kk < kScKeys / 16; ++kk)
+                        el_mma_ts(o_t, p_t + (kk >> 2) * 64 + (kk & 3) * 8, vd + kk * (2048 >> 4),
+                                  idesc_o, kk > 0 ? 1u : a0);
+                };
+                // key tiles ahead: one for both query tiles, or one for either place
+                const int ahead = tn ? 2 : 1, nqw = tn ? 1 : nq;
+                auto pos_k = [&](int i) { return tn ? sc_pos_k2(i) : sc_pos_k(i); };
+                auto pos_v = [&](int i) { return tn ? sc_pos_v2(i, n) : sc_pos_v(i, n); };
+                for (int i = 0; ok && i < min(ahead, n); ++i) {
+                    if (!(ok = wait(&full[i], 0))) break;
+                    issue_s(i, i);
+                    if (nqw == 2) issue_s(1, i);
+                    el_commit(&empty[i]);
+                }
+                for (int i = 0; ok && i < n; ++i) {
+                    const bool next = i + ahead < n;
+                    const int kp = pos_k(i + ahead), vp = pos_v(i);
+                    if (next && !(ok = wait(&full[kp % SLOTS], kp / SLOTS))) break;
+                    if (!(ok = wait(&full[vp % SLOTS], vp / SLOTS))) break;
+                    for (int k = 0; ok && k < nqw; ++k) {
+                        const int w = tn ? i & 1 : k, j = tn ? i >> 1 : i;
+                        if (!(ok = wait(&p_full[w], j))) break;
+                        issue_pv(w, vp % SLOTS, j > 0);
+                        el_commit(&o_done[w]);
+                        if (next) issue_s(w, kp % SLOTS);
+                    }
+                    if (!ok) break;
+                    el_commit(&empty[vp % SLOTS]);
+                    if (next) el_commit(&empty[kp % SLOTS]);
+                }
+                el_commit(mma_drain);
+            }
+            if (!ok && lane == 0) {
+                *s_abort = 1;
+                raise_flag(CX_DEV_WAIT_TIMEOUT);
+            }
+        } else if (warp < C::MMA_WARP) {
             // ---------------- producers: blocks pw, pw + 3, .. of each item ----------------
             const int pw = warp - C::PROD_WARP;
             const int32_t* tab = p.tables + (int64_t)b * p.table_stride;
@@ -853,10 +1090,15 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
     tc_fence_before();
     __syncthreads();
     if (*s_abort && tid == 0) {
-        const int issued = *s_issued;
+        int issued = *s_issued;
+        if (TREE) issued = max(issued, max(s_issued[1], s_issued[2]));
         for (int s = 0; s < SLOTS; ++s) {
             const int uses = issued > s ? (issued - 1 - s) / SLOTS + 1 : 0;
-            if (uses > 0) mbar_wait_bounded(&full[s], (uses - 1) & 1, nullptr, kWaitLimitNs);
+            // (TREE: a slot that not all producers came to never completes; what the others
+            // loaded into it ends well within the wait)
+            if (uses > 0)
+                mbar_wait_bounded(&full[s], (uses - 1) & 1, nullptr,
+                                  TREE ? 20000000ull : kWaitLimitNs);
         }
     }
     if (tid == C::MMA_WARP * 32) mbar_wait_bounded(mma_drain, 0, nullptr, kWaitLimitNs);
@@ -877,7 +1119,7 @@ __global__ void __launch_bounds__(256) scored_tc_join_kernel(const ScoredTcParam
     const int cta = (int)(job >> 8), wr = (int)(job & 255), w = wr >> 7, r = wr & 127;
     if (cta >= p.batch * p.hk * p.n_ctiles) return;
     int b, h, ctile;
-    sc_place(p, cta, lane, b, h, ctile);
+    sc_place<TREE>(p, cta, lane, b, h, ctile);
     const int qs = p.q_start ? p.q_start[b] : b;
     const int T = p.q_start ? p.q_start[b + 1] - qs : 1;
     const int t = (ctile * 2 + w) * p.tpt + r / p.group;

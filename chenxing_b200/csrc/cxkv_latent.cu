@@ -43,12 +43,12 @@ static LatPlan latent_plan(const cx_latent_pool* pool, const cx_attn_batch* b) {
 }
 
 // Parts that the generic kernel splits a context into: CTAs for about four an SM, at
-// least 64 keys a part.
+// least 32 keys a part, at most 256 parts (latent_generic_join).
 static int latent_split(const cx_latent_pool* pool, const cx_attn_batch* b, int64_t units) {
     int64_t keys = b->table_stride * pool->block_size;
     if (b->window > 0) keys = std::min(keys, b->window + b->max_q_len);
     const int64_t want = 4ll * std::max(num_sms(), 1) / std::max<int64_t>(units, 1);
-    return (int)std::max<int64_t>(1, std::min(std::min(want, keys / 64), (int64_t)256));
+    return (int)std::max<int64_t>(1, std::min(std::min(want, keys / 32), (int64_t)256));
 }
 
 static int64_t generic_tiles(const cx_attn_batch* b) {

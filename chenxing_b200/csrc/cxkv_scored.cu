@@ -27,14 +27,14 @@ size_t cx_paged_attend_workspace_bytes(const cx_pool* pool, const cx_attn_batch*
         return 0;
     cx_attn_batch b = *batch;
     if (!b.q_start || b.max_q_len < 1) b.max_q_len = 1;
-    return cx::attend_workspace(pool, &b);
+    return cx::attend_workspace(pool, &b, false);
 }
 
 int cx_paged_attend_kind(const cx_pool* pool, const cx_attn_batch* batch, int32_t q_dtype) {
     if (!pool || !batch || pool->n_kv_heads <= 0) return CX_KERNEL_GENERIC;
     cx_attn_batch b = *batch;
     if (!b.q_start || b.max_q_len < 1) b.max_q_len = 1;
-    return cx::attend_kind(pool, &b, q_dtype, true);
+    return cx::attend_kind(pool, &b, q_dtype, true, false);
 }
 
 }  // extern "C"

@@ -28,4 +28,19 @@ int cx_paged_attend_tree(const cx_pool* pool, int64_t layer, const cx_attn_batch
                                q, q_dtype, out, workspace, workspace_bytes, replan, stream);
 }
 
+size_t cx_paged_attend_tree_workspace_bytes(const cx_pool* pool, const cx_attn_batch* batch) {
+    if (!pool || !batch || pool->n_kv_heads <= 0 || batch->n_q_heads <= 0 || batch->batch < 0)
+        return 0;
+    cx_attn_batch b = *batch;
+    if (!b.q_start || b.max_q_len < 1) b.max_q_len = 1;
+    return cx::attend_workspace(pool, &b, true);
+}
+
+int cx_paged_attend_tree_kind(const cx_pool* pool, const cx_attn_batch* batch, int32_t q_dtype) {
+    if (!pool || !batch || pool->n_kv_heads <= 0) return CX_KERNEL_GENERIC;
+    cx_attn_batch b = *batch;
+    if (!b.q_start || b.max_q_len < 1) b.max_q_len = 1;
+    return cx::attend_kind(pool, &b, q_dtype, true, true);
+}
+
 }  // extern "C"

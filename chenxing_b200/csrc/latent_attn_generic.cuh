@@ -1,11 +1,13 @@
 // Attention over a latent cache on CUDA cores, fp32 throughout: fp32 pools, block
 // sizes other than 16, 32 and 64, rows that TMA cannot load.
 //
-// A warp takes every fourth key of its CTA's part of the context and holds 4 packed
-// rows' queries and outputs in registers, one element in 32 a lane: a key's row is
-// read once, from global memory, and serves the score and the output.  Four dot
-// products are summed over the lanes with 6 + 4 shuffles.  The four warps, and the
-// parts of a context that is split over CTAs, are joined by their maxima.
+// A warp takes 2 or 4 neighbouring keys of its CTA's part of the context at a time and
+// holds 4 packed rows' queries and outputs in registers, one element in 32 a lane: a
+// key's row is read once, from global memory, and serves the score and the output.  Four
+// dot products are summed over the lanes with 6 + 4 shuffles.  The four warps, and
+// the parts of a context that is split over CTAs, are joined by their maxima.
+// 4 sequences of up to 1,024 fp32 keys of 128 + 32, 8 heads: one key at a time 29 us and
+// 27 to join its parts, GENERIC us with four and the parts' references side by side.
 #pragma once
 
 #include "latent_attn_tc.cuh"
@@ -117,53 +119,72 @@ __global__ void __launch_bounds__(kLgWarps * 32) latent_generic_kernel(const Lat
         return pool + ((g.layer64 * g.n_blocks64 + id) * p.block_size + (k - blk * p.block_size)) *
                           p.dim;
     };
-    for (int k = k_lo + warp; k < k_hi; k += kLgWarps) {
-        bool sees[kLgRows], any = false;
+    constexpr int NK = KE <= 10 ? 4 : 2;
+    for (int k0 = k_lo + warp * NK; k0 < k_hi; k0 += kLgWarps * NK) {
+        unsigned sees[NK];                        // bit r: row r sees the key
+        const KT* src[NK];
+        float x[NK][KE];
 #pragma unroll
-        for (int r = 0; r < kLgRows; ++r) {
-            sees[r] = k >= lo[r] && k <= up[r];
-            if (p.tree.masks && k >= base && k <= last[r]) {
-                const int t = (r0 + r) / p.heads;
-                sees[r] = tree_bits(p.tree, qs + t, t, k - base) & 1u;
+        for (int j = 0; j < NK; ++j) {
+            const int k = k0 + j;
+            sees[j] = 0;
+#pragma unroll
+            for (int r = 0; r < kLgRows; ++r) {
+                bool see = k >= lo[r] && k <= up[r];
+                if (p.tree.masks && k >= base && k <= last[r]) {
+                    const int t = (r0 + r) / p.heads;
+                    see = tree_bits(p.tree, qs + t, t, k - base) & 1u;
+                }
+                if (k < k_hi && see) sees[j] |= 1u << r;
             }
-            any |= sees[r];
+            src[j] = sees[j] ? row_of(k) : nullptr;
+            if (!src[j]) sees[j] = 0;
         }
-        if (!any) continue;
-        const KT* src = row_of(k);
-        if (!src) continue;
-        float x[KE];
 #pragma unroll
-        for (int e = 0; e < KE; ++e) {
-            const int d = lane + 32 * e;
-            x[e] = d < p.dim ? Conv<KT>::to_f(src[d]) : 0.f;
-        }
-        float s[kLgRows];
+        for (int j = 0; j < NK; ++j)
 #pragma unroll
-        for (int r = 0; r < kLgRows; ++r) {
-            float a0 = 0.f, a1 = 0.f;
-#pragma unroll
-            for (int e = 0; e < KE; e += 2) {
-                a0 = fmaf(q[r][e], x[e], a0);
-                if (e + 1 < KE) a1 = fmaf(q[r][e + 1], x[e + 1], a1);
+            for (int e = 0; e < KE; ++e) {
+                const int d = lane + 32 * e;
+                x[j][e] = sees[j] && d < p.dim ? Conv<KT>::to_f(src[j][d]) : 0.f;
             }
-            s[r] = a0 + a1;
+        float s[NK][kLgRows];
+#pragma unroll
+        for (int j = 0; j < NK; ++j) {
+#pragma unroll
+            for (int r = 0; r < kLgRows; ++r) {
+                float a0 = 0.f, a1 = 0.f;
+#pragma unroll
+                for (int e = 0; e < KE; e += 2) {
+                    a0 = fmaf(q[r][e], x[j][e], a0);
+                    if (e + 1 < KE) a1 = fmaf(q[r][e + 1], x[j][e + 1], a1);
+                }
+                s[j][r] = a0 + a1;
+            }
+            warp_sum4(s[j], lane);
         }
-        warp_sum4(s, lane);
 #pragma unroll
         for (int r = 0; r < kLgRows; ++r) {
-            if (!sees[r]) continue;               // adds nothing, whatever it holds
-            const float z = s[r] * g.scale;
-            if (z > m[r]) {
-                const float f = expf(m[r] - z);
-                m[r] = z;
+            float top = m[r];
+#pragma unroll
+            for (int j = 0; j < NK; ++j) {
+                s[j][r] *= g.scale;
+                if ((sees[j] >> r) & 1u) top = fmaxf(top, s[j][r]);
+            }
+            if (top > m[r]) {
+                const float f = expf(m[r] - top);
+                m[r] = top;
                 l[r] *= f;
 #pragma unroll
                 for (int e = 0; e < KE; ++e) o[r][e] *= f;
             }
-            const float w = expf(z - m[r]);
-            l[r] += w;
 #pragma unroll
-            for (int e = 0; e < KE; ++e) o[r][e] = fmaf(w, x[e], o[r][e]);
+            for (int j = 0; j < NK; ++j) {
+                if (!((sees[j] >> r) & 1u)) continue;     // adds nothing, whatever it holds
+                const float w = expf(s[j][r] - top);
+                l[r] += w;
+#pragma unroll
+                for (int e = 0; e < KE; ++e) o[r][e] = fmaf(w, x[j][e], o[r][e]);
+            }
         }
     }
     // ---- the four warps' states, then the output or this CTA's part ----
@@ -207,25 +228,36 @@ __global__ void __launch_bounds__(kLgWarps * 32) latent_generic_kernel(const Lat
     }
 }
 
-// Joins the parts of a context that was split: one CTA per 4 rows.
+// Joins the parts of a context that was split: one CTA per row.  Lanes fetch the parts'
+// references side by side; there are at most 256.
 __global__ void __launch_bounds__(128) latent_generic_join(const LatGenParams g) {
     const LatParams& p = g.a;
     const int unit = (int)blockIdx.x, b = unit / g.row_tiles, rt = unit - b * g.row_tiles;
+    const int r = blockIdx.y, lane = threadIdx.x & 31;
     const int qs = p.q_start ? p.q_start[b] : b;
     const int T = p.q_start ? min(max(p.q_start[b + 1] - qs, 0), p.max_q) : 1;
-    const int r0 = rt * kLgRows, nr = min(kLgRows, T * p.heads - r0);
+    const int r0 = rt * kLgRows;
+    if (r0 + r >= T * p.heads) return;
     const int mrow = p.dc + 2;
-    for (int e = threadIdx.x; e < nr * p.dc; e += blockDim.x) {
-        const int r = e / p.dc, d = e - r * p.dc;
-        const float* src = g.part + ((int64_t)unit * g.n_split * kLgRows + r) * mrow;
-        const int64_t step = (int64_t)kLgRows * mrow;
-        float M = -INFINITY, L = 0.f, O = 0.f;
-        for (int s = 0; s < g.n_split; ++s) M = fmaxf(M, src[s * step + p.dc]);
-        for (int s = 0; M != -INFINITY && s < g.n_split; ++s) {
-            const float f = expf(src[s * step + p.dc] - M);
-            L = fmaf(src[s * step + p.dc + 1], f, L);
-            O = fmaf(src[s * step + d], f, O);
-        }
+    const float* src = g.part + ((int64_t)unit * g.n_split * kLgRows + r) * mrow;
+    const int64_t step = (int64_t)kLgRows * mrow;
+    __shared__ float s_f[256];
+    float M = -INFINITY, L = 0.f;
+    for (int s = lane; s < g.n_split; s += 32) M = fmaxf(M, src[s * step + p.dc]);
+#pragma unroll
+    for (int w = 16; w; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
+    for (int s = lane; s < g.n_split; s += 32) {
+        const float f = M == -INFINITY ? 0.f : expf(src[s * step + p.dc] - M);
+        L = fmaf(src[s * step + p.dc + 1], f, L);
+        if (threadIdx.x < 32) s_f[s] = f;
+    }
+#pragma unroll
+    for (int w = 16; w; w >>= 1) L += __shfl_xor_sync(0xffffffffu, L, w);
+    __syncthreads();
+    for (int d = threadIdx.x; d < p.dc; d += 128) {
+        float O = 0.f;
+#pragma unroll 8
+        for (int s = 0; s < g.n_split; ++s) O = fmaf(src[s * step + d], s_f[s], O);
         store_as(p.out, p.out_dtype, ((int64_t)qs * p.heads + r0 + r) * p.dc + d,
                  L > 0.f ? O / L : 0.f);
     }
@@ -245,7 +277,7 @@ static int launch_latent_generic(const LatGenParams& g, cudaStream_t st) {
         latent_generic_kernel<KT, 18><<<grid, kLgWarps * 32, smem, st>>>(g);
     int rc = check_launch("latent_generic_kernel");
     if (rc || g.n_split == 1) return rc;
-    latent_generic_join<<<(unsigned)units, 128, 0, st>>>(g);
+    latent_generic_join<<<dim3((unsigned)units, kLgRows), 128, 0, st>>>(g);
     return check_launch("latent_generic_join");
 }
 

@@ -284,102 +284,15 @@ __device__ __forceinline__ uint4 lat_q8(const LatParams& p, int64_t lat, int64_t
                       Half16<E>::pack(x[4], x[5]), Half16<E>::pack(x[6], x[7]));
 }
 
-// Upper word of a descriptor of 128-byte swizzled lines in groups of 8, 1024 bytes
-// apart (tc_sdesc); the lower one holds the address and the leading offset.
-constexpr uint32_t kLatDescHi = (1024u >> 4) | 1u << 14 | 2u << 29;
-
-__device__ __forceinline__ uint32_t lat_desc_lo(const void* p, uint32_t lbo) {
-    return ((smem_addr(p) >> 4) & 0x3FFFu) | (lbo >> 4) << 16;
-}
-
-// tcgen05.mma, tcgen05.commit and a TMA load by one elected thread of a warp that comes
-// here as a whole, with the same operands in every lane: only then do they stay in
-// uniform registers.  An MMA issued by a thread in a branch of its own took 180
-// cycles here whatever its shape (a tile of 52 of them 8,600), one whose thread is
-// chosen by a comparison 50, by elect.sync 25 to 49, which is what the tensor pipe
-// takes for it (64 keys: 25 / 26 / 33 cycles at 16 / 32 / 64 rows; 128 columns: 40 / 41
-// / 49).
-__device__ __forceinline__ void lat_mma(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo,
-                                        uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "elect.sync _|q, 0xffffffff;\n\t"
-        "mov.b64 a, {%1, %5};\n\t"
-        "mov.b64 b, {%2, %5};\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(kLatDescHi)
-        : "memory");
-}
-__device__ __forceinline__ void lat_commit(uint64_t* bar) {
-    asm volatile(
-        "{\n\t.reg .pred q;\n\t"
-        "elect.sync _|q, 0xffffffff;\n\t"
-        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
-            smem_addr(bar))
-        : "memory");
-}
-// Arrival of one elected thread that adds `bytes` to what the phase waits for.
-__device__ __forceinline__ void lat_expect(uint32_t bar, uint32_t bytes) {
-    asm volatile(
-        "{\n\t.reg .pred q;\n\t"
-        "elect.sync _|q, 0xffffffff;\n\t"
-        "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
-        "r"(bytes)
-        : "memory");
-}
-__device__ __forceinline__ void lat_tma(uint32_t dst, const void* tmap, uint32_t bar, int x, int y,
-                                         int z) {
-    asm volatile(
-        "{\n\t.reg .pred q;\n\t"
-        "elect.sync _|q, 0xffffffff;\n\t"
-        "@q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %4}], [%5];\n\t}" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(bar)
-        : "memory");
-}
 // The 256 bytes at `src` into L2 (a load whose value nobody waits for).
 __device__ __forceinline__ void lat_prefetch(const void* src) {
     asm volatile("{\n\t.reg .b32 x;\n\tld.global.L1::no_allocate.L2::256B.b32 x, [%0];\n\t}" ::"l"(src));
 }
-__device__ __forceinline__ uint32_t warp_uniform(uint32_t x) {
-    return __shfl_sync(0xffffffffu, x, 0);
-}
-
 // Asynchronous 16-byte copy to shared memory; zeros when `there` is not set.
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src),
                  "r"(there ? 16 : 0)
                  : "memory");
-}
-
-// A bounded wait of a whole warp on an mbarrier phase, and whether it completed.  A
-// try suspends for up to half a microsecond; `tries` of them, or *abort, end it.  (One
-// loop in one piece, which the warp leaves together: behind a loop that its threads
-// leave one by one, an MMA takes up to 370 cycles.)
-__device__ __forceinline__ bool lat_wait(uint64_t* bar, uint32_t parity, volatile int* abort,
-                                         uint32_t tries) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b32 n, a;\n\t"
-        "mov.b32 n, %4;\n\t"
-        "mov.b32 %0, 1;\n\t"
-        "TRY:\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 500;\n\t"
-        "@p bra DONE;\n\t"
-        "ld.volatile.shared.b32 a, [%3];\n\t"
-        "setp.ne.b32 p, a, 0;\n\t"
-        "@p bra FAIL;\n\t"
-        "sub.u32 n, n, 1;\n\t"
-        "setp.ne.b32 p, n, 0;\n\t"
-        "@p bra TRY;\n\t"
-        "FAIL:\n\t"
-        "mov.b32 %0, 0;\n\t"
-        "DONE:\n\t}"
-        : "=&r"(ok)
-        : "r"(smem_addr(bar)), "r"(parity), "r"(smem_addr(const_cast<int*>(abort))), "r"(tries)
-        : "memory");
-    return __all_sync(0xffffffffu, ok != 0);
 }
 
 template <typename E>
@@ -643,7 +556,7 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
                             lat_prefetch(row + o);
                     }
                 }
-                ok = lat_wait(&s_full[tile & 1], (tile >> 1) & 1, s_abort, p.tries);
+                ok = el_wait(&s_full[tile & 1], (tile >> 1) & 1, s_abort, p.tries);
                 tc_fence_after();
                 float v[NW / 2];
                 lat_ld_s<NW>(tmem + C::S_COL + (tile & 1) * N + wg * NW + lane_base, v);
@@ -719,7 +632,7 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
                     moved = bar_red_or(1, SMT, moved);
                     if (moved && i > 0) {
                         // O^T holds the tiles before this one
-                        ok = lat_wait(o_done, (tile - 1) & 1, s_abort, p.tries);
+                        ok = el_wait(o_done, (tile - 1) & 1, s_abort, p.tries);
                         if (!(ok = bar_red_and(1, SMT, ok))) break;
                         tc_fence_after();
 #pragma unroll 1
@@ -749,7 +662,7 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
                 }
                 // ---- P^T over the last tile's, when O^T has read that ----
                 if (tile > 0)
-                    ok = lat_wait(o_done, (tile - 1) & 1, s_abort, p.tries);
+                    ok = el_wait(o_done, (tile - 1) & 1, s_abort, p.tries);
                 if (!ok) {
                     *s_abort = 1;               // the next vote ends the loop for all
                     continue;
@@ -807,7 +720,7 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
                     y += __shfl_xor_sync(0xffffffffu, y, 16);
                     if (lane < 4) s_red[quad * 64 + col0 + 8 * j + e] = y;
                 }
-            ok = lat_wait(o_done, (tile - 1) & 1, s_abort, p.tries);
+            ok = el_wait(o_done, (tile - 1) & 1, s_abort, p.tries);
             if (!(ok = bar_red_and(1, SMT, ok))) break;
             tc_fence_after();
             const int64_t part = ((int64_t)blockIdx.x * 2 + slot) * N;
@@ -933,21 +846,21 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
                     // the pieces that O^T does not read are free first
                     const int q = j + NM < NP ? j + NM : j + NM - NP, ch = 2 * q + w0;
                     if (use > 0) {
-                        go = lat_wait(&empty[s * kLatMaxPieces + q], (use - 1) & 1, s_abort,
+                        go = el_wait(&empty[s * kLatMaxPieces + q], (use - 1) & 1, s_abort,
                                       p.tries);
                         if (!go) break;
                     }
                     const uint32_t bar = bar0 + q * 8, dst = dst0 + ch * kLatChunk;
-                    lat_expect(bar, ch < NCH ? kLatChunk : 0);
+                    el_expect(bar, ch < NCH ? kLatChunk : 0);
                     if (ch >= NCH) continue;
                     // (a condition at every box would triple what they take)
                     if (nb == 4) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            lat_tma(dst + k * 2048, &tm, bar, ch * 64, row4[k], z4[k]);
+                            el_tma(dst + k * 2048, &tm, bar, ch * 64, row4[k], z4[k]);
                     } else {
                         for (int k = 0; k < nb; ++k)
-                            lat_tma(dst + k * br * 128, &tm, bar, ch * 64,
+                            el_tma(dst + k * br * 128, &tm, bar, ch * 64,
                                     __shfl_sync(0xffffffffu, row, k),
                                     __shfl_sync(0xffffffffu, z, k));
                     }
@@ -965,13 +878,13 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
         // ---------------- MMA issuers: whole warps, one thread's instructions ----------------
         const bool is_s = warp == SW;
         const uint32_t tm = warp_uniform(tmem);
-        const uint32_t c_lo = warp_uniform(lat_desc_lo(s_c, kLatChunk));
-        const uint32_t b_lo = warp_uniform(lat_desc_lo(is_s ? s_q : s_p, 16));
+        const uint32_t c_lo = warp_uniform(el_desc_lo(s_c, kLatChunk));
+        const uint32_t b_lo = warp_uniform(el_desc_lo(is_s ? s_q : s_p, 16));
         bool ok = true;
         int st = 0;                               // stage of the next tile
         uint32_t use = 0;                         // parity of its fill
         for (int range = 0;; ++range) {
-            ok = lat_wait(q_full, range & 1, s_abort, p.tries);
+            ok = el_wait(q_full, range & 1, s_abort, p.tries);
             const int n = (int)warp_uniform(s_n[range & 1]);
             if (!ok || n == 0) break;
             for (int i = 0; ok && i < n; ++i, ++tile) {
@@ -982,10 +895,10 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
                     const uint32_t d = warp_uniform(tm + C::S_COL + b * N);
                     // S^T of two tiles before was read
                     if (tile >= 2)
-                        ok = lat_wait(&p_full[b], ((tile >> 1) - 1) & 1, s_abort, p.tries);
+                        ok = el_wait(&p_full[b], ((tile >> 1) - 1) & 1, s_abort, p.tries);
                     for (int j = 0; ok && j < NP; ++j) {
                         const int q = j + NM < NP ? j + NM : j + NM - NP;
-                        ok = lat_wait(&full[st * kLatMaxPieces + q], use, s_abort,
+                        ok = el_wait(&full[st * kLatMaxPieces + q], use, s_abort,
                                                    p.tries);
                         if (!ok) break;
                         tc_fence_after();
@@ -996,7 +909,7 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
                         auto steps = [&](auto k_end) {
 #pragma unroll
                             for (int k = 0; k < decltype(k_end)::value; ++k)
-                                lat_mma(d, ad + (((k >> 2) * kLatChunk + (k & 3) * 32) >> 4),
+                                el_mma(d, ad + (((k >> 2) * kLatChunk + (k & 3) * 32) >> 4),
                                         qd + (((k >> 2) * C::Q_CHUNK + (k & 3) * 32) >> 4), idesc,
                                         k > 0 ? 1u : acc);
                         };
@@ -1004,12 +917,12 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
                             steps(std::integral_constant<int, 8>{});
                         else
                             steps(std::integral_constant<int, 4>{});
-                        if (q >= NM) lat_commit(&empty[st * kLatMaxPieces + q]);
+                        if (q >= NM) el_commit(&empty[st * kLatMaxPieces + q]);
                     }
-                    if (ok) lat_commit(&s_full[b]);
+                    if (ok) el_commit(&s_full[b]);
                 } else {
                     constexpr uint32_t idesc = lat_idesc<E>(128, N, 1, 1);
-                    ok = lat_wait(&p_full[tile & 1], (tile >> 1) & 1, s_abort,
+                    ok = el_wait(&p_full[tile & 1], (tile >> 1) & 1, s_abort,
                                                p.tries);
                     if (!ok) break;
                     tc_fence_after();
@@ -1019,12 +932,12 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
                         for (int mm = 0; mm < decltype(nm)::value; ++mm) {
 #pragma unroll
                             for (int kk = 0; kk < kLatKeys / 16; ++kk)
-                                lat_mma(tm + mm * N, cd + ((mm * 2 * kLatChunk + kk * 2048) >> 4),
+                                el_mma(tm + mm * N, cd + ((mm * 2 * kLatChunk + kk * 2048) >> 4),
                                         b_lo + kk * (2048 >> 4), idesc, kk > 0 ? 1u : acc);
-                            lat_commit(&empty[st * kLatMaxPieces + mm]);
+                            el_commit(&empty[st * kLatMaxPieces + mm]);
                         }
                     });
-                    lat_commit(o_done);
+                    el_commit(o_done);
                 }
                 if (++st == ST) {
                     st = 0;
@@ -1037,7 +950,7 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
             *s_abort = 1;
             raise_flag(CX_DEV_WAIT_TIMEOUT);
         }
-        lat_commit(&drain[is_s ? 0 : 1]);         // completes once this warp's MMAs have
+        el_commit(&drain[is_s ? 0 : 1]);         // completes once this warp's MMAs have
     }
 
     // ---- teardown: drain this CTA's own copies and MMAs, then free TMEM ----

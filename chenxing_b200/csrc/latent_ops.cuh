@@ -97,15 +97,9 @@ __global__ void __launch_bounds__(288) latent_append_vec_kernel(const LatAppendP
     const int64_t t = blockIdx.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
     const int units = p.dr / 16;                      // units of 8 pairs a head
-    int64_t pos = 0;
     const bool turn = p.positions != nullptr;
-    if (turn) {
-        pos = p.positions[t];
-        if (pos < 0 || pos >= p.table_rows) {
-            if (threadIdx.x == 0) raise_flag(CX_DEV_BAD_POSITION);
-            return;
-        }
-    }
+    const int64_t pos = turn ? p.positions[t] : 0;
+    const bool in_table = !turn || (pos >= 0 && pos < p.table_rows);
     const int half = p.dr / 2;
     // first elements of unit u's two runs of 8
     auto run_a = [&](int u) { return p.interleaved ? 16 * u : 8 * u; };
@@ -114,23 +108,35 @@ __global__ void __launch_bounds__(288) latent_append_vec_kernel(const LatAppendP
     auto angles = [&](int u, RopePair (&r)[8]) {
         const float* c = p.cos_table + pos * p.dr + 8 * u;
         const float* s = p.sin_table + pos * p.dr + 8 * u;
+        float t[4][8];
+        auto eight = [&](const float* src, float (&x)[8]) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(src));
+            const float4 b = __ldg(reinterpret_cast<const float4*>(src) + 1);
+            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+            x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+        };
+        eight(c, t[0]);
+        eight(s, t[1]);
         const int o = p.interleaved ? 0 : half;
+        eight(c + o, t[2]);
+        eight(s + o, t[3]);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            r[k] = {__ldg(c + k), __ldg(s + k), __ldg(c + o + k), __ldg(s + o + k)};
+        for (int k = 0; k < 8; ++k) r[k] = {t[0][k], t[1][k], t[2][k], t[3][k]};
     };
     auto rotate = [&](const RopePair (&r)[8], float (&a)[8], float (&b)[8]) {
+        if (p.interleaved) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            if (p.interleaved) {
-                float* v = k < 4 ? a + 2 * k : b + 2 * (k - 4);
-                r[k].turn(v[0], v[1]);
-            } else {
-                r[k].turn(a[k], b[k]);
+            for (int k = 0; k < 4; ++k) {
+                r[k].turn(a[2 * k], a[2 * k + 1]);
+                r[k + 4].turn(b[2 * k], b[2 * k + 1]);
             }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) r[k].turn(a[k], b[k]);
         }
     };
-    if (warp == 0) {
+    if (!in_table && threadIdx.x == 0) raise_flag(CX_DEV_BAD_POSITION);
+    if (warp == 0 && in_table) {
         int64_t row;
         if (lat_slot(p, t, row)) {
             const int64_t dst = row * (p.dc + p.dr), src = t * p.latent_tok;
@@ -179,18 +185,24 @@ __global__ void __launch_bounds__(288) latent_append_vec_kernel(const LatAppendP
         }
         if (n_warps > 1) return;
     }
-    if (!p.q) return;
+    if (!p.q || (warp == 0 && n_warps > 1)) return;
     // units of the queries: 32 % units == 0, so that a lane keeps one unit's angles
     const int w0 = n_warps > 1 ? warp - 1 : 0, nw = n_warps > 1 ? n_warps - 1 : 1;
     const int u = lane % units, per_warp = 32 / units;
     RopePair r[8];
-    if (turn) angles(u, r);
+    bool first = true;
     for (int h = w0 * per_warp + lane / units; h < p.heads; h += nw * per_warp) {
         float a[8], b[8];
         const int64_t src = t * p.q_tok + h * p.q_head, dst = (t * p.heads + h) * p.dr;
         load8_as(p.q, p.dtype, src + run_a(u), a);
         load8_as(p.q, p.dtype, src + run_b(u), b);
-        if (turn) rotate(r, a, b);
+        // (the first queries are asked for before the position is waited for)
+        if (!in_table) return;
+        if (turn) {
+            if (first) angles(u, r);
+            first = false;
+            rotate(r, a, b);
+        }
         store8_as(p.q_out, p.q_out_dtype, dst + run_a(u), a);
         store8_as(p.q_out, p.q_out_dtype, dst + run_b(u), b);
     }
@@ -314,16 +326,21 @@ struct AcceptParams {
     int32_t block_size, heads, row_words, planes;   // planes: layers * pools * heads
 };
 
-// A thread owns one word (V) of a plane's rows (plane: layer, pool, head) of one
-// sequence and moves it for every node in order, 8 at a time: a path ascends, so
-// that its k-th node is at or behind position k, and what a group of 8 overwrites
-// no later one reads.  No two threads share a word, so that rows which are both
-// a source and a destination need no synchronisation.
+// A thread owns words (V) of the planes' rows (plane: layer, pool, head) of one sequence
+// and moves each for every node in order, 8 at a time: a path ascends, so that its k-th
+// node is at or behind position k, and what a group of 8 overwrites no later one
+// reads.  No two threads share a word, so that rows which are both a source and a
+// destination need no synchronisation.  Rows of 256 bytes are read where they lie: 64
+// sequences x 5 nodes x 24 layers of 8 heads of 128, 28 MB, ACCEPT us.
 template <typename V>
 __global__ void __launch_bounds__(256) accept_kernel(const AcceptParams p) {
     const int b = blockIdx.y;
     __shared__ int64_t s_from[32], s_to[32];
     __shared__ int s_n, s_more;
+    const int lane = threadIdx.x & 31;
+    const int32_t* path = p.paths + b * p.path_stride;
+    const int32_t* tab = p.tables + b * p.table_stride;
+    int n = lane < p.path_len ? path[lane] : -1;      // (beside the lengths, not behind them)
     const int q0 = p.q_start ? p.q_start[b] : b, T = p.q_start ? p.q_start[b + 1] - q0 : 1;
     const int64_t ctx = p.ctx_lens[b], cap = p.table_stride * p.block_size, base = ctx - T;
     if (T <= 0) return;
@@ -331,21 +348,16 @@ __global__ void __launch_bounds__(256) accept_kernel(const AcceptParams p) {
         if (threadIdx.x == 0 && blockIdx.x == 0) raise_flag(CX_DEV_BAD_QLEN);
         return;
     }
-    const int64_t w = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int plane = (int)(w / p.row_words), word = (int)(w - (int64_t)plane * p.row_words);
-    const bool mine = plane < p.planes;
-    const int h = plane % p.heads, pl = (plane / p.heads) % p.n_pools,
-              layer = plane / (p.heads * p.n_pools);
-    V* mem = mine ? static_cast<V*>(p.pool[pl]) + layer * p.layer_words : nullptr;
-    // word offset of position 0 of this plane's head, in a block
-    const int64_t head0 = (int64_t)h * p.block_size * p.row_words + word;
-    const int32_t* tab = p.tables + b * p.table_stride;
+    const int64_t words = (int64_t)p.planes * p.row_words;
+    int before = -1;                                  // the last node of the 32 before
     for (int64_t k0 = 0; k0 < p.path_len; k0 += 32) {
         if (threadIdx.x < 32) {
-            const int64_t k = k0 + threadIdx.x;
-            const int32_t* path = p.paths + b * p.path_stride;
-            const int n = k < p.path_len ? path[k] : -1, before = k > 0 ? path[min(k, p.path_len) - 1] : -1;
-            bool good = n >= 0 && n < T && n > before && (k == 0 || before >= 0);
+            const int64_t k = k0 + lane;
+            if (k0 > 0) n = k < p.path_len ? path[k] : -1;
+            int prev = __shfl_up_sync(0xffffffffu, n, 1);
+            if (lane == 0) prev = before;
+            before = __shfl_sync(0xffffffffu, n, 31);
+            bool good = n >= 0 && n < T && n > prev && (k == 0 || prev >= 0);
             int64_t from = 0, to = 0;
             if (good) {
                 const int64_t f = base + n, t = base + k;
@@ -360,26 +372,33 @@ __global__ void __launch_bounds__(256) accept_kernel(const AcceptParams p) {
             } else if (n >= 0 && blockIdx.x == 0) {
                 raise_flag(CX_DEV_BAD_PATH);
             }
-            s_from[threadIdx.x] = from;
-            s_to[threadIdx.x] = to;
+            s_from[lane] = from;
+            s_to[lane] = to;
             const unsigned all = __ballot_sync(0xffffffffu, good);
-            if (threadIdx.x == 0) {
+            if (lane == 0) {
                 s_n = all == 0xffffffffu ? 32 : __ffs((int)~all) - 1;   // up to the first that is not
                 s_more = all == 0xffffffffu;
             }
         }
         __syncthreads();
-        const int n = s_n;
-        for (int i0 = 0; mine && i0 < n; i0 += 8) {
-            V x[8];
+        const int count = s_n;
+        for (int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x; w < words;
+             w += (int64_t)gridDim.x * 256) {
+            const int plane = (int)(w / p.row_words), word = (int)(w - (int64_t)plane * p.row_words);
+            const int h = plane % p.heads, pl = (plane / p.heads) % p.n_pools,
+                      layer = plane / (p.heads * p.n_pools);
+            // word offset of position 0 of this plane's head, in a block
+            V* mem = static_cast<V*>(pl ? p.pool[1] : p.pool[0]) + layer * p.layer_words +
+                     (int64_t)h * p.block_size * p.row_words + word;
+            for (int i0 = 0; i0 < count; i0 += 8) {
+                V x[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i0 + i < n && s_from[i0 + i] != s_to[i0 + i])
-                    x[i] = mem[s_from[i0 + i] + head0];
+                for (int i = 0; i < 8; ++i)
+                    if (i0 + i < count && s_from[i0 + i] != s_to[i0 + i]) x[i] = mem[s_from[i0 + i]];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i0 + i < n && s_from[i0 + i] != s_to[i0 + i])
-                    mem[s_to[i0 + i] + head0] = x[i];
+                for (int i = 0; i < 8; ++i)
+                    if (i0 + i < count && s_from[i0 + i] != s_to[i0 + i]) mem[s_to[i0 + i]] = x[i];
+            }
         }
         if (!s_more) return;
         __syncthreads();
@@ -476,6 +495,7 @@ static int latent_append(const cx_latent_pool* pool, int64_t layer, const cx_lat
     const int units = p.dr / 16;
     auto al = [](const void* x) { return reinterpret_cast<uintptr_t>(x); };
     const uintptr_t bytes = al(p.latent) | al(p.rope) | al(p.pool) | al(weight) |
+                            (positions ? al(p.cos_table) | al(p.sin_table) : 0) |
                             (uintptr_t)(p.latent_tok * src) | (uintptr_t)(p.rope_tok * src) |
                             (has_q ? al(p.q) | al(q_out) | (uintptr_t)(p.q_tok * src) |
                                          (uintptr_t)(p.q_head * src)
@@ -499,7 +519,9 @@ static int accept_paths(AcceptParams p, int64_t batch, int64_t row_bytes, int64_
     p.row_words = (int)(row_bytes / v);
     p.layer_words = p.n_blocks * p.heads * p.block_size * p.row_words;
     const int64_t planes = layers * p.n_pools * p.heads;
-    const int64_t blocks = (planes * p.row_words + 255) / 256;
+    // (about eight CTAs an SM in all)
+    const int64_t most = (planes * p.row_words + 255) / 256, fair = 8ll * num_sms() / batch;
+    const int64_t blocks = std::max<int64_t>(1, std::min(most, fair));
     if (planes > INT32_MAX || blocks > INT32_MAX || batch > 65535)
         return fail(CX_ERR_UNSUPPORTED, "accepted paths: pool or batch too large");
     p.planes = (int)planes;

@@ -341,11 +341,15 @@ typedef struct cx_tree {
 
 /* cx_paged_attend for drafted trees (batch->q_start given): committed keys are
  * seen as there (a prefix ends at base), drafted keys by the masks.  Everything
- * else, workspace and plan included, is cx_paged_attend's. */
+ * else is cx_paged_attend's, but for the workspace's size and the kernel of a shape
+ * (cx_paged_attend_tree_workspace_bytes, cx_paged_attend_tree_kind); a plan made by
+ * one does not serve the other. */
 int cx_paged_attend_tree(const cx_pool* pool, int64_t layer, const cx_attn_batch* batch,
                          const cx_attn_mods* mods, const cx_tree* tree, const void* q,
                          int32_t q_dtype, void* out, void* workspace, size_t workspace_bytes,
                          int32_t replan, void* stream);
+size_t cx_paged_attend_tree_workspace_bytes(const cx_pool* pool, const cx_attn_batch* batch);
+int cx_paged_attend_tree_kind(const cx_pool* pool, const cx_attn_batch* batch, int32_t q_dtype);
 
 /* After verification: the K and V of the accepted nodes, in every layer, move to
  * the positions behind the committed context: of sequence b, node

@@ -44,20 +44,25 @@ SHAPES = [
     # fp32, mma.sync and generic kernels
     (8, 2, 64, F32, [1, 8, 5, 0, 13], [1, 8, 300, 40, 77]),
     (4, 4, 128, F32, [16, 3], [16, 700]),
-    (8, 2, 128, BF, [1, 13, 15, 0, 6], [1, 13, 290, 16, 95]),
-    (8, 8, 64, F16, [60, 7, 33], [60, 500, 49]),
-    (6, 2, 128, BF, [20, 9], [200, 64]),
-    (4, 1, 64, BF, [15, 2], [1030, 2]),
+    (8, 2, 128, BF, [1, 8, 5, 0, 6], [1, 8, 290, 16, 95]),
+    (8, 8, 64, F16, [32, 7, 20], [32, 500, 49]),
+    (6, 2, 128, BF, [10, 9], [200, 64]),
+    (4, 1, 64, BF, [4, 2], [1030, 2]),
     (4, 2, 80, BF, [9, 21], [50, 300]),
     (6, 3, 40, F32, [12, 1], [100, 17]),
     (8, 2, 64, F32, [40, 20], [100, 317]),
-    # tcgen05
+    # tcgen05: one query tile in two places
     (8, 2, 128, BF, [26, 10, 1, 0, 17], [26, 600, 129, 16, 140]),
     (32, 8, 128, BF, [26, 12], [1000, 127]),
+    (8, 8, 64, F16, [60, 7, 33], [60, 500, 49]),
+    (4, 1, 64, BF, [15, 9], [1030, 9]),
+    (12, 4, 128, F16, [11, 40, 3], [128, 385, 257]),
+    # and two, or their keys over many CTAs
     (4, 4, 64, F16, [130, 64, 200], [130, 500, 333]),
     (14, 2, 64, BF, [40, 19], [300, 19]),
     (6, 2, 128, F16, [90, 43], [211, 43]),
-    (5, 1, 128, F16, [30, 13], [4000, 40]),         # its keys over many CTAs
+    (5, 1, 128, F16, [30, 13], [4000, 40]),
+    (2, 1, 128, BF, [30], [9000]),
 ]
 
 
@@ -75,10 +80,11 @@ def test_kernels_of_the_shapes():
         kinds.append(_case("plain", "star", hq, sizes, ctx, hk=hk, d=d, dtype=dtype)
                      .batch().kernel_kind(dtype, dtype))
     assert kinds == ["fma", "fma", "mma", "mma", "mma", "mma", "generic", "generic", "generic"] \
-        + ["tcgen05"] * 6
+        + ["tcgen05"] * 10
 
 
-@pytest.mark.parametrize("hq,hk,d,dtype,n", [(8, 2, 128, BF, 13), (8, 2, 128, BF, 40),
+@pytest.mark.parametrize("hq,hk,d,dtype,n", [(8, 2, 128, BF, 7), (8, 2, 128, BF, 13),
+                                             (8, 2, 128, BF, 40),
                                              (8, 2, 64, F32, 8), (4, 2, 96, F16, 8)])
 def test_a_chain_is_what_verify_gives(hq, hk, d, dtype, n):
     """A tree without branches has the bits of the chain's verification."""
