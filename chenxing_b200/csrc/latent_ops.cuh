@@ -33,24 +33,31 @@ __device__ __forceinline__ float load_as(const void* p, int32_t dtype, int64_t i
                               : __half2float(static_cast<const __half*>(p)[i]);
 }
 
-// 8 elements (16-byte aligned where they start) of a run-time type.
-__device__ __forceinline__ void load8_as(const void* p, int32_t dtype, int64_t i, float (&x)[8]) {
-    if (dtype == CX_F32) {
+// 8 elements, 16-byte aligned, as they lie in memory: asked for at once, looked at
+// when they are needed.
+template <typename E> struct Raw8 {
+    uint4 u;
+    __device__ __forceinline__ void load(const void* p, int64_t i) {
+        u = __ldg(reinterpret_cast<const uint4*>(static_cast<const E*>(p) + i));
+    }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f2_get(Half16<E>::unpack(w[k]), x[2 * k], x[2 * k + 1]);
+    }
+};
+template <> struct Raw8<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const void* p, int64_t i) {
         const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-        const float4 a = __ldg(s), b = __ldg(s + 1);
+        a = __ldg(s);
+        b = __ldg(s + 1);
+    }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
         x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
         x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-        return;
     }
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i));
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const f2 v = dtype == CX_BF16 ? Half16<__nv_bfloat16>::unpack(w[k])
-                                      : Half16<__half>::unpack(w[k]);
-        f2_get(v, x[2 * k], x[2 * k + 1]);
-    }
-}
+};
 
 __device__ __forceinline__ void store8_as(void* p, int32_t dtype, int64_t i, const float (&x)[8]) {
     if (dtype == CX_F32) {
@@ -92,65 +99,75 @@ __device__ __forceinline__ bool lat_slot(const LatAppendParams& p, int64_t t, in
 
 // One block per token.  Warp 0 has the pool row, the other warps 32 units of 8 pairs
 // of the queries each: with rows of 16-byte multiples a lane holds 8 pairs, whose
-// angles it loads once for all its heads.
-__global__ void __launch_bounds__(288) latent_append_vec_kernel(const LatAppendParams p) {
+// angles it loads once for all its heads.  All that a lane needs first (rows, slot,
+// position) is asked for before any of it is looked at; then come the angles and the
+// weights.  8,192 tokens, 32 heads, bf16, 90 MB: APPEND us; with loads that are
+// converted where they are made, one after the other, 47.
+template <typename E>
+__global__ void __launch_bounds__(288, 4) latent_append_vec_kernel(const LatAppendParams p) {
     const int64_t t = blockIdx.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
-    const int units = p.dr / 16;                      // units of 8 pairs a head
+    const int units = p.dr / 16, half = p.dr / 2;     // units of 8 pairs a head
     const bool turn = p.positions != nullptr;
     const int64_t pos = turn ? p.positions[t] : 0;
-    const bool in_table = !turn || (pos >= 0 && pos < p.table_rows);
-    const int half = p.dr / 2;
     // first elements of unit u's two runs of 8
     auto run_a = [&](int u) { return p.interleaved ? 16 * u : 8 * u; };
     auto run_b = [&](int u) { return p.interleaved ? 16 * u + 8 : half + 8 * u; };
-    // the angles of unit u (pair k: elements 2k, 2k + 1 of the 16, or k of either run)
-    auto angles = [&](int u, RopePair (&r)[8]) {
-        const float* c = p.cos_table + pos * p.dr + 8 * u;
-        const float* s = p.sin_table + pos * p.dr + 8 * u;
-        float t[4][8];
-        auto eight = [&](const float* src, float (&x)[8]) {
-            const float4 a = __ldg(reinterpret_cast<const float4*>(src));
-            const float4 b = __ldg(reinterpret_cast<const float4*>(src) + 1);
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-            x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-        };
-        eight(c, t[0]);
-        eight(s, t[1]);
-        const int o = p.interleaved ? 0 : half;
-        eight(c + o, t[2]);
-        eight(s + o, t[3]);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) r[k] = {t[0][k], t[1][k], t[2][k], t[3][k]};
-    };
-    auto rotate = [&](const RopePair (&r)[8], float (&a)[8], float (&b)[8]) {
+    // unit u's pairs turned: elements 2k, 2k + 1 of the 16, or k of either run
+    auto rotate = [&](int u, float (&a)[8], float (&b)[8]) {
+        const float4* c = reinterpret_cast<const float4*>(p.cos_table + pos * p.dr + 8 * u);
+        const float4* s = reinterpret_cast<const float4*>(p.sin_table + pos * p.dr + 8 * u);
         if (p.interleaved) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                r[k].turn(a[2 * k], a[2 * k + 1]);
-                r[k + 4].turn(b[2 * k], b[2 * k + 1]);
-            }
+            const float4 c0 = __ldg(c), c1 = __ldg(c + 1), s0 = __ldg(s), s1 = __ldg(s + 1);
+            RopePair{c0.x, s0.x, c0.x, s0.x}.turn(a[0], a[1]);
+            RopePair{c0.y, s0.y, c0.y, s0.y}.turn(a[2], a[3]);
+            RopePair{c0.z, s0.z, c0.z, s0.z}.turn(a[4], a[5]);
+            RopePair{c0.w, s0.w, c0.w, s0.w}.turn(a[6], a[7]);
+            RopePair{c1.x, s1.x, c1.x, s1.x}.turn(b[0], b[1]);
+            RopePair{c1.y, s1.y, c1.y, s1.y}.turn(b[2], b[3]);
+            RopePair{c1.z, s1.z, c1.z, s1.z}.turn(b[4], b[5]);
+            RopePair{c1.w, s1.w, c1.w, s1.w}.turn(b[6], b[7]);
         } else {
+            const int o = half / 4;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) r[k].turn(a[k], b[k]);
+            for (int k = 0; k < 2; ++k) {
+                const float4 cx = __ldg(c + k), sx = __ldg(s + k), cy = __ldg(c + o + k),
+                             sy = __ldg(s + o + k);
+                RopePair{cx.x, sx.x, cy.x, sy.x}.turn(a[4 * k], b[4 * k]);
+                RopePair{cx.y, sx.y, cy.y, sy.y}.turn(a[4 * k + 1], b[4 * k + 1]);
+                RopePair{cx.z, sx.z, cy.z, sy.z}.turn(a[4 * k + 2], b[4 * k + 2]);
+                RopePair{cx.w, sx.w, cy.w, sy.w}.turn(a[4 * k + 3], b[4 * k + 3]);
+            }
         }
     };
-    if (!in_table && threadIdx.x == 0) raise_flag(CX_DEV_BAD_POSITION);
-    if (warp == 0 && in_table) {
-        int64_t row;
-        if (lat_slot(p, t, row)) {
-            const int64_t dst = row * (p.dc + p.dr), src = t * p.latent_tok;
-            const int n8 = p.dc / 8;                  // up to 2 runs of 8 a lane held, more read twice
-            float x[2][8], sum = 0.f;
-            for (int i = lane, k = 0; i < n8; i += 32, ++k) {
-                float y[8];
-                load8_as(p.latent, p.dtype, src + i * 8, y);
+    const bool pool_row = warp == 0;
+    if (pool_row) {
+        const int64_t slot = p.slots[t], src = t * p.latent_tok;
+        const int n8 = p.dc / 8;                      // (dc <= 512: up to 2 runs of 8 a lane)
+        Raw8<E> lat[2], ra, rb;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    sum = fmaf(y[e], y[e], sum);
-                    if (k == 0) x[0][e] = y[e];
-                    if (k == 1) x[1][e] = y[e];
-                }
+        for (int k = 0; k < 2; ++k)
+            if (lane + 32 * k < n8) lat[k].load(p.latent, src + (lane + 32 * k) * 8);
+        if (lane < units) {
+            ra.load(p.rope, t * p.rope_tok + run_a(lane));
+            rb.load(p.rope, t * p.rope_tok + run_b(lane));
+        }
+        const bool in_table = !turn || (pos >= 0 && pos < p.table_rows);
+        if (lane == 0) {
+            if (!in_table)
+                raise_flag(CX_DEV_BAD_POSITION);
+            else if (slot >= p.n_slots)
+                raise_flag(CX_DEV_BAD_SLOT);
+        }
+        if (in_table && slot >= 0 && slot < p.n_slots) {
+            const int64_t dst = (p.layer_row0 + slot) * (p.dc + p.dr);
+            float x[2][8], sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                if (lane + 32 * k >= n8) continue;
+                lat[k].get(x[k]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum = fmaf(x[k][e], x[k][e], sum);
             }
             float f = 1.f;
             if (p.weight) {
@@ -158,51 +175,50 @@ __global__ void __launch_bounds__(288) latent_append_vec_kernel(const LatAppendP
                 for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
                 f = rsqrtf(sum / (float)p.dc + p.eps);
             }
-            for (int i = lane, k = 0; i < n8; i += 32, ++k) {
-                float y[8], w[8];
-                if (k >= 2) load8_as(p.latent, p.dtype, src + i * 8, y);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = k == 0 ? x[0][e] : k == 1 ? x[1][e] : y[e];
+            for (int k = 0; k < 2; ++k) {
+                const int i = (lane + 32 * k) * 8;
+                if (lane + 32 * k >= n8) continue;
                 if (p.weight) {
-                    load8_as(p.weight, p.weight_dtype, i * 8, w);
+                    float w[8];
+                    if (p.weight_dtype == CX_F32) {
+                        Raw8<float> r;
+                        r.load(p.weight, i);
+                        r.get(w);
+                    } else {
+                        Raw8<E> r;
+                        r.load(p.weight, i);
+                        r.get(w);
+                    }
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = y[e] * f * w[e];
+                    for (int e = 0; e < 8; ++e) x[k][e] = x[k][e] * f * w[e];
                 }
-                store8_as(p.pool, p.pool_dtype, dst + i * 8, y);
+                store8_as(p.pool, p.pool_dtype, dst + i, x[k]);
             }
             if (lane < units) {
                 float a[8], b[8];
-                load8_as(p.rope, p.dtype, t * p.rope_tok + run_a(lane), a);
-                load8_as(p.rope, p.dtype, t * p.rope_tok + run_b(lane), b);
-                if (turn) {
-                    RopePair r[8];
-                    angles(lane, r);
-                    rotate(r, a, b);
-                }
+                ra.get(a);
+                rb.get(b);
+                if (turn) rotate(lane, a, b);
                 store8_as(p.pool, p.pool_dtype, dst + p.dc + run_a(lane), a);
                 store8_as(p.pool, p.pool_dtype, dst + p.dc + run_b(lane), b);
             }
         }
-        if (n_warps > 1) return;
     }
-    if (!p.q || (warp == 0 && n_warps > 1)) return;
+    if (!p.q || (pool_row && n_warps > 1)) return;
     // units of the queries: 32 % units == 0, so that a lane keeps one unit's angles
     const int w0 = n_warps > 1 ? warp - 1 : 0, nw = n_warps > 1 ? n_warps - 1 : 1;
     const int u = lane % units, per_warp = 32 / units;
-    RopePair r[8];
-    bool first = true;
     for (int h = w0 * per_warp + lane / units; h < p.heads; h += nw * per_warp) {
+        Raw8<E> ra, rb;
         float a[8], b[8];
         const int64_t src = t * p.q_tok + h * p.q_head, dst = (t * p.heads + h) * p.dr;
-        load8_as(p.q, p.dtype, src + run_a(u), a);
-        load8_as(p.q, p.dtype, src + run_b(u), b);
-        // (the first queries are asked for before the position is waited for)
-        if (!in_table) return;
-        if (turn) {
-            if (first) angles(u, r);
-            first = false;
-            rotate(r, a, b);
-        }
+        ra.load(p.q, src + run_a(u));
+        rb.load(p.q, src + run_b(u));
+        if (turn && (pos < 0 || pos >= p.table_rows)) return;
+        ra.get(a);
+        rb.get(b);
+        if (turn) rotate(u, a, b);
         store8_as(p.q_out, p.q_out_dtype, dst + run_a(u), a);
         store8_as(p.q_out, p.q_out_dtype, dst + run_b(u), b);
     }
@@ -505,7 +521,13 @@ static int latent_append(const cx_latent_pool* pool, int64_t layer, const cx_lat
         const int per_warp = 32 / units;
         int warps = has_q ? 1 + (p.heads + per_warp - 1) / per_warp : 1;
         if (warps > 9) warps = 9;
-        latent_append_vec_kernel<<<(unsigned)p.n_tokens, warps * 32, 0, st>>>(p);
+        const unsigned n = (unsigned)p.n_tokens;
+        if (p.dtype == CX_F32)
+            latent_append_vec_kernel<float><<<n, warps * 32, 0, st>>>(p);
+        else if (p.dtype == CX_BF16)
+            latent_append_vec_kernel<__nv_bfloat16><<<n, warps * 32, 0, st>>>(p);
+        else
+            latent_append_vec_kernel<__half><<<n, warps * 32, 0, st>>>(p);
         return check_launch("latent_append_vec_kernel");
     }
     latent_append_kernel<<<(unsigned)p.n_tokens, 128, 0, st>>>(p);
