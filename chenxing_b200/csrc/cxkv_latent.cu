@@ -36,7 +36,8 @@ static LatPlan latent_plan(const cx_latent_pool* pool, const cx_attn_batch* b) {
     const int sms = std::max(num_sms(), x.sub);
     int64_t keys = b->table_stride * pool->block_size;
     if (b->window > 0) keys = std::min(keys, b->window + b->max_q_len + 2 * kLatKeys);
-    const int64_t tiles = x.units * ((keys + kLatKeys - 1) / kLatKeys + kLatRangeCost);
+    const int cost = lat_range_cost((int)(pool->latent_dim + pool->rope_dim));
+    const int64_t tiles = x.units * ((keys + kLatKeys - 1) / kLatKeys + cost);
     const int64_t want = std::max<int64_t>(1, (tiles + kLatMinTiles - 1) / kLatMinTiles);
     x.grid = (int)std::min<int64_t>(sms / x.sub, want) * x.sub;
     return x;
@@ -117,7 +118,6 @@ static int latent_attend(const cx_latent_pool* pool, int64_t layer, const cx_att
     p.qr_tok = q->rope_token_stride;
     p.qr_head = q->rope_head_stride;
     p.out = out;
-    p.pool = pool->kv;
     p.batch = (int)b.batch;
     p.heads = (int)b.n_q_heads;
     p.max_q = (int)b.max_q_len;
@@ -151,7 +151,7 @@ static int latent_attend(const cx_latent_pool* pool, int64_t layer, const cx_att
         }
     }
     const LatPlan x = latent_plan(pool, &b);
-    if (x.units * (cap / kLatKeys + 1 + kLatRangeCost) > INT32_MAX)
+    if (x.units * (cap / kLatKeys + 13) > INT32_MAX)
         return bad(CX_ERR_UNSUPPORTED, "batch x context too large");
     p.rtiles = x.rtiles;
     p.sub = x.sub;
@@ -165,6 +165,7 @@ static int latent_attend(const cx_latent_pool* pool, int64_t layer, const cx_att
     p.desc = reinterpret_cast<int32_t*>(w);
     p.part_ml = reinterpret_cast<float*>(w + (size_t)x.grid * 32);
     p.part_o = p.part_ml + (size_t)x.grid * 2 * x.n * 2;   // (16-byte aligned)
+    p.range_cost = lat_range_cost(p.dim);
     p.box_rows = latent_box_rows(pool->block_size);
     CUtensorMap tm;
     rc = make_latent_tmap(&tm, pool);

@@ -55,19 +55,23 @@ constexpr int kLatP = kLatKeys * 128;          // P^T: a line of up to 64 rows p
 constexpr int kLatProd = 2;                   // producer warps
 constexpr int kLatMaxStages = 4;
 constexpr int kLatMaxPieces = (kLatMaxDim + 127) / 128;
-constexpr int kLatAhead = 3;                  // tiles from the one in work to the one asked for
 constexpr int kLatMinTiles = 4;       // tiles per CTA before another CTA starts
-// What a range costs its CTA beside its tiles (output, first tile), in tiles: with shares
-// of equal tiles the CTAs that two ranges meet in took 72 instead of 66 us (64 x 8k
-// tokens, 16 heads).
-constexpr int kLatRangeCost = 3;
+
+// What a range costs its CTA beside its tiles (output, first tile), in tiles.  With
+// shares of equal tiles the CTAs that two ranges meet in took 72 us where the others
+// took 66 (64 x 8k tokens, 16 heads).  In time it is about the same for all widths, and a
+// tile's time goes with its width: 5 tiles of 576 columns (3: 70.0, 5: 69.5, 7: 70.4 us), 9
+// of 320 (trees over latents of 256 + 64, 3: 78, 5: 72, 9: 69).
+static int lat_range_cost(int dim) {
+    const int c = 2880 / dim;
+    return c < 4 ? 4 : c > 12 ? 12 : c;
+}
 
 struct LatParams {
     const int32_t* tables;
     int64_t table_stride;
     const int32_t* ctx_lens;
     const int32_t* q_start;     // NULL: one query token per sequence
-    const void* pool;
     TreeMask tree;
     const void* q_lat;
     const void* q_rope;
@@ -80,7 +84,7 @@ struct LatParams {
     int32_t n_blocks, block_size, layer, window, dc, dim;
     int32_t q_dtype, out_dtype, q_vec;
     int32_t stages;             // tiles in shared memory
-    int32_t box_rows;
+    int32_t box_rows, range_cost;
     float scale_log2;
     uint32_t tries;             // of a wait
 };
@@ -90,8 +94,8 @@ struct LatUnit {
     int b, T, qs, ctx, base;    // base: committed tokens (ctx - T)
     int r0, n_rows;             // packed rows [r0, r0 + n_rows) of the sequence
     int tile0, n_tiles;         // of the `sub` row tiles that run side by side
-    __device__ __forceinline__ int cost() const {
-        return n_tiles > 0 ? n_tiles + kLatRangeCost : 0;
+    __device__ __forceinline__ int cost(const LatParams& p) const {
+        return n_tiles > 0 ? n_tiles + p.range_cost : 0;
     }
 };
 
@@ -117,7 +121,7 @@ __device__ __forceinline__ LatUnit lat_unit(const LatParams& p, int u, int sub_i
     return x;
 }
 
-// A run of tiles of one unit.  Shares are counted in cost: a unit's first kLatRangeCost
+// A run of tiles of one unit.  Shares are counted in cost: a unit's first range_cost
 // are no tiles.
 struct LatSeg {
     LatUnit x;
@@ -130,9 +134,9 @@ struct LatCursor {
     __device__ __forceinline__ bool next(const LatParams& p, int sub_id, int N, LatSeg& s) {
         while (left > 0 && u < p.n_units) {
             s.x = lat_unit(p, u, sub_id, N);
-            const int take = min(left, s.x.cost() - off);
-            s.from = max(off - kLatRangeCost, 0);
-            s.to = off + take - kLatRangeCost;
+            const int take = min(left, s.x.cost(p) - off);
+            s.from = max(off - p.range_cost, 0);
+            s.to = off + take - p.range_cost;
             left -= max(take, 0);
             ++u;
             off = 0;
@@ -284,10 +288,6 @@ __device__ __forceinline__ uint4 lat_q8(const LatParams& p, int64_t lat, int64_t
                       Half16<E>::pack(x[4], x[5]), Half16<E>::pack(x[6], x[7]));
 }
 
-// The 256 bytes at `src` into L2 (a load whose value nobody waits for).
-__device__ __forceinline__ void lat_prefetch(const void* src) {
-    asm volatile("{\n\t.reg .b32 x;\n\tld.global.L1::no_allocate.L2::256B.b32 x, [%0];\n\t}" ::"l"(src));
-}
 // Asynchronous 16-byte copy to shared memory; zeros when `there` is not set.
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src),
@@ -348,6 +348,25 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
     float* s_alpha = reinterpret_cast<float*>(misc + 512);            // [64], after s_vis
     float* s_red = reinterpret_cast<float*>(misc + 1024);             // [4][64]
 
+    // ---- what needs nothing of the kernels before: it may still run beside them ----
+    if (tid == 0) {
+        for (int s = 0; s < ST * kLatMaxPieces; ++s) {
+            mbar_init(&full[s], kLatProd);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(&s_full[0], 1);
+        mbar_init(&s_full[1], 1);
+        mbar_init(&p_full[0], SW);
+        mbar_init(&p_full[1], SW);
+        mbar_init(o_done, 1);
+        mbar_init(q_full, SW);
+        mbar_init(&drain[0], 1);
+        mbar_init(&drain[1], 1);
+        *s_abort = 0;
+        for (int k = 0; k < kLatProd; ++k) s_issued[k] = 0;
+        fence_mbar_init();
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
     if (tid == 0) p.desc[(int64_t)blockIdx.x * 8] = 0;
 
@@ -375,7 +394,7 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
         const int per = (p.n_units + C::THREADS - 1) / C::THREADS;
         const int u0 = min(p.n_units, tid * per), u1 = min(p.n_units, u0 + per);
         int sum = 0;
-        for (int u = u0; u < u1; ++u) sum += lat_unit(p, u, 0, N).cost();
+        for (int u = u0; u < u1; ++u) sum += lat_unit(p, u, 0, N).cost(p);
         int incl = sum;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -401,7 +420,7 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
         if (before <= w0 && w0 < before + sum) {
             int u = u0, at = before;
             for (; u < u1; ++u) {
-                const int n = lat_unit(p, u, 0, N).cost();
+                const int n = lat_unit(p, u, 0, N).cost(p);
                 if (w0 < at + n) break;
                 at += n;
             }
@@ -410,23 +429,6 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
             s_start[2] = w1 - w0;
             s_start[3] = W;
         }
-    }
-    if (tid == 0) {
-        for (int s = 0; s < ST * kLatMaxPieces; ++s) {
-            mbar_init(&full[s], kLatProd);
-            mbar_init(&empty[s], 1);
-        }
-        mbar_init(&s_full[0], 1);
-        mbar_init(&s_full[1], 1);
-        mbar_init(&p_full[0], SW);
-        mbar_init(&p_full[1], SW);
-        mbar_init(o_done, 1);
-        mbar_init(q_full, SW);
-        mbar_init(&drain[0], 1);
-        mbar_init(&drain[1], 1);
-        *s_abort = 0;
-        for (int k = 0; k < kLatProd; ++k) s_issued[k] = 0;
-        fence_mbar_init();
     }
     if (warp == SW) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -534,28 +536,8 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
                 m[j][0] = m[j][1] = -INFINITY;
                 l[j][0] = l[j][1] = 0.f;
             }
-            // Rows of the tiles behind those in shared memory are asked into L2, two or four
-            // threads a row: what follows an O^T is then a load from L2.
-            constexpr int kPer = SMT / kLatKeys;
-            const int pf_row = tid / kPer, row_bytes = p.dim * 2;
-            auto pf_block = [&](int i) {
-                const int key = first_k + i * kLatKeys + pf_row;
-                return i < n && key < x.ctx ? tab[key / bs] : -1;
-            };
-            int pf_id = pf_block(kLatAhead);
             for (int i = 0; i < n; ++i, ++tile) {
                 const int k0 = first_k + i * kLatKeys;
-                {
-                    const int id = pf_id, key = k0 + kLatAhead * kLatKeys + pf_row;
-                    pf_id = pf_block(i + 1 + kLatAhead);
-                    if (id >= 0 && id < p.n_blocks) {
-                        const char* row = static_cast<const char*>(p.pool) +
-                                          (((int64_t)p.layer * p.n_blocks + id) * bs + key % bs) *
-                                              row_bytes;
-                        for (int o = tid % kPer * 256; o < row_bytes; o += kPer * 256)
-                            lat_prefetch(row + o);
-                    }
-                }
                 ok = el_wait(&s_full[tile & 1], (tile >> 1) & 1, s_abort, p.tries);
                 tc_fence_after();
                 float v[NW / 2];
@@ -983,6 +965,7 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
 // side by side, then every thread adds up four columns of all parts.
 template <int N>
 __global__ void __launch_bounds__(256) latent_join_kernel(const LatParams p) {
+    asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int4 d = *reinterpret_cast<const int4*>(p.desc + (int64_t)blockIdx.x * 8);
     const int parts = d.x, slot = d.y, n_rows = d.z;
@@ -1070,18 +1053,23 @@ static int launch_latent_tc(const CUtensorMap& tm, LatParams p, int grid, cudaSt
     LatCfg<N>::ring(p.dc, p.dim, p.stages, smem);
     auto kern = latent_tc_kernel<N, E>;
     CX_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    kern<<<grid, LatCfg<N>::THREADS, smem, st>>>(tm, p);
-    int rc = check_launch("latent_tc_kernel");
-    if (rc) return rc;
+    // (both kernels start beside the end of the one before them and wait for it)
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid, N / 2);
-    cfg.blockDim = 256;
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = LatCfg<N>::THREADS;
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
+    CX_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tm, p));
+    int rc = check_launch("latent_tc_kernel");
+    if (rc) return rc;
+    cfg.gridDim = dim3(grid, N / 2);
+    cfg.blockDim = 256;
+    cfg.dynamicSmemBytes = 0;
     CX_CUDA_CHECK(cudaLaunchKernelEx(&cfg, latent_join_kernel<N>, p));
     return check_launch("latent_join_kernel");
 }

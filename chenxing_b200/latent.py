@@ -28,6 +28,15 @@ from .radix_kv import _BlockPool, _check_cow_slots
 __all__ = ["LatentPagedKVCache", "LatentBatch"]
 
 
+def _rows2(x, device: torch.device) -> torch.Tensor:
+    """``x`` (tokens, dim) on ``device`` with its innermost dimension contiguous."""
+    if not (isinstance(x, torch.Tensor) and x.dtype != torch.float64 and x.device == device):
+        x = to_device(x, device)
+    if x.dim() != 2:
+        raise ValueError(f"latent and k_rope must have two dimensions, got {tuple(x.shape)}")
+    return x if x.shape[1] <= 1 or x.stride(1) == 1 else x.contiguous()
+
+
 class LatentBatch(PagedBatch):
     """``PagedBatch`` of a latent cache: tables, lengths, ``window`` and
     ``tree_parents`` as there, no score modifiers.  ``scale`` is that of the model's
@@ -170,47 +179,46 @@ class LatentPagedKVCache(_BlockPool):
         if rope.head_dim != self.rope_dim:
             raise ValueError(f"RoPE tables of {rope.head_dim} dims for a rotary part of "
                              f"{self.rope_dim}")
-        if not _lib.same_device(rope.device, self.device):
+        if rope.device != self.device and not _lib.same_device(rope.device, self.device):
             raise ValueError(f"RoPE tables on {rope.device}, the cache on {self.device}")
         return self._append(layer, latent, k_rope, slot_mapping, positions, rope, q_rope, weight,
                             eps, q_out_dtype)
 
     def _append(self, layer, latent, k_rope, slots, positions, rope, q_rope, weight, eps,
                 q_out_dtype):
-        dev = self.device
-        lt, kt = rows_on_device(latent, dev), rows_on_device(k_rope, dev)
-        lt, kt = (t if t.dim() != 2 or t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
-                  for t in (lt, kt))
-        T = lt.shape[0] if lt.dim() else 0
-        if lt.shape != (T, self.latent_dim) or kt.shape != (T, self.rope_dim):
-            raise ValueError(f"latent and k_rope must be (T, {self.latent_dim}) and "
-                             f"(T, {self.rope_dim}), got {tuple(lt.shape)} / {tuple(kt.shape)}")
-        code = _lib.cx_dtype(lt.dtype)
+        dev, dc, dr = self.device, self.latent_dim, self.rope_dim
+        lt, kt = _rows2(latent, dev), _rows2(k_rope, dev)
+        dt, T = lt.dtype, lt.shape[0]
+        if lt.shape[1] != dc or kt.shape != (T, dr):
+            raise ValueError(f"latent and k_rope must be (T, {dc}) and (T, {dr}), got "
+                             f"{tuple(lt.shape)} / {tuple(kt.shape)}")
+        code = _lib.cx_dtype(dt)
         qt = qo = None
         hq, qs, q_code = 0, (0, 0), _lib.CX_F32
         if q_rope is not None:
             qt = rows_on_device(q_rope, dev)
-            if qt.dim() != 3 or qt.shape[0] != T or qt.shape[2] != self.rope_dim:
-                raise ValueError(f"q_rope must be ({T}, Hq, {self.rope_dim}), got "
-                                 f"{tuple(qt.shape)}")
+            if qt.dim() != 3 or qt.shape[0] != T or qt.shape[2] != dr:
+                raise ValueError(f"q_rope must be ({T}, Hq, {dr}), got {tuple(qt.shape)}")
             hq, qs = qt.shape[1], qt.stride()
-        if kt.dtype != lt.dtype or (qt is not None and qt.dtype != lt.dtype):
+        if kt.dtype != dt or (qt is not None and qt.dtype != dt):
             raise TypeError("latent, k_rope and q_rope must have one element type")
         st = index_on_device(slots, dev)
         ps = None if positions is None else index_on_device(positions, dev)
         if st.numel() != T or (ps is not None and ps.numel() != T):
             raise ValueError("slot_mapping and positions need one entry per token")
-        w, w_code = None, _lib.CX_F32
-        if weight is not None:
-            w = to_device(weight, dev)
-            if w.numel() != self.latent_dim:
-                raise ValueError(f"weight must have {self.latent_dim} elements, got {w.numel()}")
-            if w.dtype == lt.dtype:
+        w, w_code = weight, _lib.CX_F32
+        if w is not None:
+            if not (isinstance(w, torch.Tensor) and w.is_cuda and w.device == dev
+                    and w.is_contiguous()):
+                w = to_device(w, dev)
+            if w.numel() != dc:
+                raise ValueError(f"weight must have {dc} elements, got {w.numel()}")
+            if w.dtype == dt:
                 w_code = code
             elif w.dtype != torch.float32:
                 w = w.float()
         if qt is not None:
-            qo = qt.new_empty((T, hq, self.rope_dim), dtype=q_out_dtype or qt.dtype)
+            qo = qt.new_empty((T, hq, dr), dtype=q_out_dtype or dt)
             q_code = _lib.cx_dtype(qo.dtype)
         rows = _lib.CxLatentRows(lt.data_ptr(), kt.data_ptr(), _lib.ptr(qt), lt.stride(0),
                                  kt.stride(0), qs[0], qs[1], T, hq, code, 0)
@@ -248,7 +256,8 @@ class LatentPagedKVCache(_BlockPool):
         dev, dc, dr = self.device, self.latent_dim, self.rope_dim
         rows, hq = batch.total_q, batch.n_q_heads
         if isinstance(q, (tuple, list)):
-            ql, qr = (rows_on_device(x, dev) for x in q)
+            ql, qr = q
+            ql, qr = rows_on_device(ql, dev), rows_on_device(qr, dev)
         else:
             q = rows_on_device(q, dev)
             ql, qr = q[..., :dc], q[..., dc:]
@@ -270,8 +279,8 @@ class LatentPagedKVCache(_BlockPool):
         code, out_code = _lib.cx_dtype(ql.dtype), _lib.cx_dtype(out.dtype)
         if rows == 0:
             return out
-        qs = _lib.CxLatentQ(ql.data_ptr(), qr.data_ptr(), ql.stride(0), ql.stride(1), qr.stride(0),
-                            qr.stride(1), code, 0)
+        ls, rs = ql.stride(), qr.stride()
+        qs = _lib.CxLatentQ(ql.data_ptr(), qr.data_ptr(), ls[0], ls[1], rs[0], rs[1], code, 0)
         with _lib.on_device(dev):
             _lib.check(_lib.lib().cx_latent_attend(
                 self._pool, int(layer), batch.c_struct(), batch._tree, qs, out.data_ptr(),
