@@ -106,6 +106,7 @@ struct MmaParams {
     int32_t* counters;   // [batch * n_groups] merge tickets, zero between calls
     float* partials;     // [(P + batch*n_groups)][hg][rows][D + 2]
     ScoreMod mod;        // MOD instantiations (and the plan: prefix blocks)
+    int32_t min_units;   // least units of a CTA's chunk; 0: kMinUnitsPerCta
     int32_t plan_kind;   // 0: cx_paged_decode / _verify; cx_paged_attend: 1, with a prefix 3
 };
 
@@ -212,7 +213,8 @@ static __global__ void __launch_bounds__(1024) paged_plan_kernel(MmaParams p, in
             W = 0;
         }
         p.seq_start[B] = (int)W;
-        long long want = (W + kMinUnitsPerCta - 1) / kMinUnitsPerCta;
+        const int least = p.min_units > 0 ? p.min_units : kMinUnitsPerCta;
+        long long want = (W + least - 1) / least;
         long long pe = want < grid ? want : grid;
         if (pe < 1) pe = 1;
         const long long chunk = W > 0 ? (W + pe - 1) / pe : 1;

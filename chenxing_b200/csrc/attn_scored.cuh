@@ -122,6 +122,12 @@ static int attend_split(const cx_pool* pool, int64_t layer, const cx_attn_batch&
     p.mod.slopes = m.alibi_slopes;
     p.mod.prefix = m.prefix_lens;
     p.plan_kind = m.prefix_lens ? 3 : 1;
+    // A tree's 16 or 32 fp32 rows are much work for a unit's few warps: a CTA for every
+    // unit while there are CTAs, and no range of more than three parts is left to its last
+    // CTA (8 trees of 8 nodes, 32 rows, behind up to 512 keys: chunks of 4 units 80 us,
+    // of 1 unit 72, and with ranges of 4 parts joined apart 55).
+    const bool fine = TREE && pool->dtype == CX_F32 && rows > 8;
+    if (fine) p.min_units = 1;
     p.mod.q_stride = m.q_stride;
     p.mod.out = out;
     p.mod.out_dtype = m.out_dtype;
@@ -153,7 +159,7 @@ static int attend_split(const cx_pool* pool, int64_t layer, const cx_attn_batch&
     // and the rest over 400, 227 -> 150 us, against 4 us more for 128 even ones (173 ->
     // 178).  Single tokens and fp32 gain nothing there (141 -> 147 us).
     if (2 * b.batch * sh.n_groups <= grid)
-        p.mod.join_min = 4;
+        p.mod.join_min = fine ? 3 : 4;
     else if (b.max_q_len > 1 && pool->dtype != CX_F32)
         p.mod.join_min = 16;
     switch (pool->dtype) {

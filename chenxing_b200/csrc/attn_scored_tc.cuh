@@ -242,7 +242,8 @@ __device__ __forceinline__ void sc_place(const ScoredTcParams& p, int cta, int l
 // tile would run as one chain S -> softmax -> P -> PV -> next S, with half of the
 // softmax warps idle: both query tiles then hold its rows and take the key tiles in
 // turn (`turns`), each with its own maxima, sums and O, which are joined at the end.  64
-// trees of 26 nodes (104 rows) behind 1k to 8k keys, 8 KV heads of 128: 391 -> TURNS us.
+// trees of 26 nodes (104 rows) behind 1k to 8k keys, 8 KV heads of 128: 377 us as a chain, 371 in two places with the
+// loads and MMAs issued as by the kernel without trees, 294 with elected threads.
 template <int DH, typename E, bool CAP, bool ALIBI, bool TREE = false>
 __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
     scored_tc_kernel(const __grid_constant__ CUtensorMap tmk,

