@@ -116,6 +116,12 @@ __device__ __forceinline__ void store_as(void* p, int32_t dtype, int64_t i, floa
         static_cast<__half*>(p)[i] = __float2half_rn(x);
 }
 
+__device__ __forceinline__ float load_as(const void* p, int32_t dtype, int64_t i) {
+    return dtype == CX_F32    ? static_cast<const float*>(p)[i]
+           : dtype == CX_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i])
+                              : __half2float(static_cast<const __half*>(p)[i]);
+}
+
 // Elements `i`, `i + 1` (i even, the array 8-byte aligned) of such an array.
 __device__ __forceinline__ void store2_as(void* p, int32_t dtype, int64_t i, float x, float y) {
     if (dtype == CX_F32)

@@ -43,17 +43,26 @@ static LatPlan latent_plan(const cx_latent_pool* pool, const cx_attn_batch* b) {
     return x;
 }
 
-// Parts that the generic kernel splits a context into: CTAs for about four an SM, at
-// least 32 keys a part, at most 256 parts (latent_generic_join).
-static int latent_split(const cx_latent_pool* pool, const cx_attn_batch* b, int64_t units) {
-    int64_t keys = b->table_stride * pool->block_size;
-    if (b->window > 0) keys = std::min(keys, b->window + b->max_q_len);
-    const int64_t want = 4ll * std::max(num_sms(), 1) / std::max<int64_t>(units, 1);
-    return (int)std::max<int64_t>(1, std::min(std::min(want, keys / 32), (int64_t)256));
+// Rows of a unit of the fp32 kernels: latent_rows_kernel from 17 rows of a sequence on (62
+// tokens of 64 heads behind 1,200 keys of 384 + 64: 1,188 us with units of 4 rows, 558 with
+// 32; 16 rows behind 4,000 of 512 + 64: 150 and 174).
+static int generic_unit_rows(const cx_attn_batch* b) {
+    return b->n_q_heads * b->max_q_len > 16 ? kLrRows : kLgRows;
 }
 
 static int64_t generic_tiles(const cx_attn_batch* b) {
-    return (b->n_q_heads * b->max_q_len + kLgRows - 1) / kLgRows;
+    const int64_t u = generic_unit_rows(b);
+    return (b->n_q_heads * b->max_q_len + u - 1) / u;
+}
+
+// Parts that the fp32 kernels split a context into: CTAs for four an SM (of 32 rows: two),
+// at least 32 keys a part, at most 256 parts (latent_generic_join).
+static int latent_split(const cx_latent_pool* pool, const cx_attn_batch* b, int64_t units) {
+    int64_t keys = b->table_stride * pool->block_size;
+    if (b->window > 0) keys = std::min(keys, b->window + b->max_q_len);
+    const int64_t want = (generic_unit_rows(b) == kLrRows ? 2ll : 4ll) * std::max(num_sms(), 1) /
+                         std::max<int64_t>(units, 1);
+    return (int)std::max<int64_t>(1, std::min(std::min(want, keys / 32), (int64_t)256));
 }
 
 static size_t latent_workspace(const cx_latent_pool* pool, const cx_attn_batch* b, bool tc) {
@@ -64,7 +73,7 @@ static size_t latent_workspace(const cx_latent_pool* pool, const cx_attn_batch* 
     }
     const int64_t units = b->batch * generic_tiles(b);
     const int s = latent_split(pool, b, units);
-    return s == 1 ? 256 : 256 + (size_t)units * s * kLgRows * (pool->latent_dim + 2) * 4;
+    return s == 1 ? 256 : 256 + (size_t)units * s * generic_unit_rows(b) * (pool->latent_dim + 2) * 4;
 }
 
 static int latent_attend(const cx_latent_pool* pool, int64_t layer, const cx_attn_batch* bt,
@@ -141,6 +150,7 @@ static int latent_attend(const cx_latent_pool* pool, int64_t layer, const cx_att
         const int64_t tiles = generic_tiles(&b), units = b.batch * tiles;
         if (units > INT32_MAX) return bad(CX_ERR_UNSUPPORTED, "too many rows");
         g.row_tiles = (int)tiles;
+        g.unit_rows = generic_unit_rows(&b);
         g.n_split = latent_split(pool, &b, units);
         g.scale = scale;
         g.part = reinterpret_cast<float*>(static_cast<char*>(ws) + 256);

@@ -27,12 +27,6 @@ struct LatAppendParams {
     float eps;
 };
 
-__device__ __forceinline__ float load_as(const void* p, int32_t dtype, int64_t i) {
-    return dtype == CX_F32    ? static_cast<const float*>(p)[i]
-           : dtype == CX_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i])
-                              : __half2float(static_cast<const __half*>(p)[i]);
-}
-
 // 8 elements, 16-byte aligned, as they lie in memory: asked for at once, looked at
 // when they are needed.
 template <typename E> struct Raw8 {

@@ -35,7 +35,8 @@ def test_decode(hq, dc, dr, dtype, bs):
 
 
 @pytest.mark.parametrize("hq,dc,dr,dtype", [
-    (16, 512, 64, BF), (5, 256, 64, F16), (128, 512, 64, BF), (1, 128, 32, BF), (3, 128, 32, F32)])
+    (16, 512, 64, BF), (5, 256, 64, F16), (128, 512, 64, BF), (1, 128, 32, BF), (3, 128, 32, F32),
+    (16, 512, 64, F32), (12, 300, 6, F32), (5, 50, 6, BF), (2, 383, 10, F16), (9, 257, 2, F32)])
 @pytest.mark.parametrize("window", [None, 1, 37, 100])
 @pytest.mark.parametrize("ctx,q_lens", [
     ([1, 5, 17, 64, 200, 66, 333], [1, 5, 4, 0, 5, 2, 3]),
@@ -46,7 +47,8 @@ def test_chains(hq, dc, dr, dtype, window, ctx, q_lens):
 
 
 @pytest.mark.parametrize("hq,dc,dr,dtype,bs", [
-    (16, 512, 64, BF, 16), (4, 256, 64, F16, 32), (2, 128, 32, F32, 16), (128, 512, 64, BF, 16)])
+    (16, 512, 64, BF, 16), (4, 256, 64, F16, 32), (2, 128, 32, F32, 16), (128, 512, 64, BF, 16),
+    (1, 64, 8, F32, 16), (7, 320, 64, F32, 5), (3, 64, 16, BF, 24)])
 @pytest.mark.parametrize("kind", ["random", "star", "chain", "deep"])
 @pytest.mark.parametrize("window", [None, 3, 50])
 def test_trees(hq, dc, dr, dtype, bs, kind, window):
@@ -91,6 +93,17 @@ def test_scales_and_growing_scores(dtype, scale):
         t, pos = torch.tensor(c.tables[b]), torch.arange(rows.shape[0])
         c.cache.kv_pool[0][t.cuda()[pos.cuda() // 16], pos.cuda() % 16] = rows.to(dtype).cuda()
     c.check(c.run(out_dtype=F32))
+
+
+@pytest.mark.parametrize("hq,dc,dr,dtype,bs", [(8, 128, 32, F32, 16), (64, 384, 64, F32, 16),
+                                               (3, 50, 6, BF, 16), (40, 70, 2, F16, 1)])
+def test_cut_contexts_of_the_fp32_kernels(hq, dc, dr, dtype, bs):
+    c = LatentCase(hq=hq, dc=dc, dr=dr, ctx=[3000, 1, 0, 777], dtype=dtype, bs=bs, seed=12)
+    batch = c.batch()
+    assert batch.kernel_kind(dtype) == "generic"
+    a = c.run(batch, out_dtype=F32)
+    c.check(a)
+    assert torch.equal(a, c.run(batch, out_dtype=F32))
 
 
 def test_last_layer_and_larger_table():
