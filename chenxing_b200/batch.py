@@ -65,22 +65,29 @@ def _same_start(a, b) -> bool:
     return list(a[:n]) == list(b[:n]) and (n > 0 or len(a) == len(b))
 
 
+def tree_rows(parents, q_lens):
+    """(q_lens, each row's node, each row's parent) of a drafted tree per sequence, rows
+    concatenated, int64; ValueError unless every parent comes before its node or is -1."""
+    q_lens = np.asarray(q_lens, dtype=np.int64).reshape(-1)
+    if len(parents) != q_lens.shape[0] or any(len(p) != n for p, n in zip(parents, q_lens)):
+        raise ValueError("tree_parents must be one list per sequence with one parent per query "
+                         "token")
+    own = np.concatenate([np.arange(n) for n in q_lens] or [np.zeros(0, np.int64)]).astype(np.int64)
+    up = np.concatenate([np.asarray(p, dtype=np.int64).reshape(-1) for p in parents]
+                        or [np.zeros(0, np.int64)])
+    if np.any(up < -1) or np.any(up >= own):
+        raise ValueError("tree_parents: a node's parent comes before it, or is -1")
+    return q_lens, own, up
+
+
 def tree_arrays(parents, q_lens, window: int = 0):
     """(masks, depths) of a drafted tree per sequence, rows concatenated: masks
     (rows, words) uint32, bit u set where the row sees node u (itself and its
     ancestors, with ``window`` > 0 the nearest ``window`` of them); depths (rows,)
     int32, a node's ancestors.  ``parents[b][i]``: node i's parent, below i, or -1
     behind the committed context."""
-    q_lens = np.asarray(q_lens, dtype=np.int64).reshape(-1)
-    if len(parents) != q_lens.shape[0] or any(len(p) != n for p, n in zip(parents, q_lens)):
-        raise ValueError("tree_parents must be one list per sequence with one parent per query "
-                         "token")
+    q_lens, own, up = tree_rows(parents, q_lens)
     total, words = int(q_lens.sum()), max(1, -(-int(q_lens.max(initial=1)) // 32))
-    own = np.concatenate([np.arange(n) for n in q_lens] or [np.zeros(0, np.int64)]).astype(np.int64)
-    up = np.concatenate([np.asarray(p, dtype=np.int64).reshape(-1) for p in parents]
-                        or [np.zeros(0, np.int64)])
-    if np.any(up < -1) or np.any(up >= own):
-        raise ValueError("tree_parents: a node's parent comes before it, or is -1")
     first = np.repeat(np.cumsum(q_lens) - q_lens, q_lens)
     up = np.where(up < 0, -1, up + first)                   # rows
     masks = np.zeros((total, words), dtype=np.uint32)
@@ -138,6 +145,7 @@ class PagedBatch:
                  window: int | None = None, scale: float | None = None,
                  table_stride: int | None = None, softcap: float | None = None,
                  alibi_slopes=None, prefix_lens=None, tree_parents=None) -> None:
+        self._check_cache(cache)
         self.cache = cache
         self.device = cache.device
         self.n_q_heads = int(n_q_heads)
@@ -262,6 +270,10 @@ class PagedBatch:
             self._ws = torch.zeros(need, dtype=torch.uint8, device=self.device)
             self._ws_bytes = need
 
+    def _check_cache(self, cache) -> None:
+        if hasattr(cache, "latent_dim"):
+            raise TypeError("a latent cache takes a LatentBatch")
+
     def _workspace_need(self) -> int:
         pool = self.cache.cx_pool()
         if self.is_tree:
@@ -325,6 +337,8 @@ class PagedBatch:
 def _attend(cache, layer: int, q, batch: PagedBatch, out, replan, out_dtype, fn_name: str):
     if batch.cache is not cache:
         raise ValueError("PagedBatch belongs to a different cache")
+    if hasattr(cache, "latent_dim"):
+        raise TypeError("a latent cache attends through its own decode_batch and verify_batch")
     if out_dtype is None:
         out_dtype = torch.float32 if out is None else out.dtype
     if batch.takes_attend(out_dtype):

@@ -9,8 +9,9 @@ namespace cx {
 int copy_dev_flags_latent(cudaStream_t s, unsigned int* v) { return copy_dev_flags(s, v); }
 int clear_dev_flags_latent(cudaStream_t s) { return clear_dev_flags(s); }
 
-// Whether the tcgen05 kernel takes the call: 16-bit pools whose rows TMA can load.
-// `vec` is not needed (it reads queries of any alignment).
+// Whether the tcgen05 kernel takes the call: 16-bit pools whose rows TMA can load
+// (queries of any alignment), and no queries of the other 16-bit type, whose range or
+// precision the pool's does not hold.
 static bool latent_tc(const cx_latent_pool* pool, int32_t q_dtype) {
     const int64_t dim = pool->latent_dim + pool->rope_dim;
     return pool->dtype != CX_F32 && (q_dtype == CX_F32 || q_dtype == pool->dtype) &&

@@ -55,7 +55,7 @@ constexpr int kLatP = kLatKeys * 128;          // P^T: a line of up to 64 rows p
 constexpr int kLatProd = 2;                   // producer warps
 constexpr int kLatMaxStages = 4;
 constexpr int kLatMaxPieces = (kLatMaxDim + 127) / 128;
-constexpr int kLatMinTiles = 4;       // tiles per CTA before another CTA starts
+constexpr int kLatMinTiles = 4;       // cost (in tiles) of a CTA before another starts
 
 // What a range costs its CTA beside its tiles (output, first tile), in tiles.  With
 // shares of equal tiles the CTAs that two ranges meet in took 72 us where the others

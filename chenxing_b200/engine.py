@@ -41,7 +41,7 @@ import numpy as np
 import torch
 
 from ._arrays import upload
-from .batch import PagedBatch, slot_mapping
+from .batch import PagedBatch, slot_mapping, tree_rows
 from .latent import LatentBatch, LatentPagedKVCache
 from .radix_kv import RadixPagedKVCache
 
@@ -86,10 +86,10 @@ class BatchedKVEngine:
 
     _latent = False
 
-    def __init__(self, cache: RadixPagedKVCache | LatentPagedKVCache, *, n_q_heads: int, window: int | None = None,
-                 scale: float | None = None, free_private_blocks: bool = False,
-                 publish_mode: str = "reference", softcap: float | None = None,
-                 alibi_slopes=None) -> None:
+    def __init__(self, cache: RadixPagedKVCache | LatentPagedKVCache, *, n_q_heads: int,
+                 window: int | None = None, scale: float | None = None,
+                 free_private_blocks: bool = False, publish_mode: str = "reference",
+                 softcap: float | None = None, alibi_slopes=None) -> None:
         if publish_mode not in ("reference", "suffix"):
             raise ValueError("publish_mode must be 'reference' or 'suffix'")
         self._latent = isinstance(cache, LatentPagedKVCache)
@@ -239,6 +239,8 @@ class BatchedKVEngine:
             raise ValueError("tree_parents needs attend=True")
         if self._latent and prefix_lens is not None:
             raise ValueError("a latent cache takes no prefix_lens")
+        if tree_parents is not None:     # (refused before a table grows)
+            tree_rows(tree_parents, [1] * len(seq_ids) if q_lens is None else q_lens)
         p = self.plan_host(seq_ids, q_lens)
         c = self.cache
         dev = c.device
@@ -379,6 +381,8 @@ class BatchedKVEngine:
         paths = [list(map(int, p)) for p in paths]
         if any(s.n_tokens != n for s, n in zip(plan.seqs, plan.n_past)):
             raise RuntimeError("accept() after the plan's sequences moved on")
+        if len({id(s) for s in plan.seqs}) != len(plan.seqs):
+            raise ValueError("accept() of a plan that has a sequence twice")
         self.cache.accept_paths(plan.batch, paths)
         for s, p in zip(plan.seqs, paths):
             s.n_tokens += len(p)

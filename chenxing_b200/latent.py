@@ -49,13 +49,22 @@ class LatentBatch(PagedBatch):
     def __init__(self, cache, block_tables, ctx_lens, *, n_q_heads: int, scale: float,
                  q_lens=None, window: int | None = None, table_stride: int | None = None,
                  tree_parents=None) -> None:
-        if not isinstance(cache, LatentPagedKVCache):
-            raise TypeError("LatentBatch needs a LatentPagedKVCache")
         if int(n_q_heads) < 1:
             raise ValueError("n_q_heads must be positive")
         super().__init__(cache, block_tables, ctx_lens, n_q_heads=n_q_heads, q_lens=q_lens,
                          window=window, scale=float(scale), table_stride=table_stride,
                          tree_parents=tree_parents)
+
+    def set(self, block_tables, ctx_lens, q_lens=None, prefix_lens=None,
+            tree_parents=None) -> None:
+        """``PagedBatch.set``, without ``prefix_lens``."""
+        if prefix_lens is not None:
+            raise ValueError("a latent cache takes no prefix_lens")
+        super().set(block_tables, ctx_lens, q_lens, tree_parents=tree_parents)
+
+    def _check_cache(self, cache) -> None:
+        if not isinstance(cache, LatentPagedKVCache):
+            raise TypeError("LatentBatch needs a LatentPagedKVCache")
 
     def _workspace_need(self) -> int:
         return int(_lib.lib().cx_latent_attend_workspace_bytes(self.cache.cx_pool(), self._c))

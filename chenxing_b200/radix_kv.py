@@ -480,6 +480,8 @@ class _BlockPool(RadixIndex):
                 raise ValueError(f"paths must be ({batch.batch}, n), got {tuple(paths.shape)}")
             if paths.dtype.is_floating_point or paths.dtype == torch.bool or paths.is_complex():
                 raise TypeError("paths must be integers")
+            if paths.dtype in (torch.int64, torch.uint32, torch.uint64):   # (no node, not another)
+                paths = paths.to(torch.int64).clamp(-1, np.iinfo(np.int32).max)
             t = paths.to(self.device, torch.int32, non_blocking=True)
             if t.shape[1] > 1 and t.stride(1) != 1 or t.stride(0) < t.shape[1]:
                 t = t.contiguous()

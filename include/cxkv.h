@@ -248,7 +248,8 @@ int cx_paged_decode_static(const cx_pool* pool, int64_t layer, const cx_attn_bat
                            const void* q, int32_t q_dtype, float* out, void* stream);
 
 /* Limit, in nanoseconds, of every pipeline wait inside the split-K kernels of
- * later decode / verify calls, all kernels of cx_paged_attend and the staged
+ * later decode / verify calls, all kernels of cx_paged_attend and
+ * cx_paged_attend_tree, the tcgen05 kernel of cx_latent_attend and the staged
  * form of cx_kv_append_norm_rope in this process (0 restores the default, 2 s;
  * the tcgen05 kernels of cx_paged_verify keep that).  A
  * wait that runs out makes its CTA stop, wait (with the default limit) for its
@@ -440,11 +441,12 @@ typedef struct cx_latent_q {
  * selects 1/sqrt(latent_dim + rope_dim); a model's scale is that of its heads before
  * they were absorbed.  What the pool holds where no query row sees it does not
  * reach the result; at a position that only some rows see, it must be finite.
- * 16-bit pools with block_size 16, 32 or 64 and (latent_dim + rope_dim) a multiple of
- * 8, at least 64, take a tcgen05 kernel, which rounds fp32 queries and the
- * probabilities to the pool's type (the denominator sums the rounded ones); all
- * else, and queries of the other 16-bit type, an fp32 kernel.  The plan is made in the call: a workspace
- * holds nothing between calls, but calls that overlap need one each. */
+ * 16-bit pools on a 16-byte boundary with block_size a multiple of 8 and
+ * (latent_dim + rope_dim) a multiple of 8, at least 64, take a tcgen05 kernel, which
+ * rounds fp32 queries and the probabilities to the pool's type (the denominator sums
+ * the rounded ones); all else, and queries of the other 16-bit type, an fp32 kernel.
+ * The plan is made in the call: a workspace holds nothing between calls, but calls
+ * that overlap need one each. */
 int cx_latent_attend(const cx_latent_pool* pool, int64_t layer, const cx_attn_batch* batch,
                      const cx_tree* tree, const cx_latent_q* q, void* out, int32_t out_dtype,
                      void* workspace, size_t workspace_bytes, void* stream);
