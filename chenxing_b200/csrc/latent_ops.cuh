@@ -92,13 +92,17 @@ __device__ __forceinline__ bool lat_slot(const LatAppendParams& p, int64_t t, in
 }
 
 // One block per token.  Warp 0 has the pool row, the other warps 32 units of 8 pairs
-// of the queries each: with rows of 16-byte multiples a lane holds 8 pairs, whose
+// of the queries at a time: with rows of 16-byte multiples a lane holds 8 pairs, whose
 // angles it loads once for all its heads.  All that a lane needs first (rows, slot,
 // position) is asked for before any of it is looked at; then come the angles and the
-// weights.  8,192 tokens, 32 heads, bf16, 90 MB: 28 us; with loads that are
-// converted where they are made, one after the other, 47.
+// weights.  8,192 tokens, 32 heads, bf16, 90 MB: 23 us; with a head a lane, twice the
+// warps and 56 registers, which spill, 27 (64 tokens: 2.5 and 2.7); with loads that are converted where they
+// are made, one after the other, 47.
+constexpr int kLaHeads = 2;       // heads a lane asks for at once
+constexpr int kLaWarps = 5;
 template <typename E>
-__global__ void __launch_bounds__(288, 4) latent_append_vec_kernel(const LatAppendParams p) {
+__global__ void __launch_bounds__(kLaWarps * 32, 5)
+    latent_append_vec_kernel(const LatAppendParams p) {
     const int64_t t = blockIdx.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
     const int units = p.dr / 16, half = p.dr / 2;     // units of 8 pairs a head
@@ -107,12 +111,29 @@ __global__ void __launch_bounds__(288, 4) latent_append_vec_kernel(const LatAppe
     // first elements of unit u's two runs of 8
     auto run_a = [&](int u) { return p.interleaved ? 16 * u : 8 * u; };
     auto run_b = [&](int u) { return p.interleaved ? 16 * u + 8 : half + 8 * u; };
-    // unit u's pairs turned: elements 2k, 2k + 1 of the 16, or k of either run
-    auto rotate = [&](int u, float (&a)[8], float (&b)[8]) {
+    // the angles of unit u's pairs: c[0 .. 1] and s[0 .. 1] of either pair element, or of
+    // the first, c[2 .. 3] and s[2 .. 3] of the second
+    struct Angles {
+        float4 c[4], s[4];
+    };
+    auto angles = [&](int u) {
+        Angles g;
         const float4* c = reinterpret_cast<const float4*>(p.cos_table + pos * p.dr + 8 * u);
         const float4* s = reinterpret_cast<const float4*>(p.sin_table + pos * p.dr + 8 * u);
+        const int o = p.interleaved ? 0 : half / 4;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            g.c[k] = __ldg(c + k);
+            g.s[k] = __ldg(s + k);
+            g.c[2 + k] = __ldg(c + o + k);
+            g.s[2 + k] = __ldg(s + o + k);
+        }
+        return g;
+    };
+    // the pairs turned: elements 2k, 2k + 1 of the 16, or k of either run
+    auto rotate = [&](const Angles& g, float (&a)[8], float (&b)[8]) {
         if (p.interleaved) {
-            const float4 c0 = __ldg(c), c1 = __ldg(c + 1), s0 = __ldg(s), s1 = __ldg(s + 1);
+            const float4 c0 = g.c[0], c1 = g.c[1], s0 = g.s[0], s1 = g.s[1];
             RopePair{c0.x, s0.x, c0.x, s0.x}.turn(a[0], a[1]);
             RopePair{c0.y, s0.y, c0.y, s0.y}.turn(a[2], a[3]);
             RopePair{c0.z, s0.z, c0.z, s0.z}.turn(a[4], a[5]);
@@ -122,11 +143,9 @@ __global__ void __launch_bounds__(288, 4) latent_append_vec_kernel(const LatAppe
             RopePair{c1.z, s1.z, c1.z, s1.z}.turn(b[4], b[5]);
             RopePair{c1.w, s1.w, c1.w, s1.w}.turn(b[6], b[7]);
         } else {
-            const int o = half / 4;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const float4 cx = __ldg(c + k), sx = __ldg(s + k), cy = __ldg(c + o + k),
-                             sy = __ldg(s + o + k);
+                const float4 cx = g.c[k], sx = g.s[k], cy = g.c[2 + k], sy = g.s[2 + k];
                 RopePair{cx.x, sx.x, cy.x, sy.x}.turn(a[4 * k], b[4 * k]);
                 RopePair{cx.y, sx.y, cy.y, sy.y}.turn(a[4 * k + 1], b[4 * k + 1]);
                 RopePair{cx.z, sx.z, cy.z, sy.z}.turn(a[4 * k + 2], b[4 * k + 2]);
@@ -193,7 +212,7 @@ __global__ void __launch_bounds__(288, 4) latent_append_vec_kernel(const LatAppe
                 float a[8], b[8];
                 ra.get(a);
                 rb.get(b);
-                if (turn) rotate(lane, a, b);
+                if (turn) rotate(angles(lane), a, b);
                 store8_as(p.pool, p.pool_dtype, dst + p.dc + run_a(lane), a);
                 store8_as(p.pool, p.pool_dtype, dst + p.dc + run_b(lane), b);
             }
@@ -202,19 +221,35 @@ __global__ void __launch_bounds__(288, 4) latent_append_vec_kernel(const LatAppe
     if (!p.q || (pool_row && n_warps > 1)) return;
     // units of the queries: 32 % units == 0, so that a lane keeps one unit's angles
     const int w0 = n_warps > 1 ? warp - 1 : 0, nw = n_warps > 1 ? n_warps - 1 : 1;
-    const int u = lane % units, per_warp = 32 / units;
-    for (int h = w0 * per_warp + lane / units; h < p.heads; h += nw * per_warp) {
-        Raw8<E> ra, rb;
-        float a[8], b[8];
-        const int64_t src = t * p.q_tok + h * p.q_head, dst = (t * p.heads + h) * p.dr;
-        ra.load(p.q, src + run_a(u));
-        rb.load(p.q, src + run_b(u));
-        if (turn && (pos < 0 || pos >= p.table_rows)) return;
-        ra.get(a);
-        rb.get(b);
-        if (turn) rotate(u, a, b);
-        store8_as(p.q_out, p.q_out_dtype, dst + run_a(u), a);
-        store8_as(p.q_out, p.q_out_dtype, dst + run_b(u), b);
+    const int u = lane % units, step = nw * (32 / units);
+    Angles g;
+    for (int h0 = w0 * (32 / units) + lane / units, first = 1; h0 < p.heads;
+         h0 += kLaHeads * step, first = 0) {
+        Raw8<E> ra[kLaHeads], rb[kLaHeads];
+#pragma unroll
+        for (int k = 0; k < kLaHeads; ++k) {
+            const int h = h0 + k * step;
+            if (h >= p.heads) continue;
+            const int64_t src = t * p.q_tok + h * p.q_head;
+            ra[k].load(p.q, src + run_a(u));
+            rb[k].load(p.q, src + run_b(u));
+        }
+        if (first && turn) {
+            if (pos < 0 || pos >= p.table_rows) return;
+            g = angles(u);
+        }
+#pragma unroll
+        for (int k = 0; k < kLaHeads; ++k) {
+            const int h = h0 + k * step;
+            if (h >= p.heads) continue;
+            float a[8], b[8];
+            const int64_t dst = (t * p.heads + h) * p.dr;
+            ra[k].get(a);
+            rb[k].get(b);
+            if (turn) rotate(g, a, b);
+            store8_as(p.q_out, p.q_out_dtype, dst + run_a(u), a);
+            store8_as(p.q_out, p.q_out_dtype, dst + run_b(u), b);
+        }
     }
 }
 
@@ -513,8 +548,8 @@ static int latent_append(const cx_latent_pool* pool, int64_t layer, const cx_lat
     const bool vec = (bytes & 15) == 0 && p.dc % 8 == 0 && p.dr % 16 == 0 && 32 % units == 0;
     if (vec) {
         const int per_warp = 32 / units;
-        int warps = has_q ? 1 + (p.heads + per_warp - 1) / per_warp : 1;
-        if (warps > 9) warps = 9;
+        const int per_q = per_warp * kLaHeads;
+        const int warps = !has_q ? 1 : std::min(kLaWarps, 1 + (p.heads + per_q - 1) / per_q);
         const unsigned n = (unsigned)p.n_tokens;
         if (p.dtype == CX_F32)
             latent_append_vec_kernel<float><<<n, warps * 32, 0, st>>>(p);
