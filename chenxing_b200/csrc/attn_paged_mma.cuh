@@ -106,7 +106,6 @@ struct MmaParams {
     int32_t* counters;   // [batch * n_groups] merge tickets, zero between calls
     float* partials;     // [(P + batch*n_groups)][hg][rows][D + 2]
     ScoreMod mod;        // MOD instantiations (and the plan: prefix blocks)
-    int32_t min_units;   // least units of a CTA's chunk; 0: kMinUnitsPerCta
     int32_t plan_kind;   // 0: cx_paged_decode / _verify; cx_paged_attend: 1, with a prefix 3
 };
 
@@ -213,8 +212,7 @@ static __global__ void __launch_bounds__(1024) paged_plan_kernel(MmaParams p, in
             W = 0;
         }
         p.seq_start[B] = (int)W;
-        const int least = p.min_units > 0 ? p.min_units : kMinUnitsPerCta;
-        long long want = (W + least - 1) / least;
+        long long want = (W + kMinUnitsPerCta - 1) / kMinUnitsPerCta;
         long long pe = want < grid ? want : grid;
         if (pe < 1) pe = 1;
         const long long chunk = W > 0 ? (W + pe - 1) / pe : 1;
@@ -1581,10 +1579,17 @@ static int launch_f32_d(const MmaShape& sh, const CUtensorMap& tk, const CUtenso
     const int rt = f32_rt(p.rows);
 #define CX_CASE(HG_, RT_) \
     if (sh.hg == HG_ && rt == RT_) return launch_f32_cfg<D, HG_, RT_, MOD, TREE>(tk, tv, p, st, grid);
-    CX_CASE(1, 4) CX_CASE(1, 8) CX_CASE(1, 16)
-    CX_CASE(2, 4) CX_CASE(2, 8) CX_CASE(2, 16)
+    // (trees of more rows have a kernel of their own, attn_tree_f32.cuh)
+    CX_CASE(1, 4) CX_CASE(1, 8)
+    CX_CASE(2, 4) CX_CASE(2, 8)
     if constexpr (D == 64) {
-        CX_CASE(4, 4) CX_CASE(4, 8) CX_CASE(4, 16)
+        CX_CASE(4, 4) CX_CASE(4, 8)
+    }
+    if constexpr (!TREE) {
+        CX_CASE(1, 16) CX_CASE(2, 16)
+        if constexpr (D == 64) {
+            CX_CASE(4, 16)
+        }
     }
 #undef CX_CASE
     return fail(CX_ERR_UNSUPPORTED, "paged attention: no fp32 kernel for this row/head shape");

@@ -6,6 +6,7 @@
 
 #include "cx_common.cuh"  // unity build: included from cxkv_scored.cu after the kernels
 #include "attn_scored_tc.cuh"
+#include "attn_tree_f32.cuh"
 
 namespace cx {
 
@@ -33,13 +34,15 @@ static bool tc_shape(const cx_pool* pool, const cx_attn_batch* b, bool tree) {
 // The split-K kernels: up to 64 packed rows.
 static bool split_shape(const cx_pool* pool, const cx_attn_batch* b, bool tree) {
     const int64_t rows = b->n_q_heads / pool->n_kv_heads * b->max_q_len;
-    return tma_shape(pool, b) && rows >= 1 && rows <= 64 && !tc_shape(pool, b, tree);
+    return tma_shape(pool, b) && rows >= 1 && rows <= 64 && !tc_shape(pool, b, tree) &&
+           !(tree && pool->dtype == CX_F32 && rows >= kTrRows0);
 }
 
 // The kernel of a call.  `vec`: q, its token stride and out are 16-byte aligned.
 // 16-bit pools take queries of their own type or fp32, fp32 pools any type.
 static int attend_kind(const cx_pool* pool, const cx_attn_batch* b, int32_t q_dtype, bool vec,
                        bool tree) {
+    if (tree && tree_rows_shape(pool, b)) return CX_KERNEL_FMA;
     if (!vec) return CX_KERNEL_GENERIC;
     if (pool->dtype == CX_F32) return split_shape(pool, b, tree) ? CX_KERNEL_FMA : CX_KERNEL_GENERIC;
     if (q_dtype != CX_F32 && q_dtype != pool->dtype) return CX_KERNEL_GENERIC;
@@ -75,6 +78,7 @@ static size_t attend_workspace(const cx_pool* pool, const cx_attn_batch* b, bool
                             : (size_t)(n_ctiles * b->batch * pool->n_kv_heads) * n_split * 256 *
                                   (pool->head_dim + 2) * 4;
     }
+    if (tree && tree_rows_shape(pool, b)) return tree_rows_workspace(pool, b);
     if (!split_shape(pool, b, tree)) return 256;
     return ws_layout(b->batch, unit_shape(pool, rows), rows, pool->head_dim, grid_size()).total;
 }
@@ -122,12 +126,6 @@ static int attend_split(const cx_pool* pool, int64_t layer, const cx_attn_batch&
     p.mod.slopes = m.alibi_slopes;
     p.mod.prefix = m.prefix_lens;
     p.plan_kind = m.prefix_lens ? 3 : 1;
-    // A tree's 16 or 32 fp32 rows are much work for a unit's few warps: a CTA for every
-    // unit while there are CTAs, and no range of more than three parts is left to its last
-    // CTA (8 trees of 8 nodes, 32 rows, behind up to 512 keys: chunks of 4 units 80 us,
-    // of 1 unit 72, and with ranges of 4 parts joined apart 55).
-    const bool fine = TREE && pool->dtype == CX_F32 && rows > 8;
-    if (fine) p.min_units = 1;
     p.mod.q_stride = m.q_stride;
     p.mod.out = out;
     p.mod.out_dtype = m.out_dtype;
@@ -159,7 +157,7 @@ static int attend_split(const cx_pool* pool, int64_t layer, const cx_attn_batch&
     // and the rest over 400, 227 -> 150 us, against 4 us more for 128 even ones (173 ->
     // 178).  Single tokens and fp32 gain nothing there (141 -> 147 us).
     if (2 * b.batch * sh.n_groups <= grid)
-        p.mod.join_min = fine ? 3 : 4;
+        p.mod.join_min = 4;
     else if (b.max_q_len > 1 && pool->dtype != CX_F32)
         p.mod.join_min = 16;
     switch (pool->dtype) {
@@ -308,6 +306,11 @@ static int attend_scored(const cx_pool* pool, int64_t layer, const cx_attn_batch
     const uintptr_t al = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) |
                          static_cast<uintptr_t>(m.q_stride * elem_bytes(q_dtype));
     cudaStream_t st = as_stream(stream);
+    if constexpr (TREE) {
+        if (tree_rows_shape(pool, &b))
+            return attend_tree_rows<TREE>(pool, layer, b, m, tree, scale, q, q_dtype, out, ws,
+                                          ws_bytes, st);
+    }
     const int kind = attend_kind(pool, &b, q_dtype, (al & 15) == 0, TREE);
     if (kind == CX_KERNEL_MMA || kind == CX_KERNEL_FMA)
         return attend_split<TREE>(pool, layer, b, m, tree, scale, q, q_dtype, out, ws, ws_bytes, replan,

@@ -161,6 +161,13 @@ __device__ __forceinline__ int tree_key_pos(const TreeMask& t, int64_t q0, int n
     return u >= 0 && u < n ? base + __ldg(t.depths + q0 + u) : base + u;
 }
 
+// Asynchronous 16-byte copy to shared memory; zeros when `there` is not set.
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
+                 "r"(there ? 16 : 0)
+                 : "memory");
+}
+
 // ---- packed fp32 pairs ------------------------------------------------------
 using f2 = unsigned long long;
 __device__ __forceinline__ f2 f2_of(float lo, float hi) {

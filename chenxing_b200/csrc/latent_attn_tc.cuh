@@ -288,13 +288,6 @@ __device__ __forceinline__ uint4 lat_q8(const LatParams& p, int64_t lat, int64_t
                       Half16<E>::pack(x[4], x[5]), Half16<E>::pack(x[6], x[7]));
 }
 
-// Asynchronous 16-byte copy to shared memory; zeros when `there` is not set.
-__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src),
-                 "r"(there ? 16 : 0)
-                 : "memory");
-}
-
 template <typename E>
 __host__ __device__ constexpr uint32_t lat_idesc(int m, int n, int a_mn, int b_mn) {
     return sc_idesc<E>(m, n, b_mn) | ((uint32_t)a_mn << 15);

@@ -153,6 +153,36 @@ def test_bad_block_ids_leave_their_keys_out():
     assert bool(((out[0].double().cpu() - want[0]).abs() <= tol[0]).all())
 
 
+@pytest.mark.parametrize("hq,q_lens", [(4, None), (16, [3])])
+def test_bad_block_ids_in_fp32(hq, q_lens):
+    from chenxing_b200 import _lib
+    c = LatentCase(hq=hq, dc=128, dr=32, ctx=[200], q_lens=q_lens, dtype=F32, seed=9)
+    batch = c.batch()
+    batch.block_tables[0, 3] = 10 ** 6
+    batch.block_tables[0, 7] = -5
+    out = c.run(batch)
+    assert _lib.device_flags(clear=True) == 2
+    c.check(out, hidden=list(range(48, 64)) + list(range(112, 128)))
+
+
+@pytest.mark.parametrize("hq,dtype", [(16, BF), (64, F16), (8, F32), (40, F32)])
+def test_batches_on_two_streams_at_once(hq, dtype):
+    """A batch a stream, each with a workspace of its own; the same calls one by one."""
+    c = LatentCase(hq=hq, dc=256, dr=64, ctx=[2500, 333], dtype=dtype, seed=4)
+    batches = [c.batch() for _ in range(2)]
+    want = c.run(batches[0], out_dtype=dtype)
+    c.check(want)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for _ in range(5):
+        for b, st in zip(batches, streams):
+            with torch.cuda.stream(st):
+                outs.append(c.run(b, out_dtype=dtype))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
 def test_wait_limit():
     """Waits that run out end the call with an error, and the next call is right."""
     from chenxing_b200 import _lib

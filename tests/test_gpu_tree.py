@@ -51,6 +51,8 @@ SHAPES = [
     (4, 2, 80, BF, [9, 21], [50, 300]),
     (6, 3, 40, F32, [12, 1], [100, 17]),
     (8, 2, 64, F32, [40, 20], [100, 317]),
+    (4, 1, 64, F32, [2, 1, 0], [700, 20, 9]),
+    (3, 1, 128, F32, [3, 40], [5000, 41]),
     # tcgen05: one query tile in two places
     (8, 2, 128, BF, [26, 10, 1, 0, 17], [26, 600, 129, 16, 140]),
     (32, 8, 128, BF, [26, 12], [1000, 127]),
@@ -79,8 +81,8 @@ def test_kernels_of_the_shapes():
     for hq, hk, d, dtype, sizes, ctx in SHAPES:
         kinds.append(_case("plain", "star", hq, sizes, ctx, hk=hk, d=d, dtype=dtype)
                      .batch().kernel_kind(dtype, dtype))
-    assert kinds == ["fma", "fma", "mma", "mma", "mma", "mma", "generic", "generic", "generic"] \
-        + ["tcgen05"] * 10
+    assert kinds == ["fma", "fma", "mma", "mma", "mma", "mma", "generic", "generic", "fma", "fma",
+                     "fma"] + ["tcgen05"] * 10
 
 
 @pytest.mark.parametrize("hq,hk,d,dtype,n", [(8, 2, 128, BF, 7), (8, 2, 128, BF, 13),
@@ -104,6 +106,63 @@ def test_type_mixes(dtype, q_dtype, out_dtype, n):
     c = _case("plain", "random", 8, [n, 3], [70, 300], hk=2, d=128, dtype=dtype, q_dtype=q_dtype,
               strided=True)
     c.check(c.run(out_dtype=out_dtype))
+
+
+@pytest.mark.parametrize("bs", [1, 5, 64])
+def test_blocks_of_other_sizes(bs):
+    c = _case("alibi-cap-window", "random", 8, [21, 0, 4], [150, 7, 4], hk=2, d=64, dtype=F32, bs=bs)
+    assert c.batch().kernel_kind(F32) == "fma"
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("hq,dtype,n", [(8, F32, 2), (8, F32, 9), (8, BF, 6), (8, BF, 26)])
+@pytest.mark.parametrize("prefix", [None, [21]])
+def test_bad_block_ids_leave_their_keys_out(hq, dtype, n, prefix):
+    from chenxing_b200 import _lib
+    c = _case("plain", "random", hq, [n], [200 + n], hk=2, d=64, dtype=dtype, prefix=prefix)
+    batch = c.batch()
+    batch.block_tables[0, 3] = 10 ** 6
+    batch.block_tables[0, 7] = -5
+    out = c.run(batch, out_dtype=dtype)
+    assert _lib.device_flags(clear=True) == 2
+    c.check(out, list(range(48, 64)) + list(range(112, 128)))
+
+
+def test_batches_on_two_streams_at_once():
+    """A batch a stream, each with a workspace of its own; the same calls one by one."""
+    shapes = [(8, 2, 64, F32, [9, 12]), (8, 2, 128, BF, [26, 12]), (8, 2, 128, BF, [3, 6])]
+    for hq, hk, d, dtype, sizes in shapes:
+        c = _case("alibi", "random", hq, sizes, [2500, 333], hk=hk, d=d, dtype=dtype)
+        batches = [c.batch() for _ in range(2)]
+        want = c.run(batches[0])
+        c.check(want)
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        outs = []
+        for _ in range(5):
+            for b, st in zip(batches, streams):
+                with torch.cuda.stream(st):
+                    outs.append(c.run(b))
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs)
+
+
+def test_two_graphs_share_a_workspace():
+    c = _case("plain", "deep", 8, [9, 30], [1500, 333], hk=2, d=64, dtype=F32)
+    batch = c.batch()
+    want = c.run(batch)
+    outs = [torch.empty_like(want) for _ in range(2)]
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for g, o in zip(graphs, outs):
+        with torch.cuda.graph(g):
+            c.run(batch, out=o)
+    for _ in range(2):
+        for o in outs:
+            o.zero_()
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs)
 
 
 def test_float32_output_takes_the_tree_too():
