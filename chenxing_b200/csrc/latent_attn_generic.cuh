@@ -198,6 +198,7 @@ __global__ void __launch_bounds__(kLgWarps * 32) latent_generic_kernel(const Lat
             }
         }
     }
+    asm volatile("griddepcontrol.launch_dependents;");
     // ---- the four warps' states, then the output or this CTA's part ----
     extern __shared__ float gsm[];                // [warp][row][dc + 2]
     const int mrow = p.dc + 2;
@@ -422,6 +423,7 @@ __global__ void __launch_bounds__(kLrWarps * 32, 1) latent_rows_kernel(const Lat
         }
         __syncwarp();
     }
+    asm volatile("griddepcontrol.launch_dependents;");
     if (bad && lane == 0) raise_flag(CX_DEV_BAD_BLOCK);
     const int64_t row0 = (int64_t)qs * p.heads + r0;
     const int mrow = p.dc + 2;
@@ -457,6 +459,7 @@ __global__ void __launch_bounds__(kLrWarps * 32, 1) latent_rows_kernel(const Lat
 // Joins the parts of a context that was split: one CTA per row.  Lanes fetch the parts'
 // references side by side; there are at most 256.
 __global__ void __launch_bounds__(128) latent_generic_join(const LatGenParams g) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const LatParams& p = g.a;
     const int unit = (int)blockIdx.x, b = unit / g.row_tiles, rt = unit - b * g.row_tiles;
     const int r = blockIdx.y, lane = threadIdx.x & 31;
@@ -489,6 +492,20 @@ __global__ void __launch_bounds__(128) latent_generic_join(const LatGenParams g)
     }
 }
 
+static int launch_latent_generic_join(const LatGenParams& g, int64_t units, cudaStream_t st) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)units, g.unit_rows);
+    cfg.blockDim = 128;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    CX_CUDA_CHECK(cudaLaunchKernelEx(&cfg, latent_generic_join, g));
+    return check_launch("latent_generic_join");
+}
+
 template <typename KT>
 static int launch_latent_generic(const LatGenParams& g, cudaStream_t st) {
     const int64_t units = (int64_t)g.a.batch * g.row_tiles;
@@ -511,8 +528,7 @@ static int launch_latent_generic(const LatGenParams& g, cudaStream_t st) {
                        : nc == 3 ? go(latent_rows_kernel<KT, 3>)
                                  : go(latent_rows_kernel<KT, 4>);
         if (rc || g.n_split == 1) return rc;
-        latent_generic_join<<<dim3((unsigned)units, g.unit_rows), 128, 0, st>>>(g);
-        return check_launch("latent_generic_join");
+        return launch_latent_generic_join(g, units, st);
     }
     if (g.a.dim <= 192)
         latent_generic_kernel<KT, 6><<<grid, kLgWarps * 32, smem, st>>>(g);
@@ -522,8 +538,7 @@ static int launch_latent_generic(const LatGenParams& g, cudaStream_t st) {
         latent_generic_kernel<KT, 18><<<grid, kLgWarps * 32, smem, st>>>(g);
     int rc = check_launch("latent_generic_kernel");
     if (rc || g.n_split == 1) return rc;
-    latent_generic_join<<<dim3((unsigned)units, g.unit_rows), 128, 0, st>>>(g);
-    return check_launch("latent_generic_join");
+    return launch_latent_generic_join(g, units, st);
 }
 
 }  // namespace cx
