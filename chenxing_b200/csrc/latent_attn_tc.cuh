@@ -329,8 +329,10 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
     uint64_t* s_full = empty + kLatMaxStages * kLatMaxPieces;     // [2] S^T of a tile is there
     uint64_t* p_full = s_full + 2;                // [2] P^T written, O^T rescaled
     uint64_t* o_done = p_full + 2;                // O^T of a tile is done
-    uint64_t* q_full = o_done + 1;                // Q of a range is there
-    uint64_t* drain = q_full + 1;                 // [2] last commits of the MMA warps
+    // [2] Q of a range is there, by the range's parity: behind a range of one tile the
+    // softmax warps come to the next range's before the PV warp need have seen this one's
+    uint64_t* q_full = o_done + 1;
+    uint64_t* drain = q_full + 2;                 // [2] last commits of the MMA warps
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drain + 2);
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
     volatile int* s_issued = s_abort + 1;         // [kLatProd] tiles whose loads were begun
@@ -352,7 +354,8 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
         mbar_init(&p_full[0], SW);
         mbar_init(&p_full[1], SW);
         mbar_init(o_done, 1);
-        mbar_init(q_full, SW);
+        mbar_init(&q_full[0], SW);
+        mbar_init(&q_full[1], SW);
         mbar_init(&drain[0], 1);
         mbar_init(&drain[1], 1);
         *s_abort = 0;
@@ -495,12 +498,13 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
         };
         int ranges = 0;
         auto q_ready = [&](int n) {                  // n tiles; 0: no further range
+            uint64_t* there = &q_full[ranges & 1];
             if (tid == 0) s_n[ranges & 1] = n;
             ++ranges;
             if (q_async) asm volatile("cp.async.wait_all;" ::: "memory");
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(q_full);
+            if (lane == 0) mbar_arrive(there);
         };
         bool more = cur.next(p, sub_id, N, seg);
         if (more) load_q(seg.x);
@@ -859,7 +863,7 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
         int st = 0;                               // stage of the next tile
         uint32_t use = 0;                         // parity of its fill
         for (int range = 0;; ++range) {
-            ok = el_wait(q_full, range & 1, s_abort, p.tries);
+            ok = el_wait(&q_full[range & 1], (range >> 1) & 1, s_abort, p.tries);
             const int n = (int)warp_uniform(s_n[range & 1]);
             if (!ok || n == 0) break;
             for (int i = 0; ok && i < n; ++i, ++tile) {
