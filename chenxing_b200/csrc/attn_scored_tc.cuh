@@ -717,7 +717,11 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
                     x[256 + w * 128 + r] = l;
                 }
                 if (!ok) *s_abort = 1;
+                // (the other place's O as well is read below: its warps saw its last product
+                // finish and met these here)
+                tc_fence_before();
                 named_bar_sync(2, C::SOFTMAX);
+                tc_fence_after();
                 ok = __all_sync(0xffffffffu, !*s_abort);
                 const float m0 = x[r], m1 = x[128 + r], M = fmaxf(m0, m1);
                 const float f0 = M == -INFINITY ? 0.f : exp2f(m0 - M);

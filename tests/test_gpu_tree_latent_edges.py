@@ -1,9 +1,10 @@
 """Edges of the drafted trees, the accepted paths and the latent cache (bounds:
 tree_cases)."""
+import numpy as np
 import pytest
 import torch
 
-from tree_cases import LatentCase
+from tree_cases import LatentCase, TreeCase, random_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -32,4 +33,21 @@ def test_many_ranges_of_one_tile(hq, dc, dr, dtype, q_lens):
     a = c.run(batch, out_dtype=dtype)
     c.check(a)
     for _ in range(5):
+        assert torch.equal(a, c.run(batch, out_dtype=dtype))
+
+
+@pytest.mark.parametrize("hq,hk,d,dtype", [(8, 2, 128, BF), (4, 4, 64, F16)])
+def test_two_places_that_end_apart(hq, hk, d, dtype):
+    """Trees of one query tile, held in two places, behind 1 to 10 key tiles: the places
+    have as many or differ by one, and each is read by the other's warps."""
+    rng = np.random.default_rng(d)
+    ctx = [60 + 128 * i for i in range(10)] + [128 * i + 1 for i in range(1, 10)]
+    n = 15 if hq > hk else 40
+    parents = [random_tree(rng, n, "random") for _ in ctx]
+    c = TreeCase(hq=hq, hk=hk, d=d, dtype=dtype, ctx=ctx, parents=parents, seed=d)
+    batch = c.batch()
+    assert batch.kernel_kind(dtype, dtype) == "tcgen05"
+    a = c.run(batch, out_dtype=dtype)
+    c.check(a)
+    for _ in range(30):
         assert torch.equal(a, c.run(batch, out_dtype=dtype))
