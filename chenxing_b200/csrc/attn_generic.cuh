@@ -411,10 +411,10 @@ __global__ void __launch_bounds__(kGenWarps * 32) attn_generic_kernel(GenericPar
         float M = -INFINITY;
         for (int w = 0; w < kGenWarps; ++w) M = fmaxf(M, s_m[((size_t)w * kGenRows + r) * mrow + DV]);
         float Lsum = 0.f, O = 0.f;
-        if (M != -INFINITY) {
+        if (MOD || M != -INFINITY) {
             for (int w = 0; w < kGenWarps; ++w) {
                 const float* src = s_m + ((size_t)w * kGenRows + r) * mrow;
-                const float wgt = expf(src[DV] - M);
+                const float wgt = expf(src[DV] - ref_base(M));
                 Lsum += src[DV + 1] * wgt;
                 O += src[d] * wgt;
             }
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(kGenWarps * 32) attn_generic_kernel(GenericPar
         const int64_t R = r0 + r, i = R / G, h = kh * G + R % G;
         const int64_t ooff = PAGED ? ((q0 + i) * p.hq + h) * p.dv : ((b * p.hq + h) * sq + i) * p.dv;
         if constexpr (MOD)
-            store_as(p.mod_out, p.mod.out_dtype, ooff + d, Lsum > 0.f ? O / Lsum : 0.f);
+            store_as(p.mod_out, p.mod.out_dtype, ooff + d, Lsum == 0.f ? 0.f : O / Lsum);
         else
             p.out[ooff + d] = Lsum > 0.f ? O / Lsum : 0.f;
     }

@@ -415,23 +415,20 @@ __device__ __forceinline__ void ks_merge(const MmaParams& p, const float* merge,
             float L = 0.f, o[D / 32];
 #pragma unroll
             for (int k = 0; k < D / 32; ++k) o[k] = 0.f;
-            if (M != -INFINITY) {
-                for (int s2 = 0; s2 < KS; ++s2) {
-                    const float* r = row0 + s2 * step;
-                    const float wgt = exp2f(r[D] - M);
-                    L += r[D + 1] * wgt;
+            for (int s2 = 0; s2 < KS; ++s2) {
+                const float* r = row0 + s2 * step;
+                const float wgt = exp2f(r[D] - ref_base(M));
+                L += r[D + 1] * wgt;
 #pragma unroll
-                    for (int k = 0; k < D / 64; ++k) {
-                        const float2 v =
-                            *reinterpret_cast<const float2*>(r + k * 64 + 2 * lane);
-                        o[2 * k] += v.x * wgt;
-                        o[2 * k + 1] += v.y * wgt;
-                    }
+                for (int k = 0; k < D / 64; ++k) {
+                    const float2 v = *reinterpret_cast<const float2*>(r + k * 64 + 2 * lane);
+                    o[2 * k] += v.x * wgt;
+                    o[2 * k + 1] += v.y * wgt;
                 }
             }
             if (seg.whole) {
                 const int64_t orow = (qs + R / G) * Hq + (int64_t)(seg.g * HG + eh) * G + R % G;
-                const float inv = L > 0.f ? 1.f / L : 0.f;
+                const float inv = sum_inv(L);
 #pragma unroll
                 for (int k = 0; k < D / 64; ++k)
                     put2<MOD>(p, orow * D + k * 64 + 2 * lane, o[2 * k] * inv,
@@ -551,7 +548,7 @@ __device__ __forceinline__ void ticket_merge(const MmaParams& p, const Seg& seg,
                         Mn = fmaxf(Mn, __shfl_xor_sync(0xffffffffu, Mn, s2));
                     Mn = fmaxf(Mn, M[u]);
                     // (a partial that saw no key: weight 0, its columns are 0)
-                    const float base = Mn == -INFINITY ? 0.f : Mn;
+                    const float base = ref_base(Mn);
                     const float a = exp2f(M[u] - base);
                     w[u] = exp2f(m - base);
                     float ls = l * w[u];
@@ -584,7 +581,7 @@ __device__ __forceinline__ void ticket_merge(const MmaParams& p, const Seg& seg,
                 if (q >= n_rows) continue;
                 const int eh = q / rows_b, R = q - eh * rows_b;
                 const int64_t orow = (qs + R / G) * Hq + (int64_t)(seg.g * HG + eh) * G + R % G;
-                const float inv = L[u] > 0.f ? 1.f / L[u] : 0.f;
+                const float inv = sum_inv(L[u]);
 #pragma unroll
                 for (int k = 0; k < D / 64; ++k)
                     put2<MOD>(p, orow * D + k * 64 + 2 * lane, o[u][2 * k] * inv,
@@ -694,7 +691,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const MmaParams p) {
         for (int s2 = 16; s2; s2 >>= 1) Mn = fmaxf(Mn, __shfl_xor_sync(0xffffffffu, Mn, s2));
         Mn = fmaxf(Mn, M);
         // (a partial that saw no key: weight 0, its columns are 0)
-        const float base = Mn == -INFINITY ? 0.f : Mn;
+        const float base = ref_base(Mn);
         const float a = exp2f(M - base), w = exp2f(m - base);
         float ls = l * w;
 #pragma unroll
@@ -729,7 +726,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const MmaParams p) {
     M = s_m[0];
 #pragma unroll
     for (int w = 1; w < 8; ++w) M = fmaxf(M, s_m[w]);
-    const float base = M == -INFINITY ? 0.f : M;
+    const float base = ref_base(M);
     float x = 0.f, y = 0.f;
     L = 0.f;
 #pragma unroll
@@ -739,7 +736,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const MmaParams p) {
         x += s_o[w][d] * wgt;
         y += s_o[w][d + 1] * wgt;
     }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const float inv = sum_inv(L);
     const int64_t orow = (qs + R / G) * p.hq + (int64_t)(g * p.hg + eh) * G + R % G;
     put2<true>(p, orow * D + d, x * inv, y * inv);
 }
@@ -1348,7 +1345,7 @@ __global__ void __launch_bounds__(MOD ? MmaCfg<D, MT, HG>::THREADS_MOD
                 if (R >= rows_b) continue;
                 const float mm = half ? m1 : m0, ll = half ? l1 : l0;
                 if (seg.whole) {
-                    const float inv = ll > 0.f ? 1.f / ll : 0.f;
+                    const float inv = MOD ? sum_inv(ll) : ll > 0.f ? 1.f / ll : 0.f;
                     const int64_t orow = (qs + R / G) * Hq + (int64_t)h * G + R % G;
 #pragma unroll
                     for (int n = 0; n < C::NT; ++n)

@@ -724,8 +724,7 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
                 tc_fence_after();
                 ok = __all_sync(0xffffffffu, !*s_abort);
                 const float m0 = x[r], m1 = x[128 + r], M = fmaxf(m0, m1);
-                const float f0 = M == -INFINITY ? 0.f : exp2f(m0 - M);
-                const float f1 = M == -INFINITY ? 0.f : exp2f(m1 - M);
+                const float f0 = exp2f(m0 - ref_base(M)), f1 = exp2f(m1 - ref_base(M));
                 const float L = x[256 + r] * f0 + x[384 + r] * f1;
                 const bool two = g.n_tiles > 1;              // (the second has an O)
                 const int64_t o_row = ((int64_t)(qs + (g.t0 + r / G)) * p.hq + h * G + r % G) * D;
@@ -738,7 +737,7 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
                         to[D + 1] = L;
                     }
                 }
-                const float inv = to ? 1.f : L > 0.f ? 1.f / L : 0.f;
+                const float inv = to ? 1.f : sum_inv(L);
                 // a quarter of the columns a thread: 16 at a time
                 const uint32_t tm_c = tmem + 2 * kScKeys + lane_off;
 #pragma unroll 1
@@ -776,7 +775,7 @@ __global__ void __launch_bounds__(ScCfg<DH>::THREADS, 1)
                 }
             }
             if (ok) {
-                const float inv = part ? 1.f : l > 0.f ? 1.f / l : 0.f;
+                const float inv = part ? 1.f : sum_inv(l);
                 const int64_t o_row = ((int64_t)(qs + t_e) * p.hq + head_e) * D + c * (D / 2);
 #pragma unroll 1
                 for (int k = 0; k < D / 64; ++k) {
@@ -1137,14 +1136,13 @@ __global__ void __launch_bounds__(256) scored_tc_join_kernel(const ScoredTcParam
 #pragma unroll
     for (int e = 0; e < D / 32; ++e) o[e] = 0.f;
     for (int s = 0; s < p.n_split; ++s) {
-        const float m = src[s * STEP + D];
-        if (m == -INFINITY) continue;          // a part that saw no key
-        const float f = exp2f(m - M);
-        L = fmaf(src[s * STEP + D + 1], f, L);
+        const float m = src[s * STEP + D], f = exp2f(m - ref_base(M));
+        L = fmaf(src[s * STEP + D + 1], f, L);  // (of a part of NaN: NaN)
+        if (m == -INFINITY) continue;           // a part that saw no key
 #pragma unroll
         for (int e = 0; e < D / 32; ++e) o[e] = fmaf(src[s * STEP + e * 32 + lane], f, o[e]);
     }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const float inv = sum_inv(L);
     const int64_t row = ((int64_t)(qs + t) * p.hq + h * p.group + r % p.group) * D;
 #pragma unroll
     for (int e = 0; e < D / 32; ++e) store_as(p.out, p.out_dtype, row + e * 32 + lane, o[e] * inv);

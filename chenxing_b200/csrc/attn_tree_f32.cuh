@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kTrWarps * 32, 2) tree_rows_kernel(const TreeR
                 m[r] = top;
                 moved = true;
             }
-            pr[r] = see ? expf(s - m[r]) : 0.f;
+            pr[r] = see ? expf(s - ref_base(m[r])) : 0.f;
             l[r] = fmaf(l[r], corr[r], pr[r]);
         }
         s_p[lane] = make_float4(pr[0], pr[1], pr[2], pr[3]);
@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kTrWarps * 32, 2) tree_rows_kernel(const TreeR
             if (lane == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(m[r], L);
         } else {
             const int R = x.r0 + R0 + r;
-            const float inv = L > 0.f ? 1.f / L : 0.f;
+            const float inv = sum_inv(L);
             const int64_t row = (int64_t)(x.qs + R / G) * p.hq + x.kh * G + R % G;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(D) tree_rows_join(const TreeRowsParams p) {
 #pragma unroll
     for (int w = 16; w; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
     for (int s = lane; s < p.n_split; s += 32) {
-        const float f = M == -INFINITY ? 0.f : expf(src[s * STEP + D] - M);
+        const float f = expf(src[s * STEP + D] - ref_base(M));
         L = fmaf(src[s * STEP + D + 1], f, L);
         if (threadIdx.x < 32) s_f[s] = f;
     }
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(D) tree_rows_join(const TreeRowsParams p) {
     const int R = x.r0 + r;
     store_as(p.out, p.out_dtype,
              ((int64_t)(x.qs + R / p.group) * p.hq + x.kh * p.group + R % p.group) * D + threadIdx.x,
-             L > 0.f ? O / L : 0.f);
+             L == 0.f ? 0.f : O / L);
 }
 
 // fp32 pools with heads of 64 or 128 on 16-byte rows, blocks of any size.

@@ -168,6 +168,16 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool ther
                  : "memory");
 }
 
+// ---- ends of a softmax ------------------------------------------------------
+// A row's weight from its sum of exponentials: 0 where it saw no key.  NaN stays NaN (a
+// comparison with `> 0` would turn a row of NaN scores into zeros).
+__device__ __forceinline__ float sum_inv(float l) { return l == 0.f ? 0.f : 1.f / l; }
+
+// The reference that exponentials are taken against: 0 for a part whose scores have no
+// maximum.  The weight of its sum is then 0 (2^-inf), and 0 * NaN hands on the NaN of scores
+// that were no numbers.
+__device__ __forceinline__ float ref_base(float m) { return m == -INFINITY ? 0.f : m; }
+
 // ---- packed fp32 pairs ------------------------------------------------------
 using f2 = unsigned long long;
 __device__ __forceinline__ f2 f2_of(float lo, float hi) {

@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kLgWarps * 32) latent_generic_kernel(const Lat
 #pragma unroll
             for (int j = 0; j < NK; ++j) {
                 if (!((sees[j] >> r) & 1u)) continue;     // adds nothing, whatever it holds
-                const float w = expf(s[j][r] - top);
+                const float w = expf(s[j][r] - ref_base(top));
                 l[r] += w;
 #pragma unroll
                 for (int e = 0; e < KE; ++e) o[r][e] = fmaf(w, x[j][e], o[r][e]);
@@ -221,8 +221,8 @@ __global__ void __launch_bounds__(kLgWarps * 32) latent_generic_kernel(const Lat
         const size_t step = (size_t)kLgRows * mrow;
         float M = -INFINITY, L = 0.f, O = 0.f;
         for (int w = 0; w < kLgWarps; ++w) M = fmaxf(M, src[w * step + p.dc]);
-        for (int w = 0; M != -INFINITY && w < kLgWarps; ++w) {
-            const float f = expf(src[w * step + p.dc] - M);
+        for (int w = 0; w < kLgWarps; ++w) {
+            const float f = expf(src[w * step + p.dc] - ref_base(M));
             L = fmaf(src[w * step + p.dc + 1], f, L);
             O = fmaf(src[w * step + d], f, O);
         }
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kLgWarps * 32) latent_generic_kernel(const Lat
                 dst[p.dc + 1] = L;
             }
         } else {
-            store_as(p.out, p.out_dtype, (row0 + r) * p.dc + d, L > 0.f ? O / L : 0.f);
+            store_as(p.out, p.out_dtype, (row0 + r) * p.dc + d, L == 0.f ? 0.f : O / L);
         }
     }
 }
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(kLrWarps * 32, 1) latent_rows_kernel(const Lat
                 m[r] = top;
                 moved = true;
             }
-            pr[r] = see ? expf(x - m[r]) : 0.f;
+            pr[r] = see ? expf(x - ref_base(m[r])) : 0.f;
             l[r] = fmaf(l[r], corr[r], pr[r]);
         }
         s_p[lane] = make_float4(pr[0], pr[1], pr[2], pr[3]);
@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(kLrWarps * 32, 1) latent_rows_kernel(const Lat
                          ? g.part + (((int64_t)unit * g.n_split + blockIdx.y) * kLrRows + R0 + r) *
                                         mrow
                          : nullptr;
-        const float inv = L > 0.f ? 1.f / L : 0.f;
+        const float inv = sum_inv(L);
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(128) latent_generic_join(const LatGenParams g)
 #pragma unroll
     for (int w = 16; w; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
     for (int s = lane; s < g.n_split; s += 32) {
-        const float f = M == -INFINITY ? 0.f : expf(src[s * step + p.dc] - M);
+        const float f = expf(src[s * step + p.dc] - ref_base(M));
         L = fmaf(src[s * step + p.dc + 1], f, L);
         if (threadIdx.x < 32) s_f[s] = f;
     }
@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(128) latent_generic_join(const LatGenParams g)
 #pragma unroll 8
         for (int s = 0; s < g.n_split; ++s) O = fmaf(src[s * step + d], s_f[s], O);
         store_as(p.out, p.out_dtype, ((int64_t)qs * p.heads + r0 + r) * p.dc + d,
-                 L > 0.f ? O / L : 0.f);
+                 L == 0.f ? 0.f : O / L);
     }
 }
 

@@ -632,8 +632,7 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
                 uint32_t pk[NW / 4];
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
-                    const float b0 = m[j][0] == -INFINITY ? 0.f : m[j][0];
-                    const float b1 = m[j][1] == -INFINITY ? 0.f : m[j][1];
+                    const float b0 = ref_base(m[j][0]), b1 = ref_base(m[j][1]);
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
                         pk[2 * j + t] = Half16<E>::pack(ex2_sfu(v[4 * j + 2 * t] - b0),
@@ -705,7 +704,7 @@ __global__ void __launch_bounds__(LatCfg<N>::THREADS, 1)
             const int64_t part = ((int64_t)blockIdx.x * 2 + slot) * N;
             if (tid < N) {
                 const float L = (s_red[tid] + s_red[64 + tid]) + (s_red[128 + tid] + s_red[192 + tid]);
-                s_alpha[tid] = whole ? (L > 0.f ? 1.f / L : 0.f) : 1.f;
+                s_alpha[tid] = whole ? sum_inv(L) : 1.f;
                 if (!whole) p.part_ml[(part + tid) * 2 + 1] = L;
             }
             if (!whole && quad == 0 && lane < 4) {
@@ -981,8 +980,8 @@ __global__ void __launch_bounds__(256) latent_join_kernel(const LatParams p) {
         float top = fmaxf(ml.x, M);
 #pragma unroll
         for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-        if (top == -INFINITY) continue;           // parts that saw no key
-        const float old = exp2f(M - top), f = exp2f(ml.x - top);
+        // (parts that saw no key: weight 0; of parts of NaN the sums are NaN)
+        const float base = ref_base(top), old = exp2f(M - base), f = exp2f(ml.x - base);
         M = top;
         float sum = ml.y * f;
 #pragma unroll
@@ -1010,7 +1009,7 @@ __global__ void __launch_bounds__(256) latent_join_kernel(const LatParams p) {
             }
         }
     }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const float inv = sum_inv(L);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (col + e < p.dc) store_as(p.out, p.out_dtype, row * p.dc + col + e, o[e] * inv);

@@ -302,7 +302,8 @@ typedef struct cx_attn_mods {
  *     seen = j < prefix  or  (j <= pos and (window <= 0 or j > pos - window))
  * over keys j < ctx_lens[b].  out is [rows][n_q_heads][head_dim] of
  * out_dtype, rounded once from the fp32 accumulators; a row that sees no key is
- * zero.  out may be q itself (one type, contiguous), but not overlap it
+ * zero, one that sees a score of NaN is NaN.  out may be q itself (one type,
+ * contiguous), but not overlap it
  * otherwise.
  * What the pool holds at positions that no query row of a sequence sees (past
  * the context in its last block, left of every row's window) does not reach the
@@ -437,7 +438,8 @@ typedef struct cx_latent_q {
  *     out  = sum_j softmax(s)[j] row_j[:latent_dim]
  * over the keys that cx_paged_decode (q_start NULL) or cx_paged_verify would show it,
  * or with `tree` those of cx_paged_attend_tree.  out is [rows][n_q_heads][latent_dim]
- * of out_dtype, rounded once from fp32; a row that sees no key is zero.  scale NaN
+ * of out_dtype, rounded once from fp32; a row that sees no key is zero, one that sees a
+ * score of NaN is NaN.  scale NaN
  * selects 1/sqrt(latent_dim + rope_dim); a model's scale is that of its heads before
  * they were absorbed.  What the pool holds where no query row sees it does not
  * reach the result; at a position that only some rows see, it must be finite.

@@ -1,9 +1,12 @@
 """Edges of the drafted trees, the accepted paths and the latent cache (bounds:
 tree_cases)."""
+import math
+
 import numpy as np
 import pytest
 import torch
 
+from scored_cases import ScoredCase, alibi
 from tree_cases import LatentCase, TreeCase, random_tree
 
 pytestmark = pytest.mark.gpu
@@ -51,3 +54,64 @@ def test_two_places_that_end_apart(hq, hk, d, dtype):
     c.check(a)
     for _ in range(30):
         assert torch.equal(a, c.run(batch, out_dtype=dtype))
+
+
+def _check_nan_rows(c, out, rows):
+    """`rows` (token, head) hold NaN throughout, every other row is as without them."""
+    bad = torch.zeros(out.shape[:2], dtype=torch.bool)
+    for r in rows:
+        bad[r] = True
+    got = out.double().cpu()
+    assert bool(torch.isnan(got[bad]).all()), "a row of NaN queries came out finite"
+    got[bad] = c.expected(out.dtype, "any")[0][bad] if isinstance(c, LatentCase) \
+        else c.expected(out.dtype)[0][bad]
+    c.check(got.to(out.dtype))
+
+
+@pytest.mark.parametrize("ctx", [[40, 200], [3000, 70]])
+@pytest.mark.parametrize("hq,hk,d,dtype,n", [
+    (8, 2, 64, F32, 2), (8, 2, 64, F32, 8), (8, 2, 128, BF, 7), (32, 4, 64, F16, 6),
+    (8, 2, 128, BF, 9), (4, 4, 64, F16, 9), (8, 2, 80, BF, 9)])
+# (a capped infinity is the cap)
+@pytest.mark.parametrize("value,mods", [
+    (math.nan, dict()), (math.inf, dict()), (math.nan, dict(softcap=20.0, slopes="alibi"))])
+def test_nan_queries_of_trees(value, ctx, hq, hk, d, dtype, n, mods):
+    """A NaN or infinite query element gives NaN scores (an infinite one scores +inf and
+    -inf, whose softmax is NaN): the row is NaN whatever kernel takes it and however its
+    keys are cut, and the others are untouched."""
+    mods = dict(mods)
+    if mods.get("slopes"):
+        mods["slopes"] = alibi(hq)
+    rng = np.random.default_rng(d)
+    c = TreeCase(hq=hq, hk=hk, d=d, dtype=dtype, ctx=ctx,
+                 parents=[random_tree(rng, n, "random") for _ in ctx], seed=d, **mods)
+    rows = [(0, 1), (n + 1, hq - 1)]
+    for r in rows:
+        c.q_dev[r][3] = value
+    _check_nan_rows(c, c.run(out_dtype=dtype), rows)
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("ctx", [[40, 200], [3000, 70]])
+@pytest.mark.parametrize("hq,dc,dr,dtype,n", [
+    (4, 128, 32, F32, 1), (6, 300, 6, F32, 2), (20, 256, 64, F32, 3), (16, 512, 64, BF, 1),
+    (16, 256, 64, F16, 3), (40, 512, 64, BF, 9)])
+def test_nan_queries_of_latents(value, ctx, hq, dc, dr, dtype, n):
+    c = LatentCase(hq=hq, dc=dc, dr=dr, dtype=dtype, ctx=ctx, q_lens=[n, n], seed=dc)
+    rows = [(0, 1), (2 * n - 1, hq - 1)]
+    for r in rows:
+        c.q_dev[0][r][3] = value
+    _check_nan_rows(c, c.run(out_dtype=dtype), rows)
+
+
+@pytest.mark.parametrize("ctx", [[40, 200], [3000, 70]])
+@pytest.mark.parametrize("hq,hk,d,dtype,n", [(8, 2, 64, F32, 3), (8, 2, 128, BF, 5),
+                                             (4, 4, 64, F16, 100), (8, 2, 80, BF, 9)])
+def test_nan_queries_of_scored_chains(ctx, hq, hk, d, dtype, n):
+    n = min(n, min(ctx))
+    c = ScoredCase(hq=hq, hk=hk, d=d, dtype=dtype, ctx=ctx, q_lens=[n, n], softcap=20.0,
+                   slopes=alibi(hq), seed=d)
+    rows = [(0, 1), (2 * n - 1, hq - 1)]
+    for r in rows:
+        c.q_dev[r][3] = math.nan
+    _check_nan_rows(c, c.run(out_dtype=dtype), rows)
