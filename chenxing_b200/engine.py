@@ -371,11 +371,11 @@ class BatchedKVEngine:
         return self.cache.decode_batch(layer, q, plan.batch, out, out_dtype=out_dtype)
 
     def accept(self, plan: StepPlan, paths) -> None:
-        """End a verified step with one path of each sequence's tree (or of its
-        chain): lists of query rows of ``plan``, ascending.  Their K/V move behind the
-        committed context in every layer, and as many positions are committed
-        (``commit`` is for steps that keep every row).  The tokens are the
-        caller's to record (``extend_tokens``)."""
+        """End a verified step with one path of each sequence's tree: lists of query
+        rows of ``plan``, each the parent of the next; of a chain, its first rows.
+        Their K/V move behind the committed context in every layer, and as many
+        positions are committed (``commit`` is for steps that keep every row).  The
+        tokens are the caller's to record (``extend_tokens``)."""
         if plan.batch is None:
             raise RuntimeError("plan(..., attend=False) has no attention batch")
         paths = [list(map(int, p)) for p in paths]
@@ -383,6 +383,8 @@ class BatchedKVEngine:
             raise RuntimeError("accept() after the plan's sequences moved on")
         if len({id(s) for s in plan.seqs}) != len(plan.seqs):
             raise ValueError("accept() of a plan that has a sequence twice")
+        if not plan.tree and any(p != list(range(len(p))) for p in paths):
+            raise ValueError("a path of a chain is its first rows")
         self.cache.accept_paths(plan.batch, paths)
         for s, p in zip(plan.seqs, paths):
             s.n_tokens += len(p)

@@ -471,8 +471,12 @@ class _BlockPool(RadixIndex):
 
         paths: lists of node numbers, or an integer tensor (B, n) in which a negative
         entry ends a path (a device tensor is read in stream order, so that a
-        captured graph takes each replay's paths).  A path ascends strictly; lists are
-        checked here, a tensor by the kernel ("bad path of accepted nodes")."""
+        captured graph takes each replay's paths).  A path ascends strictly, and over a
+        batch with ``tree_parents`` each node is the parent of the next, from a node
+        behind the committed context on.  Lists are checked here; of a tensor the kernel
+        checks that it ascends over drafted rows ("bad path of accepted nodes"), not the
+        parents.  Without ``tree_parents`` the batch knows no tree: which rows belong
+        together is the caller's to say."""
         if batch.cache is not self:
             raise ValueError("the batch belongs to a different cache")
         if isinstance(paths, torch.Tensor):
@@ -492,6 +496,10 @@ class _BlockPool(RadixIndex):
             for p, n in zip(rows, batch.q_lens_host):
                 if any(not 0 <= x < n for x in p) or any(a >= b for a, b in zip(p, p[1:])):
                     raise ValueError("a path must ascend over the sequence's query rows")
+            for p, up in zip(rows, batch.tree_parents or ()):
+                if any(up[x] != y for x, y in zip(p, [-1] + p)):
+                    raise ValueError("a path must go from a node behind the committed context "
+                                     "to a child each")
             a = np.full((len(rows), max(map(len, rows), default=0)), -1, dtype=np.int32)
             for b, p in enumerate(rows):
                 a[b, :len(p)] = p
