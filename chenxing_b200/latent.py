@@ -161,16 +161,12 @@ class LatentPagedKVCache(_BlockPool):
         as they are; a negative slot stores nothing.  ``cow``: (src, dst, n_valid), the
         first n_valid slots of block src are copied into block dst of this layer
         first."""
+        if not 0 <= layer < self.n_layers:       # (to the block copy -1 is every layer)
+            raise IndexError(f"layer {layer} outside [0, {self.n_layers})")
         if cow is not None:
             _check_cow_slots(slot_mapping, cow, self.block_size)
-            src, dst, n = (to_device(c, self.device, float_only=False).to(torch.int32)
-                           for c in cow)
-            with _lib.on_device(self.device):
-                _lib.check(_lib.lib().cx_latent_block_copy(
-                    self._pool, int(layer), src.data_ptr(), dst.data_ptr(), n.data_ptr(),
-                    src.numel(), self.block_size, _lib.raw_stream(self.device)),
-                    "cx_latent_block_copy")
-        self._append(layer, latent, k_rope, slot_mapping, None, None, None, None, 0.0, None)
+            cow = tuple(to_device(c, self.device, float_only=False).to(torch.int32) for c in cow)
+        self._append(layer, latent, k_rope, slot_mapping, None, None, None, None, 0.0, None, cow)
 
     def append_norm_rope(self, layer: int, latent, k_rope, slot_mapping, positions, rope,
                          q_rope=None, *, weight=None, eps: float = 1e-6, q_out_dtype=None):
@@ -194,7 +190,7 @@ class LatentPagedKVCache(_BlockPool):
                             eps, q_out_dtype)
 
     def _append(self, layer, latent, k_rope, slots, positions, rope, q_rope, weight, eps,
-                q_out_dtype):
+                q_out_dtype, cow=None):
         dev, dc, dr = self.device, self.latent_dim, self.rope_dim
         lt, kt = _rows2(latent, dev), _rows2(k_rope, dev)
         dt, T = lt.dtype, lt.shape[0]
@@ -238,6 +234,11 @@ class LatentPagedKVCache(_BlockPool):
                                   rope.cos.data_ptr(), rope.sin.data_ptr(), rope.rows,
                                   rope.head_dim)
         with _lib.on_device(dev):
+            if cow is not None:                  # (nothing is copied for rows that are refused)
+                src, dst, n = cow
+                _lib.check(_lib.lib().cx_latent_block_copy(
+                    self._pool, int(layer), src.data_ptr(), dst.data_ptr(), n.data_ptr(),
+                    src.numel(), self.block_size, _lib.raw_stream(dev)), "cx_latent_block_copy")
             _lib.check(_lib.lib().cx_latent_append(
                 self._pool, int(layer), rows, st.data_ptr(), _lib.ptr(ps), how, _lib.ptr(qo),
                 q_code, _lib.raw_stream(dev)), "cx_latent_append")

@@ -59,3 +59,28 @@ def test_engine_keeps_the_first_rows_of_a_chain():
     assert moved == [] and s.n_tokens == plan.n_past[0]
     e.accept(plan, [[0, 1]])
     assert moved == [[[0, 1]]] and s.n_tokens == plan.n_past[0] + 2
+
+
+# ---------------------------------------------------------------------------
+# rows of the latent cache
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("layer", [-1, 2])
+def test_append_with_copies_checks_the_layer_first(monkeypatch, layer):
+    """The block copy takes -1 for every layer: an append must not come that far."""
+    called = []
+    monkeypatch.setattr(_lib, "on_device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(_lib, "raw_stream", lambda d: None)
+    monkeypatch.setattr(_lib, "lib", lambda: SimpleNamespace(
+        cx_latent_block_copy=lambda *a: called.append("copy") or 0,
+        cx_latent_append=lambda *a: called.append("append") or 0))
+    c = _latent_cache()
+    rows = torch.zeros(1, 128), torch.zeros(1, 64), [40]
+    with pytest.raises(IndexError):
+        c.append_batch(layer, *rows, cow=([1], [2], [8]))
+    with pytest.raises(IndexError):
+        c.append_batch(layer, *rows)
+    with pytest.raises(ValueError):                        # rows that are refused: no copy either
+        c.append_batch(1, rows[0][:, :64], *rows[1:], cow=([1], [2], [8]))
+    assert called == []
+    c.append_batch(1, *rows, cow=([1], [2], [8]))
+    assert called == ["copy", "append"]
