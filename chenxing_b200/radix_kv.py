@@ -384,8 +384,11 @@ class RadixIndex:
 def _check_cow_slots(slots, cow, block_size: int) -> None:
     """Raise ValueError if a slot lands inside the copied prefix of a
     copy-on-write destination block (the copy and the stores of one append
-    launch run concurrently).  Device tensors are not inspected: reading them
-    would synchronise the stream."""
+    launch run concurrently), or if the three of ``cow`` differ in length (the copy
+    reads as many of each as there are sources).  Device tensors are not inspected
+    further: reading them would synchronise the stream."""
+    if len({x.numel() if isinstance(x, torch.Tensor) else np.size(x) for x in cow}) != 1:
+        raise ValueError("copy-on-write: src, dst and n_valid differ in length")
     if any(isinstance(x, torch.Tensor) and x.is_cuda for x in (slots, *cow)):
         return
     s = np.asarray(slots.numpy() if isinstance(slots, torch.Tensor) else slots,

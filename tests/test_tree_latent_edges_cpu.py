@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from chenxing_b200 import BatchedKVEngine, PagedBatch, _lib
+from chenxing_b200 import BatchedKVEngine, PagedBatch, RadixPagedKVCache, _lib
 from chenxing_b200.engine import KVSequence, StepPlan
 from test_latent_refusals_cpu import _latent_cache, _Recorder
 
@@ -84,3 +84,19 @@ def test_append_with_copies_checks_the_layer_first(monkeypatch, layer):
     assert called == []
     c.append_batch(1, *rows, cow=([1], [2], [8]))
     assert called == ["copy", "append"]
+
+
+@pytest.mark.parametrize("cow", [([1, 3], [2], [8]), ([1], [2, 4], [8]), ([1, 3], [2, 4], [8]),
+                                 (torch.tensor([1, 3]), torch.tensor([2, 4]), torch.tensor([8]))])
+@pytest.mark.parametrize("latent", [False, True])
+def test_copies_of_one_length(cow, latent):
+    """The copies read as many destinations and counts as there are sources."""
+    if latent:
+        c, rows = _latent_cache(), (torch.zeros(1, 128), torch.zeros(1, 64))
+    else:
+        c = object.__new__(RadixPagedKVCache)
+        c.block_size, c.device = 16, torch.device("cpu")
+        rows = torch.zeros(1, 2, 64), torch.zeros(1, 2, 64)
+    c._append = c.append_slots = lambda *a: pytest.fail("came as far as the launch")
+    with pytest.raises(ValueError):
+        c.append_batch(0, *rows, [100], cow=cow)
