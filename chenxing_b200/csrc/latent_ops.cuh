@@ -388,9 +388,11 @@ __global__ void __launch_bounds__(256) accept_kernel(const AcceptParams p) {
     int n = lane < p.path_len ? path[lane] : -1;      // (beside the lengths, not behind them)
     const int q0 = p.q_start ? p.q_start[b] : b, T = p.q_start ? p.q_start[b + 1] - q0 : 1;
     const int64_t ctx = p.ctx_lens[b], cap = p.table_stride * p.block_size, base = ctx - T;
-    if (T <= 0) return;
-    if (base < 0 || ctx > cap) {
-        if (threadIdx.x == 0 && blockIdx.x == 0) raise_flag(CX_DEV_BAD_QLEN);
+    if (T <= 0 || base < 0 || ctx > cap) {
+        // (a row without nodes or context, as a padded batch has them: nothing to move, and
+        // nothing wrong unless its path asks for some)
+        if (threadIdx.x == 0 && blockIdx.x == 0 && n >= 0)
+            raise_flag(T <= 0 ? CX_DEV_BAD_PATH : CX_DEV_BAD_QLEN);
         return;
     }
     const int64_t words = (int64_t)p.planes * p.row_words;

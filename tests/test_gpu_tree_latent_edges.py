@@ -115,3 +115,43 @@ def test_nan_queries_of_scored_chains(ctx, hq, hk, d, dtype, n):
     for r in rows:
         c.q_dev[r][3] = math.nan
     _check_nan_rows(c, c.run(out_dtype=dtype), rows)
+
+
+@pytest.mark.parametrize("latent", [False, True])
+@pytest.mark.parametrize("as_tensor", [False, True])
+def test_accept_of_rows_without_nodes(latent, as_tensor):
+    """A padded row (no context) of a decode batch, and a sequence without nodes: empty
+    paths raise nothing, and the others move; a path that asks such a row for a node
+    raises the flag of its fault."""
+    from chenxing_b200 import (LatentBatch, LatentPagedKVCache, PagedBatch, RadixPagedKVCache,
+                               _lib)
+    if latent:
+        cache = LatentPagedKVCache(6, 16, 2, 64, 16, dtype=BF, host_io=False)
+        pools, make = [cache.kv_pool], LatentBatch
+        kw = dict(n_q_heads=4, scale=1.0)
+    else:
+        cache = RadixPagedKVCache(6, 16, 2, 2, 64, dtype=BF, host_io=False)
+        pools, make = [cache.k_pool, cache.v_pool], PagedBatch
+        kw = dict(n_q_heads=4)
+    gen = torch.Generator().manual_seed(1)
+    for p in pools:
+        p.copy_(torch.randn(p.shape, generator=gen).to(BF))
+    before = [p.clone() for p in pools]
+
+    def accept(batch, paths):
+        width = max(map(len, paths)) + 1
+        cache.accept_paths(batch, torch.tensor([p + [-1] * (width - len(p)) for p in paths],
+                                               device="cuda") if as_tensor else paths)
+        return _lib.device_flags(clear=True)
+
+    decode = make(cache, [[1], [], [3, 4]], [5, 0, 20], **kw)
+    assert accept(decode, [[0], [], [0]]) == 0             # (in place already)
+    drafted = make(cache, [[1], [], [3, 4], [5]], [5, 0, 20, 7], q_lens=[3, 0, 4, 0], **kw)
+    assert all(torch.equal(p, b) for p, b in zip(pools, before))
+    assert accept(drafted, [[1, 2], [], [0, 3], []]) == 0
+    for p, b in zip(pools, before):
+        assert torch.equal(p[:, 1, 2:4], b[:, 1, 3:5])
+        assert torch.equal(p[:, 4, 1], b[:, 4, 3]) and torch.equal(p[:, 4, 0], b[:, 4, 0])
+    if as_tensor:
+        assert accept(drafted, [[], [], [], [0]]) == 64    # no such node
+        assert accept(decode, [[], [0], []]) == 16         # no context
