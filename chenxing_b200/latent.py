@@ -186,6 +186,9 @@ class LatentPagedKVCache(_BlockPool):
                              f"{self.rope_dim}")
         if rope.device != self.device and not _lib.same_device(rope.device, self.device):
             raise ValueError(f"RoPE tables on {rope.device}, the cache on {self.device}")
+        if positions is None:
+            raise ValueError("append_norm_rope needs positions (append_batch stores rows as they "
+                             "are)")
         return self._append(layer, latent, k_rope, slot_mapping, positions, rope, q_rope, weight,
                             eps, q_out_dtype)
 

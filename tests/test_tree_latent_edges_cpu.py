@@ -100,3 +100,13 @@ def test_copies_of_one_length(cow, latent):
     c._append = c.append_slots = lambda *a: pytest.fail("came as far as the launch")
     with pytest.raises(ValueError):
         c.append_batch(0, *rows, [100], cow=cow)
+
+
+def test_rotation_needs_positions(monkeypatch):
+    """Without them the shared key part would be stored unrotated."""
+    monkeypatch.setattr(_lib, "lib", lambda: pytest.fail("came as far as the launch"))
+    c = _latent_cache()
+    rope = SimpleNamespace(head_dim=64, device=torch.device("cpu"), interleaved=0, rows=8,
+                           cos=torch.zeros(8, 64), sin=torch.zeros(8, 64))
+    with pytest.raises(ValueError):
+        c.append_norm_rope(0, torch.zeros(3, 128), torch.zeros(3, 64), torch.arange(3), None, rope)
