@@ -10,8 +10,10 @@ int copy_dev_flags_latent(cudaStream_t s, unsigned int* v) { return copy_dev_fla
 int clear_dev_flags_latent(cudaStream_t s) { return clear_dev_flags(s); }
 
 // Whether the tcgen05 kernel takes the call: 16-bit pools whose rows TMA can load
-// (queries of any alignment), and no queries of the other 16-bit type, whose range or
-// precision the pool's does not hold.
+// (queries of any alignment), with queries of the pool's type or fp32, which are rounded to
+// it as by the kernels over K/V pools (fp32 beyond fp16's 65504 becomes infinite, and the row
+// NaN).  Queries of the other 16-bit type are rare and lose range or precision: they go to
+// the fp32 kernels, which convert nothing.
 static bool latent_tc(const cx_latent_pool* pool, int32_t q_dtype) {
     const int64_t dim = pool->latent_dim + pool->rope_dim;
     return pool->dtype != CX_F32 && (q_dtype == CX_F32 || q_dtype == pool->dtype) &&

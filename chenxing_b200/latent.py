@@ -251,7 +251,11 @@ class LatentPagedKVCache(_BlockPool):
         """One query token per sequence: q = (q_latent (B, Hq, latent_dim), q_rope (B,
         Hq, rope_dim)), of one type and any token and head strides, or one tensor
         (B, Hq, latent_dim + rope_dim) -> (B, Hq, latent_dim), float32 unless ``out`` or
-        ``out_dtype`` says bfloat16 or float16."""
+        ``out_dtype`` says bfloat16 or float16.  Over a 16-bit pool the tcgen05 kernel
+        rounds float32 queries to the pool's type first (over float16 those beyond 65504
+        become infinite, and their rows NaN) and the probabilities before the second
+        product; ``LatentBatch.kernel_kind`` names the kernel, "generic" is fp32
+        throughout."""
         if batch.verify:
             raise ValueError("decode_batch needs a LatentBatch built without q_lens")
         return self._attend(layer, q, batch, out, out_dtype)

@@ -445,7 +445,8 @@ typedef struct cx_latent_q {
  * reach the result; at a position that only some rows see, it must be finite.
  * 16-bit pools on a 16-byte boundary with block_size a multiple of 8 and
  * (latent_dim + rope_dim) a multiple of 8, at least 64, take a tcgen05 kernel, which
- * rounds fp32 queries and the probabilities to the pool's type (the denominator sums
+ * rounds fp32 queries (beyond 65504 over fp16: to infinity, and the row is NaN) and the
+ * probabilities to the pool's type (the denominator sums
  * the rounded ones); all else, and queries of the other 16-bit type, an fp32 kernel.
  * The plan is made in the call: a workspace holds nothing between calls, but calls
  * that overlap need one each. */

@@ -155,3 +155,17 @@ def test_accept_of_rows_without_nodes(latent, as_tensor):
     if as_tensor:
         assert accept(drafted, [[], [], [], [0]]) == 64    # no such node
         assert accept(decode, [[], [0], []]) == 16         # no context
+
+
+def test_fp32_queries_beyond_fp16():
+    """Rounded to the pool's type they are infinite: the row is NaN, no other is touched.
+    Over a bf16 pool, and where the fp32 kernels take the call, the same query is finite."""
+    for dtype, bs in ((F16, 16), (BF, 16), (F16, 20)):
+        c = LatentCase(hq=16, dc=128, dr=64, ctx=[200, 70], dtype=dtype, q_dtype=F32, bs=bs, seed=3)
+        kind = c.batch().kernel_kind(F32)
+        assert kind == ("generic" if bs == 20 else "tcgen05")
+        c.q_dev[0][1, 2, 5] = 1e5
+        if dtype == F16 and kind == "tcgen05":
+            _check_nan_rows(c, c.run(out_dtype=F32), [(1, 2)])
+        else:
+            assert bool(torch.isfinite(c.run(out_dtype=F32)).all())
