@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from scored_cases import ScoredCase, alibi
+from scored_cases import HALF, ScoredCase, alibi
 from tree_cases import LatentCase, TreeCase, random_tree
 
 pytestmark = pytest.mark.gpu
@@ -169,3 +169,133 @@ def test_fp32_queries_beyond_fp16():
             _check_nan_rows(c, c.run(out_dtype=F32), [(1, 2)])
         else:
             assert bool(torch.isfinite(c.run(out_dtype=F32)).all())
+
+
+# ---------------------------------------------------------------------------
+# placement of tcgen05 trees, chains as trees, long chunks
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("B", [32, 33, 64, 100, 128, 129])
+@pytest.mark.parametrize("lengths", ["equal", "distinct", "some"])
+def test_many_trees_on_tcgen05(B, lengths):
+    """The longest contexts start first, ranked 32 at a time up to 128 sequences: every
+    sequence's rows are written once, with ties, ranks across the groups of 32 and
+    sequences without nodes; long tables cut the keys over several CTAs up to 64."""
+    rng = np.random.default_rng(B)
+    sizes = [9 if lengths == "equal" or i % 7 else 0 for i in range(B)]
+    if lengths == "equal":
+        ctx = [40] * B
+    elif lengths == "distinct":
+        ctx = (12 + rng.permutation(B)).tolist()
+    else:
+        ctx = [12 + int(x) for x in rng.integers(0, 4, B) * 16]
+    ctx[B // 2] = 1100
+    c = TreeCase(hq=4, hk=1, d=64, dtype=BF, ctx=ctx, seed=B,
+                 parents=[random_tree(rng, n, "random") for n in sizes])
+    batch = c.batch()
+    assert batch.kernel_kind(BF, BF) == "tcgen05"
+    a = c.run(batch, out_dtype=BF)
+    c.check(a)
+    assert torch.equal(a, c.run(batch, out_dtype=BF))
+
+
+@pytest.mark.parametrize("hq,hk,d,dtype,n,same", [
+    (8, 2, 128, BF, 7, True), (8, 8, 64, F16, 20, True), (4, 2, 96, F16, 8, True),
+    (8, 2, 64, F32, 2, True), (8, 2, 128, BF, 13, False), (8, 2, 64, F32, 8, False),
+    (8, 2, 128, BF, 40, False)])
+def test_a_chain_as_a_tree(hq, hk, d, dtype, n, same):
+    """`same`: chain and tree run one kernel, whose sums then have one order, bit for bit;
+    elsewhere both are within their bounds, and so of each other."""
+    from chenxing_b200 import PagedBatch
+    c = TreeCase(hq=hq, hk=hk, d=d, dtype=dtype, ctx=[n + 200, n + 31], softcap=30.0, window=19,
+                 q_scale=4.0, parents=[random_tree(None, n, "chain")] * 2, seed=d)
+    tree_batch = c.batch()
+    chain_batch = PagedBatch(c.cache, c.tables, c.ctx, n_q_heads=hq, q_lens=c.q_lens,
+                             window=c.window, softcap=c.softcap, scale=c.scale)
+    tree, chain = c.run(tree_batch, out_dtype=dtype), c.run(chain_batch, out_dtype=dtype)
+    c.check(tree)
+    c.check(chain)
+    if same:
+        assert tree_batch.kernel_kind(dtype, dtype) == chain_batch.kernel_kind(dtype, dtype)
+        assert torch.equal(tree, chain)
+    _, tol = c.expected(dtype)
+    assert bool(((tree - chain).double().abs().cpu() <= 2 * tol).all())
+
+
+@pytest.mark.parametrize("hq,dc,dr,dtype", [(16, 512, 64, BF), (4, 256, 64, F16), (3, 128, 32, F32)])
+@pytest.mark.parametrize("window", [None, 100])
+def test_long_chunks_over_latents(hq, dc, dr, dtype, window):
+    c = LatentCase(hq=hq, dc=dc, dr=dr, ctx=[700, 301, 64], q_lens=[300, 301, 5], dtype=dtype,
+                   window=window, seed=dr)
+    c.check(c.run(out_dtype=dtype))
+
+
+# ---------------------------------------------------------------------------
+# the engine: 16-bit pools, a tree behind a tail block that two sequences share
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("latent", [False, True])
+def test_engine_tree_behind_a_shared_tail(latent, dtype):
+    """Sequence 1 shares sequence 0's partly filled tail block, drafts a tree behind it and
+    keeps a path: the block is copied first, sequence 0 keeps its rows, and the cache holds
+    for sequence 1 what decoding the path alone would have left."""
+    from chenxing_b200 import BatchedKVEngine, LatentPagedKVCache, RadixPagedKVCache, RopeTables
+    hq, L = 8, 2
+
+    def engine():
+        if latent:
+            return BatchedKVEngine(LatentPagedKVCache(32, 16, L, 128, 64, dtype=dtype,
+                                                      host_io=False), n_q_heads=hq, scale=0.07)
+        return BatchedKVEngine(RadixPagedKVCache(32, 16, L, 2, 64, dtype=dtype, host_io=False),
+                               n_q_heads=hq)
+
+    gen = torch.Generator().manual_seed(3)
+    rope = RopeTables(256, 64)
+    one = torch.ones(64, device="cuda")
+
+    def rows(n):
+        make = (lambda *s: torch.randn(n, *s, generator=gen).to(dtype).cuda())
+        kv = [(make(128), make(64)) if latent else (make(2, 64), make(2, 64)) for _ in range(L)]
+        return kv, [make(hq, 192 if latent else 64) for _ in range(L)]
+
+    def step(eng, ids, q_lens, new, qs, **kw):
+        plan = eng.plan(ids, q_lens, verify=True, **kw)
+        outs = []
+        for layer, (k, v) in enumerate(new):
+            q = eng.append_rope(plan, layer, k, v, rope, qs[layer][..., -64:],
+                                **({} if latent else dict(k_weight=one)))
+            outs.append(eng.attend(plan, layer, (qs[layer][..., :128], q) if latent else q))
+        return plan, outs
+
+    def read(eng, i, layer, n):
+        return eng.cache.read_layer(eng.seqs[i].block_table, n, layer)
+
+    eng, ref = engine(), engine()
+    tokens = list(range(21))
+    first, q0 = rows(21)
+    n0 = 15                                        # committed of sequence 1, in a shared block
+    for e, i, n in ((eng, 0, 21), (ref, 0, 21), (ref, 1, n0)):
+        e.add(i, tokens[:n])
+        plan, _ = step(e, [i], [n], [(k[:n], v[:n]) for k, v in first], [q[:n] for q in q0])
+        e.commit(plan)
+    assert eng.add(1, tokens[:n0] + [90], share_tail_from=0).n_tokens == n0
+    assert eng.seqs[1].block_table == eng.seqs[0].block_table[:1]
+    kept = [[t.clone() for t in read(eng, 0, layer, 21)] for layer in range(L)]
+    new, qs = rows(6)
+    plan, outs = step(eng, [1], [6], new, qs, tree_parents=[[-1, -1, 0, 1, 1, 4]])
+    assert eng.seqs[1].block_table[0] != eng.seqs[0].block_table[0]
+    path = [1, 4, 5]
+    eng.accept(plan, [path])
+    keep = torch.tensor(path).cuda()
+    plan, want = step(ref, [1], [3], [(k[keep], v[keep]) for k, v in new], [q[keep] for q in qs])
+    ref.commit(plan)
+    assert eng.seqs[1].n_tokens == ref.seqs[1].n_tokens == n0 + 3
+    for layer in range(L):
+        for x, y in zip(read(eng, 1, layer, n0 + 3), read(ref, 1, layer, n0 + 3)):
+            assert torch.equal(x, y)
+        for x, y in zip(read(eng, 0, layer, 21), kept[layer]):
+            assert torch.equal(x, y)
+        # the same scores to fp32; each side rounds its probabilities to the pool's type (of
+        # sums of p |v| up to max |v|), fp16 those below its smallest step too
+        v = read(ref, 1, layer, n0 + 3)[0 if latent else 1].float().abs().max()
+        bound = 2 * (HALF[dtype] + 2.0 ** -16 + (n0 + 3) * 2.0 ** -25) * v
+        assert bool(((outs[layer][keep] - want[layer]).abs() <= bound).all())
