@@ -288,8 +288,9 @@ class PagedBatch:
 
     def row_positions(self) -> np.ndarray:
         """The position of every query row (int64, rows concatenated): where its
-        rotation turns it to.  A node of a tree stands by its depth."""
-        base = np.repeat(self.ctx_host - self.q_lens_host, self.q_lens_host)
+        rotation turns it to.  A node of a tree stands by its depth; the row of a padded
+        sequence (context 0) at 0, which every table has."""
+        base = np.repeat(np.maximum(self.ctx_host - self.q_lens_host, 0), self.q_lens_host)
         if self.is_tree:
             return base + self.depths_host
         return base + np.concatenate([np.arange(n) for n in self.q_lens_host]

@@ -110,3 +110,9 @@ def test_rotation_needs_positions(monkeypatch):
                            cos=torch.zeros(8, 64), sin=torch.zeros(8, 64))
     with pytest.raises(ValueError):
         c.append_norm_rope(0, torch.zeros(3, 128), torch.zeros(3, 64), torch.arange(3), None, rope)
+
+
+def test_positions_of_padded_rows(lib):
+    """A position of -1 is outside every rotation table and would raise a device flag."""
+    b = PagedBatch(_Recorder(), [[0, 1], [], [2]], [20, 0, 5], n_q_heads=4)
+    assert b.row_positions().tolist() == [19, 0, 4]
