@@ -66,26 +66,16 @@ static inline int check_pool(const cx_pool* p) {
 // reads and clears them all.
 static __device__ unsigned int g_dev_flags = 0;
 
-// Starts the copy of this translation unit's word to `v` on `s`, or its clearing;
-// the caller synchronises.
-static int copy_dev_flags(cudaStream_t s, unsigned int* v) {
-    CX_CUDA_CHECK(cudaMemcpyFromSymbolAsync(v, g_dev_flags, sizeof(*v), 0,
-                                            cudaMemcpyDeviceToHost, s));
-    return CX_OK;
-}
-static int clear_dev_flags(cudaStream_t s) {
-    static const unsigned int zero = 0;
-    CX_CUDA_CHECK(cudaMemcpyToSymbolAsync(g_dev_flags, &zero, sizeof(zero), 0,
-                                          cudaMemcpyHostToDevice, s));
-    return CX_OK;
+// This translation unit's word on the current device; nullptr: none.
+static unsigned int* dev_flags() {
+    void* p = nullptr;
+    return cudaGetSymbolAddress(&p, g_dev_flags) == cudaSuccess ? static_cast<unsigned int*>(p)
+                                                                : nullptr;
 }
 
-int copy_dev_flags_scored(cudaStream_t s, unsigned int* v);   // of cxkv_scored.cu
-int clear_dev_flags_scored(cudaStream_t s);
-int copy_dev_flags_tree(cudaStream_t s, unsigned int* v);     // of cxkv_tree.cu
-int clear_dev_flags_tree(cudaStream_t s);
-int copy_dev_flags_latent(cudaStream_t s, unsigned int* v);   // of cxkv_latent.cu
-int clear_dev_flags_latent(cudaStream_t s);
+unsigned int* dev_flags_scored();   // of cxkv_scored.cu
+unsigned int* dev_flags_tree();     // of cxkv_tree.cu
+unsigned int* dev_flags_latent();   // of cxkv_latent.cu
 
 __device__ __forceinline__ void raise_flag(unsigned int bit) {
     atomicOr(&g_dev_flags, bit);

@@ -6,8 +6,7 @@
 
 namespace cx {
 
-int copy_dev_flags_latent(cudaStream_t s, unsigned int* v) { return copy_dev_flags(s, v); }
-int clear_dev_flags_latent(cudaStream_t s) { return clear_dev_flags(s); }
+unsigned int* dev_flags_latent() { return dev_flags(); }
 
 // Whether the tcgen05 kernel takes the call: 16-bit pools whose rows TMA can load
 // (queries of any alignment), with queries of the pool's type or fp32, which are rounded to

@@ -8,8 +8,7 @@
 
 namespace cx {
 
-int copy_dev_flags_tree(cudaStream_t s, unsigned int* v) { return copy_dev_flags(s, v); }
-int clear_dev_flags_tree(cudaStream_t s) { return clear_dev_flags(s); }
+unsigned int* dev_flags_tree() { return dev_flags(); }
 
 }  // namespace cx
 

@@ -299,3 +299,49 @@ def test_engine_tree_behind_a_shared_tail(latent, dtype):
         v = read(ref, 1, layer, n0 + 3)[0 if latent else 1].float().abs().max()
         bound = 2 * (HALF[dtype] + 2.0 ** -16 + (n0 + 3) * 2.0 ** -25) * v
         assert bool(((outs[layer][keep] - want[layer]).abs() <= bound).all())
+
+
+# ---------------------------------------------------------------------------
+# device flags
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("unit", ["scored", "tree", "latent"])
+def test_flags_of_every_unit_are_read_and_cleared(unit):
+    from chenxing_b200 import _lib
+    if unit == "latent":
+        c = LatentCase(hq=4, dc=128, dr=64, ctx=[100], dtype=BF, poison=False)
+    elif unit == "tree":
+        c = TreeCase(hq=8, hk=2, d=64, ctx=[100], parents=[[-1, 0]], poison=False)
+    else:
+        c = ScoredCase(hq=8, hk=2, d=64, ctx=[100], softcap=30.0, poison=False)
+    batch = c.batch()
+    batch.block_tables[0, 2] = c.cache.n_blocks + 5
+    c.run(batch, out_dtype=BF)
+    assert [_lib.device_flags(clear=x) for x in (False, False, True, True, False)] == [2, 2, 2, 0, 0]
+
+
+@pytest.mark.parametrize("clear", [False, True])
+def test_reading_the_flags_copies_once(clear):
+    """One launch collects the words of all units, one copy brings them to the host."""
+    from torch.profiler import ProfilerActivity, profile
+
+    from chenxing_b200 import _lib
+    with profile(activities=[ProfilerActivity.CPU, ProfilerActivity.CUDA],
+                 acc_events=True) as prof:
+        assert _lib.device_flags(clear=clear) == 0
+    calls = {e.key: e.count for e in prof.key_averages()}
+    if not calls.get("cudaStreamSynchronize"):
+        pytest.skip("the profiler sees no runtime calls here")
+    assert calls["cudaStreamSynchronize"] == calls.get("cudaMemcpyAsync") == 1
+    assert calls.get("cudaLaunchKernel", 0) + calls.get("cudaLaunchKernelExC", 0) == 1
+
+
+def test_flags_read_on_streams_by_many_threads():
+    from concurrent.futures import ThreadPoolExecutor
+
+    from chenxing_b200 import _lib
+
+    def read(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            return [_lib.device_flags(clear=i % 2 == 0) for _ in range(50)]
+    with ThreadPoolExecutor(8) as pool:
+        assert not any(sum(pool.map(read, range(8)), []))
