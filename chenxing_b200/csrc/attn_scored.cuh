@@ -23,7 +23,14 @@ static bool tma_shape(const cx_pool* pool, const cx_attn_batch* b) {
 // The tcgen05 kernel: 16-bit pools from 64 packed rows (query tokens x GQA
 // group) of more than one token, and groups that the split-K kernels' 64 rows
 // do not hold.  Trees, whose rows it takes as one query tile in two places, from
-// kTreeTcRows on.
+// kTreeTcRows on, where mma.sync comes to its third row tile of 16.  Microseconds, mma.sync
+// / tcgen05, at 16, 32, 36, 48 and 64 rows:
+//   64 x 4,000 keys, 32 / 8 heads of 128:  192/236  231/240  308/241  317/243  449/248
+//   64 x 4,000 keys, 32 heads of 64:       381/716  610/735  778/740  786/746  1318/750
+//    4 x 1,000 keys, 32 / 8 heads of 128:   34/21    42/22    45/22    53/23    38/24
+//    1 x 8,000 keys, 32 heads of 64:        35/32    48/32    54/33    60/33    70/34
+// (full batches decide: below 33 rows a batch that leaves SMs idle would be better on
+// tcgen05)
 constexpr int64_t kTreeTcRows = 33;
 static bool tc_shape(const cx_pool* pool, const cx_attn_batch* b, bool tree) {
     const int64_t G = b->n_q_heads / pool->n_kv_heads, rows = G * b->max_q_len;

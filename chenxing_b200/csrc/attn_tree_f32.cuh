@@ -9,7 +9,9 @@
 // read), a lane's columns of every key for the outputs (heads of 64: half of the warp
 // takes every other key).  Keys are counted through the visible ones alone, the prefix's
 // and then the window's, so that parts are even whatever lies between.  It is bound by
-// shared memory: 5 reads for 16 products a lane of the scores, 2 for 16 of the outputs.
+// shared memory.  In passes of 128 bytes a warp: 8 for 16 products a lane of the scores (4 of
+// the lanes' own keys, 4 broadcasts), 5 for 16 of the outputs of heads of 128 (4, and 1 of
+// weights).
 // 8 trees of 8 nodes, 8 / 2 heads of 64, behind up to 512 keys: 17 us where the split-K
 // kernel for chains (which still has fewer rows: 32 trees of 4 behind up to 4,096 keys
 // 86 us there, 143 here) took 35 to 52; 100 nodes of 4 heads behind 2,000 keys 66, the

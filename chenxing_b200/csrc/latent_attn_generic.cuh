@@ -12,8 +12,8 @@
 // latent_rows_kernel, more rows: 32 rows share tiles of 32 keys in shared memory, two
 // in turn.  A warp has 4 rows: a lane's key against them for the scores (a query
 // element is one broadcast read), a lane's columns of every key for the outputs.  It
-// is bound by shared memory (8 reads for 16 products of the scores, 17 for 64 of the
-// outputs of 512) and by one CTA an SM: 14 TFLOP/s for 62 tokens of 64 heads behind 1,200
+// is bound by shared memory (in passes of 128 bytes a warp: 8 for 16 products a lane of the
+// scores, 17 for 64 of the outputs of 512) and by one CTA an SM: 14 TFLOP/s for 62 tokens of 64 heads behind 1,200
 // keys of 384 + 64, 558 us.
 //
 // Parts of a context that is split over CTAs are joined by their maxima.

@@ -95,9 +95,10 @@ __device__ __forceinline__ bool lat_slot(const LatAppendParams& p, int64_t t, in
 // of the queries at a time: with rows of 16-byte multiples a lane holds 8 pairs, whose
 // angles it loads once for all its heads.  All that a lane needs first (rows, slot,
 // position) is asked for before any of it is looked at; then come the angles and the
-// weights.  8,192 tokens, 32 heads, bf16, 90 MB: 23 us; with a head a lane, twice the
-// warps and 56 registers, which spill, 27 (64 tokens: 2.5 and 2.7); with loads that are converted where they
-// are made, one after the other, 47.
+// weights.  8,192 tokens, 32 heads, bf16, 90 MB: 23 us.  72 registers a lane: it still spills,
+// 96 bytes in 16 bits and 172 in fp32.  With a head a lane, twice the warps and 56 registers,
+// which spill more, 27 (64 tokens: 2.5 and 2.7); with loads that are converted where they are
+// made, one after the other, 47.
 constexpr int kLaHeads = 2;       // heads a lane asks for at once
 constexpr int kLaWarps = 5;
 template <typename E>
